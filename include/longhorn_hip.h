@@ -370,6 +370,96 @@ int lhq_gemm_fp8_e4m3(const uint8_t* A, const uint8_t* Bt, const float* A_scale,
                       const float* B_scale, float* C, int M, int N, int K, float alpha,
                       float beta, void* stream);
 
+/* ---- 8-bit key/value cache and attention over it ------------------------- */
+/* No reference counterpart on the quantized-GEMM path: what a decode step
+ * runs between its quantized projections.
+ *
+ * The cache is paged.  A page holds 64 tokens of every kv head as codes, one
+ * byte a value (format LHQ_KV_INT8: two's complement in [-127, 127];
+ * LHQ_KV_FP8: e4m3), with one fp32 scale for each (token, head) and for keys
+ * and values apart; a value is code * scale.  Dp = head_dim rounded up to 32:
+ *   k_codes  [num_pages][n_kv_heads][64][Dp]
+ *   v_codes  [num_pages][n_kv_heads][Dp][64]  channel-major; token t of a page
+ *     at byte 16*((t>>2)&3) + 8*(t>>5) + 4*((t>>4)&1) + (t&3) of a row: the
+ *     operand order of the 16x16x32 MFMA, as in the W4 layout above
+ *   k_scales, v_scales  [num_pages][n_kv_heads][64] fp32
+ * codes zero past head_dim, all four 16-byte aligned.  lhq_kv_codes_bytes and
+ * lhq_kv_scales_bytes give the size of each (0 for dims that are refused).
+ * The caller hands out pages: block_table [n_seqs][max_pages] names the page
+ * of the cache that holds tokens 64p .. 64p+63 of a sequence.  An entry
+ * outside [0, num_pages) is no page: nothing is written there, it reads as
+ * zeros and attention does not see its tokens.  Two sequences may share pages
+ * that neither of them writes.
+ *
+ * Rows of new tokens: sequence s owns rows [offsets[s], offsets[s+1]) (device
+ * table [n_seqs + 1], as in the grouped GEMMs), its row i being the token at
+ * position start[s] + i.  row_capacity bounds offsets[n_seqs]; table values
+ * outside [0, row_capacity] are clamped to it.  head_dim <= 256. */
+#define LHQ_KV_INT8 0
+#define LHQ_KV_FP8 1
+int64_t lhq_kv_codes_bytes(int num_pages, int n_kv_heads, int head_dim);
+int64_t lhq_kv_scales_bytes(int num_pages, int n_kv_heads);
+/* Quantize new tokens into the cache, by the rule of the per-row quantizers
+ * above with a row = one token of one head, bit for bit (quant.cpp:52-63,
+ * 195-206).  Row r of k (of v) starts at element r * k_stride (v_stride), its
+ * heads one after the other, so both may be slices of one projection's output.
+ * rows (device, [row_capacity], or NULL: the identity) names the row of k and
+ * v that becomes row i of the list -- the accepted ones of drafted tokens; one
+ * outside [0, n_rows) is skipped.  A position listed twice gets either token. */
+int lhq_kv_write_f32(const float* k, const float* v, int64_t k_stride, int64_t v_stride,
+                     const int32_t* rows, const int32_t* offsets, const int32_t* start,
+                     const int32_t* block_table, uint8_t* k_codes, float* k_scales,
+                     uint8_t* v_codes, float* v_scales, int format, int n_seqs, int n_rows,
+                     int row_capacity, int max_pages, int num_pages, int n_kv_heads, int head_dim,
+                     void* stream);
+int lhq_kv_write_bf16(const uint16_t* k, const uint16_t* v, int64_t k_stride, int64_t v_stride,
+                      const int32_t* rows, const int32_t* offsets, const int32_t* start,
+                      const int32_t* block_table, uint8_t* k_codes, float* k_scales,
+                      uint8_t* v_codes, float* v_scales, int format, int n_seqs, int n_rows,
+                      int row_capacity, int max_pages, int num_pages, int n_kv_heads, int head_dim,
+                      void* stream);
+/* Read cached tokens back: k_out, v_out [row_capacity, n_kv_heads, head_dim]
+ * get code * scale (bf16: rounded once).  Rows that the table names no
+ * sequence for are left as they are. */
+int lhq_kv_read_f32(const uint8_t* k_codes, const float* k_scales, const uint8_t* v_codes,
+                    const float* v_scales, const int32_t* offsets, const int32_t* start,
+                    const int32_t* block_table, float* k_out, float* v_out, int format, int n_seqs,
+                    int row_capacity, int max_pages, int num_pages, int n_kv_heads, int head_dim,
+                    void* stream);
+int lhq_kv_read_bf16(const uint8_t* k_codes, const float* k_scales, const uint8_t* v_codes,
+                     const float* v_scales, const int32_t* offsets, const int32_t* start,
+                     const int32_t* block_table, uint16_t* k_out, uint16_t* v_out, int format,
+                     int n_seqs, int row_capacity, int max_pages, int num_pages, int n_kv_heads,
+                     int head_dim, void* stream);
+/* Attention of new tokens -- one a sequence in plain decode, a drafted tree in
+ * speculative decode -- over the first lengths[s] tokens of the cache and over
+ * one another:  out = softmax(scale * q K^T) V per query head, query head i
+ * reading kv head i / (n_heads / n_kv_heads); bf16 in and out, fp32 sums.
+ * tree [row_capacity]: bit j of a row's word lets it see the sequence's new
+ * token j (NULL: those up to itself); bits past the sequence's last token are
+ * ignored.  k_new, v_new are the new tokens' own keys and values, not yet in
+ * the cache (strides as above; both NULL: only the cache is seen).  A row that
+ * sees nothing gives zeros.  max_new <= 64 bounds the new tokens of a
+ * sequence; of one that has more, those past max_new are not computed and
+ * their rows of out [row_capacity, n_heads, head_dim] are left as they are.
+ * lengths are clamped to [0, 64 * max_pages].  scale must be finite and
+ * positive.
+ * workspace: the sequences' tokens are split over workgroups, whose partial
+ * sums meet there and are added in order of position (deterministic).  Up to
+ * lhq_kv_attn_workspace_bytes bytes are used; with less, or NULL, there are
+ * fewer splits.  Device memory, 16-byte aligned, any contents, not shared with
+ * a call running concurrently. */
+int64_t lhq_kv_attn_workspace_bytes(int n_seqs, int row_capacity, int max_new, int max_pages,
+                                    int n_heads, int n_kv_heads, int head_dim);
+int lhq_kv_attn_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k_new, int64_t k_stride,
+                     const uint16_t* v_new, int64_t v_stride, const uint64_t* tree,
+                     const int32_t* offsets, const int32_t* lengths, const int32_t* block_table,
+                     const uint8_t* k_codes, const float* k_scales, const uint8_t* v_codes,
+                     const float* v_scales, uint16_t* out, int format, int n_seqs,
+                     int row_capacity, int max_new, int max_pages, int num_pages, int n_heads,
+                     int n_kv_heads, int head_dim, float scale, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
 /* ---- fp32 GEMM: gemm.hpp:13-29 / gemm.cpp:5-75 -------------------------- */
 /* lh::gemm semantics (beta first; beta == 0 never reads C). */
 int lhq_gemm_f32(const float* A, const float* B, float* C, int M, int N, int K,

@@ -84,6 +84,14 @@ SIGNATURES = {
     "lhq_gemm_w8a8_bf16": [_p, _p, _p, _p, _p, _i, _i, _i, _p],
     "lhq_gemm_w8a8_i32": [_p, _p, _p, _i, _i, _i, _p],
     "lhq_gemm_fp8_e4m3": [_p, _p, _p, _p, _p, _i, _i, _i, _f, _f, _p],
+    "lhq_kv_codes_bytes": [_i, _i, _i],
+    "lhq_kv_scales_bytes": [_i, _i],
+    "lhq_kv_write_f32": [_p, _p, _i64, _i64] + [_p] * 8 + [_i] * 8 + [_p],
+    "lhq_kv_write_bf16": [_p, _p, _i64, _i64] + [_p] * 8 + [_i] * 8 + [_p],
+    "lhq_kv_read_f32": [_p] * 9 + [_i] * 7 + [_p],
+    "lhq_kv_read_bf16": [_p] * 9 + [_i] * 7 + [_p],
+    "lhq_kv_attn_workspace_bytes": [_i] * 7,
+    "lhq_kv_attn_bf16": [_p, _i64, _p, _i64, _p, _i64] + [_p] * 9 + [_i] * 9 + [_f, _p, _i64, _p],
     "lhq_gemm_f32": [_p, _p, _p, _i, _i, _i, _f, _f, _p],
     "lhq_gemm_f32_ref": [_p, _p, _p, _i, _i, _i, _f, _f, _p],
     "lhq_gemm_f32_batched": [_p, _p, _p, _i, _i, _i, _i, _f, _f, _p],
@@ -107,6 +115,9 @@ _RESTYPES = {
     "lhq_w4_scales_bytes": _i64,
     "lhq_w4_zeros_bytes": _i64,
     "lhq_b8_prepacked_bytes": _i64,
+    "lhq_kv_codes_bytes": _i64,
+    "lhq_kv_scales_bytes": _i64,
+    "lhq_kv_attn_workspace_bytes": _i64,
     "lhq_gemm_w4a16_workspace_bytes": _i64,
     "lhq_gemm_w4a16_bf16_workspace_bytes": _i64,
     "lhq_gemm_w4a16_bf16_grouped_workspace_bytes": _i64,

@@ -1,0 +1,110 @@
+// kvcommon.hpp -- the paged 8-bit key/value cache: layout, argument checks and
+// the device-side list of (sequence, page) tiles that its kernels walk.
+//
+// A page holds kKvPage = 64 tokens of every kv head, one byte a value, with
+// Dp = head_dim rounded up to 32 (the k extent of one 16x16x32 MFMA):
+//   keys    [page][head][64 tokens][Dp]   a token's row is contiguous
+//   values  [page][head][Dp][64 tokens]   a channel's row holds the page's
+//     tokens in kv_slot order, so that 8 adjacent bytes are the k elements
+//     that one lane of a 16x16x32 MFMA takes from two score tiles that the
+//     lane itself holds (see kvattn.hip)
+//   scales  [page][head][64] fp32, for keys and for values
+// Values past head_dim in a row are zero codes.
+#pragma once
+
+#include "common.hpp"
+
+namespace lhq {
+
+constexpr int kKvPage = 64;
+constexpr int kKvMaxDim = 256;
+constexpr int kKvMaxNew = 64;  // new tokens of one sequence: a 64-bit mask each
+
+__host__ __device__ constexpr int kv_padded(int D) { return (D + 31) / 32 * 32; }
+// Place of page token t in a value row: lane group g = (t >> 2) & 3 owns bytes
+// 16g .. 16g+15: token 32s + 16h + 4g + r at 16g + 8s + 4h + r.
+__host__ __device__ constexpr int kv_slot(int t) {
+    return 16 * ((t >> 2) & 3) + 8 * (t >> 5) + 4 * ((t >> 4) & 1) + (t & 3);
+}
+
+struct KvCache {
+    uint8_t* k;
+    float* ks;
+    uint8_t* v;
+    float* vs;
+    const int32_t* table;  // [n_seqs][max_pages]
+    int max_pages, num_pages, heads, D;
+    __host__ __device__ int Dp() const { return kv_padded(D); }
+    // The pool page that holds page p of sequence s, or -1.
+    __device__ int page(int s, int64_t p) const {
+        if (p < 0 || p >= max_pages) return -1;
+        const int id = table[static_cast<int64_t>(s) * max_pages + p];
+        return id >= 0 && id < num_pages ? id : -1;
+    }
+    __device__ int64_t code_base(int page, int h) const {
+        return (static_cast<int64_t>(page) * heads + h) * kKvPage * Dp();
+    }
+    __device__ int64_t scale_base(int page, int h) const {
+        return (static_cast<int64_t>(page) * heads + h) * kKvPage;
+    }
+};
+
+// Rows [lo, hi) of sequence s by the offsets table, inside [0, capacity]
+// whatever the table holds.
+struct KvRows { int lo, hi; };
+__device__ __forceinline__ KvRows kv_rows(const int32_t* offsets, int s, int capacity) {
+    const int lo = min(max(offsets[s], 0), capacity);
+    return {lo, min(max(offsets[s + 1], lo), capacity)};
+}
+
+// The unit with number `unit` in the list that has count(s) units of sequence
+// 0, then those of sequence 1, ...: its sequence and its number within it, the
+// same in every lane; seq = n_seqs past the end of the list.  Each wave scans
+// the sequences by itself, 64 at a time (no barrier; a batch of 64 is one step).
+struct KvUnit { int seq; int64_t nth; };
+template <typename Count>
+__device__ __forceinline__ KvUnit kv_find_unit(int64_t unit, int n_seqs, Count count) {
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < n_seqs; base += 64) {
+        const int s = base + lane;
+        const int64_t mine = s < n_seqs ? count(s) : 0;
+        int64_t sum = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int64_t v = __shfl_up(sum, d, 64);
+            if (lane >= d) sum += v;
+        }
+        const uint64_t over = __ballot(sum > unit);
+        if (over) {
+            const int l = __builtin_ctzll(over);
+            return {base + l, unit - __shfl(sum - mine, l, 64)};
+        }
+        unit -= __shfl(sum, 63, 64);
+    }
+    return {n_seqs, 0};
+}
+
+// Checks that all entry points of the cache share; `fn` names the caller.
+inline int kv_check(const char* fn, const KvCache& c, int format, int n_seqs, int row_capacity) {
+    LHQ_REQUIRE(format == LHQ_KV_INT8 || format == LHQ_KV_FP8, "%s: unknown cache format %d", fn, format);
+    LHQ_REQUIRE(n_seqs >= 0 && row_capacity >= 0, "%s: bad counts (%d sequences, %d rows)", fn, n_seqs, row_capacity);
+    LHQ_REQUIRE(c.max_pages >= 0 && c.num_pages >= 0 && c.heads > 0 && c.D > 0,
+                "%s: bad cache dims (pages %d of %d, heads %d, head_dim %d)", fn, c.max_pages, c.num_pages, c.heads,
+                c.D);
+    LHQ_SUPPORTED(c.D <= kKvMaxDim, "%s: head_dim %d is over %d", fn, c.D, kKvMaxDim);
+    LHQ_SUPPORTED(c.heads <= 65535, "%s: %d kv heads are over 65535", fn, c.heads);
+    LHQ_SUPPORTED(static_cast<int64_t>(c.max_pages) * kKvPage < (int64_t{1} << 31),
+                  "%s: sequences of 2^31 tokens", fn);
+    return LHQ_OK;
+}
+// The pointers, wanted once there is something to do.
+inline int kv_check_pointers(const char* fn, const KvCache& c) {
+    LHQ_REQUIRE(c.num_pages == 0 || (c.k && c.ks && c.v && c.vs), "%s: null cache pointer", fn);
+    LHQ_REQUIRE(c.max_pages == 0 || c.table, "%s: null block table", fn);
+    auto odd = [](const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; };
+    LHQ_REQUIRE(!odd(c.k, 16) && !odd(c.v, 16), "%s: cache codes must be 16-byte aligned", fn);
+    LHQ_REQUIRE(!odd(c.ks, 16) && !odd(c.vs, 16), "%s: cache scales must be 16-byte aligned", fn);
+    return LHQ_OK;
+}
+
+}  // namespace lhq

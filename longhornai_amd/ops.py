@@ -246,3 +246,168 @@ def gemm_w8a8_i32(Aq, Bt, M, N, K, C=None):
         C = empty((M, N), np.int32)
     lib().call("lhq_gemm_w8a8_i32", P(Aq), P(Bt), P(C), M, N, K, stream())
     return C
+
+
+# ---------------------------------------------------------------------------
+# 8-bit key/value cache and attention over it
+# ---------------------------------------------------------------------------
+
+KV_PAGE = 64
+_KV_FORMATS = {"int8": 0, "fp8": 1}  # LHQ_KV_INT8, LHQ_KV_FP8
+
+
+@dataclass
+class KvCache:
+    """The buffers of a paged 8-bit cache (layout in include/longhorn_hip.h):
+    codes uint8 (keys [pages, heads, 64, Dp], values [pages, heads, Dp, 64]),
+    scales fp32 [pages, heads, 64].  ``fmt`` is "int8" or "fp8"."""
+    fmt: str
+    n_pages: int
+    n_kv_heads: int
+    head_dim: int
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scales: torch.Tensor
+    v_scales: torch.Tensor
+
+    def __post_init__(self):
+        if self.fmt not in _KV_FORMATS:
+            raise ValueError(f"KvCache: format {self.fmt!r} is not one of {sorted(_KV_FORMATS)}")
+        L, dims = lib(), (self.n_pages, self.n_kv_heads, self.head_dim)
+        codes, scales = L.lhq_kv_codes_bytes(*dims), L.lhq_kv_scales_bytes(*dims[:2])
+        if codes <= 0 or scales <= 0:
+            raise ValueError(f"KvCache: bad dims pages={dims[0]} heads={dims[1]} head_dim={dims[2]}")
+        for name, t, dt, nbytes in (("k", self.k, torch.uint8, codes), ("v", self.v, torch.uint8, codes),
+                                    ("k_scales", self.k_scales, torch.float32, scales),
+                                    ("v_scales", self.v_scales, torch.float32, scales)):
+            if t.dtype != dt or not t.is_contiguous() or t.numel() * t.element_size() != nbytes:
+                raise ValueError(f"KvCache: {name} must be {nbytes} contiguous bytes of {dt}, "
+                                 f"got {tuple(t.shape)} {t.dtype}")
+
+    def pointers(self):
+        return self.k.data_ptr(), self.k_scales.data_ptr(), self.v.data_ptr(), self.v_scales.data_ptr()
+
+
+def kv_cache(fmt: str, n_pages: int, n_kv_heads: int, head_dim: int) -> KvCache:
+    """A cache of its own memory; its tokens hold nothing until they are written."""
+    L = lib()
+    codes, scales = L.lhq_kv_codes_bytes(n_pages, n_kv_heads, head_dim), L.lhq_kv_scales_bytes(n_pages, n_kv_heads)
+    if codes <= 0 or scales <= 0:
+        raise ValueError(f"kv_cache: bad dims pages={n_pages} heads={n_kv_heads} head_dim={head_dim}")
+    return KvCache(fmt, n_pages, n_kv_heads, head_dim, zeros((codes,), np.uint8), zeros((codes,), np.uint8),
+                   zeros((scales // 4,), np.float32), zeros((scales // 4,), np.float32))
+
+
+def _kv_rows(fn: str, name: str, t: torch.Tensor, heads: int, D: int, dtypes) -> int:
+    """Checks new tokens' rows [n, heads * D] or [n, heads, D], heads packed;
+    returns the stride between rows."""
+    if t.dtype not in dtypes:
+        raise ValueError(f"{fn}: {name} is {t.dtype}, not one of {[str(d) for d in dtypes]}")
+    shape, st = t.shape, t.stride()
+    if tuple(shape[1:]) == (heads * D,):
+        packed = st[1] == 1 or heads * D == 1
+    elif tuple(shape[1:]) == (heads, D):
+        packed = (st[2] == 1 or D == 1) and (st[1] == D or heads == 1)
+    else:
+        raise ValueError(f"{fn}: {name} has shape {tuple(shape)}, not [n, {heads} * {D}]")
+    if not packed:
+        raise ValueError(f"{fn}: the heads of a row of {name} must lie one after the other (strides {tuple(st)})")
+    return st[0] if shape[0] > 1 else max(st[0], heads * D)
+
+
+def _kv_tables(fn: str, offsets: torch.Tensor, start: torch.Tensor, table: torch.Tensor):
+    """Checks the int32 device tables; returns (sequences, pages of a table row)."""
+    if offsets.dtype != torch.int32 or start.dtype != torch.int32 or table.dtype != torch.int32:
+        raise ValueError(f"{fn}: offsets, positions and block table must be int32")
+    B = start.shape[0]
+    if offsets.shape[0] != B + 1 or table.dim() != 2 or table.shape[0] != B:
+        raise ValueError(f"{fn}: {B} positions with {offsets.shape[0]} offsets and a block table of "
+                         f"{tuple(table.shape)}")
+    if not (offsets.is_contiguous() and start.is_contiguous() and table.is_contiguous()):
+        raise ValueError(f"{fn}: offsets, positions and block table must be contiguous")
+    return B, table.shape[1]
+
+
+def kv_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, start: torch.Tensor,
+             block_table: torch.Tensor, rows: torch.Tensor | None = None) -> None:
+    """Quantize new tokens into the cache.  k, v: fp32, or bf16 as int16 bits,
+    [n, heads * head_dim] (rows may be strided); sequence s's rows
+    offsets[s] .. offsets[s+1] go to its positions from start[s] on.  ``rows``
+    (int32): the row of k and v for each row of that list (one outside them is
+    skipped)."""
+    H, D = cache.n_kv_heads, cache.head_dim
+    ks = _kv_rows("kv_write", "k", k, H, D, (torch.int16, torch.float32))
+    vs = _kv_rows("kv_write", "v", v, H, D, (k.dtype,))
+    B, width = _kv_tables("kv_write", offsets, start, block_table)
+    if v.shape[0] != k.shape[0]:
+        raise ValueError(f"kv_write: {k.shape[0]} rows of keys and {v.shape[0]} of values")
+    if rows is not None and (rows.dtype != torch.int32 or not rows.is_contiguous()):
+        raise ValueError("kv_write: rows must be contiguous int32")
+    n = k.shape[0] if rows is None else rows.numel()
+    lib().call("lhq_kv_write_f32" if k.dtype == torch.float32 else "lhq_kv_write_bf16", P(k), P(v), ks, vs, P(rows),
+               P(offsets), P(start), P(block_table), *cache.pointers(), _KV_FORMATS[cache.fmt], B, k.shape[0], n,
+               width, cache.n_pages, H, D, stream())
+
+
+def kv_read(cache: KvCache, offsets: torch.Tensor, start: torch.Tensor, block_table: torch.Tensor, n: int,
+            bf16: bool = True, out: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """Cached tokens as values: row i of sequence s's rows offsets[s] ..
+    offsets[s+1] is its position start[s] + i.  n rows in all; returns (k, v)
+    [n, heads, head_dim], bf16 as int16 bits or fp32."""
+    H, D = cache.n_kv_heads, cache.head_dim
+    B, width = _kv_tables("kv_read", offsets, start, block_table)
+    dt = torch.int16 if bf16 else torch.float32
+    if out is None:
+        both = torch.empty((2, n, H, D), dtype=dt, device=cache.k.device)
+        out = both[0], both[1]
+    for t in out:
+        if t.dtype != dt or tuple(t.shape) != (n, H, D) or not t.is_contiguous():
+            raise ValueError(f"kv_read: outputs must be contiguous [{n}, {H}, {D}] {dt}")
+    lib().call("lhq_kv_read_bf16" if bf16 else "lhq_kv_read_f32", *cache.pointers(), P(offsets), P(start),
+               P(block_table), P(out[0]), P(out[1]), _KV_FORMATS[cache.fmt], B, n, width, cache.n_pages, H, D,
+               stream())
+    return out
+
+
+def kv_attn_workspace(cache: KvCache, n_seqs: int, n: int, max_new: int, max_pages: int,
+                      n_heads: int) -> torch.Tensor | None:
+    """A device workspace of the size lhq_kv_attn_bf16 can use (None: it needs none)."""
+    nbytes = lib().lhq_kv_attn_workspace_bytes(n_seqs, n, max_new, max_pages, n_heads, cache.n_kv_heads,
+                                               cache.head_dim)
+    return empty((nbytes,), np.uint8) if nbytes > 0 else None
+
+
+def kv_attn(cache: KvCache, q: torch.Tensor, offsets: torch.Tensor, lengths: torch.Tensor,
+            block_table: torch.Tensor, k_new: torch.Tensor | None, v_new: torch.Tensor | None,
+            tree: torch.Tensor | None = None, scale: float | None = None, max_new: int = 1,
+            workspace: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of new tokens (q [n, heads * head_dim], bf16 as int16 bits)
+    over the first lengths[s] cached tokens of their sequence and over the new
+    ones (k_new, v_new) that tree (int64, a bit for each) names -- None: those
+    up to the token itself.  Returns out [n, heads, head_dim], int16 bits."""
+    H, D = cache.n_kv_heads, cache.head_dim
+    B, width = _kv_tables("kv_attn", offsets, lengths, block_table)
+    n, heads = q.shape[0], (q.shape[1] // D if q.dim() == 2 else q.shape[1])
+    bits = (torch.int16,)
+    qs = _kv_rows("kv_attn", "q", q, heads, D, bits)
+    if heads % H != 0:
+        raise ValueError(f"kv_attn: {heads} query heads over {H} kv heads")
+    if (k_new is None) != (v_new is None):
+        raise ValueError("kv_attn: new keys without values, or values without keys")
+    ks = vs = 0
+    if k_new is not None:
+        ks = _kv_rows("kv_attn", "k_new", k_new, H, D, bits)
+        vs = _kv_rows("kv_attn", "v_new", v_new, H, D, bits)
+        if k_new.shape[0] != n or v_new.shape[0] != n:
+            raise ValueError(f"kv_attn: {n} queries with {k_new.shape[0]} new keys and {v_new.shape[0]} values")
+    if tree is not None and (tree.dtype != torch.int64 or tree.numel() != n or not tree.is_contiguous()):
+        raise ValueError(f"kv_attn: tree must hold {n} contiguous int64 words")
+    if out is None:
+        out = torch.empty((n, heads, D), dtype=torch.int16, device=q.device)
+    elif out.dtype != torch.int16 or out.numel() != n * heads * D or not out.is_contiguous():
+        raise ValueError(f"kv_attn: out must be contiguous [{n}, {heads}, {D}] int16")
+    nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    lib().call("lhq_kv_attn_bf16", P(q), qs, P(k_new), ks, P(v_new), vs, P(tree), P(offsets), P(lengths),
+               P(block_table), *cache.pointers(), P(out), _KV_FORMATS[cache.fmt], B, n, max_new, width, cache.n_pages,
+               heads, H, D, D ** -0.5 if scale is None else scale, P(workspace), nbytes, stream())
+    return out
