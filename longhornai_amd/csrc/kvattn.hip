@@ -5,12 +5,43 @@
 //   o   = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m)     new ones its mask names
 // Keys and values of cached tokens are code * scale; a token whose page is
 // missing is not seen; a query that sees nothing gives zeros.
+//
+// One pass over the cache with a running maximum and sum.  A wave owns 16 * NQ
+// queries of one kv head (the new tokens' query heads that share it) and every
+// NW-th page of a range; it reads the page from memory into registers and works
+// on it there, so no wave waits for another until the end, where the waves of
+// the workgroup join their sums in LDS.  Both products are 16x16x32 MFMAs on
+// transposed tiles: S^T = K Q^T leaves a lane with 4 adjacent tokens of one
+// query for each 16-token tile, which is what it needs as the B operand of
+// O^T = V^T P^T when the value codes lie in kv_slot order -- no exchange
+// between lanes, and a query's maximum and rescaling factor are one register.
+// Precision: key codes are exact in bf16 and meet the queries' own bf16; value
+// codes are exact in fp16, and a weight times its value scale is rounded once
+// to fp16 (2^-11 of itself).  To keep that product in fp16's normal range it
+// is held relative to 2^e, e the running exponent of the largest value scale.
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kvcommon.hpp"
 
 namespace lhq {
 namespace {
+
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+
+// The running maximum follows the scores only when one is over it by more
+// than 2^kLag (rarely, after the first pages): weights go up to 2^kLag and,
+// times value scales held at 2^kTop, stay within fp16's 65504.
+constexpr float kLag = 4.0f;
+constexpr int kTop = 11;
+
+constexpr int kJoinRows = 16;
+// A call is split until it has about this many workgroups (two of four waves
+// fit a CU), a split has this many pages at least, a sequence at most this
+// many splits (one lane each when they are joined).
+constexpr int kTargetGroups = 1024, kLeastPages = 16, kMostSplits = 64;
 
 struct AttnArgs {
     const uint16_t* q;
@@ -25,79 +56,528 @@ struct AttnArgs {
     KvCache c;
     uint16_t* out;
     int n_seqs, capacity, max_new, heads;
-    float scale;
+    float scale2;          // scale * log2 e: weights are powers of two
+    bool vec, vec_out;     // rows of q and k_new: 16-byte loads; of out: 8-byte stores
+    int pages_per_split;   // a sequence of p pages has ceil(p / this) splits
+    int splits;            // the most of one sequence
+    float* ws_ml;          // [row][query head][split] {maximum, sum}
+    float* ws_o;           // [row][query head][split][Dp]
 };
 
+__device__ __forceinline__ int cached(const AttnArgs& a, int s) {
+    return static_cast<int>(min<int64_t>(max(a.lengths[s], 0), static_cast<int64_t>(a.c.max_pages) * kKvPage));
+}
+__device__ __forceinline__ int split_count(const AttnArgs& a, int length) {
+    const int pages = (length + kKvPage - 1) / kKvPage;
+    return max(1, (pages + a.pages_per_split - 1) / a.pages_per_split);
+}
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Four codes as two pairs of bf16 or of fp16 (exact either way).
 template <bool FP8>
-__device__ __forceinline__ float code_value(uint8_t b) {
-    if constexpr (FP8) return e4m3_to_f32(b);
-    else return static_cast<float>(static_cast<int8_t>(b));
+__device__ __forceinline__ u32x2_t codes_bf16(uint32_t w) {
+    if constexpr (FP8) {
+        return {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false)),
+                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))};
+    } else {
+        auto f = [w](int j) { return static_cast<float>(static_cast<int8_t>(w >> (8 * j))); };
+        return {pack_bf16x2(f(0), f(1)), pack_bf16x2(f(2), f(3))};
+    }
+}
+template <bool FP8>
+__device__ __forceinline__ u32x2_t codes_f16(uint32_t w) {
+    if constexpr (FP8) {
+        return {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false)),
+                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true))};
+    } else {
+        // code + 128 in the mantissa of 1024, less 1152
+        const uint32_t b = w ^ 0x80808080u;
+        constexpr uint32_t kExp = 0x64646464u;
+        const f16x2_t off = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+        auto pair = [off](uint32_t u) {
+            return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, u) + off);
+        };
+        return {pair(__builtin_amdgcn_perm(kExp, b, 0x04010400u)), pair(__builtin_amdgcn_perm(kExp, b, 0x04030402u))};
+    }
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {  // rounds to nearest even
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(lhq_f32x2{a, b}, f16x2_t));
+}
+__device__ __forceinline__ f32x4_t mfma_f16_16x16x32(u32x4_t a, u32x4_t b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
+                                                  0, 0, 0);
 }
 
-// One wave per (new token, query head); 64 keys at a time, one a lane, then
-// every lane its channels d = lane + 64 i.
-template <bool FP8>
-__global__ __launch_bounds__(64) void kv_attn_plain_kernel(AttnArgs a) {
-    __shared__ float qs[kKvMaxDim], ps[64];
-    const int row = blockIdx.x, hq = blockIdx.y, lane = threadIdx.x;
-    const int D = a.c.D, Dp = a.c.Dp(), h = hq / (a.heads / a.c.heads);
-    const KvUnit u = kv_find_unit(row, a.n_seqs, [&](int s) {
+// Eight bf16 of a row from channel ch on, those past D as zero.
+__device__ __forceinline__ u32x4_t load_channels(const uint16_t* row, int ch, int D, bool vec) {
+    u32x4_t w = {0, 0, 0, 0};
+    if (vec) {
+        if (ch < D) w = *reinterpret_cast<const u32x4_t*>(row + ch);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (ch + j < D) w[j / 2] |= static_cast<uint32_t>(row[ch + j]) << (16 * (j & 1));
+    }
+    return w;
+}
+
+// The first channel of lane group g in k step i: 64 channels are two steps, of
+// which a group takes 16 adjacent ones (one 16-byte load of key codes); the
+// 32 left over when the steps are odd in number give 8 to a group.
+template <int KS>
+__device__ __forceinline__ int step_channel(int i, int g) {
+    return i < KS / 2 * 2 ? 64 * (i / 2) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g;
+}
+
+// The waves of a workgroup at most; two a SIMD where 256 registers hold a
+// wave's page, queries and sums, else one.
+template <int KS, int NQ>
+constexpr bool two_a_simd() { return KS <= 4 && NQ <= 2; }
+template <int KS, int NQ>
+constexpr int most_waves() { return two_a_simd<KS, NQ>() ? 8 : 4; }
+
+// LDS of a workgroup: each wave's sums [QB][Dp + 4], maxima and sums of
+// weights [2][QB]; before that (NQ > 1) the queries as MFMA operands.
+template <int KS, int NQ>
+constexpr size_t lds_bytes(int waves) {
+    return static_cast<size_t>(waves) * (16 * NQ) * (32 * KS + 4 + 2) * 4;
+}
+
+// Four channels of a result row from channel ch on.
+__device__ __forceinline__ void store_row(uint16_t* row, int ch, int D, const f32x4_t& sum, float weight, bool vec) {
+    f32x4_t y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = weight == 0.0f ? 0.0f : sum[j] / weight;  // nothing seen: zeros
+    if (vec) {
+        if (ch < D) *reinterpret_cast<u32x2_t*>(row + ch) = u32x2_t{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (ch + j < D) row[ch + j] = f32_to_bf16(y[j]);
+    }
+}
+
+template <int KS, int NQ, bool FP8>
+__global__ __launch_bounds__((64 * most_waves<KS, NQ>()), (two_a_simd<KS, NQ>() ? 2 : 1)) void kv_attn_kernel(AttnArgs a) {
+    constexpr int Dp = 32 * KS, QB = 16 * NQ, CT = 2 * KS, kPitch = Dp + 4;
+    extern __shared__ __attribute__((aligned(16))) float attn_lds[];
+    u32x4_t* q_lds = reinterpret_cast<u32x4_t*>(attn_lds);
+    const int H = a.c.heads, G = a.heads / H, D = a.c.D;
+    const int h = blockIdx.x % H;
+    const KvUnit u = kv_find_unit(blockIdx.x / H, a.n_seqs, [&](int s) {
         const KvRows r = kv_rows(a.offsets, s, a.capacity);
-        return static_cast<int64_t>(r.hi - r.lo);
+        const int T = min(r.hi - r.lo, a.max_new);
+        return static_cast<int64_t>((T * G + QB - 1) / QB) * split_count(a, cached(a, s));
     });
-    if (u.seq >= a.n_seqs || u.nth >= a.max_new) return;
-    const KvRows r = kv_rows(a.offsets, u.seq, a.capacity);
-    const int tok = r.lo + static_cast<int>(u.nth), T = min(r.hi - r.lo, a.max_new);
-    const int64_t L = min<int64_t>(max(a.lengths[u.seq], 0), static_cast<int64_t>(a.c.max_pages) * kKvPage);
-    for (int d = lane; d < D; d += 64) qs[d] = bf16_to_f32(a.q[tok * a.q_stride + hq * D + d]) * a.scale;
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, o[kKvMaxDim / 64] = {};
-    auto step = [&](bool seen, float s, auto value) {
-        if (!__ballot(seen)) return;
-        float top = seen ? s : -INFINITY;
-        for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-        const float mn = fmaxf(m, top);
-        const float f = m == -INFINITY ? 0.0f : expf(m - mn), p = seen ? expf(s - mn) : 0.0f;
-        m = mn;
-        float sum = p;
-        for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x, 64);
-        l = l * f + sum;
-        ps[lane] = p;
-        __syncthreads();
-        for (int i = 0; i < kKvMaxDim / 64; ++i) {
-            const int d = lane + 64 * i;
-            if (d >= D) break;
-            float acc = o[i] * f;
-            for (int t = 0; t < 64; ++t)
-                if (ps[t] != 0.0f) acc += ps[t] * value(t, d);
-            o[i] = acc;
-        }
-        __syncthreads();
+    if (u.seq >= a.n_seqs) return;
+    const KvRows rows = kv_rows(a.offsets, u.seq, a.capacity);
+    const int T = min(rows.hi - rows.lo, a.max_new), R = T * G, blocks = (R + QB - 1) / QB;
+    const int L = cached(a, u.seq), pages = (L + kKvPage - 1) / kKvPage, splits = split_count(a, L);
+    const int split = static_cast<int>(u.nth) / blocks, r0 = (static_cast<int>(u.nth) % blocks) * QB;
+    const int p0 = static_cast<int>(static_cast<int64_t>(pages) * split / splits);
+    const int p1 = static_cast<int>(static_cast<int64_t>(pages) * (split + 1) / splits);
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), NW = blockDim.x >> 6;
+
+    // Queries as B operands: column c of tile t is row r0 + 16 t + c of the (token, head of the group) list.
+    auto load_q = [&](int t, int i) -> u32x4_t {
+        const int r = r0 + 16 * t + c;
+        if (r >= R) return {0, 0, 0, 0};
+        return load_channels(a.q + (rows.lo + r / G) * a.q_stride + (h * G + r % G) * D, step_channel<KS>(i, g), D,
+                             a.vec);
     };
-    for (int64_t p = 0; p * kKvPage < L; ++p) {
-        const int page = a.c.page(u.seq, p);
-        if (page < 0) continue;
-        const uint8_t* kc = a.c.k + a.c.code_base(page, h);
-        const uint8_t* vc = a.c.v + a.c.code_base(page, h);
-        const float *ks = a.c.ks + a.c.scale_base(page, h), *vs = a.c.vs + a.c.scale_base(page, h);
-        const bool in = p * kKvPage + lane < L;
-        float s = 0.0f;
-        if (in)
-            for (int d = 0; d < D; ++d) s += qs[d] * code_value<FP8>(kc[lane * Dp + d]);
-        step(in, in ? s * ks[lane] : 0.0f, [&](int t, int d) { return vs[t] * code_value<FP8>(vc[d * kKvPage + kv_slot(t)]); });
+    u32x4_t q_reg[NQ == 1 ? KS : 1];
+    if constexpr (NQ == 1) {
+#pragma unroll
+        for (int i = 0; i < KS; ++i) q_reg[i] = load_q(0, i);
+    } else {
+        for (int n = wave; n < NQ * KS; n += NW) q_lds[n * 64 + lane] = load_q(n / KS, n % KS);
+        __syncthreads();
     }
-    if (a.k_new) {
-        float s = 0.0f;
-        const uint64_t seen = a.tree ? a.tree[tok] : ~uint64_t{0} >> (63 - u.nth);
-        const bool in = lane < T && ((seen >> lane) & 1);
-        if (in)
-            for (int d = 0; d < D; ++d) s += qs[d] * bf16_to_f32(a.k_new[(r.lo + lane) * a.k_stride + h * D + d]);
-        step(in, s, [&](int t, int d) { return bf16_to_f32(a.v_new[(r.lo + t) * a.v_stride + h * D + d]); });
+    auto query = [&](int t, int i) -> u32x4_t {
+        if constexpr (NQ == 1) return q_reg[i];
+        else return q_lds[(t * KS + i) * 64 + lane];
+    };
+
+    f32x4_t o[NQ][CT], x[NQ][4];
+    float m[NQ], l[NQ];
+    int e = -200;  // (under every exponent: the first value scale that is not zero sets it)
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+        m[t] = -INFINITY;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < CT; ++i) o[t][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
-    for (int i = 0; i < kKvMaxDim / 64; ++i) {
-        const int d = lane + 64 * i;
-        if (d < D) a.out[(static_cast<int64_t>(tok) * a.heads + hq) * D + d] = f32_to_bf16(l == 0.0f ? 0.0f : o[i] / l);
+    // Sums from here on are relative to 2^to (to > e).
+    auto raise = [&](int to) {
+#pragma unroll
+        for (int t = 0; t < NQ; ++t)
+#pragma unroll
+            for (int i = 0; i < CT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[t][i][j] = ldexpf(o[t][i][j], max(e - to, -400));
+        e = to;
+    };
+    // The exponent that a maximum over lanes asks for; infinite and NaN ones ask for the largest.
+    auto exponent = [](float v) { return v < INFINITY ? __builtin_amdgcn_frexp_expf(v) : 128; };
+    auto across = [](float v) {  // maximum over the four lane groups
+        v = fmaxf(v, __shfl_xor(v, 16, 64));
+        return fmaxf(v, __shfl_xor(v, 32, 64));
+    };
+    // x (scores of 64 tokens) -> weights; times w they are the operands p of the second product.
+    auto weigh = [&](const f32x4_t (&w)[4], u32x4_t (&p)[NQ][2]) {
+#pragma unroll
+        for (int t = 0; t < NQ; ++t) {
+            float top = x[t][0][0];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) top = fmaxf(top, x[t][i][j]);
+            if (__ballot(top > m[t] + kLag)) {
+                const float mn = fmaxf(m[t], across(top));
+                const float f = mn == -INFINITY ? 1.0f : exp2_(m[t] - mn);
+                m[t] = mn;
+                l[t] *= f;
+#pragma unroll
+                for (int i = 0; i < CT; ++i) o[t][i] *= f;
+            }
+            const float ref = m[t] == -INFINITY ? 0.0f : m[t];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f32x4_t y;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    y[j] = exp2_(x[t][i][j] - ref);
+                    l[t] += y[j];
+                }
+                p[t][i / 2][2 * (i & 1)] = pack_f16x2(y[0] * w[i][0], y[1] * w[i][1]);
+                p[t][i / 2][2 * (i & 1) + 1] = pack_f16x2(y[2] * w[i][2], y[3] * w[i][3]);
+            }
+        }
+    };
+
+    // ---- cached tokens: pages p0 + wave, + NW, ... ----
+    uint32_t k[4][2 * KS];
+    u32x4_t v[CT];
+    f32x4_t ks[4], vs[4];
+    auto load_keys = [&](int page) {
+        const uint8_t* base = a.c.k + a.c.code_base(page, h);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const uint8_t* row = base + (16 * t + c) * Dp;
+#pragma unroll
+            for (int i = 0; i < KS / 2; ++i) {
+                const u32x4_t w = *reinterpret_cast<const u32x4_t*>(row + 64 * i + 16 * g);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) k[t][4 * i + j] = w[j];
+            }
+            if constexpr (KS % 2) {
+                const u32x2_t w = *reinterpret_cast<const u32x2_t*>(row + 32 * (KS - 1) + 8 * g);
+                k[t][2 * KS - 2] = w[0];
+                k[t][2 * KS - 1] = w[1];
+            }
+            ks[t] = *reinterpret_cast<const f32x4_t*>(a.c.ks + a.c.scale_base(page, h) + 16 * t + 4 * g);
+        }
+    };
+    auto load_values = [&](int page) {
+        const uint8_t* base = a.c.v + a.c.code_base(page, h);
+#pragma unroll
+        for (int i = 0; i < CT; ++i) v[i] = *reinterpret_cast<const u32x4_t*>(base + (16 * i + c) * kKvPage + 16 * g);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            vs[t] = *reinterpret_cast<const f32x4_t*>(a.c.vs + a.c.scale_base(page, h) + 16 * t + 4 * g);
+    };
+    const int mine = p0 + wave < p1 ? (p1 - p0 - wave + NW - 1) / NW : 0;
+    int ids = 0;
+    auto page_id = [&](int it) {  // 64 entries of the block table at a time, one a lane
+        if ((it & 63) == 0) {
+            const int p = p0 + wave + (it + lane) * NW;
+            ids = p < p1 ? a.c.page(u.seq, p) : -1;
+        }
+        return __builtin_amdgcn_readlane(ids, it & 63);
+    };
+    int page = -1;
+    if (mine > 0) {
+        page = page_id(0);
+        load_keys(max(page, 0));  // (a missing page's place is taken by page 0, of which no token is seen)
+        load_values(max(page, 0));
     }
+    for (int it = 0; it < mine; ++it) {
+        if constexpr (NQ > 1) asm volatile("" ::: "memory");  // the queries stay in LDS
+        const int left = page < 0 ? 0 : min(L - (p0 + wave + it * NW) * kKvPage, kKvPage);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) x[n][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                const u32x2_t lo = codes_bf16<FP8>(k[t][2 * i]), hi = codes_bf16<FP8>(k[t][2 * i + 1]);
+                const u32x4_t key = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) x[n][t] = mfma_bf16_16x16x32(key, query(n, i), x[n][t]);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const f32x4_t s = ks[t] * a.scale2;
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) x[n][t] *= s;
+        }
+        const int next = it + 1 < mine ? page_id(it + 1) : -1;
+        if (it + 1 < mine) load_keys(max(next, 0));
+        if (left < kKvPage) {  // the last page: whatever it holds past the length
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                uint32_t bytes = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const bool in = 16 * t + 4 * g + j < left;
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) x[n][t][j] = in ? x[n][t][j] : -INFINITY;
+                    vs[t][j] = in ? vs[t][j] : 0.0f;
+                    bytes |= in ? 0xffu << (8 * j) : 0u;
+                }
+#pragma unroll
+                for (int i = 0; i < CT; ++i) v[i][t] &= bytes;
+            }
+        }
+        float top = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(vs[t][j]));
+        if (__ballot(top > ldexpf(1.0f, e))) raise(max(e, __builtin_amdgcn_readfirstlane(exponent(across(top)))));
+        f32x4_t w[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[t][j] = ldexpf(vs[t][j], kTop - e);
+        u32x4_t p[NQ][2];
+        weigh(w, p);
+#pragma unroll
+        for (int i = 0; i < CT; ++i)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const u32x2_t lo = codes_f16<FP8>(v[i][2 * s]), hi = codes_f16<FP8>(v[i][2 * s + 1]);
+                const u32x4_t val = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) o[n][i] = mfma_f16_16x16x32(val, p[n][s], o[n][i]);
+            }
+        if (it + 1 < mine) load_values(max(next, 0));
+        page = next;
+    }
+
+    // ---- the new tokens, by the wave whose turn it is after the sequence's last page ----
+    if (a.k_new && split == splits - 1 && wave == (p1 - p0) % NW) {
+        uint64_t seen[NQ];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            const int r = r0 + 16 * n + c, t = r / G;
+            seen[n] = r >= R ? 0 : a.tree ? a.tree[rows.lo + t] : ~uint64_t{0} >> (63 - t);
+            seen[n] &= ~uint64_t{0} >> (64 - T);
+        }
+        float big = 0.0f;
+        bool odd = false;  // values that are not finite: kept out of the product
+        auto value = [&](int t, int ch) {
+            if (t >= T || ch >= D) return 0.0f;
+            const float y = bf16_to_f32(a.v_new[(rows.lo + t) * a.v_stride + h * D + ch]);
+            odd |= !(fabsf(y) < INFINITY);
+            return fabsf(y) < INFINITY ? y : 0.0f;
+        };
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) x[n][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            if (16 * t >= T) continue;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                u32x4_t key = {0, 0, 0, 0};
+                if (16 * t + c < T)
+                    key = load_channels(a.k_new + (rows.lo + 16 * t + c) * a.k_stride + h * D, step_channel<KS>(i, g),
+                                        D, a.vec);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) x[n][t] = mfma_bf16_16x16x32(key, query(n, i), x[n][t]);
+            }
+            for (int i = 0; i < CT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) big = fmaxf(big, fabsf(value(16 * t + 4 * g + j, 16 * i + c)));
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    x[n][t][j] = (seen[n] >> (16 * t + 4 * g + j)) & 1 ? x[n][t][j] * a.scale2 : -INFINITY;
+        for (int s = 32; s; s >>= 1) big = fmaxf(big, __shfl_xor(big, s, 64));
+        // the values themselves as fp16, their largest under 2^15 (fp16's normal range holds 2^-29 of that)
+        const int want = __builtin_amdgcn_readfirstlane(exponent(big)) - 15;
+        if (big > 0.0f && want > e) raise(want);
+        const float one = ldexpf(1.0f, kTop);
+        const f32x4_t w[4] = {{one, one, one, one}, {one, one, one, one}, {one, one, one, one}, {one, one, one, one}};
+        u32x4_t p[NQ][2];
+        weigh(w, p);
+#pragma unroll
+        for (int i = 0; i < CT; ++i)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (32 * s >= T) continue;
+                u32x4_t val;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const int t = 32 * s + 16 * (b / 2) + 4 * g + 2 * (b & 1);
+                    val[b] = pack_f16x2(ldexpf(value(t, 16 * i + c), -e), ldexpf(value(t + 1, 16 * i + c), -e));
+                }
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) o[n][i] = mfma_f16_16x16x32(val, p[n][s], o[n][i]);
+            }
+        if (__ballot(odd))  // a query that sees such a value takes it as it is, the others do not
+            for (int t = 0; t < T; ++t)
+#pragma unroll
+                for (int i = 0; i < CT; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int ch = 16 * i + 4 * g + j;
+                        const float y = ch < D ? bf16_to_f32(a.v_new[(rows.lo + t) * a.v_stride + h * D + ch]) : 0.0f;
+                        if (!(fabsf(y) < INFINITY))
+#pragma unroll
+                            for (int n = 0; n < NQ; ++n)
+                                if ((seen[n] >> t) & 1) o[n][i][j] += y;
+                    }
+    }
+
+    // ---- the waves' sums meet in LDS ----
+    if constexpr (NQ > 1) __syncthreads();  // (the queries' place is taken)
+    float* mine_o = attn_lds + wave * QB * (kPitch + 2);
+    float* mine_ml = mine_o + QB * kPitch;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        float sum = l[n];
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (g == 0) {
+            mine_ml[16 * n + c] = m[n];
+            mine_ml[QB + 16 * n + c] = sum;
+        }
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+            f32x4_t y;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = ldexpf(o[n][i][j], e - kTop);
+            *reinterpret_cast<f32x4_t*>(mine_o + (16 * n + c) * kPitch + 16 * i + 4 * g) = y;
+        }
+    }
+    __syncthreads();
+    for (int n = threadIdx.x; n < QB * (Dp / 4); n += blockDim.x) {
+        const int qr = n / (Dp / 4), ch = 4 * (n % (Dp / 4)), r = r0 + qr;
+        if (r >= R) break;
+        const float* at = attn_lds + qr * kPitch + ch;
+        const float* ml = attn_lds + QB * kPitch + qr;
+        float top = -INFINITY;
+        for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[w * QB * (kPitch + 2)]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+        float weight = 0.0f;
+        for (int w = 0; w < NW; ++w) {
+            const float f = exp2_(ml[w * QB * (kPitch + 2)] - ref);
+            weight += ml[w * QB * (kPitch + 2) + QB] * f;
+            sum += *reinterpret_cast<const f32x4_t*>(at + w * QB * (kPitch + 2)) * f;
+        }
+        const int64_t row = static_cast<int64_t>(rows.lo + r / G) * a.heads + h * G + r % G;
+        if (splits == 1) {
+            store_row(a.out + row * D, ch, D, sum, weight, a.vec_out);
+        } else {
+            const int64_t part = row * a.splits + split;
+            *reinterpret_cast<f32x4_t*>(a.ws_o + part * Dp + ch) = sum;
+            if (ch == 0) {
+                a.ws_ml[2 * part] = top;
+                a.ws_ml[2 * part + 1] = weight;
+            }
+        }
+    }
+}
+
+// Joins the splits of a sequence's rows, in order of position: a workgroup
+// takes 16 (new token, query head) rows of one kv head, a wave one at a time.
+__global__ __launch_bounds__(256) void kv_attn_join_kernel(AttnArgs a) {
+    const int H = a.c.heads, G = a.heads / H, D = a.c.D, Dp = a.c.Dp(), h = blockIdx.x % H;
+    const KvUnit u = kv_find_unit(blockIdx.x / H, a.n_seqs, [&](int s) {
+        const KvRows r = kv_rows(a.offsets, s, a.capacity);
+        return static_cast<int64_t>((min(r.hi - r.lo, a.max_new) * G + kJoinRows - 1) / kJoinRows);
+    });
+    if (u.seq >= a.n_seqs) return;
+    const int splits = split_count(a, cached(a, u.seq));
+    if (splits == 1) return;  // (its rows are there already)
+    const KvRows rows = kv_rows(a.offsets, u.seq, a.capacity);
+    const int R = min(rows.hi - rows.lo, a.max_new) * G, lane = threadIdx.x & 63;
+    // lanes that share the splits of 4 channels
+    const int share = Dp <= 64 ? 4 : Dp <= 128 ? 2 : 1, ch = 4 * (lane & (64 / share - 1)), first = lane / (64 / share);
+    for (int i = threadIdx.x >> 6; i < kJoinRows; i += 4) {
+        const int r = static_cast<int>(u.nth) * kJoinRows + i;
+        if (r >= R) return;
+        const int64_t row = static_cast<int64_t>(rows.lo + r / G) * a.heads + h * G + r % G, part = row * a.splits;
+        const float m = lane < splits ? a.ws_ml[2 * (part + lane)] : -INFINITY;
+        float top = m;
+        for (int s = 32; s; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+        const float f = exp2_(m - (top == -INFINITY ? 0.0f : top));
+        float weight = lane < splits ? a.ws_ml[2 * (part + lane) + 1] * f : 0.0f;
+        for (int s = 32; s; s >>= 1) weight += __shfl_xor(weight, s, 64);
+        f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < splits; s += share) {
+            const float fs = __shfl(f, s + first, 64);
+            if (s + first < splits && ch < Dp)
+                sum += *reinterpret_cast<const f32x4_t*>(a.ws_o + (part + s + first) * Dp + ch) * fs;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (share >= 2) sum[j] += __shfl_xor(sum[j], 32, 64);
+            if (share == 4) sum[j] += __shfl_xor(sum[j], 16, 64);
+        }
+        if (first == 0) store_row(a.out + row * D, ch, D, sum, weight, a.vec_out);
+    }
+}
+
+// How a call is laid out: query tiles of a wave, waves of a workgroup,
+// splits of a sequence, workgroups.
+struct Plan {
+    int tiles, waves, pages_per_split, splits;
+    int64_t units, join_units;  // per kv head
+    int64_t ml_bytes, bytes;
+};
+int64_t unit_bound(int n_seqs, int capacity, int max_new, int G, int block) {
+    const int64_t seqs = std::min(n_seqs, capacity);
+    return std::min(static_cast<int64_t>(capacity) * G / block + seqs,
+                    seqs * ((static_cast<int64_t>(max_new) * G + block - 1) / block));
+}
+Plan make_plan(int n_seqs, int capacity, int max_new, int max_pages, int heads, int kv_heads, int D, int64_t ws_bytes) {
+    const int G = heads / kv_heads, KS = kv_padded(D) / 32;
+    Plan p{};
+    p.tiles = max_new * G <= 16 ? 1 : 2;
+    p.units = unit_bound(n_seqs, capacity, max_new, G, 16 * p.tiles);
+    p.join_units = unit_bound(n_seqs, capacity, max_new, G, kJoinRows);
+    const int64_t groups = std::max<int64_t>(1, p.units * kv_heads), rows = static_cast<int64_t>(capacity) * heads;
+    int64_t splits = std::min<int64_t>({(kTargetGroups + groups - 1) / groups, max_pages / kLeastPages, kMostSplits});
+    for (splits = std::max<int64_t>(splits, 1);; --splits) {
+        p.ml_bytes = splits == 1 ? 0 : (rows * splits * 8 + 15) / 16 * 16;
+        p.bytes = splits == 1 ? 0 : p.ml_bytes + rows * splits * 32 * KS * 4;
+        if (p.bytes <= ws_bytes) break;
+    }
+    p.pages_per_split = std::max<int>(1, (max_pages + splits - 1) / splits);
+    p.splits = static_cast<int>(splits);
+    p.waves = KS <= 4 && groups * splits <= 256 ? 8 : 4;
+    return p;
+}
+
+template <int KS, int NQ, bool FP8>
+int launch(const char* fn, const AttnArgs& a, const Plan& p, hipStream_t s) {
+    constexpr auto kern = &kv_attn_kernel<KS, NQ, FP8>;
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    if (attr != hipSuccess) return set_error(LHQ_ERR_HIP, "%s: dynamic LDS attribute: %s", fn, hipGetErrorString(attr));
+    const unsigned grid = static_cast<unsigned>(p.units * a.c.heads * p.splits);
+    kern<<<grid, 64 * p.waves, lds_bytes<KS, NQ>(p.waves), s>>>(a);
+    return check_launch(fn);
 }
 
 }  // namespace
@@ -109,8 +589,10 @@ extern "C" {
 
 int64_t lhq_kv_attn_workspace_bytes(int n_seqs, int row_capacity, int max_new, int max_pages, int n_heads,
                                     int n_kv_heads, int head_dim) {
-    (void)n_seqs, (void)row_capacity, (void)max_new, (void)max_pages, (void)n_heads, (void)n_kv_heads, (void)head_dim;
-    return 0;
+    if (n_seqs < 0 || row_capacity < 0 || max_new < 0 || max_new > kKvMaxNew || max_pages < 0 || n_kv_heads <= 0 ||
+        n_heads <= 0 || n_heads % n_kv_heads != 0 || head_dim <= 0 || head_dim > kKvMaxDim)
+        return 0;
+    return make_plan(n_seqs, row_capacity, max_new, max_pages, n_heads, n_kv_heads, head_dim, INT64_MAX).bytes;
 }
 
 int lhq_kv_attn_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k_new, int64_t k_stride,
@@ -142,11 +624,44 @@ int lhq_kv_attn_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k_new,
     if (n_seqs == 0 || row_capacity == 0 || max_new == 0) return LHQ_OK;
     if (int st = kv_check_pointers(fn, c)) return st;
     LHQ_REQUIRE(q && offsets && lengths && out, "%s: null pointer", fn);
-    const AttnArgs a{q,     q_stride, k_new, k_stride, v_new,        v_stride, tree,    offsets,
-                     lengths, c,      out,   n_seqs,   row_capacity, max_new,  n_heads, scale};
-    const dim3 grid(row_capacity, n_heads);
-    if (format == LHQ_KV_FP8) kv_attn_plain_kernel<true><<<grid, 64, 0, as_stream(stream)>>>(a);
-    else kv_attn_plain_kernel<false><<<grid, 64, 0, as_stream(stream)>>>(a);
+    auto odd = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; };
+    AttnArgs a{q,        q_stride, k_new,  k_stride,     v_new,   v_stride, tree, offsets, lengths, c, out,
+               n_seqs, row_capacity, max_new, n_heads,  scale * 1.4426950408889634f};
+    if (num_pages == 0) a.c.max_pages = 0;  // (no page to stand in for a missing one)
+    a.vec = head_dim % 8 == 0 && !odd(q, 16) && q_stride % 8 == 0 &&
+            (!k_new || (!odd(k_new, 16) && k_stride % 8 == 0));
+    a.vec_out = head_dim % 4 == 0 && !odd(out, 8);
+    const Plan p = make_plan(n_seqs, row_capacity, max_new, max_pages, n_heads, n_kv_heads, head_dim,
+                             workspace ? workspace_bytes : 0);
+    LHQ_SUPPORTED(p.units * n_kv_heads * p.splits < INT32_MAX && p.join_units * n_kv_heads < INT32_MAX,
+                  "%s: %lld query blocks of %d heads are over the grid", fn, static_cast<long long>(p.units), n_kv_heads);
+    a.pages_per_split = p.pages_per_split;
+    a.splits = p.splits;
+    a.ws_ml = static_cast<float*>(workspace);
+    a.ws_o = a.ws_ml + p.ml_bytes / 4;
+    const hipStream_t s = as_stream(stream);
+    int st = LHQ_OK;
+    auto go = [&](auto ks) {
+        auto with = [&](auto nq, auto fp8) { st = launch<ks(), nq(), fp8()>(fn, a, p, s); };
+        auto fmt = [&](auto nq) {
+            if (format == LHQ_KV_FP8) with(nq, std::true_type{});
+            else with(nq, std::false_type{});
+        };
+        if (p.tiles == 1) fmt(std::integral_constant<int, 1>{});
+        else fmt(std::integral_constant<int, 2>{});
+    };
+    switch (kv_padded(head_dim) / 32) {
+        case 1: go(std::integral_constant<int, 1>{}); break;
+        case 2: go(std::integral_constant<int, 2>{}); break;
+        case 3: go(std::integral_constant<int, 3>{}); break;
+        case 4: go(std::integral_constant<int, 4>{}); break;
+        case 5: go(std::integral_constant<int, 5>{}); break;
+        case 6: go(std::integral_constant<int, 6>{}); break;
+        case 7: go(std::integral_constant<int, 7>{}); break;
+        default: go(std::integral_constant<int, 8>{}); break;
+    }
+    if (st != LHQ_OK || p.splits == 1) return st;
+    kv_attn_join_kernel<<<static_cast<unsigned>(p.join_units * n_kv_heads), 256, 0, s>>>(a);
     return check_launch(fn);
 }
 
