@@ -30,6 +30,7 @@ namespace {
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
 
 // The running maximum follows the scores only when one is over it by more
 // than 2^kLag (rarely, after the first pages): weights go up to 2^kLag and,
@@ -41,7 +42,7 @@ constexpr int kJoinRows = 16;
 // A call is split until it has about this many workgroups (two of four waves
 // fit a CU), a split has this many pages at least, a sequence at most this
 // many splits (one lane each when they are joined).
-constexpr int kTargetGroups = 1024, kLeastPages = 16, kMostSplits = 64;
+constexpr int kMostSplits = 64;
 
 struct AttnArgs {
     const uint16_t* q;
@@ -57,7 +58,7 @@ struct AttnArgs {
     uint16_t* out;
     int n_seqs, capacity, max_new, heads;
     float scale2;          // scale * log2 e: weights are powers of two
-    bool vec, vec_out;     // rows of q and k_new: 16-byte loads; of out: 8-byte stores
+    bool vec_out;          // rows of out: 8-byte stores
     int pages_per_split;   // a sequence of p pages has ceil(p / this) splits
     int splits;            // the most of one sequence
     float* ws_ml;          // [row][query head][split] {maximum, sum}
@@ -108,17 +109,41 @@ __device__ __forceinline__ f32x4_t mfma_f16_16x16x32(u32x4_t a, u32x4_t b, f32x4
                                                   0, 0, 0);
 }
 
-// Eight bf16 of a row from channel ch on, those past D as zero.
-__device__ __forceinline__ u32x4_t load_channels(const uint16_t* row, int ch, int D, bool vec) {
-    u32x4_t w = {0, 0, 0, 0};
-    if (vec) {
-        if (ch < D) w = *reinterpret_cast<const u32x4_t*>(row + ch);
+// Eight bf16 of a row from channel ch on, those past D as zero: one 16-byte
+// load at any alignment, of the row's last 8 channels where fewer are left
+// (and shifted down).  SMALL: D may be under 8.
+template <bool SMALL>
+__device__ __forceinline__ u32x4_t load_channels(const uint16_t* row, int ch, int D) {
+    uint64_t w[2] = {0, 0};
+    if (SMALL && D < 8) {
+        if (ch == 0)
+#pragma unroll 1
+            for (int j = D - 1; j >= 0; --j) {
+                w[1] = (w[1] << 16) | (w[0] >> 48);
+                w[0] = (w[0] << 16) | row[j];
+            }
     } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (ch + j < D) w[j / 2] |= static_cast<uint32_t>(row[ch + j]) << (16 * (j & 1));
+        const int at = min(ch, D - 8), down = 16 * (ch - at), by = down & 63;
+        __builtin_memcpy(w, row + at, 16);
+        if (D % 8) {
+            const uint64_t lo = down >= 64 ? w[1] : w[0], hi = down >= 64 ? 0 : w[1];
+            w[0] = (lo >> by) | ((hi << 1) << (63 - by));
+            w[1] = hi >> by;
+        }
+        if (ch >= D) w[0] = w[1] = 0;
     }
-    return w;
+    return {static_cast<uint32_t>(w[0]), static_cast<uint32_t>(w[0] >> 32), static_cast<uint32_t>(w[1]),
+            static_cast<uint32_t>(w[1] >> 32)};
+}
+
+// The arguments once more, from where the launch left them: a kernel that
+// takes the ones of a later stage from here does not hold them through its
+// main loop (they would be spilled there).
+typedef const __attribute__((address_space(4))) AttnArgs* LateArgs;
+__device__ __forceinline__ LateArgs late_args() {
+    auto p = (LateArgs)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
 }
 
 // The first channel of lane group g in k step i: 64 channels are two steps, of
@@ -163,19 +188,24 @@ __global__ __launch_bounds__((64 * most_waves<KS, NQ>()), (two_a_simd<KS, NQ>() 
     extern __shared__ __attribute__((aligned(16))) float attn_lds[];
     u32x4_t* q_lds = reinterpret_cast<u32x4_t*>(attn_lds);
     const int H = a.c.heads, G = a.heads / H, D = a.c.D;
-    const int h = blockIdx.x % H;
-    const KvUnit u = kv_find_unit(blockIdx.x / H, a.n_seqs, [&](int s) {
+    const int h = blockIdx.x;
+    int lane_lo = 0, lane_T = 0, lane_L = 0;
+    const KvUnit u = kv_find_unit(blockIdx.y + blockIdx.z * gridDim.y, a.n_seqs, [&](int s) {
         const KvRows r = kv_rows(a.offsets, s, a.capacity);
-        const int T = min(r.hi - r.lo, a.max_new);
-        return static_cast<int64_t>((T * G + QB - 1) / QB) * split_count(a, cached(a, s));
+        lane_lo = r.lo;
+        lane_T = min(r.hi - r.lo, a.max_new);
+        lane_L = cached(a, s);
+        return static_cast<uint32_t>((lane_T * G + QB - 1) / QB) * split_count(a, lane_L);
     });
     if (u.seq >= a.n_seqs) return;
-    const KvRows rows = kv_rows(a.offsets, u.seq, a.capacity);
-    const int T = min(rows.hi - rows.lo, a.max_new), R = T * G, blocks = (R + QB - 1) / QB;
-    const int L = cached(a, u.seq), pages = (L + kKvPage - 1) / kKvPage, splits = split_count(a, L);
-    const int split = static_cast<int>(u.nth) / blocks, r0 = (static_cast<int>(u.nth) % blocks) * QB;
-    const int p0 = static_cast<int>(static_cast<int64_t>(pages) * split / splits);
-    const int p1 = static_cast<int>(static_cast<int64_t>(pages) * (split + 1) / splits);
+    const int lo = __builtin_amdgcn_readlane(lane_lo, u.lane);  // its first row
+    const int T = __builtin_amdgcn_readlane(lane_T, u.lane), R = T * G, blocks = (R + QB - 1) / QB;
+    const int L = __builtin_amdgcn_readlane(lane_L, u.lane);
+    const int pages = (L + kKvPage - 1) / kKvPage, splits = split_count(a, L);
+    const int split = u.nth / blocks, r0 = (u.nth % blocks) * QB;
+    // (under 2^25 pages and 64 splits)
+    const int p0 = static_cast<uint32_t>(pages * split) / static_cast<uint32_t>(splits);
+    const int p1 = (static_cast<uint32_t>(pages) * (split + 1)) / static_cast<uint32_t>(splits);
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), NW = blockDim.x >> 6;
 
@@ -183,8 +213,7 @@ __global__ __launch_bounds__((64 * most_waves<KS, NQ>()), (two_a_simd<KS, NQ>() 
     auto load_q = [&](int t, int i) -> u32x4_t {
         const int r = r0 + 16 * t + c;
         if (r >= R) return {0, 0, 0, 0};
-        return load_channels(a.q + (rows.lo + r / G) * a.q_stride + (h * G + r % G) * D, step_channel<KS>(i, g), D,
-                             a.vec);
+        return load_channels<KS == 1>(a.q + (lo + r / G) * a.q_stride + (h * G + r % G) * D, step_channel<KS>(i, g), D);
     };
     u32x4_t q_reg[NQ == 1 ? KS : 1];
     if constexpr (NQ == 1) {
@@ -369,39 +398,47 @@ __global__ __launch_bounds__((64 * most_waves<KS, NQ>()), (two_a_simd<KS, NQ>() 
     }
 
     // ---- the new tokens, by the wave whose turn it is after the sequence's last page ----
-    if (a.k_new && split == splits - 1 && wave == (p1 - p0) % NW) {
+    const LateArgs late = late_args();
+    if (late->k_new && split == splits - 1 && wave == (p1 - p0) % NW) {
         uint64_t seen[NQ];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             const int r = r0 + 16 * n + c, t = r / G;
-            seen[n] = r >= R ? 0 : a.tree ? a.tree[rows.lo + t] : ~uint64_t{0} >> (63 - t);
+            seen[n] = r >= R ? 0 : late->tree ? late->tree[lo + t] : ~uint64_t{0} >> (63 - t);
             seen[n] &= ~uint64_t{0} >> (64 - T);
         }
-        float big = 0.0f;
-        bool odd = false;  // values that are not finite: kept out of the product
-        auto value = [&](int t, int ch) {
-            if (t >= T || ch >= D) return 0.0f;
-            const float y = bf16_to_f32(a.v_new[(rows.lo + t) * a.v_stride + h * D + ch]);
-            odd |= !(fabsf(y) < INFINITY);
-            return fabsf(y) < INFINITY ? y : 0.0f;
+        // Value rows of 32 tokens as they come, all loads in flight together: channel 16 i + c of tokens
+        // t and t + 1, t = 32 s + 16 (j / 2) + 4 g + 2 (j % 2), clamped to a row and a channel that are there.
+        const uint16_t* new_values = late->v_new + lo * late->v_stride + h * D;
+        uint32_t raw[CT][4];
+        auto load_raw = [&](int s) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int t = 32 * s + 16 * (j / 2) + 4 * g + 2 * (j % 2);
+                const uint16_t* row = new_values + min(t, T - 1) * late->v_stride;
+                const uint16_t* odd = new_values + min(t + 1, T - 1) * late->v_stride;
+#pragma unroll
+                for (int i = 0; i < CT; ++i) {
+                    const int ch = min(16 * i + c, D - 1);
+                    raw[i][j] = row[ch] | static_cast<uint32_t>(odd[ch]) << 16;
+                }
+            }
         };
+        load_raw(0);
+        const uint16_t* new_keys = late->k_new + lo * late->k_stride + h * D;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
             for (int n = 0; n < NQ; ++n) x[n][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
             if (16 * t >= T) continue;
+            const uint16_t* row = new_keys + min(16 * t + c, T - 1) * late->k_stride;
+            u32x4_t key[KS];
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                u32x4_t key = {0, 0, 0, 0};
-                if (16 * t + c < T)
-                    key = load_channels(a.k_new + (rows.lo + 16 * t + c) * a.k_stride + h * D, step_channel<KS>(i, g),
-                                        D, a.vec);
+            for (int i = 0; i < KS; ++i) key[i] = load_channels<KS == 1>(row, step_channel<KS>(i, g), D);
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) x[n][t] = mfma_bf16_16x16x32(key, query(n, i), x[n][t]);
-            }
-            for (int i = 0; i < CT; ++i)
+            for (int i = 0; i < KS; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) big = fmaxf(big, fabsf(value(16 * t + 4 * g + j, 16 * i + c)));
+                for (int n = 0; n < NQ; ++n) x[n][t] = mfma_bf16_16x16x32(key[i], query(n, i), x[n][t]);
         }
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
@@ -410,41 +447,70 @@ __global__ __launch_bounds__((64 * most_waves<KS, NQ>()), (two_a_simd<KS, NQ>() 
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     x[n][t][j] = (seen[n] >> (16 * t + 4 * g + j)) & 1 ? x[n][t][j] * a.scale2 : -INFINITY;
-        for (int s = 32; s; s >>= 1) big = fmaxf(big, __shfl_xor(big, s, 64));
-        // the values themselves as fp16, their largest under 2^15 (fp16's normal range holds 2^-29 of that)
-        const int want = __builtin_amdgcn_readfirstlane(exponent(big)) - 15;
-        if (big > 0.0f && want > e) raise(want);
         const float one = ldexpf(1.0f, kTop);
         const f32x4_t w[4] = {{one, one, one, one}, {one, one, one, one}, {one, one, one, one}, {one, one, one, one}};
         u32x4_t p[NQ][2];
         weigh(w, p);
+        uint64_t odd = 0;  // lanes that met a value that is not finite
+#pragma unroll 1
+        for (int s = 0; 32 * s < T; ++s) {
+            if (s > 0) load_raw(s);
+            u16x2_t size = {0, 0};
+            auto grow = [&] {
+                size = u16x2_t{0, 0};
 #pragma unroll
-        for (int i = 0; i < CT; ++i)
+                for (int i = 0; i < CT; ++i)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                if (32 * s >= T) continue;
+                    for (int j = 0; j < 4; ++j)
+                        size = __builtin_elementwise_max(size, __builtin_bit_cast(u16x2_t, raw[i][j] & 0x7fff7fffu));
+            };
+            grow();
+            const uint64_t not_finite = __ballot(max(size[0], size[1]) >= 0x7f80);
+            if (not_finite) {  // kept out of the product, in which they would reach queries that do not see them
+                odd |= not_finite;
+                asm volatile("");  // (a branch, not 64 selects that every call makes)
+#pragma unroll
+                for (int i = 0; i < CT; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if ((raw[i][j] & 0x7f80u) == 0x7f80u) raw[i][j] &= 0xffff0000u;
+                        if ((raw[i][j] & 0x7f800000u) == 0x7f800000u) raw[i][j] &= 0xffffu;
+                    }
+                grow();
+            }
+            float big = bf16_to_f32(max(size[0], size[1]));
+            for (int d = 32; d; d >>= 1) big = fmaxf(big, __shfl_xor(big, d, 64));
+            // the values themselves as fp16, their largest under 2^15 (fp16's normal range holds 2^-29 of that)
+            const int want = __builtin_amdgcn_readfirstlane(exponent(big)) - 15;
+            if (big > 0.0f && want > e) raise(want);
+#pragma unroll
+            for (int i = 0; i < CT; ++i) {
                 u32x4_t val;
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const int t = 32 * s + 16 * (b / 2) + 4 * g + 2 * (b & 1);
-                    val[b] = pack_f16x2(ldexpf(value(t, 16 * i + c), -e), ldexpf(value(t + 1, 16 * i + c), -e));
-                }
+                for (int j = 0; j < 4; ++j)
+                    val[j] = pack_f16x2(ldexpf(__uint_as_float(raw[i][j] << 16), -e),
+                                        ldexpf(__uint_as_float(raw[i][j] & 0xffff0000u), -e));
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) o[n][i] = mfma_f16_16x16x32(val, p[n][s], o[n][i]);
+                for (int n = 0; n < NQ; ++n) o[n][i] = mfma_f16_16x16x32(val, p[n][0], o[n][i]);
             }
-        if (__ballot(odd))  // a query that sees such a value takes it as it is, the others do not
-            for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) p[n][0] = p[n][1];
+        }
+        if (odd)  // a query that sees such a value takes it as it is, the others do not
+#pragma unroll 1
+            for (int t = 0; t < T; ++t) {
+                const uint16_t* row = new_values + t * late->v_stride;
 #pragma unroll
                 for (int i = 0; i < CT; ++i)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int ch = 16 * i + 4 * g + j;
-                        const float y = ch < D ? bf16_to_f32(a.v_new[(rows.lo + t) * a.v_stride + h * D + ch]) : 0.0f;
-                        if (!(fabsf(y) < INFINITY))
+                        const float y = bf16_to_f32(row[min(ch, D - 1)]);
 #pragma unroll
-                            for (int n = 0; n < NQ; ++n)
-                                if ((seen[n] >> t) & 1) o[n][i][j] += y;
+                        for (int n = 0; n < NQ; ++n)
+                            o[n][i][j] += !(fabsf(y) < INFINITY) && ((seen[n] >> t) & 1) ? y : 0.0f;
                     }
+            }
     }
 
     // ---- the waves' sums meet in LDS ----
@@ -484,15 +550,15 @@ __global__ __launch_bounds__((64 * most_waves<KS, NQ>()), (two_a_simd<KS, NQ>() 
             weight += ml[w * QB * (kPitch + 2) + QB] * f;
             sum += *reinterpret_cast<const f32x4_t*>(at + w * QB * (kPitch + 2)) * f;
         }
-        const int64_t row = static_cast<int64_t>(rows.lo + r / G) * a.heads + h * G + r % G;
+        const int64_t row = static_cast<int64_t>(lo + r / G) * late->heads + h * G + r % G;
         if (splits == 1) {
-            store_row(a.out + row * D, ch, D, sum, weight, a.vec_out);
+            store_row(late->out + row * D, ch, D, sum, weight, late->vec_out);
         } else {
-            const int64_t part = row * a.splits + split;
-            *reinterpret_cast<f32x4_t*>(a.ws_o + part * Dp + ch) = sum;
+            const int64_t part = row * late->splits + split;
+            *reinterpret_cast<f32x4_t*>(late->ws_o + part * Dp + ch) = sum;
             if (ch == 0) {
-                a.ws_ml[2 * part] = top;
-                a.ws_ml[2 * part + 1] = weight;
+                late->ws_ml[2 * part] = top;
+                late->ws_ml[2 * part + 1] = weight;
             }
         }
     }
@@ -501,33 +567,49 @@ __global__ __launch_bounds__((64 * most_waves<KS, NQ>()), (two_a_simd<KS, NQ>() 
 // Joins the splits of a sequence's rows, in order of position: a workgroup
 // takes 16 (new token, query head) rows of one kv head, a wave one at a time.
 __global__ __launch_bounds__(256) void kv_attn_join_kernel(AttnArgs a) {
-    const int H = a.c.heads, G = a.heads / H, D = a.c.D, Dp = a.c.Dp(), h = blockIdx.x % H;
-    const KvUnit u = kv_find_unit(blockIdx.x / H, a.n_seqs, [&](int s) {
+    const int H = a.c.heads, G = a.heads / H, D = a.c.D, Dp = a.c.Dp(), h = blockIdx.x;
+    int lane_lo = 0, lane_T = 0, lane_L = 0;
+    const KvUnit u = kv_find_unit(blockIdx.y + blockIdx.z * gridDim.y, a.n_seqs, [&](int s) {
         const KvRows r = kv_rows(a.offsets, s, a.capacity);
-        return static_cast<int64_t>((min(r.hi - r.lo, a.max_new) * G + kJoinRows - 1) / kJoinRows);
+        lane_lo = r.lo;
+        lane_T = min(r.hi - r.lo, a.max_new);
+        lane_L = cached(a, s);
+        return static_cast<uint32_t>((lane_T * G + kJoinRows - 1) / kJoinRows);
     });
     if (u.seq >= a.n_seqs) return;
-    const int splits = split_count(a, cached(a, u.seq));
+    const int splits = split_count(a, __builtin_amdgcn_readlane(lane_L, u.lane));
     if (splits == 1) return;  // (its rows are there already)
-    const KvRows rows = kv_rows(a.offsets, u.seq, a.capacity);
-    const int R = min(rows.hi - rows.lo, a.max_new) * G, lane = threadIdx.x & 63;
+    const int lo = __builtin_amdgcn_readlane(lane_lo, u.lane), R = __builtin_amdgcn_readlane(lane_T, u.lane) * G;
+    const int lane = threadIdx.x & 63;
     // lanes that share the splits of 4 channels
     const int share = Dp <= 64 ? 4 : Dp <= 128 ? 2 : 1, ch = 4 * (lane & (64 / share - 1)), first = lane / (64 / share);
     for (int i = threadIdx.x >> 6; i < kJoinRows; i += 4) {
-        const int r = static_cast<int>(u.nth) * kJoinRows + i;
+        const int r = u.nth * kJoinRows + i;
         if (r >= R) return;
-        const int64_t row = static_cast<int64_t>(rows.lo + r / G) * a.heads + h * G + r % G, part = row * a.splits;
+        const int64_t row = static_cast<int64_t>(lo + r / G) * a.heads + h * G + r % G, part = row * a.splits;
+        const float* from = a.ws_o + part * Dp + min(ch, Dp - 4);
         const float m = lane < splits ? a.ws_ml[2 * (part + lane)] : -INFINITY;
-        float top = m;
-        for (int s = 32; s; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
-        const float f = exp2_(m - (top == -INFINITY ? 0.0f : top));
-        float weight = lane < splits ? a.ws_ml[2 * (part + lane) + 1] * f : 0.0f;
-        for (int s = 32; s; s >>= 1) weight += __shfl_xor(weight, s, 64);
+        const float l = lane < splits ? a.ws_ml[2 * (part + lane) + 1] : 0.0f;
+        float f = 0.0f, weight = 0.0f;
         f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < splits; s += share) {
-            const float fs = __shfl(f, s + first, 64);
-            if (s + first < splits && ch < Dp)
-                sum += *reinterpret_cast<const f32x4_t*>(a.ws_o + (part + s + first) * Dp + ch) * fs;
+        for (int s0 = 0; s0 < splits; s0 += 8 * share) {
+            f32x4_t y[8];  // eight splits a lane in flight; past the last one, that again, unused
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                y[k] = *reinterpret_cast<const f32x4_t*>(from + min(s0 + k * share + first, splits - 1) * Dp);
+            if (s0 == 0) {
+                float top = m;
+                for (int s = 32; s; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+                f = exp2_(m - (top == -INFINITY ? 0.0f : top));
+                weight = l * f;
+                for (int s = 32; s; s >>= 1) weight += __shfl_xor(weight, s, 64);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int s = s0 + k * share + first;
+                const float fs = __shfl(f, s & 63, 64);
+                if (s < splits) sum += y[k] * fs;
+            }
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -554,6 +636,7 @@ Plan make_plan(int n_seqs, int capacity, int max_new, int max_pages, int heads, 
     const int G = heads / kv_heads, KS = kv_padded(D) / 32;
     Plan p{};
     p.tiles = max_new * G <= 16 ? 1 : 2;
+    const int kTargetGroups = tuning_knob("LHQ_KV_TARGET", p.tiles > 1 ? 512 : 1024), kLeastPages = tuning_knob("LHQ_KV_LEAST", 16);
     p.units = unit_bound(n_seqs, capacity, max_new, G, 16 * p.tiles);
     p.join_units = unit_bound(n_seqs, capacity, max_new, G, kJoinRows);
     const int64_t groups = std::max<int64_t>(1, p.units * kv_heads), rows = static_cast<int64_t>(capacity) * heads;
@@ -569,14 +652,19 @@ Plan make_plan(int n_seqs, int capacity, int max_new, int max_pages, int heads, 
     return p;
 }
 
+// kv heads, units: blockIdx.y + blockIdx.z * gridDim.y
+dim3 unit_grid(int heads, int64_t units) {
+    const unsigned y = static_cast<unsigned>(std::min<int64_t>(units, 32768));
+    return dim3(heads, y, static_cast<unsigned>((units + y - 1) / y));
+}
+
 template <int KS, int NQ, bool FP8>
 int launch(const char* fn, const AttnArgs& a, const Plan& p, hipStream_t s) {
     constexpr auto kern = &kv_attn_kernel<KS, NQ, FP8>;
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (attr != hipSuccess) return set_error(LHQ_ERR_HIP, "%s: dynamic LDS attribute: %s", fn, hipGetErrorString(attr));
-    const unsigned grid = static_cast<unsigned>(p.units * a.c.heads * p.splits);
-    kern<<<grid, 64 * p.waves, lds_bytes<KS, NQ>(p.waves), s>>>(a);
+    kern<<<unit_grid(a.c.heads, p.units * p.splits), 64 * p.waves, lds_bytes<KS, NQ>(p.waves), s>>>(a);
     return check_launch(fn);
 }
 
@@ -628,12 +716,10 @@ int lhq_kv_attn_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k_new,
     AttnArgs a{q,        q_stride, k_new,  k_stride,     v_new,   v_stride, tree, offsets, lengths, c, out,
                n_seqs, row_capacity, max_new, n_heads,  scale * 1.4426950408889634f};
     if (num_pages == 0) a.c.max_pages = 0;  // (no page to stand in for a missing one)
-    a.vec = head_dim % 8 == 0 && !odd(q, 16) && q_stride % 8 == 0 &&
-            (!k_new || (!odd(k_new, 16) && k_stride % 8 == 0));
     a.vec_out = head_dim % 4 == 0 && !odd(out, 8);
     const Plan p = make_plan(n_seqs, row_capacity, max_new, max_pages, n_heads, n_kv_heads, head_dim,
                              workspace ? workspace_bytes : 0);
-    LHQ_SUPPORTED(p.units * n_kv_heads * p.splits < INT32_MAX && p.join_units * n_kv_heads < INT32_MAX,
+    LHQ_SUPPORTED(p.units * p.splits < INT32_MAX && p.units * p.splits * n_kv_heads * p.waves < INT32_MAX / 64,
                   "%s: %lld query blocks of %d heads are over the grid", fn, static_cast<long long>(p.units), n_kv_heads);
     a.pages_per_split = p.pages_per_split;
     a.splits = p.splits;
@@ -661,7 +747,7 @@ int lhq_kv_attn_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k_new,
         default: go(std::integral_constant<int, 8>{}); break;
     }
     if (st != LHQ_OK || p.splits == 1) return st;
-    kv_attn_join_kernel<<<static_cast<unsigned>(p.join_units * n_kv_heads), 256, 0, s>>>(a);
+    kv_attn_join_kernel<<<unit_grid(n_kv_heads, p.join_units), 256, 0, s>>>(a);
     return check_launch(fn);
 }
 

@@ -101,23 +101,26 @@ __device__ __forceinline__ float code_value(uint32_t w, int j) {
 }
 
 // Pages that n tokens from position `start` on touch.
-__device__ __forceinline__ int64_t tile_count(int64_t start, int64_t n) {
-    return n > 0 ? ((start + n - 1) >> 6) - (start >> 6) + 1 : 0;
+__device__ __forceinline__ uint32_t tile_count(int64_t start, int64_t n) {
+    return n > 0 ? static_cast<uint32_t>(((start + n - 1) >> 6) - (start >> 6) + 1) : 0u;
 }
 
 // The tile of a workgroup: tokens [t0, t1) of page `p` of sequence seq; token
 // t is row row0 + t of the list of new rows.
 struct Tile { int seq, t0, t1; int64_t p, row0; };
 __device__ __forceinline__ Tile find_tile(const int32_t* offsets, const int32_t* start, int n_seqs, int capacity) {
+    KvRows mine{0, 0};
+    int mine_start = 0;
     const KvUnit u = kv_find_unit(blockIdx.x, n_seqs, [&](int s) {
-        const KvRows r = kv_rows(offsets, s, capacity);
-        return tile_count(start[s], r.hi - r.lo);
+        mine = kv_rows(offsets, s, capacity);
+        mine_start = start[s];
+        return tile_count(mine_start, mine.hi - mine.lo);
     });
     if (u.seq >= n_seqs) return {n_seqs, 0, 0, 0, 0};
-    const KvRows r = kv_rows(offsets, u.seq, capacity);
-    const int64_t s0 = start[u.seq], p = (s0 >> 6) + u.nth;
-    const int64_t a = s0 - (p << 6), b = a + (r.hi - r.lo);
-    return {u.seq, static_cast<int>(max<int64_t>(a, 0)), static_cast<int>(min<int64_t>(b, kKvPage)), p, r.lo - a};
+    const int lo = __builtin_amdgcn_readlane(mine.lo, u.lane), hi = __builtin_amdgcn_readlane(mine.hi, u.lane);
+    const int64_t s0 = __builtin_amdgcn_readlane(mine_start, u.lane), p = (s0 >> 6) + u.nth;
+    const int64_t a = s0 - (p << 6), b = a + (hi - lo);
+    return {u.seq, static_cast<int>(max<int64_t>(a, 0)), static_cast<int>(min<int64_t>(b, kKvPage)), p, lo - a};
 }
 
 // Write: one workgroup per (tile, head).  1 << LB lanes (eight channels each)

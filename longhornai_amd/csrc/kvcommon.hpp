@@ -57,31 +57,43 @@ __device__ __forceinline__ KvRows kv_rows(const int32_t* offsets, int s, int cap
     return {lo, min(max(offsets[s + 1], lo), capacity)};
 }
 
+// Sums over the lanes up to each one, of numbers under 2^32, held at 2^32 - 1.
+__device__ __forceinline__ uint32_t kv_scan(uint32_t x) {
+#define LHQ_SCAN_STEP(ctrl, rows)                                                                           \
+    x = __builtin_elementwise_add_sat(                                                                      \
+        x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), ctrl, rows, 0xf, false)))
+    LHQ_SCAN_STEP(0x111, 0xf);  // row_shr:1, 2, 4, 8: within 16 lanes
+    LHQ_SCAN_STEP(0x112, 0xf);
+    LHQ_SCAN_STEP(0x114, 0xf);
+    LHQ_SCAN_STEP(0x118, 0xf);
+    LHQ_SCAN_STEP(0x142, 0xa);  // row_bcast:15 to rows 1 and 3
+    LHQ_SCAN_STEP(0x143, 0xc);  // row_bcast:31 to the upper half
+#undef LHQ_SCAN_STEP
+    return x;
+}
+
 // The unit with number `unit` in the list that has count(s) units of sequence
-// 0, then those of sequence 1, ...: its sequence and its number within it, the
-// same in every lane; seq = n_seqs past the end of the list.  Each wave scans
-// the sequences by itself, 64 at a time (no barrier; a batch of 64 is one step).
-struct KvUnit { int seq; int64_t nth; };
+// 0, then those of sequence 1, ...: its sequence, its number within it and the
+// lane that counted the sequence (what count left in that lane's variables is
+// the sequence's), the same in every lane; seq = n_seqs past the end of the
+// list.  Each wave scans the sequences by itself, 64 at a time (no barrier; a
+// batch of 64 is one step).  A sum held at 2^32 - 1 is over every unit.
+struct KvUnit { int seq, nth, lane; };
 template <typename Count>
-__device__ __forceinline__ KvUnit kv_find_unit(int64_t unit, int n_seqs, Count count) {
+__device__ __forceinline__ KvUnit kv_find_unit(uint32_t unit, int n_seqs, Count count) {
     const int lane = threadIdx.x & 63;
     for (int base = 0; base < n_seqs; base += 64) {
         const int s = base + lane;
-        const int64_t mine = s < n_seqs ? count(s) : 0;
-        int64_t sum = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t v = __shfl_up(sum, d, 64);
-            if (lane >= d) sum += v;
-        }
+        const uint32_t sum = kv_scan(s < n_seqs ? count(s) : 0u);
         const uint64_t over = __ballot(sum > unit);
         if (over) {
             const int l = __builtin_ctzll(over);
-            return {base + l, unit - __shfl(sum - mine, l, 64)};
+            const uint32_t before = l > 0 ? __builtin_amdgcn_readlane(sum, l - 1) : 0u;
+            return {base + l, static_cast<int>(unit - before), l};
         }
-        unit -= __shfl(sum, 63, 64);
+        unit -= __builtin_amdgcn_readlane(sum, 63);
     }
-    return {n_seqs, 0};
+    return {n_seqs, 0, 0};
 }
 
 // Checks that all entry points of the cache share; `fn` names the caller.

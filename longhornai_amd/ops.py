@@ -256,7 +256,7 @@ KV_PAGE = 64
 _KV_FORMATS = {"int8": 0, "fp8": 1}  # LHQ_KV_INT8, LHQ_KV_FP8
 
 
-@dataclass
+@dataclass(frozen=True)
 class KvCache:
     """The buffers of a paged 8-bit cache (layout in include/longhorn_hip.h):
     codes uint8 (keys [pages, heads, 64, Dp], values [pages, heads, Dp, 64]),
@@ -298,34 +298,43 @@ def kv_cache(fmt: str, n_pages: int, n_kv_heads: int, head_dim: int) -> KvCache:
                    zeros((scales // 4,), np.float32), zeros((scales // 4,), np.float32))
 
 
-def _kv_rows(fn: str, name: str, t: torch.Tensor, heads: int, D: int, dtypes) -> int:
+# These checks run before every call, ahead of kernels of a few microseconds:
+# each attribute of a tensor is read once, the usual case decided first.
+
+def _kv_rows(fn: str, name: str, t: torch.Tensor, heads: int, D: int, dtypes) -> tuple[int, int]:
     """Checks new tokens' rows [n, heads * D] or [n, heads, D], heads packed;
-    returns the stride between rows."""
+    returns (rows, the stride between them)."""
+    shape, st = t.shape, t.stride()
     if t.dtype not in dtypes:
         raise ValueError(f"{fn}: {name} is {t.dtype}, not one of {[str(d) for d in dtypes]}")
-    shape, st = t.shape, t.stride()
-    if tuple(shape[1:]) == (heads * D,):
-        packed = st[1] == 1 or heads * D == 1
-    elif tuple(shape[1:]) == (heads, D):
+    width = heads * D
+    if len(shape) == 2 and shape[1] == width:
+        packed = st[1] == 1 or width == 1
+    elif len(shape) == 3 and shape[1] == heads and shape[2] == D:
         packed = (st[2] == 1 or D == 1) and (st[1] == D or heads == 1)
     else:
         raise ValueError(f"{fn}: {name} has shape {tuple(shape)}, not [n, {heads} * {D}]")
     if not packed:
         raise ValueError(f"{fn}: the heads of a row of {name} must lie one after the other (strides {tuple(st)})")
-    return st[0] if shape[0] > 1 else max(st[0], heads * D)
+    n = shape[0]
+    return n, st[0] if n > 1 else max(st[0], width)
 
 
 def _kv_tables(fn: str, offsets: torch.Tensor, start: torch.Tensor, table: torch.Tensor):
     """Checks the int32 device tables; returns (sequences, pages of a table row)."""
-    if offsets.dtype != torch.int32 or start.dtype != torch.int32 or table.dtype != torch.int32:
+    i32 = torch.int32
+    if offsets.dtype is not i32 or start.dtype is not i32 or table.dtype is not i32:
         raise ValueError(f"{fn}: offsets, positions and block table must be int32")
-    B = start.shape[0]
-    if offsets.shape[0] != B + 1 or table.dim() != 2 or table.shape[0] != B:
+    B, shape = start.shape[0], table.shape
+    if offsets.shape[0] != B + 1 or len(shape) != 2 or shape[0] != B:
         raise ValueError(f"{fn}: {B} positions with {offsets.shape[0]} offsets and a block table of "
-                         f"{tuple(table.shape)}")
+                         f"{tuple(shape)}")
     if not (offsets.is_contiguous() and start.is_contiguous() and table.is_contiguous()):
         raise ValueError(f"{fn}: offsets, positions and block table must be contiguous")
-    return B, table.shape[1]
+    return B, shape[1]
+
+
+_KV_BITS, _KV_ROWS = (torch.int16,), (torch.int16, torch.float32)
 
 
 def kv_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, start: torch.Tensor,
@@ -336,17 +345,18 @@ def kv_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, offsets: torch.Te
     (int32): the row of k and v for each row of that list (one outside them is
     skipped)."""
     H, D = cache.n_kv_heads, cache.head_dim
-    ks = _kv_rows("kv_write", "k", k, H, D, (torch.int16, torch.float32))
-    vs = _kv_rows("kv_write", "v", v, H, D, (k.dtype,))
+    dt = k.dtype
+    n_rows, ks = _kv_rows("kv_write", "k", k, H, D, _KV_ROWS)
+    n_values, vs = _kv_rows("kv_write", "v", v, H, D, (dt,))
     B, width = _kv_tables("kv_write", offsets, start, block_table)
-    if v.shape[0] != k.shape[0]:
-        raise ValueError(f"kv_write: {k.shape[0]} rows of keys and {v.shape[0]} of values")
+    if n_values != n_rows:
+        raise ValueError(f"kv_write: {n_rows} rows of keys and {n_values} of values")
     if rows is not None and (rows.dtype != torch.int32 or not rows.is_contiguous()):
         raise ValueError("kv_write: rows must be contiguous int32")
-    n = k.shape[0] if rows is None else rows.numel()
-    lib().call("lhq_kv_write_f32" if k.dtype == torch.float32 else "lhq_kv_write_bf16", P(k), P(v), ks, vs, P(rows),
-               P(offsets), P(start), P(block_table), *cache.pointers(), _KV_FORMATS[cache.fmt], B, k.shape[0], n,
-               width, cache.n_pages, H, D, stream())
+    n = n_rows if rows is None else rows.numel()
+    lib().call("lhq_kv_write_f32" if dt == torch.float32 else "lhq_kv_write_bf16", k.data_ptr(), v.data_ptr(), ks, vs,
+               P(rows), offsets.data_ptr(), start.data_ptr(), block_table.data_ptr(), *cache.pointers(),
+               _KV_FORMATS[cache.fmt], B, n_rows, n, width, cache.n_pages, H, D, stream())
 
 
 def kv_read(cache: KvCache, offsets: torch.Tensor, start: torch.Tensor, block_table: torch.Tensor, n: int,
@@ -358,14 +368,15 @@ def kv_read(cache: KvCache, offsets: torch.Tensor, start: torch.Tensor, block_ta
     B, width = _kv_tables("kv_read", offsets, start, block_table)
     dt = torch.int16 if bf16 else torch.float32
     if out is None:
-        both = torch.empty((2, n, H, D), dtype=dt, device=cache.k.device)
-        out = both[0], both[1]
-    for t in out:
-        if t.dtype != dt or tuple(t.shape) != (n, H, D) or not t.is_contiguous():
-            raise ValueError(f"kv_read: outputs must be contiguous [{n}, {H}, {D}] {dt}")
-    lib().call("lhq_kv_read_bf16" if bf16 else "lhq_kv_read_f32", *cache.pointers(), P(offsets), P(start),
-               P(block_table), P(out[0]), P(out[1]), _KV_FORMATS[cache.fmt], B, n, width, cache.n_pages, H, D,
-               stream())
+        k = cache.k.new_empty((n, H, D), dtype=dt)
+        out = k, torch.empty_like(k)
+    else:
+        for t in out:
+            if t.dtype != dt or tuple(t.shape) != (n, H, D) or not t.is_contiguous():
+                raise ValueError(f"kv_read: outputs must be contiguous [{n}, {H}, {D}] {dt}")
+    lib().call("lhq_kv_read_bf16" if bf16 else "lhq_kv_read_f32", *cache.pointers(), offsets.data_ptr(),
+               start.data_ptr(), block_table.data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
+               _KV_FORMATS[cache.fmt], B, n, width, cache.n_pages, H, D, stream())
     return out
 
 
@@ -387,27 +398,28 @@ def kv_attn(cache: KvCache, q: torch.Tensor, offsets: torch.Tensor, lengths: tor
     up to the token itself.  Returns out [n, heads, head_dim], int16 bits."""
     H, D = cache.n_kv_heads, cache.head_dim
     B, width = _kv_tables("kv_attn", offsets, lengths, block_table)
-    n, heads = q.shape[0], (q.shape[1] // D if q.dim() == 2 else q.shape[1])
-    bits = (torch.int16,)
-    qs = _kv_rows("kv_attn", "q", q, heads, D, bits)
+    shape = q.shape
+    heads = shape[1] // D if len(shape) == 2 else shape[1]
+    n, qs = _kv_rows("kv_attn", "q", q, heads, D, _KV_BITS)
     if heads % H != 0:
         raise ValueError(f"kv_attn: {heads} query heads over {H} kv heads")
     if (k_new is None) != (v_new is None):
         raise ValueError("kv_attn: new keys without values, or values without keys")
     ks = vs = 0
     if k_new is not None:
-        ks = _kv_rows("kv_attn", "k_new", k_new, H, D, bits)
-        vs = _kv_rows("kv_attn", "v_new", v_new, H, D, bits)
-        if k_new.shape[0] != n or v_new.shape[0] != n:
-            raise ValueError(f"kv_attn: {n} queries with {k_new.shape[0]} new keys and {v_new.shape[0]} values")
+        n_keys, ks = _kv_rows("kv_attn", "k_new", k_new, H, D, _KV_BITS)
+        n_values, vs = _kv_rows("kv_attn", "v_new", v_new, H, D, _KV_BITS)
+        if n_keys != n or n_values != n:
+            raise ValueError(f"kv_attn: {n} queries with {n_keys} new keys and {n_values} values")
     if tree is not None and (tree.dtype != torch.int64 or tree.numel() != n or not tree.is_contiguous()):
         raise ValueError(f"kv_attn: tree must hold {n} contiguous int64 words")
     if out is None:
-        out = torch.empty((n, heads, D), dtype=torch.int16, device=q.device)
+        out = q.new_empty((n, heads, D))
     elif out.dtype != torch.int16 or out.numel() != n * heads * D or not out.is_contiguous():
         raise ValueError(f"kv_attn: out must be contiguous [{n}, {heads}, {D}] int16")
     nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    lib().call("lhq_kv_attn_bf16", P(q), qs, P(k_new), ks, P(v_new), vs, P(tree), P(offsets), P(lengths),
-               P(block_table), *cache.pointers(), P(out), _KV_FORMATS[cache.fmt], B, n, max_new, width, cache.n_pages,
-               heads, H, D, D ** -0.5 if scale is None else scale, P(workspace), nbytes, stream())
+    lib().call("lhq_kv_attn_bf16", q.data_ptr(), qs, P(k_new), ks, P(v_new), vs, P(tree), offsets.data_ptr(),
+               lengths.data_ptr(), block_table.data_ptr(), *cache.pointers(), out.data_ptr(), _KV_FORMATS[cache.fmt],
+               B, n, max_new, width, cache.n_pages, heads, H, D, D ** -0.5 if scale is None else scale, P(workspace),
+               nbytes, stream())
     return out
