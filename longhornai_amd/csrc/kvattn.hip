@@ -28,6 +28,7 @@
 namespace lhq {
 namespace {
 
+#define LHQ_LDS_AS __attribute__((address_space(3)))
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
 typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
@@ -38,7 +39,7 @@ typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
 constexpr float kLag = 4.0f;
 constexpr int kTop = 11;
 
-constexpr int kJoinRows = 16;
+constexpr int kJoinRows = 4;
 // A call is split until it has about this many workgroups (two of four waves
 // fit a CU), a split has this many pages at least, a sequence at most this
 // many splits (one lane each when they are joined).
@@ -154,19 +155,73 @@ __device__ __forceinline__ int step_channel(int i, int g) {
     return i < KS / 2 * 2 ? 64 * (i / 2) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g;
 }
 
+// A page's keys in LDS: rows of Dp bytes, the 16-byte chunk j of row r in place
+// j ^ key_swizzle(r).  The lanes of an operand read have 16 rows and one chunk
+// for each lane group; with this the 16 lanes that LDS serves at a time (lane
+// bit 5 and the parity of bits 2..4 are the same in them) meet 16 different
+// 16-byte bank groups.  Rows of an odd number of 32 bytes do so as they are.
+// Keys come in by LDS DMA because a wave reads 64 adjacent chunks that way: in
+// operand order, 16 rows apart, the same loads reach 9.7 TB/s of the L2's 33.
+template <int KS>
+__device__ __forceinline__ int key_swizzle(int r) {
+    if constexpr (KS == 2) return (r >> 1) & 2;
+    else if constexpr (KS == 4) return (r >> 1) & 7;
+    else if constexpr (KS == 6) return (r >> 2) & 2;
+    else if constexpr (KS == 8) return ((r & 1) << 2) | ((r & 2) << 2) | ((r >> 2) & 2);
+    else return 0;
+}
+// LDS DMA: 16 bytes a lane, from this lane's address to `to` + 16 * lane.
+__device__ __forceinline__ void dma16(const void* from, void* to) {
+    __builtin_amdgcn_global_load_lds(from, (LHQ_LDS_AS void*)to, 16, 0, 0);
+}
+// The n-th of a page's 2 KS key DMAs (1 KiB): to + 16 * lane gets this lane's chunk.
+template <int KS>
+__device__ __forceinline__ void fetch_keys(const uint8_t* page, uint8_t* to, int n) {
+    const int at = 64 * n + (threadIdx.x & 63);
+    dma16(page + 16 * (at ^ key_swizzle<KS>(at / (2 * KS))), to + 1024 * n);
+}
+// S^T of a page whose keys lie in LDS at `keys`.
+template <int KS, int NQ, bool FP8>
+__device__ __forceinline__ void score(const uint8_t* keys, const u32x4_t (&q)[NQ][KS], f32x4_t (&x)[NQ][4]) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    // (a step of channels at a time over all tiles: no product waits for the one before it)
+#pragma unroll
+    for (int i = 0; i < KS; i += 2) {
+        u32x4_t w[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const uint8_t* row = keys + (16 * t + c) * 32 * KS;
+            if (i + 1 < KS) {
+                w[t] = *reinterpret_cast<const u32x4_t*>(row + 16 * ((2 * i + g) ^ key_swizzle<KS>(c)));
+            } else {
+                const u32x2_t y = *reinterpret_cast<const u32x2_t*>(row + 32 * i + 8 * g);
+                w[t][0] = y[0], w[t][1] = y[1];
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < 2 && i + b < KS; ++b)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const u32x2_t lo = codes_bf16<FP8>(w[t][2 * b]), hi = codes_bf16<FP8>(w[t][2 * b + 1]);
+                const u32x4_t key = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+                    x[n][t] = mfma_bf16_16x16x32(key, q[n][i + b], i + b == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : x[n][t]);
+            }
+    }
+}
+
 // The waves of a workgroup at most; two a SIMD where 256 registers hold a
 // wave's page, queries and sums, else one.
-template <int KS, int NQ>
-constexpr bool two_a_simd() { return KS <= 4 && NQ <= 2; }
-template <int KS, int NQ>
-constexpr int most_waves() { return two_a_simd<KS, NQ>() ? 8 : 4; }
+template <int KS>
+constexpr int most_waves() { return KS <= 4 ? 8 : 4; }
 
-// LDS of a workgroup: each wave's sums [QB][Dp + 4], maxima and sums of
-// weights [2][QB]; before that (NQ > 1) the queries as MFMA operands.
+// LDS of a wave: its page, then its sums [QB][Dp + 4] and its maxima and sums of
+// weights [2][QB].
 template <int KS, int NQ>
-constexpr size_t lds_bytes(int waves) {
-    return static_cast<size_t>(waves) * (16 * NQ) * (32 * KS + 4 + 2) * 4;
-}
+constexpr int sums_floats() { return 16 * NQ * (32 * KS + 4 + 2); }
+template <int KS>
+constexpr int page_bytes() { return 4 * KS * 1024; }
 
 // Four channels of a result row from channel ch on.
 __device__ __forceinline__ void store_row(uint16_t* row, int ch, int D, const f32x4_t& sum, float weight, bool vec) {
@@ -182,241 +237,192 @@ __device__ __forceinline__ void store_row(uint16_t* row, int ch, int D, const f3
     }
 }
 
-template <int KS, int NQ, bool FP8>
-__global__ __launch_bounds__((64 * most_waves<KS, NQ>()), (two_a_simd<KS, NQ>() ? 2 : 1)) void kv_attn_kernel(AttnArgs a) {
-    constexpr int Dp = 32 * KS, QB = 16 * NQ, CT = 2 * KS, kPitch = Dp + 4;
-    extern __shared__ __attribute__((aligned(16))) float attn_lds[];
-    u32x4_t* q_lds = reinterpret_cast<u32x4_t*>(attn_lds);
-    const int H = a.c.heads, G = a.heads / H, D = a.c.D;
-    const int h = blockIdx.x;
+// A workgroup's share: rows [r0, ...) of the (new token, query head of the kv
+// head) list of a sequence, and its pages [p0, p1).
+struct Unit {
+    int seq, h, G, lo, T, R, r0, L, pages, split, splits, p0, p1;
+};
+// BLOCK rows a workgroup; false past the end of the list.
+__device__ __forceinline__ bool find_share(const AttnArgs& a, int block, Unit& u) {
+    u.h = blockIdx.x;
+    u.G = a.heads / a.c.heads;
     int lane_lo = 0, lane_T = 0, lane_L = 0;
-    const KvUnit u = kv_find_unit(blockIdx.y + blockIdx.z * gridDim.y, a.n_seqs, [&](int s) {
+    const KvUnit f = kv_find_unit(blockIdx.y + blockIdx.z * gridDim.y, a.n_seqs, [&](int s) {
         const KvRows r = kv_rows(a.offsets, s, a.capacity);
         lane_lo = r.lo;
         lane_T = min(r.hi - r.lo, a.max_new);
         lane_L = cached(a, s);
-        return static_cast<uint32_t>((lane_T * G + QB - 1) / QB) * split_count(a, lane_L);
+        return static_cast<uint32_t>((lane_T * u.G + block - 1) / block) * split_count(a, lane_L);
     });
-    if (u.seq >= a.n_seqs) return;
-    const int lo = __builtin_amdgcn_readlane(lane_lo, u.lane);  // its first row
-    const int T = __builtin_amdgcn_readlane(lane_T, u.lane), R = T * G, blocks = (R + QB - 1) / QB;
-    const int L = __builtin_amdgcn_readlane(lane_L, u.lane);
-    const int pages = (L + kKvPage - 1) / kKvPage, splits = split_count(a, L);
-    const int split = u.nth / blocks, r0 = (u.nth % blocks) * QB;
+    if (f.seq >= a.n_seqs) return false;
+    u.seq = f.seq;
+    u.lo = __builtin_amdgcn_readlane(lane_lo, f.lane);
+    u.T = __builtin_amdgcn_readlane(lane_T, f.lane);
+    u.R = u.T * u.G;
+    u.L = __builtin_amdgcn_readlane(lane_L, f.lane);
+    u.pages = (u.L + kKvPage - 1) / kKvPage;
+    u.splits = split_count(a, u.L);
+    const int blocks = (u.R + block - 1) / block;
+    u.split = f.nth / blocks;
+    u.r0 = (f.nth % blocks) * block;
     // (under 2^25 pages and 64 splits)
-    const int p0 = static_cast<uint32_t>(pages * split) / static_cast<uint32_t>(splits);
-    const int p1 = (static_cast<uint32_t>(pages) * (split + 1)) / static_cast<uint32_t>(splits);
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), NW = blockDim.x >> 6;
-
-    // Queries as B operands: column c of tile t is row r0 + 16 t + c of the (token, head of the group) list.
-    auto load_q = [&](int t, int i) -> u32x4_t {
-        const int r = r0 + 16 * t + c;
-        if (r >= R) return {0, 0, 0, 0};
-        return load_channels<KS == 1>(a.q + (lo + r / G) * a.q_stride + (h * G + r % G) * D, step_channel<KS>(i, g), D);
-    };
-    u32x4_t q_reg[NQ == 1 ? KS : 1];
-    if constexpr (NQ == 1) {
+    u.p0 = static_cast<uint32_t>(u.pages * u.split) / static_cast<uint32_t>(u.splits);
+    u.p1 = (static_cast<uint32_t>(u.pages) * (u.split + 1)) / static_cast<uint32_t>(u.splits);
+    return true;
+}
+// The operands of the 16 queries from row r on, column lane & 15 (past the
+// last row: that one again, whose results no one reads).
+template <int KS>
+__device__ __forceinline__ void load_queries(const AttnArgs& a, const Unit& u, int r, u32x4_t (&q)[KS]) {
+    const int lane = threadIdx.x & 63, row = min(r + (lane & 15), u.R - 1), t = row / u.G;
+    const uint16_t* from = a.q + (u.lo + t) * a.q_stride + (u.h * u.G + row - t * u.G) * a.c.D;
 #pragma unroll
-        for (int i = 0; i < KS; ++i) q_reg[i] = load_q(0, i);
-    } else {
-        for (int n = wave; n < NQ * KS; n += NW) q_lds[n * 64 + lane] = load_q(n / KS, n % KS);
-        __syncthreads();
-    }
-    auto query = [&](int t, int i) -> u32x4_t {
-        if constexpr (NQ == 1) return q_reg[i];
-        else return q_lds[(t * KS + i) * 64 + lane];
-    };
+    for (int i = 0; i < KS; ++i) q[i] = load_channels<KS == 1>(from, step_channel<KS>(i, lane >> 4), a.c.D);
+}
 
+// What a wave holds: sums o (channels 16 i + 4 g + j of query 16 n + c at
+// o[n][i][j], c = lane & 15, g = lane >> 4), scores or weights x of 64 tokens
+// (token 16 t + 4 g + j at x[n][t][j]), the running maximum m and this lane's
+// part l of the sum of weights.
+template <int KS, int NQ>
+struct Sums {
+    static constexpr int CT = 2 * KS, QB = 16 * NQ, kPitch = 32 * KS + 4;
     f32x4_t o[NQ][CT], x[NQ][4];
     float m[NQ], l[NQ];
-    int e = -200;  // (under every exponent: the first value scale that is not zero sets it)
+    int e;       // o is relative to 2^(e - kTop)
+    bool fresh;  // no scores so far
+
+    __device__ __forceinline__ void clear() {
+        fresh = true;
+        e = -200;  // (under every exponent: the first value scale that is not zero sets it)
 #pragma unroll
-    for (int t = 0; t < NQ; ++t) {
-        m[t] = -INFINITY;
-        l[t] = 0.0f;
+        for (int n = 0; n < NQ; ++n) {
+            m[n] = l[n] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < CT; ++i) o[t][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < CT; ++i) o[n][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
     }
-    // Sums from here on are relative to 2^to (to > e).
-    auto raise = [&](int to) {
+    __device__ __forceinline__ void raise(int to) {  // to > e
 #pragma unroll
-        for (int t = 0; t < NQ; ++t)
+        for (int n = 0; n < NQ; ++n)
 #pragma unroll
             for (int i = 0; i < CT; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[t][i][j] = ldexpf(o[t][i][j], max(e - to, -400));
+                for (int j = 0; j < 4; ++j) o[n][i][j] = ldexpf(o[n][i][j], max(e - to, -400));
         e = to;
-    };
-    // The exponent that a maximum over lanes asks for; infinite and NaN ones ask for the largest.
-    auto exponent = [](float v) { return v < INFINITY ? __builtin_amdgcn_frexp_expf(v) : 128; };
-    auto across = [](float v) {  // maximum over the four lane groups
+    }
+    // The exponent that a maximum asks for; infinite and NaN ones ask for the largest.
+    static __device__ __forceinline__ int exponent(float v) {
+        return v < INFINITY ? __builtin_amdgcn_frexp_expf(v) : 128;
+    }
+    static __device__ __forceinline__ float across(float v) {  // maximum over the four lane groups
         v = fmaxf(v, __shfl_xor(v, 16, 64));
         return fmaxf(v, __shfl_xor(v, 32, 64));
-    };
-    // x (scores of 64 tokens) -> weights; times w they are the operands p of the second product.
-    auto weigh = [&](const f32x4_t (&w)[4], u32x4_t (&p)[NQ][2]) {
-#pragma unroll
-        for (int t = 0; t < NQ; ++t) {
-            float top = x[t][0][0];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) top = fmaxf(top, x[t][i][j]);
-            if (__ballot(top > m[t] + kLag)) {
-                const float mn = fmaxf(m[t], across(top));
-                const float f = mn == -INFINITY ? 1.0f : exp2_(m[t] - mn);
-                m[t] = mn;
-                l[t] *= f;
-#pragma unroll
-                for (int i = 0; i < CT; ++i) o[t][i] *= f;
-            }
-            const float ref = m[t] == -INFINITY ? 0.0f : m[t];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                f32x4_t y;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    y[j] = exp2_(x[t][i][j] - ref);
-                    l[t] += y[j];
-                }
-                p[t][i / 2][2 * (i & 1)] = pack_f16x2(y[0] * w[i][0], y[1] * w[i][1]);
-                p[t][i / 2][2 * (i & 1) + 1] = pack_f16x2(y[2] * w[i][2], y[3] * w[i][3]);
-            }
-        }
-    };
-
-    // ---- cached tokens: pages p0 + wave, + NW, ... ----
-    uint32_t k[4][2 * KS];
-    u32x4_t v[CT];
-    f32x4_t ks[4], vs[4];
-    auto load_keys = [&](int page) {
-        const uint8_t* base = a.c.k + a.c.code_base(page, h);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const uint8_t* row = base + (16 * t + c) * Dp;
-#pragma unroll
-            for (int i = 0; i < KS / 2; ++i) {
-                const u32x4_t w = *reinterpret_cast<const u32x4_t*>(row + 64 * i + 16 * g);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) k[t][4 * i + j] = w[j];
-            }
-            if constexpr (KS % 2) {
-                const u32x2_t w = *reinterpret_cast<const u32x2_t*>(row + 32 * (KS - 1) + 8 * g);
-                k[t][2 * KS - 2] = w[0];
-                k[t][2 * KS - 1] = w[1];
-            }
-            ks[t] = *reinterpret_cast<const f32x4_t*>(a.c.ks + a.c.scale_base(page, h) + 16 * t + 4 * g);
-        }
-    };
-    auto load_values = [&](int page) {
-        const uint8_t* base = a.c.v + a.c.code_base(page, h);
-#pragma unroll
-        for (int i = 0; i < CT; ++i) v[i] = *reinterpret_cast<const u32x4_t*>(base + (16 * i + c) * kKvPage + 16 * g);
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-            vs[t] = *reinterpret_cast<const f32x4_t*>(a.c.vs + a.c.scale_base(page, h) + 16 * t + 4 * g);
-    };
-    const int mine = p0 + wave < p1 ? (p1 - p0 - wave + NW - 1) / NW : 0;
-    int ids = 0;
-    auto page_id = [&](int it) {  // 64 entries of the block table at a time, one a lane
-        if ((it & 63) == 0) {
-            const int p = p0 + wave + (it + lane) * NW;
-            ids = p < p1 ? a.c.page(u.seq, p) : -1;
-        }
-        return __builtin_amdgcn_readlane(ids, it & 63);
-    };
-    int page = -1;
-    if (mine > 0) {
-        page = page_id(0);
-        load_keys(max(page, 0));  // (a missing page's place is taken by page 0, of which no token is seen)
-        load_values(max(page, 0));
     }
-    for (int it = 0; it < mine; ++it) {
-        if constexpr (NQ > 1) asm volatile("" ::: "memory");  // the queries stay in LDS
-        const int left = page < 0 ? 0 : min(L - (p0 + wave + it * NW) * kKvPage, kKvPage);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) x[n][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                const u32x2_t lo = codes_bf16<FP8>(k[t][2 * i]), hi = codes_bf16<FP8>(k[t][2 * i + 1]);
-                const u32x4_t key = {lo[0], lo[1], hi[0], hi[1]};
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) x[n][t] = mfma_bf16_16x16x32(key, query(n, i), x[n][t]);
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const f32x4_t s = ks[t] * a.scale2;
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) x[n][t] *= s;
-        }
-        const int next = it + 1 < mine ? page_id(it + 1) : -1;
-        if (it + 1 < mine) load_keys(max(next, 0));
-        if (left < kKvPage) {  // the last page: whatever it holds past the length
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                uint32_t bytes = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const bool in = 16 * t + 4 * g + j < left;
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) x[n][t][j] = in ? x[n][t][j] : -INFINITY;
-                    vs[t][j] = in ? vs[t][j] : 0.0f;
-                    bytes |= in ? 0xffu << (8 * j) : 0u;
-                }
-#pragma unroll
-                for (int i = 0; i < CT; ++i) v[i][t] &= bytes;
-            }
-        }
+    // Value scales of 64 tokens -> the factors of their weights.
+    __device__ __forceinline__ void factors(const f32x4_t (&vs)[4], f32x4_t (&w)[4]) {
         float top = 0.0f;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(vs[t][j]));
         if (__ballot(top > ldexpf(1.0f, e))) raise(max(e, __builtin_amdgcn_readfirstlane(exponent(across(top)))));
-        f32x4_t w[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[t][j] = ldexpf(vs[t][j], kTop - e);
-        u32x4_t p[NQ][2];
-        weigh(w, p);
+    }
+    // x (products q . k), times ks the scores -> weights; times w they are the
+    // operands p of the second product.  The maximum follows when a score is
+    // over it by more than kLag; the wave's first scores set it.
+    __device__ __forceinline__ void weigh(const f32x4_t (&ks)[4], const f32x4_t (&w)[4], u32x4_t (&p)[NQ][2]) {
+        if (fresh) {
+            fresh = false;
 #pragma unroll
-        for (int i = 0; i < CT; ++i)
+            for (int n = 0; n < NQ; ++n) {
+                float top = -INFINITY;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const u32x2_t lo = codes_f16<FP8>(v[i][2 * s]), hi = codes_f16<FP8>(v[i][2 * s + 1]);
-                const u32x4_t val = {lo[0], lo[1], hi[0], hi[1]};
+                for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) o[n][i] = mfma_f16_16x16x32(val, p[n][s], o[n][i]);
+                    for (int j = 0; j < 4; ++j) top = fmaxf(top, x[n][t][j] * ks[t][j]);
+                m[n] = across(top);
+                if (m[n] == -INFINITY) m[n] = 0.0f;  // (nothing seen: every weight is zero)
             }
-        if (it + 1 < mine) load_values(max(next, 0));
-        page = next;
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    x[n][t][j] = __builtin_fmaf(x[n][t][j], ks[t][j], -m[n]);
+                    top = fmaxf(top, x[n][t][j]);
+                }
+            if (__ballot(top > kLag)) {
+                const float to = m[n] + fmaxf(across(top), 0.0f), by = to - m[n], f = exp2_(-by);
+                m[n] = to;
+                l[n] *= f;
+#pragma unroll
+                for (int i = 0; i < CT; ++i) o[n][i] *= f;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) x[n][t] -= by;
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                f32x4_t y;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    y[j] = exp2_(x[n][t][j]);
+                    l[n] += y[j];
+                }
+                p[n][t / 2][2 * (t & 1)] = pack_f16x2(y[0] * w[t][0], y[1] * w[t][1]);
+                p[n][t / 2][2 * (t & 1) + 1] = pack_f16x2(y[2] * w[t][2], y[3] * w[t][3]);
+            }
+        }
+    }
+    // The last page's tokens past the length: scores of -inf, value scales of zero.
+    __device__ __forceinline__ void cut(int left, f32x4_t (&ks)[4], f32x4_t (&vs)[4]) {
+        asm volatile("" : "+s"(left));  // (else made selects on every page)
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool in = 16 * t + 4 * g + j < left;
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) x[n][t][j] = in ? x[n][t][j] : -INFINITY;
+                ks[t][j] = in ? ks[t][j] : 1.0f;
+                vs[t][j] = in ? vs[t][j] : 0.0f;
+            }
+    }
+    // The bytes of tokens 16 t + 4 g + (0..3) that are under `left`.
+    static __device__ __forceinline__ uint32_t bytes_in(int t, int left) {
+        const int in = min(max(left - 16 * t - 4 * ((static_cast<int>(threadIdx.x) & 63) >> 4), 0), 4);
+        return in == 4 ? 0xffffffffu : (1u << (8 * in)) - 1;
     }
 
-    // ---- the new tokens, by the wave whose turn it is after the sequence's last page ----
-    const LateArgs late = late_args();
-    if (late->k_new && split == splits - 1 && wave == (p1 - p0) % NW) {
+    // The new tokens' own keys and values, for the queries from row r0 on.
+    template <typename Query>
+    __device__ __forceinline__ void new_tokens(LateArgs late, const Unit& u, int r0, int D, Query query) {
+        const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
         uint64_t seen[NQ];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-            const int r = r0 + 16 * n + c, t = r / G;
-            seen[n] = r >= R ? 0 : late->tree ? late->tree[lo + t] : ~uint64_t{0} >> (63 - t);
-            seen[n] &= ~uint64_t{0} >> (64 - T);
+            const int r = r0 + 16 * n + c, t = r / u.G;
+            seen[n] = r >= u.R ? 0 : late->tree ? late->tree[u.lo + t] : ~uint64_t{0} >> (63 - t);
+            seen[n] &= ~uint64_t{0} >> (64 - u.T);
         }
         // Value rows of 32 tokens as they come, all loads in flight together: channel 16 i + c of tokens
         // t and t + 1, t = 32 s + 16 (j / 2) + 4 g + 2 (j % 2), clamped to a row and a channel that are there.
-        const uint16_t* new_values = late->v_new + lo * late->v_stride + h * D;
+        const uint16_t* new_values = late->v_new + u.lo * late->v_stride + u.h * D;
         uint32_t raw[CT][4];
         auto load_raw = [&](int s) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int t = 32 * s + 16 * (j / 2) + 4 * g + 2 * (j % 2);
-                const uint16_t* row = new_values + min(t, T - 1) * late->v_stride;
-                const uint16_t* odd = new_values + min(t + 1, T - 1) * late->v_stride;
+                const uint16_t* row = new_values + min(t, u.T - 1) * late->v_stride;
+                const uint16_t* odd = new_values + min(t + 1, u.T - 1) * late->v_stride;
 #pragma unroll
                 for (int i = 0; i < CT; ++i) {
                     const int ch = min(16 * i + c, D - 1);
@@ -424,14 +430,14 @@ __global__ __launch_bounds__((64 * most_waves<KS, NQ>()), (two_a_simd<KS, NQ>() 
                 }
             }
         };
-        load_raw(0);
-        const uint16_t* new_keys = late->k_new + lo * late->k_stride + h * D;
+        if constexpr (NQ == 1) load_raw(0);
+        const uint16_t* new_keys = late->k_new + u.lo * late->k_stride + u.h * D;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
             for (int n = 0; n < NQ; ++n) x[n][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-            if (16 * t >= T) continue;
-            const uint16_t* row = new_keys + min(16 * t + c, T - 1) * late->k_stride;
+            if (16 * t >= u.T) continue;
+            const uint16_t* row = new_keys + min(16 * t + c, u.T - 1) * late->k_stride;
             u32x4_t key[KS];
 #pragma unroll
             for (int i = 0; i < KS; ++i) key[i] = load_channels<KS == 1>(row, step_channel<KS>(i, g), D);
@@ -446,15 +452,18 @@ __global__ __launch_bounds__((64 * most_waves<KS, NQ>()), (two_a_simd<KS, NQ>() 
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    x[n][t][j] = (seen[n] >> (16 * t + 4 * g + j)) & 1 ? x[n][t][j] * a.scale2 : -INFINITY;
-        const float one = ldexpf(1.0f, kTop);
-        const f32x4_t w[4] = {{one, one, one, one}, {one, one, one, one}, {one, one, one, one}, {one, one, one, one}};
+                    x[n][t][j] = (seen[n] >> (16 * t + 4 * g + j)) & 1 ? x[n][t][j] : -INFINITY;
+        f32x4_t k2[4], w[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) k2[t][j] = late->scale2, w[t][j] = ldexpf(1.0f, kTop);
         u32x4_t p[NQ][2];
-        weigh(w, p);
+        weigh(k2, w, p);
         uint64_t odd = 0;  // lanes that met a value that is not finite
 #pragma unroll 1
-        for (int s = 0; 32 * s < T; ++s) {
-            if (s > 0) load_raw(s);
+        for (int s = 0; 32 * s < u.T; ++s) {
+            if (NQ > 1 || s > 0) load_raw(s);  // (early where registers are free)
             u16x2_t size = {0, 0};
             auto grow = [&] {
                 size = u16x2_t{0, 0};
@@ -468,13 +477,14 @@ __global__ __launch_bounds__((64 * most_waves<KS, NQ>()), (two_a_simd<KS, NQ>() 
             const uint64_t not_finite = __ballot(max(size[0], size[1]) >= 0x7f80);
             if (not_finite) {  // kept out of the product, in which they would reach queries that do not see them
                 odd |= not_finite;
-                asm volatile("");  // (a branch, not 64 selects that every call makes)
+                uint32_t inf = 0x7f80u;
+                asm volatile("" : "+s"(inf));  // (else made 64 selects on every call)
 #pragma unroll
                 for (int i = 0; i < CT; ++i)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        if ((raw[i][j] & 0x7f80u) == 0x7f80u) raw[i][j] &= 0xffff0000u;
-                        if ((raw[i][j] & 0x7f800000u) == 0x7f800000u) raw[i][j] &= 0xffffu;
+                        if ((raw[i][j] & inf) == inf) raw[i][j] &= 0xffff0000u;
+                        if (((raw[i][j] >> 16) & inf) == inf) raw[i][j] &= 0xffffu;
                     }
                 grow();
             }
@@ -498,7 +508,7 @@ __global__ __launch_bounds__((64 * most_waves<KS, NQ>()), (two_a_simd<KS, NQ>() 
         }
         if (odd)  // a query that sees such a value takes it as it is, the others do not
 #pragma unroll 1
-            for (int t = 0; t < T; ++t) {
+            for (int t = 0; t < u.T; ++t) {
                 const uint16_t* row = new_values + t * late->v_stride;
 #pragma unroll
                 for (int i = 0; i < CT; ++i)
@@ -513,48 +523,53 @@ __global__ __launch_bounds__((64 * most_waves<KS, NQ>()), (two_a_simd<KS, NQ>() 
             }
     }
 
-    // ---- the waves' sums meet in LDS ----
-    if constexpr (NQ > 1) __syncthreads();  // (the queries' place is taken)
-    float* mine_o = attn_lds + wave * QB * (kPitch + 2);
-    float* mine_ml = mine_o + QB * kPitch;
+    // This wave's sums to LDS, as they are (2^e applied).
+    __device__ __forceinline__ void put(float* to) {
+        const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        float sum = l[n];
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        if (g == 0) {
-            mine_ml[16 * n + c] = m[n];
-            mine_ml[QB + 16 * n + c] = sum;
-        }
+        for (int n = 0; n < NQ; ++n) {
+            float sum = l[n];
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            if (g == 0) {
+                to[QB * kPitch + 16 * n + c] = sum == 0.0f ? -INFINITY : m[n];
+                to[QB * kPitch + QB + 16 * n + c] = sum;
+            }
 #pragma unroll
-        for (int i = 0; i < CT; ++i) {
-            f32x4_t y;
+            for (int i = 0; i < CT; ++i) {
+                f32x4_t y;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = ldexpf(o[n][i][j], e - kTop);
-            *reinterpret_cast<f32x4_t*>(mine_o + (16 * n + c) * kPitch + 16 * i + 4 * g) = y;
+                for (int j = 0; j < 4; ++j) y[j] = ldexpf(o[n][i][j], e - kTop);
+                *reinterpret_cast<f32x4_t*>(to + (16 * n + c) * kPitch + 16 * i + 4 * g) = y;
+            }
         }
     }
-    __syncthreads();
+};
+
+// The waves' sums in LDS -> results, or a split's part of them.
+template <int KS, int NQ>
+__device__ __forceinline__ void join_waves(const float* lds, LateArgs late, const Unit& u, int D, int waves) {
+    constexpr int Dp = 32 * KS, QB = 16 * NQ, kPitch = Dp + 4, step = sums_floats<KS, NQ>();
     for (int n = threadIdx.x; n < QB * (Dp / 4); n += blockDim.x) {
-        const int qr = n / (Dp / 4), ch = 4 * (n % (Dp / 4)), r = r0 + qr;
-        if (r >= R) break;
-        const float* at = attn_lds + qr * kPitch + ch;
-        const float* ml = attn_lds + QB * kPitch + qr;
+        const int qr = n / (Dp / 4), ch = 4 * (n % (Dp / 4)), r = u.r0 + qr;
+        if (r >= u.R) break;
+        const float* at = lds + qr * kPitch + ch;
+        const float* ml = lds + QB * kPitch + qr;
         float top = -INFINITY;
-        for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[w * QB * (kPitch + 2)]);
+        for (int w = 0; w < waves; ++w) top = fmaxf(top, ml[w * step]);
         const float ref = top == -INFINITY ? 0.0f : top;
         f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
         float weight = 0.0f;
-        for (int w = 0; w < NW; ++w) {
-            const float f = exp2_(ml[w * QB * (kPitch + 2)] - ref);
-            weight += ml[w * QB * (kPitch + 2) + QB] * f;
-            sum += *reinterpret_cast<const f32x4_t*>(at + w * QB * (kPitch + 2)) * f;
+        for (int w = 0; w < waves; ++w) {
+            const float f = exp2_(ml[w * step] - ref);
+            weight += ml[w * step + QB] * f;
+            sum += *reinterpret_cast<const f32x4_t*>(at + w * step) * f;
         }
-        const int64_t row = static_cast<int64_t>(lo + r / G) * late->heads + h * G + r % G;
-        if (splits == 1) {
+        const int64_t row = static_cast<int64_t>(u.lo + r / u.G) * late->heads + u.h * u.G + r % u.G;
+        if (u.splits == 1) {
             store_row(late->out + row * D, ch, D, sum, weight, late->vec_out);
         } else {
-            const int64_t part = row * late->splits + split;
+            const int64_t part = row * late->splits + u.split;
             *reinterpret_cast<f32x4_t*>(late->ws_o + part * Dp + ch) = sum;
             if (ch == 0) {
                 late->ws_ml[2 * part] = top;
@@ -562,6 +577,114 @@ __global__ __launch_bounds__((64 * most_waves<KS, NQ>()), (two_a_simd<KS, NQ>() 
             }
         }
     }
+}
+
+// Every wave has the workgroup's 16 * NQ queries and pages of its own, which
+// come to its own place in LDS by DMA: the next page's keys once this one's
+// have met the queries, its values once this one's have met the weights.  No
+// wave waits for another before the end.
+template <int KS, int NQ, bool FP8>
+__global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_attn_kernel(AttnArgs a) {
+    constexpr int CT = 2 * KS;
+    extern __shared__ __attribute__((aligned(16))) uint8_t attn_lds[];
+    Unit u;
+    if (!find_share(a, 16 * NQ, u)) return;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, h = u.h, D = a.c.D;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), NW = blockDim.x >> 6;
+    uint8_t* keys = attn_lds + wave * page_bytes<KS>();
+    uint8_t* values = keys + 2 * KS * 1024;
+
+    f32x4_t ks[4], vs[4];
+    auto load_keys = [&](int page) {
+        const uint8_t* from = a.c.k + a.c.code_base(page, h);
+#pragma unroll
+        for (int n = 0; n < 2 * KS; ++n) fetch_keys<KS>(from, keys, n);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            ks[t] = *reinterpret_cast<const f32x4_t*>(a.c.ks + a.c.scale_base(page, h) + 16 * t + 4 * g);
+    };
+    auto load_values = [&](int page) {
+        asm volatile("" ::: "memory");  // (after the keys: the waits below count on the order)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            vs[t] = *reinterpret_cast<const f32x4_t*>(a.c.vs + a.c.scale_base(page, h) + 16 * t + 4 * g);
+        const uint8_t* from = a.c.v + a.c.code_base(page, h) + 16 * lane;
+#pragma unroll
+        for (int i = 0; i < CT; ++i) dma16(from + 1024 * i, values + 1024 * i);
+    };
+    // pages p0 + wave, + NW, ...
+    const int mine = u.p0 + wave < u.p1 ? (u.p1 - u.p0 - wave + NW - 1) / NW : 0;
+    int ids = 0;
+    auto page_id = [&](int it) {  // 64 entries of the block table at a time, one a lane
+        if ((it & 63) == 0) {
+            const int p = u.p0 + wave + (it + lane) * NW;
+            ids = p < u.p1 ? a.c.page(u.seq, p) : -1;
+        }
+        return __builtin_amdgcn_readlane(ids, it & 63);
+    };
+    int page = -1;
+    if (mine > 0) {
+        page = page_id(0);
+        load_keys(max(page, 0));  // (a missing page's place is taken by page 0, of which no token is seen)
+        load_values(max(page, 0));
+    }
+    u32x4_t q[NQ][KS];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) load_queries<KS>(a, u, u.r0 + 16 * n, q[n]);
+    Sums<KS, NQ> z;
+    z.clear();
+    for (int it = 0; it < mine; ++it) {
+        const int left = page < 0 ? 0 : min(u.L - (u.p0 + wave + it * NW) * kKvPage, kKvPage);
+        // The keys have landed: at least the CT loads of values were issued after them.
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CT) : "memory");
+        score<KS, NQ, FP8>(keys, q, z.x);
+        f32x4_t k2[4], f[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) k2[t] = ks[t] * a.scale2;
+        const int next = it + 1 < mine ? page_id(it + 1) : -1;
+        if (it + 1 < mine) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (this page's keys have been read)
+            load_keys(max(next, 0));
+        }
+        if (left < kKvPage) z.cut(left, k2, vs);
+        z.factors(vs, f);
+        u32x4_t w[NQ][2];
+        z.weigh(k2, f, w);
+        // The values have landed: the next page's 2 KS loads of keys were issued after them, or none.
+        if (it + 1 < mine) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * KS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        u32x4_t* val = reinterpret_cast<u32x4_t*>(values + 64 * c + 16 * g);
+        if (left < kKvPage)  // what lies past the length becomes zeros
+            for (int i = 0; i < CT; ++i)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) val[64 * i][t] &= z.bytes_in(t, left);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < CT; ++i) {
+                const u32x2_t y = *(reinterpret_cast<const u32x2_t*>(val + 64 * i) + s);
+                const u32x2_t lo = codes_f16<FP8>(y[0]), hi = codes_f16<FP8>(y[1]);
+                const u32x4_t b = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) z.o[n][i] = mfma_f16_16x16x32(b, w[n][s], z.o[n][i]);
+            }
+        if (it + 1 < mine) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (this page's values have been read)
+            load_values(max(next, 0));
+        }
+        page = next;
+    }
+
+    // the new tokens, by the wave whose turn it is after the last page
+    const LateArgs late = late_args();
+    if (late->k_new && u.split == u.splits - 1 && wave == (u.p1 - u.p0) % NW)
+        z.new_tokens(late, u, u.r0, D, [&](int n, int i) { return q[n][i]; });
+
+    __syncthreads();  // (the pages' place is taken)
+    float* sums = reinterpret_cast<float*>(attn_lds);
+    z.put(sums + wave * sums_floats<KS, NQ>());
+    __syncthreads();
+    join_waves<KS, NQ>(sums, late, u, D, NW);
 }
 
 // Joins the splits of a sequence's rows, in order of position: a workgroup
@@ -635,8 +758,9 @@ int64_t unit_bound(int n_seqs, int capacity, int max_new, int G, int block) {
 Plan make_plan(int n_seqs, int capacity, int max_new, int max_pages, int heads, int kv_heads, int D, int64_t ws_bytes) {
     const int G = heads / kv_heads, KS = kv_padded(D) / 32;
     Plan p{};
-    p.tiles = max_new * G <= 16 ? 1 : 2;
-    const int kTargetGroups = tuning_knob("LHQ_KV_TARGET", p.tiles > 1 ? 512 : 1024), kLeastPages = tuning_knob("LHQ_KV_LEAST", 16);
+    const int R = max_new * G, most = KS <= 4 ? 8 : 4;
+    p.tiles = R <= 16 ? 1 : 2;
+    const int kTargetGroups = tuning_knob("LHQ_KV_TARGET", 512), kLeastPages = tuning_knob("LHQ_KV_LEAST", 16);
     p.units = unit_bound(n_seqs, capacity, max_new, G, 16 * p.tiles);
     p.join_units = unit_bound(n_seqs, capacity, max_new, G, kJoinRows);
     const int64_t groups = std::max<int64_t>(1, p.units * kv_heads), rows = static_cast<int64_t>(capacity) * heads;
@@ -648,7 +772,7 @@ Plan make_plan(int n_seqs, int capacity, int max_new, int max_pages, int heads, 
     }
     p.pages_per_split = std::max<int>(1, (max_pages + splits - 1) / splits);
     p.splits = static_cast<int>(splits);
-    p.waves = KS <= 4 && groups * splits <= 256 ? 8 : 4;
+    p.waves = groups * splits <= 256 ? most : 4;
     return p;
 }
 
@@ -658,14 +782,20 @@ dim3 unit_grid(int heads, int64_t units) {
     return dim3(heads, y, static_cast<unsigned>((units + y - 1) / y));
 }
 
-template <int KS, int NQ, bool FP8>
-int launch(const char* fn, const AttnArgs& a, const Plan& p, hipStream_t s) {
-    constexpr auto kern = &kv_attn_kernel<KS, NQ, FP8>;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
+template <auto Kern>
+int launch(const char* fn, const AttnArgs& a, const Plan& p, size_t lds, hipStream_t s) {
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(Kern),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (attr != hipSuccess) return set_error(LHQ_ERR_HIP, "%s: dynamic LDS attribute: %s", fn, hipGetErrorString(attr));
-    kern<<<unit_grid(a.c.heads, p.units * p.splits), 64 * p.waves, lds_bytes<KS, NQ>(p.waves), s>>>(a);
+    Kern<<<unit_grid(a.c.heads, p.units * p.splits), 64 * p.waves, lds, s>>>(a);
     return check_launch(fn);
+}
+template <int KS, bool FP8>
+int launch(const char* fn, const AttnArgs& a, const Plan& p, hipStream_t s) {
+    const int wave = std::max(4 * (p.tiles == 1 ? sums_floats<KS, 1>() : sums_floats<KS, 2>()), page_bytes<KS>());
+    const size_t lds = p.waves * wave;
+    if (p.tiles == 1) return launch<&kv_attn_kernel<KS, 1, FP8>>(fn, a, p, lds, s);
+    return launch<&kv_attn_kernel<KS, 2, FP8>>(fn, a, p, lds, s);
 }
 
 }  // namespace
@@ -728,13 +858,7 @@ int lhq_kv_attn_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k_new,
     const hipStream_t s = as_stream(stream);
     int st = LHQ_OK;
     auto go = [&](auto ks) {
-        auto with = [&](auto nq, auto fp8) { st = launch<ks(), nq(), fp8()>(fn, a, p, s); };
-        auto fmt = [&](auto nq) {
-            if (format == LHQ_KV_FP8) with(nq, std::true_type{});
-            else with(nq, std::false_type{});
-        };
-        if (p.tiles == 1) fmt(std::integral_constant<int, 1>{});
-        else fmt(std::integral_constant<int, 2>{});
+        st = format == LHQ_KV_FP8 ? launch<ks(), true>(fn, a, p, s) : launch<ks(), false>(fn, a, p, s);
     };
     switch (kv_padded(head_dim) / 32) {
         case 1: go(std::integral_constant<int, 1>{}); break;
