@@ -180,35 +180,38 @@ __device__ __forceinline__ void fetch_keys(const uint8_t* page, uint8_t* to, int
     const int at = 64 * n + (threadIdx.x & 63);
     dma16(page + 16 * (at ^ key_swizzle<KS>(at / (2 * KS))), to + 1024 * n);
 }
-// S^T of a page whose keys lie in LDS at `keys`.
-template <int KS, int NQ, bool FP8>
-__device__ __forceinline__ void score(const uint8_t* keys, const u32x4_t (&q)[NQ][KS], f32x4_t (&x)[NQ][4]) {
+// A page's keys from LDS as operands: k steps 2 i and 2 i + 1 of tile t.
+template <int KS>
+__device__ __forceinline__ void read_keys(const uint8_t* keys, u32x4_t (&k)[(KS + 1) / 2][4]) {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    // (a step of channels at a time over all tiles: no product waits for the one before it)
 #pragma unroll
-    for (int i = 0; i < KS; i += 2) {
-        u32x4_t w[4];
+    for (int i = 0; i < (KS + 1) / 2; ++i)
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             const uint8_t* row = keys + (16 * t + c) * 32 * KS;
-            if (i + 1 < KS) {
-                w[t] = *reinterpret_cast<const u32x4_t*>(row + 16 * ((2 * i + g) ^ key_swizzle<KS>(c)));
+            if (2 * i + 1 < KS) {
+                k[i][t] = *reinterpret_cast<const u32x4_t*>(row + 16 * ((4 * i + g) ^ key_swizzle<KS>(c)));
             } else {
-                const u32x2_t y = *reinterpret_cast<const u32x2_t*>(row + 32 * i + 8 * g);
-                w[t][0] = y[0], w[t][1] = y[1];
+                const u32x2_t y = *reinterpret_cast<const u32x2_t*>(row + 64 * i + 8 * g);
+                k[i][t] = u32x4_t{y[0], y[1], 0, 0};
             }
         }
+}
+// S^T of a page.
+template <int KS, int NQ, bool FP8>
+__device__ __forceinline__ void score(const u32x4_t (&k)[(KS + 1) / 2][4], const u32x4_t (&q)[NQ][KS],
+                                      f32x4_t (&x)[NQ][4]) {
+    // (a step of channels at a time over all tiles: no product waits for the one before it)
 #pragma unroll
-        for (int b = 0; b < 2 && i + b < KS; ++b)
+    for (int i = 0; i < KS; ++i)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const u32x2_t lo = codes_bf16<FP8>(w[t][2 * b]), hi = codes_bf16<FP8>(w[t][2 * b + 1]);
-                const u32x4_t key = {lo[0], lo[1], hi[0], hi[1]};
+        for (int t = 0; t < 4; ++t) {
+            const u32x2_t lo = codes_bf16<FP8>(k[i / 2][t][2 * (i & 1)]), hi = codes_bf16<FP8>(k[i / 2][t][2 * (i & 1) + 1]);
+            const u32x4_t key = {lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
-                for (int n = 0; n < NQ; ++n)
-                    x[n][t] = mfma_bf16_16x16x32(key, q[n][i + b], i + b == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : x[n][t]);
-            }
-    }
+            for (int n = 0; n < NQ; ++n)
+                x[n][t] = mfma_bf16_16x16x32(key, q[n][i], i == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : x[n][t]);
+        }
 }
 
 // The waves of a workgroup at most; two a SIMD where 256 registers hold a
@@ -216,12 +219,12 @@ __device__ __forceinline__ void score(const uint8_t* keys, const u32x4_t (&q)[NQ
 template <int KS>
 constexpr int most_waves() { return KS <= 4 ? 8 : 4; }
 
-// LDS of a wave: its page, then its sums [QB][Dp + 4] and its maxima and sums of
+// LDS of a wave: its page and the factors of its tokens, then its sums [QB][Dp + 4] and its maxima and sums of
 // weights [2][QB].
 template <int KS, int NQ>
 constexpr int sums_floats() { return 16 * NQ * (32 * KS + 4 + 2); }
 template <int KS>
-constexpr int page_bytes() { return 4 * KS * 1024; }
+constexpr int page_bytes() { return 4 * KS * 1024 + 512; }
 
 // Four channels of a result row from channel ch on.
 __device__ __forceinline__ void store_row(uint16_t* row, int ch, int D, const f32x4_t& sum, float weight, bool vec) {
@@ -319,18 +322,14 @@ struct Sums {
         v = fmaxf(v, __shfl_xor(v, 16, 64));
         return fmaxf(v, __shfl_xor(v, 32, 64));
     }
-    // Value scales of 64 tokens -> the factors of their weights.
-    __device__ __forceinline__ void factors(const f32x4_t (&vs)[4], f32x4_t (&w)[4]) {
-        float top = 0.0f;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(vs[t][j]));
-        if (__ballot(top > ldexpf(1.0f, e))) raise(max(e, __builtin_amdgcn_readfirstlane(exponent(across(top)))));
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[t][j] = ldexpf(vs[t][j], kTop - e);
+    // The value scale of token `lane` -> the factor of its weights.
+    __device__ __forceinline__ float factor(float vs) {
+        float top = fabsf(vs);
+        if (__ballot(top > ldexpf(1.0f, e))) {
+            for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+            raise(max(e, __builtin_amdgcn_readfirstlane(exponent(top))));
+        }
+        return ldexpf(vs, kTop - e);
     }
     // x (products q . k), times ks the scores -> weights; times w they are the
     // operands p of the second product.  The maximum follows when a score is
@@ -381,20 +380,17 @@ struct Sums {
             }
         }
     }
-    // The last page's tokens past the length: scores of -inf, value scales of zero.
-    __device__ __forceinline__ void cut(int left, f32x4_t (&ks)[4], f32x4_t (&vs)[4]) {
+    // The last page's tokens past the length are not seen.
+    __device__ __forceinline__ void cut(int left) {
+        left = __builtin_amdgcn_readfirstlane(left);
         asm volatile("" : "+s"(left));  // (else made selects on every page)
         const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bool in = 16 * t + 4 * g + j < left;
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) x[n][t][j] = in ? x[n][t][j] : -INFINITY;
-                ks[t][j] = in ? ks[t][j] : 1.0f;
-                vs[t][j] = in ? vs[t][j] : 0.0f;
-            }
+                for (int n = 0; n < NQ; ++n) x[n][t][j] = 16 * t + 4 * g + j < left ? x[n][t][j] : -INFINITY;
     }
     // The bytes of tokens 16 t + 4 g + (0..3) that are under `left`.
     static __device__ __forceinline__ uint32_t bytes_in(int t, int left) {
@@ -402,25 +398,25 @@ struct Sums {
         return in == 4 ? 0xffffffffu : (1u << (8 * in)) - 1;
     }
 
-    // The new tokens' own keys and values, for the queries from row r0 on.
-    template <typename Query>
-    __device__ __forceinline__ void new_tokens(LateArgs late, const Unit& u, int r0, int D, Query query) {
+    // The new tokens' own keys and values: tokens t0 .. t0 + 31 that there are (at least one).
+    __device__ __forceinline__ void new_tokens(LateArgs late, const Unit& u, int t0, int D, const u32x4_t (&q)[NQ][KS]) {
         const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-        uint64_t seen[NQ];
+        uint32_t seen[NQ];  // of those 32
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-            const int r = r0 + 16 * n + c, t = r / u.G;
-            seen[n] = r >= u.R ? 0 : late->tree ? late->tree[u.lo + t] : ~uint64_t{0} >> (63 - t);
-            seen[n] &= ~uint64_t{0} >> (64 - u.T);
+            const int r = u.r0 + 16 * n + c, t = r / u.G;
+            uint64_t word = r >= u.R ? 0 : late->tree ? late->tree[u.lo + t] : ~uint64_t{0} >> (63 - t);
+            word &= ~uint64_t{0} >> (64 - u.T);
+            seen[n] = static_cast<uint32_t>(word >> t0);
         }
-        // Value rows of 32 tokens as they come, all loads in flight together: channel 16 i + c of tokens
-        // t and t + 1, t = 32 s + 16 (j / 2) + 4 g + 2 (j % 2), clamped to a row and a channel that are there.
+        // Value rows as they come, all loads in flight together: channel 16 i + c of tokens t and t + 1,
+        // t = t0 + 16 (j / 2) + 4 g + 2 (j % 2), clamped to a row and a channel that are there.
         const uint16_t* new_values = late->v_new + u.lo * late->v_stride + u.h * D;
         uint32_t raw[CT][4];
-        auto load_raw = [&](int s) {
+        auto load_raw = [&] {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int t = 32 * s + 16 * (j / 2) + 4 * g + 2 * (j % 2);
+                const int t = t0 + 16 * (j / 2) + 4 * g + 2 * (j % 2);
                 const uint16_t* row = new_values + min(t, u.T - 1) * late->v_stride;
                 const uint16_t* odd = new_values + min(t + 1, u.T - 1) * late->v_stride;
 #pragma unroll
@@ -430,99 +426,86 @@ struct Sums {
                 }
             }
         };
-        if constexpr (NQ == 1) load_raw(0);
+        if constexpr (NQ == 1) load_raw();  // (early where registers are free)
         const uint16_t* new_keys = late->k_new + u.lo * late->k_stride + u.h * D;
+        f32x4_t ks[4], f[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) x[n][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-            if (16 * t >= u.T) continue;
-            const uint16_t* row = new_keys + min(16 * t + c, u.T - 1) * late->k_stride;
+            for (int j = 0; j < 4; ++j) ks[t][j] = late->scale2, f[t][j] = ldexpf(1.0f, kTop);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) x[n][t] = f32x4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (t >= 2) continue;
+            const uint16_t* row = new_keys + min(t0 + 16 * t + c, u.T - 1) * late->k_stride;
             u32x4_t key[KS];
 #pragma unroll
             for (int i = 0; i < KS; ++i) key[i] = load_channels<KS == 1>(row, step_channel<KS>(i, g), D);
 #pragma unroll
-            for (int i = 0; i < KS; ++i)
+            for (int n = 0; n < NQ; ++n) {
+                f32x4_t y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) x[n][t] = mfma_bf16_16x16x32(key[i], query(n, i), x[n][t]);
-        }
-#pragma unroll
-        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
+                for (int i = 0; i < KS; ++i) y = mfma_bf16_16x16x32(key[i], q[n][i], y);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    x[n][t][j] = (seen[n] >> (16 * t + 4 * g + j)) & 1 ? x[n][t][j] : -INFINITY;
-        f32x4_t k2[4], w[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) k2[t][j] = late->scale2, w[t][j] = ldexpf(1.0f, kTop);
+                    if ((seen[n] >> (16 * t + 4 * g + j)) & 1) x[n][t][j] = y[j];
+            }
+        }
         u32x4_t p[NQ][2];
-        weigh(k2, w, p);
-        uint64_t odd = 0;  // lanes that met a value that is not finite
-#pragma unroll 1
-        for (int s = 0; 32 * s < u.T; ++s) {
-            if (NQ > 1 || s > 0) load_raw(s);  // (early where registers are free)
-            u16x2_t size = {0, 0};
-            auto grow = [&] {
-                size = u16x2_t{0, 0};
+        weigh(ks, f, p);
+        if constexpr (NQ > 1) load_raw();
+        u16x2_t size = {0, 0};
+        auto grow = [&] {
+            size = u16x2_t{0, 0};
 #pragma unroll
-                for (int i = 0; i < CT; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        size = __builtin_elementwise_max(size, __builtin_bit_cast(u16x2_t, raw[i][j] & 0x7fff7fffu));
-            };
-            grow();
-            const uint64_t not_finite = __ballot(max(size[0], size[1]) >= 0x7f80);
-            if (not_finite) {  // kept out of the product, in which they would reach queries that do not see them
-                odd |= not_finite;
-                uint32_t inf = 0x7f80u;
-                asm volatile("" : "+s"(inf));  // (else made 64 selects on every call)
-#pragma unroll
-                for (int i = 0; i < CT; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if ((raw[i][j] & inf) == inf) raw[i][j] &= 0xffff0000u;
-                        if (((raw[i][j] >> 16) & inf) == inf) raw[i][j] &= 0xffffu;
-                    }
-                grow();
-            }
-            float big = bf16_to_f32(max(size[0], size[1]));
-            for (int d = 32; d; d >>= 1) big = fmaxf(big, __shfl_xor(big, d, 64));
-            // the values themselves as fp16, their largest under 2^15 (fp16's normal range holds 2^-29 of that)
-            const int want = __builtin_amdgcn_readfirstlane(exponent(big)) - 15;
-            if (big > 0.0f && want > e) raise(want);
-#pragma unroll
-            for (int i = 0; i < CT; ++i) {
-                u32x4_t val;
+            for (int i = 0; i < CT; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    val[j] = pack_f16x2(ldexpf(__uint_as_float(raw[i][j] << 16), -e),
-                                        ldexpf(__uint_as_float(raw[i][j] & 0xffff0000u), -e));
+                    size = __builtin_elementwise_max(size, __builtin_bit_cast(u16x2_t, raw[i][j] & 0x7fff7fffu));
+        };
+        grow();
+        const uint64_t not_finite = __ballot(max(size[0], size[1]) >= 0x7f80);
+        if (not_finite) {  // kept out of the product, in which they would reach queries that do not see them
+            uint32_t inf = 0x7f80u;
+            asm volatile("" : "+s"(inf));  // (else made 64 selects on every call)
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) o[n][i] = mfma_f16_16x16x32(val, p[n][0], o[n][i]);
-            }
+            for (int i = 0; i < CT; ++i)
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) p[n][0] = p[n][1];
+                for (int j = 0; j < 4; ++j) {
+                    if ((raw[i][j] & inf) == inf) raw[i][j] &= 0xffff0000u;
+                    if (((raw[i][j] >> 16) & inf) == inf) raw[i][j] &= 0xffffu;
+                }
+            grow();
         }
-        if (odd)  // a query that sees such a value takes it as it is, the others do not
+        float big = bf16_to_f32(max(size[0], size[1]));
+        for (int d = 32; d; d >>= 1) big = fmaxf(big, __shfl_xor(big, d, 64));
+        // the values themselves as fp16, their largest under 2^15 (fp16's normal range holds 2^-29 of that)
+        const int want = __builtin_amdgcn_readfirstlane(exponent(big)) - 15;
+        if (big > 0.0f && want > e) raise(want);
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+            u32x4_t val;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                val[j] = pack_f16x2(ldexpf(__uint_as_float(raw[i][j] << 16), -e),
+                                    ldexpf(__uint_as_float(raw[i][j] & 0xffff0000u), -e));
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) o[n][i] = mfma_f16_16x16x32(val, p[n][0], o[n][i]);
+        }
+        if (not_finite)  // a query that sees such a value takes it as it is, the others do not
 #pragma unroll 1
-            for (int t = 0; t < u.T; ++t) {
+            for (int t = t0; t < min(u.T, t0 + 32); ++t) {
                 const uint16_t* row = new_values + t * late->v_stride;
 #pragma unroll
                 for (int i = 0; i < CT; ++i)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const int ch = 16 * i + 4 * g + j;
-                        const float y = bf16_to_f32(row[min(ch, D - 1)]);
+                        const float y = bf16_to_f32(row[min(16 * i + 4 * g + j, D - 1)]);
 #pragma unroll
                         for (int n = 0; n < NQ; ++n)
-                            o[n][i][j] += !(fabsf(y) < INFINITY) && ((seen[n] >> t) & 1) ? y : 0.0f;
+                            o[n][i][j] += !(fabsf(y) < INFINITY) && ((seen[n] >> (t - t0)) & 1) ? y : 0.0f;
                     }
             }
     }
-
     // This wave's sums to LDS, as they are (2^e applied).
     __device__ __forceinline__ void put(float* to) {
         const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
@@ -594,21 +577,17 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
     uint8_t* keys = attn_lds + wave * page_bytes<KS>();
     uint8_t* values = keys + 2 * KS * 1024;
 
-    f32x4_t ks[4], vs[4];
-    auto load_keys = [&](int page) {
+    float* factors = reinterpret_cast<float*>(values + 2 * KS * 1024);  // of scores, of weights; by token
+
+    float ks = 0.0f, vs = 0.0f;  // of token `lane`
+    auto load_page = [&](int page) {
+        ks = a.c.ks[a.c.scale_base(page, h) + lane];
+        vs = a.c.vs[a.c.scale_base(page, h) + lane];
         const uint8_t* from = a.c.k + a.c.code_base(page, h);
 #pragma unroll
         for (int n = 0; n < 2 * KS; ++n) fetch_keys<KS>(from, keys, n);
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-            ks[t] = *reinterpret_cast<const f32x4_t*>(a.c.ks + a.c.scale_base(page, h) + 16 * t + 4 * g);
-    };
-    auto load_values = [&](int page) {
-        asm volatile("" ::: "memory");  // (after the keys: the waits below count on the order)
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-            vs[t] = *reinterpret_cast<const f32x4_t*>(a.c.vs + a.c.scale_base(page, h) + 16 * t + 4 * g);
-        const uint8_t* from = a.c.v + a.c.code_base(page, h) + 16 * lane;
+        asm volatile("" ::: "memory");  // (the values last: the wait for the keys counts on it)
+        from = a.c.v + a.c.code_base(page, h) + 16 * lane;
 #pragma unroll
         for (int i = 0; i < CT; ++i) dma16(from + 1024 * i, values + 1024 * i);
     };
@@ -625,8 +604,7 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
     int page = -1;
     if (mine > 0) {
         page = page_id(0);
-        load_keys(max(page, 0));  // (a missing page's place is taken by page 0, of which no token is seen)
-        load_values(max(page, 0));
+        load_page(max(page, 0));  // (a missing page's place is taken by page 0, of which no token is seen)
     }
     u32x4_t q[NQ][KS];
 #pragma unroll
@@ -635,50 +613,55 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
     z.clear();
     for (int it = 0; it < mine; ++it) {
         const int left = page < 0 ? 0 : min(u.L - (u.p0 + wave + it * NW) * kKvPage, kKvPage);
-        // The keys have landed: at least the CT loads of values were issued after them.
+        // The keys have landed: the CT loads of values were issued after them.
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CT) : "memory");
-        score<KS, NQ, FP8>(keys, q, z.x);
-        f32x4_t k2[4], f[4];
+        u32x4_t k[(KS + 1) / 2][4], v[CT], w[NQ][2];
+        read_keys<KS>(keys, k);
+        const bool in = lane < left;  // what the last page holds past the length counts for nothing
+        factors[lane] = in ? ks * a.scale2 : 1.0f;
+        factors[64 + lane] = z.factor(in ? vs : 0.0f);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
-        for (int t = 0; t < 4; ++t) k2[t] = ks[t] * a.scale2;
+        for (int i = 0; i < CT; ++i) v[i] = *reinterpret_cast<const u32x4_t*>(values + 1024 * i + 64 * c + 16 * g);
+        __builtin_amdgcn_sched_barrier(0);  // (all reads ahead of the products)
+        score<KS, NQ, FP8>(k, q, z.x);
         const int next = it + 1 < mine ? page_id(it + 1) : -1;
         if (it + 1 < mine) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (this page's keys have been read)
-            load_keys(max(next, 0));
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (this page has been read)
+            load_page(max(next, 0));
         }
-        if (left < kKvPage) z.cut(left, k2, vs);
-        z.factors(vs, f);
-        u32x4_t w[NQ][2];
-        z.weigh(k2, f, w);
-        // The values have landed: the next page's 2 KS loads of keys were issued after them, or none.
-        if (it + 1 < mine) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * KS) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        u32x4_t* val = reinterpret_cast<u32x4_t*>(values + 64 * c + 16 * g);
-        if (left < kKvPage)  // what lies past the length becomes zeros
-            for (int i = 0; i < CT; ++i)
+        if (left < kKvPage) {
+            z.cut(left);
 #pragma unroll
-                for (int t = 0; t < 4; ++t) val[64 * i][t] &= z.bytes_in(t, left);
+            for (int t = 0; t < 4; ++t) {
+                const uint32_t bytes = z.bytes_in(t, left);
+#pragma unroll
+                for (int i = 0; i < CT; ++i) v[i][t] &= bytes;
+            }
+        }
+        f32x4_t k2[4], f[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            k2[t] = *reinterpret_cast<const f32x4_t*>(factors + 16 * t + 4 * g);
+            f[t] = *reinterpret_cast<const f32x4_t*>(factors + 64 + 16 * t + 4 * g);
+        }
+        z.weigh(k2, f, w);
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int i = 0; i < CT; ++i) {
-                const u32x2_t y = *(reinterpret_cast<const u32x2_t*>(val + 64 * i) + s);
-                const u32x2_t lo = codes_f16<FP8>(y[0]), hi = codes_f16<FP8>(y[1]);
-                const u32x4_t b = {lo[0], lo[1], hi[0], hi[1]};
+                const u32x2_t lo = codes_f16<FP8>(v[i][2 * s]), hi = codes_f16<FP8>(v[i][2 * s + 1]);
+                const u32x4_t val = {lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) z.o[n][i] = mfma_f16_16x16x32(b, w[n][s], z.o[n][i]);
+                for (int n = 0; n < NQ; ++n) z.o[n][i] = mfma_f16_16x16x32(val, w[n][s], z.o[n][i]);
             }
-        if (it + 1 < mine) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (this page's values have been read)
-            load_values(max(next, 0));
-        }
         page = next;
     }
 
-    // the new tokens, by the wave whose turn it is after the last page
+    // the new tokens, 32 at a time, by the waves whose turn it is after the last page
     const LateArgs late = late_args();
-    if (late->k_new && u.split == u.splits - 1 && wave == (u.p1 - u.p0) % NW)
-        z.new_tokens(late, u, u.r0, D, [&](int n, int i) { return q[n][i]; });
+    const int turn = __builtin_amdgcn_readfirstlane((wave + NW - (u.p1 - u.p0) % NW) % NW);  // (at least four waves for at most 64 tokens)
+    if (late->k_new && u.split == u.splits - 1 && 32 * turn < u.T) z.new_tokens(late, u, 32 * turn, D, q);
 
     __syncthreads();  // (the pages' place is taken)
     float* sums = reinterpret_cast<float*>(attn_lds);
