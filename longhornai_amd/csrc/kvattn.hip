@@ -170,15 +170,30 @@ __device__ __forceinline__ int key_swizzle(int r) {
     else if constexpr (KS == 8) return ((r & 1) << 2) | ((r & 2) << 2) | ((r >> 2) & 2);
     else return 0;
 }
-// LDS DMA: 16 bytes a lane, from this lane's address to `to` + 16 * lane.
-__device__ __forceinline__ void dma16(const void* from, void* to) {
-    __builtin_amdgcn_global_load_lds(from, (LHQ_LDS_AS void*)to, 16, 0, 0);
-}
-// The n-th of a page's 2 KS key DMAs (1 KiB): to + 16 * lane gets this lane's chunk.
-template <int KS>
-__device__ __forceinline__ void fetch_keys(const uint8_t* page, uint8_t* to, int n) {
-    const int at = 64 * n + (threadIdx.x & 63);
-    dma16(page + 16 * (at ^ key_swizzle<KS>(at / (2 * KS))), to + 1024 * n);
+// LDS DMA: 16 bytes a lane, from this lane's address + OFFSET to `to` + OFFSET +
+// 16 * lane.
+template <int OFFSET>
+__device__ __forceinline__ void dma16(const void* from, void* to);
+#define LHQ_DMA16(offset)                                                           \
+    template <>                                                                     \
+    __device__ __forceinline__ void dma16<offset>(const void* from, void* to) {     \
+        __builtin_amdgcn_global_load_lds(from, (LHQ_LDS_AS void*)to, 16, offset, 0); \
+    }
+LHQ_DMA16(0)
+LHQ_DMA16(1024)
+LHQ_DMA16(2048)
+LHQ_DMA16(3072)
+#undef LHQ_DMA16
+// 2 KS KiB of a page: KiB n from `from` + 1024 n + place(n) to `to` + 1024 n + 16 * lane.
+template <int KS, typename Place>
+__device__ __forceinline__ void fetch(const uint8_t* from, uint8_t* to, Place place) {
+#pragma unroll
+    for (int n = 0; n < 2 * KS; n += 4) {  // (four of them with one address on either side)
+        dma16<0>(from + 1024 * n + place(n), to + 1024 * n);
+        dma16<1024>(from + 1024 * n + place(n + 1), to + 1024 * n);
+        if (n + 2 < 2 * KS) dma16<2048>(from + 1024 * n + place(n + 2), to + 1024 * n);
+        if (n + 2 < 2 * KS) dma16<3072>(from + 1024 * n + place(n + 3), to + 1024 * n);
+    }
 }
 // A page's keys from LDS as operands: k steps 2 i and 2 i + 1 of tile t.
 template <int KS>
@@ -584,12 +599,11 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
         ks = a.c.ks[a.c.scale_base(page, h) + lane];
         vs = a.c.vs[a.c.scale_base(page, h) + lane];
         const uint8_t* from = a.c.k + a.c.code_base(page, h);
-#pragma unroll
-        for (int n = 0; n < 2 * KS; ++n) fetch_keys<KS>(from, keys, n);
+        fetch<KS>(from, keys, [lane](int n) -> uint32_t {
+            return 16 * (lane ^ key_swizzle<KS>((64 * n + lane) / (2 * KS)));
+        });
         asm volatile("" ::: "memory");  // (the values last: the wait for the keys counts on it)
-        from = a.c.v + a.c.code_base(page, h) + 16 * lane;
-#pragma unroll
-        for (int i = 0; i < CT; ++i) dma16(from + 1024 * i, values + 1024 * i);
+        fetch<KS>(a.c.v + a.c.code_base(page, h), values, [lane](int) -> uint32_t { return 16 * lane; });
     };
     // pages p0 + wave, + NW, ...
     const int mine = u.p0 + wave < u.p1 ? (u.p1 - u.p0 - wave + NW - 1) / NW : 0;
