@@ -57,7 +57,7 @@ struct AttnArgs {
     const int32_t* lengths;
     KvCache c;
     uint16_t* out;
-    int n_seqs, capacity, max_new, heads;
+    int n_seqs, capacity, max_new, heads, group;  // group: query heads of a kv head
     float scale2;          // scale * log2 e: weights are powers of two
     bool vec_out;          // rows of out: 8-byte stores
     int pages_per_split;   // a sequence of p pages has ceil(p / this) splits
@@ -70,6 +70,7 @@ __device__ __forceinline__ int cached(const AttnArgs& a, int s) {
     return static_cast<int>(min<int64_t>(max(a.lengths[s], 0), static_cast<int64_t>(a.c.max_pages) * kKvPage));
 }
 __device__ __forceinline__ int split_count(const AttnArgs& a, int length) {
+    if (a.splits == 1) return 1;
     const int pages = (length + kKvPage - 1) / kKvPage;
     return max(1, (pages + a.pages_per_split - 1) / a.pages_per_split);
 }
@@ -259,11 +260,22 @@ __device__ __forceinline__ void store_row(uint16_t* row, int ch, int D, const f3
 // head) list of a sequence, and its pages [p0, p1).
 struct Unit {
     int seq, h, G, lo, T, R, r0, L, pages, split, splits, p0, p1;
+    float per_token;  // 1 / G
+    // The token of row r of the list: r / G, under 64.
+    __device__ int token(int r) const {
+        const int t = static_cast<int>(static_cast<float>(r) * per_token);  // at most one off
+        return t + (r >= (t + 1) * G) - (r < t * G);
+    }
+    __device__ int64_t out_row(int r, int heads) const {
+        const int t = token(r);
+        return static_cast<int64_t>(lo + t) * heads + h * G + r - t * G;
+    }
 };
 // BLOCK rows a workgroup; false past the end of the list.
 __device__ __forceinline__ bool find_share(const AttnArgs& a, int block, Unit& u) {
     u.h = blockIdx.x;
-    u.G = a.heads / a.c.heads;
+    u.G = a.group;
+    u.per_token = 1.0f / static_cast<float>(a.group);
     int lane_lo = 0, lane_T = 0, lane_L = 0;
     const KvUnit f = kv_find_unit(blockIdx.y + blockIdx.z * gridDim.y, a.n_seqs, [&](int s) {
         const KvRows r = kv_rows(a.offsets, s, a.capacity);
@@ -281,18 +293,24 @@ __device__ __forceinline__ bool find_share(const AttnArgs& a, int block, Unit& u
     u.pages = (u.L + kKvPage - 1) / kKvPage;
     u.splits = split_count(a, u.L);
     const int blocks = (u.R + block - 1) / block;
-    u.split = f.nth / blocks;
-    u.r0 = (f.nth % blocks) * block;
-    // (under 2^25 pages and 64 splits)
-    u.p0 = static_cast<uint32_t>(u.pages * u.split) / static_cast<uint32_t>(u.splits);
-    u.p1 = (static_cast<uint32_t>(u.pages) * (u.split + 1)) / static_cast<uint32_t>(u.splits);
+    if (u.splits == 1) {
+        u.split = 0;
+        u.r0 = f.nth * block;
+        u.p0 = 0;
+        u.p1 = u.pages;
+    } else {  // (under 2^25 pages and 64 splits)
+        u.split = f.nth / blocks;
+        u.r0 = (f.nth - u.split * blocks) * block;
+        u.p0 = static_cast<uint32_t>(u.pages * u.split) / static_cast<uint32_t>(u.splits);
+        u.p1 = (static_cast<uint32_t>(u.pages) * (u.split + 1)) / static_cast<uint32_t>(u.splits);
+    }
     return true;
 }
 // The operands of the 16 queries from row r on, column lane & 15 (past the
 // last row: that one again, whose results no one reads).
 template <int KS>
 __device__ __forceinline__ void load_queries(const AttnArgs& a, const Unit& u, int r, u32x4_t (&q)[KS]) {
-    const int lane = threadIdx.x & 63, row = min(r + (lane & 15), u.R - 1), t = row / u.G;
+    const int lane = threadIdx.x & 63, row = min(r + (lane & 15), u.R - 1), t = u.token(row);
     const uint16_t* from = a.q + (u.lo + t) * a.q_stride + (u.h * u.G + row - t * u.G) * a.c.D;
 #pragma unroll
     for (int i = 0; i < KS; ++i) q[i] = load_channels<KS == 1>(from, step_channel<KS>(i, lane >> 4), a.c.D);
@@ -419,7 +437,7 @@ struct Sums {
         uint32_t seen[NQ];  // of those 32
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-            const int r = u.r0 + 16 * n + c, t = r / u.G;
+            const int r = u.r0 + 16 * n + c, t = u.token(min(r, u.R - 1));
             uint64_t word = r >= u.R ? 0 : late->tree ? late->tree[u.lo + t] : ~uint64_t{0} >> (63 - t);
             word &= ~uint64_t{0} >> (64 - u.T);
             seen[n] = static_cast<uint32_t>(word >> t0);
@@ -545,25 +563,34 @@ struct Sums {
 };
 
 // The waves' sums in LDS -> results, or a split's part of them.
-template <int KS, int NQ>
-__device__ __forceinline__ void join_waves(const float* lds, LateArgs late, const Unit& u, int D, int waves) {
+template <int KS, int NQ, int WAVES>
+__device__ __forceinline__ void join_waves(const float* lds, LateArgs late, const Unit& u, int D) {
     constexpr int Dp = 32 * KS, QB = 16 * NQ, kPitch = Dp + 4, step = sums_floats<KS, NQ>();
-    for (int n = threadIdx.x; n < QB * (Dp / 4); n += blockDim.x) {
+    for (int n = threadIdx.x; n < QB * (Dp / 4); n += 64 * WAVES) {
         const int qr = n / (Dp / 4), ch = 4 * (n % (Dp / 4)), r = u.r0 + qr;
         if (r >= u.R) break;
         const float* at = lds + qr * kPitch + ch;
         const float* ml = lds + QB * kPitch + qr;
-        float top = -INFINITY;
-        for (int w = 0; w < waves; ++w) top = fmaxf(top, ml[w * step]);
+        float m[WAVES], l[WAVES], top = -INFINITY;
+        f32x4_t o[WAVES];
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            m[w] = ml[w * step];
+            l[w] = ml[w * step + QB];
+            o[w] = *reinterpret_cast<const f32x4_t*>(at + w * step);
+        }
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, m[w]);
         const float ref = top == -INFINITY ? 0.0f : top;
         f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
         float weight = 0.0f;
-        for (int w = 0; w < waves; ++w) {
-            const float f = exp2_(ml[w * step] - ref);
-            weight += ml[w * step + QB] * f;
-            sum += *reinterpret_cast<const f32x4_t*>(at + w * step) * f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float f = exp2_(m[w] - ref);
+            weight += l[w] * f;
+            sum += o[w] * f;
         }
-        const int64_t row = static_cast<int64_t>(u.lo + r / u.G) * late->heads + u.h * u.G + r % u.G;
+        const int64_t row = u.out_row(r, late->heads);
         if (u.splits == 1) {
             store_row(late->out + row * D, ch, D, sum, weight, late->vec_out);
         } else {
@@ -681,13 +708,15 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
     float* sums = reinterpret_cast<float*>(attn_lds);
     z.put(sums + wave * sums_floats<KS, NQ>());
     __syncthreads();
-    join_waves<KS, NQ>(sums, late, u, D, NW);
+    if constexpr (KS <= 4)
+        if (NW == 8) return join_waves<KS, NQ, 8>(sums, late, u, D);
+    join_waves<KS, NQ, 4>(sums, late, u, D);
 }
 
-// Joins the splits of a sequence's rows, in order of position: a workgroup
-// takes 16 (new token, query head) rows of one kv head, a wave one at a time.
+// Joins the splits of a sequence's rows, in order of position: a wave takes one
+// (new token, query head) row of a kv head.
 __global__ __launch_bounds__(256) void kv_attn_join_kernel(AttnArgs a) {
-    const int H = a.c.heads, G = a.heads / H, D = a.c.D, Dp = a.c.Dp(), h = blockIdx.x;
+    const int G = a.group, D = a.c.D, Dp = a.c.Dp(), h = blockIdx.x;
     int lane_lo = 0, lane_T = 0, lane_L = 0;
     const KvUnit u = kv_find_unit(blockIdx.y + blockIdx.z * gridDim.y, a.n_seqs, [&](int s) {
         const KvRows r = kv_rows(a.offsets, s, a.capacity);
@@ -703,41 +732,39 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(AttnArgs a) {
     const int lane = threadIdx.x & 63;
     // lanes that share the splits of 4 channels
     const int share = Dp <= 64 ? 4 : Dp <= 128 ? 2 : 1, ch = 4 * (lane & (64 / share - 1)), first = lane / (64 / share);
-    for (int i = threadIdx.x >> 6; i < kJoinRows; i += 4) {
-        const int r = u.nth * kJoinRows + i;
-        if (r >= R) return;
-        const int64_t row = static_cast<int64_t>(lo + r / G) * a.heads + h * G + r % G, part = row * a.splits;
-        const float* from = a.ws_o + part * Dp + min(ch, Dp - 4);
-        const float m = lane < splits ? a.ws_ml[2 * (part + lane)] : -INFINITY;
-        const float l = lane < splits ? a.ws_ml[2 * (part + lane) + 1] : 0.0f;
-        float f = 0.0f, weight = 0.0f;
-        f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-        for (int s0 = 0; s0 < splits; s0 += 8 * share) {
-            f32x4_t y[8];  // eight splits a lane in flight; past the last one, that again, unused
+    const int r = u.nth * kJoinRows + (threadIdx.x >> 6);
+    if (r >= R) return;
+    const int64_t row = static_cast<int64_t>(lo + r / G) * a.heads + h * G + r % G, part = row * a.splits;
+    const float* from = a.ws_o + part * Dp + min(ch, Dp - 4);
+    const float m = lane < splits ? a.ws_ml[2 * (part + lane)] : -INFINITY;
+    const float l = lane < splits ? a.ws_ml[2 * (part + lane) + 1] : 0.0f;
+    float f = 0.0f, weight = 0.0f;
+    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < splits; s0 += 8 * share) {
+        f32x4_t y[8];  // eight splits a lane in flight; past the last one, that again, unused
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                y[k] = *reinterpret_cast<const f32x4_t*>(from + min(s0 + k * share + first, splits - 1) * Dp);
-            if (s0 == 0) {
-                float top = m;
-                for (int s = 32; s; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
-                f = exp2_(m - (top == -INFINITY ? 0.0f : top));
-                weight = l * f;
-                for (int s = 32; s; s >>= 1) weight += __shfl_xor(weight, s, 64);
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int s = s0 + k * share + first;
-                const float fs = __shfl(f, s & 63, 64);
-                if (s < splits) sum += y[k] * fs;
-            }
+        for (int k = 0; k < 8; ++k)
+            y[k] = *reinterpret_cast<const f32x4_t*>(from + min(s0 + k * share + first, splits - 1) * Dp);
+        if (s0 == 0) {
+            float top = m;
+            for (int s = 32; s; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+            f = exp2_(m - (top == -INFINITY ? 0.0f : top));
+            weight = l * f;
+            for (int s = 32; s; s >>= 1) weight += __shfl_xor(weight, s, 64);
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (share >= 2) sum[j] += __shfl_xor(sum[j], 32, 64);
-            if (share == 4) sum[j] += __shfl_xor(sum[j], 16, 64);
+        for (int k = 0; k < 8; ++k) {
+            const int s = s0 + k * share + first;
+            const float fs = __shfl(f, s & 63, 64);
+            if (s < splits) sum += y[k] * fs;
         }
-        if (first == 0) store_row(a.out + row * D, ch, D, sum, weight, a.vec_out);
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (share >= 2) sum[j] += __shfl_xor(sum[j], 32, 64);
+        if (share == 4) sum[j] += __shfl_xor(sum[j], 16, 64);
+    }
+    if (first == 0) store_row(a.out + row * D, ch, D, sum, weight, a.vec_out);
 }
 
 // How a call is laid out: query tiles of a wave, waves of a workgroup,
@@ -841,7 +868,7 @@ int lhq_kv_attn_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k_new,
     LHQ_REQUIRE(q && offsets && lengths && out, "%s: null pointer", fn);
     auto odd = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; };
     AttnArgs a{q,        q_stride, k_new,  k_stride,     v_new,   v_stride, tree, offsets, lengths, c, out,
-               n_seqs, row_capacity, max_new, n_heads,  scale * 1.4426950408889634f};
+               n_seqs, row_capacity, max_new, n_heads, n_heads / n_kv_heads, scale * 1.4426950408889634f};
     if (num_pages == 0) a.c.max_pages = 0;  // (no page to stand in for a missing one)
     a.vec_out = head_dim % 4 == 0 && !odd(out, 8);
     const Plan p = make_plan(n_seqs, row_capacity, max_new, max_pages, n_heads, n_kv_heads, head_dim,
