@@ -664,13 +664,17 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
         for (int i = 0; i < CT; ++i) v[i] = *reinterpret_cast<const u32x4_t*>(values + 1024 * i + 64 * c + 16 * g);
-        __builtin_amdgcn_sched_barrier(0);  // (all reads ahead of the products)
-        score<KS, NQ, FP8>(k, q, z.x);
         const int next = it + 1 < mine ? page_id(it + 1) : -1;
         if (it + 1 < mine) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (this page has been read)
             load_page(max(next, 0));
         }
+        __builtin_amdgcn_sched_barrier(0);
+        // The SIMD's other wave is kept off the matrix cores until this one's product is through: left
+        // alone the two run every product and every softmax at the same time, one unit idle in turn.
+        __builtin_amdgcn_s_setprio(2);
+        score<KS, NQ, FP8>(k, q, z.x);
+        __builtin_amdgcn_s_setprio(0);
         if (left < kKvPage) {
             z.cut(left);
 #pragma unroll
@@ -687,6 +691,7 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
             f[t] = *reinterpret_cast<const f32x4_t*>(factors + 64 + 16 * t + 4 * g);
         }
         z.weigh(k2, f, w);
+        __builtin_amdgcn_s_setprio(2);
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -696,6 +701,7 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) z.o[n][i] = mfma_f16_16x16x32(val, w[n][s], z.o[n][i]);
             }
+        __builtin_amdgcn_s_setprio(0);
         page = next;
     }
 
@@ -767,8 +773,8 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(AttnArgs a) {
     if (first == 0) store_row(a.out + row * D, ch, D, sum, weight, a.vec_out);
 }
 
-// How a call is laid out: query tiles of a wave, waves of a workgroup,
-// splits of a sequence, workgroups.
+// How a call is laid out: query tiles of a wave, waves of a workgroup, splits
+// of a sequence, workgroups.
 struct Plan {
     int tiles, waves, pages_per_split, splits;
     int64_t units, join_units;  // per kv head
@@ -779,24 +785,54 @@ int64_t unit_bound(int n_seqs, int capacity, int max_new, int G, int block) {
     return std::min(static_cast<int64_t>(capacity) * G / block + seqs,
                     seqs * ((static_cast<int64_t>(max_new) * G + block - 1) / block));
 }
+// Splits and waves by an estimate of the time, in us, from what small calls
+// measured.  For each 32 channels a workgroup costs 1.5 (one tile of queries)
+// or 2 to set up and to finish, a page of a wave 0.45 or 1; 0.6 of that where
+// it has a SIMD for itself, 1.1 of two tiles in workgroups of eight waves, which
+// are in step with one another.  Splitting adds the launch that joins, 4.5 and
+// 0.075 a split, and the parts' way through memory.  2048 waves are resident (1024 with over 128 channels).
+// The host knows the longest length there may be, not the lengths: the estimate
+// is that of all sequences having that and that of three tenths of the work
+// being there (ragged lengths), added.  Measured: decode of 4 x 4096 tokens in 8
+// splits 14.6 us, in one 19.4; of 16 x 2048 in one 19.2, in two 21.7; trees of
+// 12 over 2500 ragged tokens in 3 or 5 splits 24, in one 31; trees of 64 over 4 x
+// 8192 in one 97, in two 116.
 Plan make_plan(int n_seqs, int capacity, int max_new, int max_pages, int heads, int kv_heads, int D, int64_t ws_bytes) {
     const int G = heads / kv_heads, KS = kv_padded(D) / 32;
     Plan p{};
-    const int R = max_new * G, most = KS <= 4 ? 8 : 4;
-    p.tiles = R <= 16 ? 1 : 2;
-    const int kTargetGroups = tuning_knob("LHQ_KV_TARGET", 512), kLeastPages = tuning_knob("LHQ_KV_LEAST", 16);
+    p.tiles = max_new * G <= 16 ? 1 : 2;
     p.units = unit_bound(n_seqs, capacity, max_new, G, 16 * p.tiles);
     p.join_units = unit_bound(n_seqs, capacity, max_new, G, kJoinRows);
-    const int64_t groups = std::max<int64_t>(1, p.units * kv_heads), rows = static_cast<int64_t>(capacity) * heads;
-    int64_t splits = std::min<int64_t>({(kTargetGroups + groups - 1) / groups, max_pages / kLeastPages, kMostSplits});
-    for (splits = std::max<int64_t>(splits, 1);; --splits) {
-        p.ml_bytes = splits == 1 ? 0 : (rows * splits * 8 + 15) / 16 * 16;
-        p.bytes = splits == 1 ? 0 : p.ml_bytes + rows * splits * 32 * KS * 4;
-        if (p.bytes <= ws_bytes) break;
-    }
-    p.pages_per_split = std::max<int>(1, (max_pages + splits - 1) / splits);
-    p.splits = static_cast<int>(splits);
-    p.waves = groups * splits <= 256 ? most : 4;
+    const int64_t units = std::max<int64_t>(1, p.units * kv_heads), rows = static_cast<int64_t>(capacity) * heads;
+    const int64_t resident = KS <= 4 ? 2048 : 1024;
+    const double ends = (p.tiles == 1 ? 1.5 : 2.0) * KS, page = (p.tiles == 1 ? 0.45 : 1.0) * KS;
+    double best = HUGE_VAL;
+    auto consider = [&](int64_t want) {
+        const int per = std::max<int>(1, (max_pages + want - 1) / want), splits = std::max(1, (max_pages + per - 1) / per);
+        const int64_t ml_bytes = splits == 1 ? 0 : (rows * splits * 8 + 15) / 16 * 16;
+        const int64_t bytes = splits == 1 ? 0 : ml_bytes + rows * splits * 32 * KS * 4;
+        if (bytes > ws_bytes) return;
+        const int64_t groups = units * splits, some = n_seqs > 1 ? std::max<int64_t>(1, groups * 3 / 10) : groups;
+        for (int waves = 4; waves <= (KS <= 4 ? 8 : 4); waves += 4) {
+            const int64_t slots = resident / waves;
+            auto time = [&](int64_t n) {
+                const double share = waves == 8 ? (p.tiles == 1 ? 1.0 : 1.1) : KS <= 4 && n <= slots / 2 ? 0.6 : 1.0;
+                return static_cast<double>((n + slots - 1) / slots) * (ends + (per + waves - 1) / waves * page * share);
+            };
+            const double cost = time(groups) + time(some) + (splits > 1 ? 9.0 + 0.15 * splits + static_cast<double>(bytes) * 0.5e-6 : 0.0);
+            if (cost >= best) continue;
+            best = cost;
+            p.waves = waves;
+            p.splits = splits;
+            p.pages_per_split = per;
+            p.ml_bytes = ml_bytes;
+            p.bytes = bytes;
+        }
+    };
+    for (int n : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, kMostSplits})
+        if (n == 1 || n <= max_pages) consider(n);
+    for (int64_t slots : {resident / 4, resident / 8})  // as many as are resident
+        if (slots / units > 1) consider(std::min<int64_t>(slots / units, kMostSplits));
     return p;
 }
 
