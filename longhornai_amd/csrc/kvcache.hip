@@ -17,36 +17,39 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Eight elements of a row as fp32, elements from `left` on as zero.  VEC: rows
-// are 16-byte aligned and head_dim is a multiple of 8.
+// Eight elements of a row from channel d on as fp32, those past D as zero.
+// VEC: rows are 16-byte aligned and D is a multiple of 8.  No branch: loads of
+// several rows stay in flight together.
 template <bool VEC>
-__device__ __forceinline__ void load8(const float* p, int left, float (&x)[8]) {
+__device__ __forceinline__ void load8(const float* row, int d, int D, float (&x)[8]) {
     if constexpr (VEC) {
-        f32x4_t a = {0.f, 0.f, 0.f, 0.f}, b = a;
-        if (left > 0) {
-            a = *reinterpret_cast<const f32x4_t*>(p);
-            b = *reinterpret_cast<const f32x4_t*>(p + 4);
-        }
+        const float* p = row + (d < D ? d : 0);
+        const f32x4_t a = *reinterpret_cast<const f32x4_t*>(p), b = *reinterpret_cast<const f32x4_t*>(p + 4);
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = a[j], x[4 + j] = b[j];
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = j < left ? p[j] : 0.0f;
+        for (int j = 0; j < 8; ++j) x[j] = row[min(d + j, D - 1)];
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = d + (VEC ? 0 : j) < D ? x[j] : 0.0f;
 }
 template <bool VEC>
-__device__ __forceinline__ void load8(const uint16_t* p, int left, float (&x)[8]) {
+__device__ __forceinline__ void load8(const uint16_t* row, int d, int D, float (&x)[8]) {
     if constexpr (VEC) {
-        u32x4_t w = {0, 0, 0, 0};
-        if (left > 0) w = *reinterpret_cast<const u32x4_t*>(p);
+        u32x4_t w = *reinterpret_cast<const u32x4_t*>(row + (d < D ? d : 0));
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            if (d >= D) w[j] = 0;
             x[2 * j] = __uint_as_float(w[j] << 16);
             x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
         }
     } else {
+        uint16_t y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = j < left ? bf16_to_f32(p[j]) : 0.0f;
+        for (int j = 0; j < 8; ++j) y[j] = row[min(d + j, D - 1)];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = d + j < D ? bf16_to_f32(y[j]) : 0.0f;
     }
 }
 template <bool VEC>
@@ -75,7 +78,8 @@ __device__ __forceinline__ void store8(uint16_t* p, int left, const float (&x)[8
     }
 }
 
-// Codes of eight values with scale and reciprocal of a row whose maximum is m.
+// Codes of eight values with scale and reciprocal of a row whose maximum is m,
+// whatever the row holds.
 template <bool FP8>
 __device__ __forceinline__ u32x2_t quant8(const float (&x)[8], float m, float& scale) {
     scale = m > 0.0f ? m / (FP8 ? 448.0f : 127.0f) : 1.0f;
@@ -93,11 +97,22 @@ __device__ __forceinline__ u32x2_t quant8(const float (&x)[8], float m, float& s
     }
     return w;
 }
+// The values of eight codes, times their scale.
 template <bool FP8>
-__device__ __forceinline__ float code_value(uint32_t w, int j) {
-    const uint8_t b = static_cast<uint8_t>(w >> (8 * j));
-    if constexpr (FP8) return e4m3_to_f32(b);
-    else return static_cast<float>(static_cast<int8_t>(b));
+__device__ __forceinline__ void values8(u32x2_t w, float scale, float (&x)[8]) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        if constexpr (FP8) {
+            const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], true);
+            x[4 * j] = lo[0] * scale;
+            x[4 * j + 1] = lo[1] * scale;
+            x[4 * j + 2] = hi[0] * scale;
+            x[4 * j + 3] = hi[1] * scale;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[4 * j + i] = static_cast<float>(static_cast<int8_t>(w[j] >> (8 * i))) * scale;
+        }
+    }
 }
 
 // Pages that n tokens from position `start` on touch.
@@ -111,7 +126,7 @@ struct Tile { int seq, t0, t1; int64_t p, row0; };
 __device__ __forceinline__ Tile find_tile(const int32_t* offsets, const int32_t* start, int n_seqs, int capacity) {
     KvRows mine{0, 0};
     int mine_start = 0;
-    const KvUnit u = kv_find_unit(blockIdx.x, n_seqs, [&](int s) {
+    const KvUnit u = kv_find_unit(blockIdx.y + blockIdx.z * gridDim.y, n_seqs, [&](int s) {
         mine = kv_rows(offsets, s, capacity);
         mine_start = start[s];
         return tile_count(mine_start, mine.hi - mine.lo);
@@ -123,11 +138,79 @@ __device__ __forceinline__ Tile find_tile(const int32_t* offsets, const int32_t*
     return {u.seq, static_cast<int>(max<int64_t>(a, 0)), static_cast<int>(min<int64_t>(b, kKvPage)), p, lo - a};
 }
 
+// Maximum over 1 << LB adjacent lanes (8, 16 or 32), the same in all of them.
+template <int LB, typename T, typename Max>
+__device__ __forceinline__ T row_max(T m, Max max_of) {
+#define LHQ_MAX_STEP(ctrl)                                                                               \
+    m = max_of(m, __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, m), ctrl, \
+                                                                    0xf, 0xf, false)))
+    LHQ_MAX_STEP(0xB1);   // quad_perm 1, 0, 3, 2
+    LHQ_MAX_STEP(0x4E);   // quad_perm 2, 3, 0, 1
+    LHQ_MAX_STEP(0x141);  // row_half_mirror: the other quad of 8 lanes
+    if constexpr (LB >= 4) LHQ_MAX_STEP(0x140);  // row_mirror: the other half of 16
+#undef LHQ_MAX_STEP
+    if constexpr (LB >= 5) m = max_of(m, __shfl_xor(m, 16, 64));
+    return m;
+}
+__device__ __forceinline__ uint32_t magnitude(const float (&x)[8]) {  // bits of max |x|; NaN is over infinity
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+    return m;
+}
+// The same codes as quant8 for a row of finite values whose reciprocal scale is
+// finite: nothing saturates (the largest value is within a rounding of 127 or
+// 448), so int8 takes the low byte of the sum with 1.5 * 2^23, whose last bit
+// is 1, and e4m3 the conversion of values that are quartered below 2^-9.
+template <bool FP8>
+__device__ __forceinline__ u32x2_t quant8_plain(const float (&x)[8], float inv) {
+    u32x2_t w;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            y[i] = x[4 * j + i] * inv;
+            if constexpr (FP8) y[i] *= fabsf(y[i]) < 0x1p-9f ? 0.25f : 1.0f;
+            else y[i] += 12582912.0f;
+        }
+        if constexpr (FP8) {
+            const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+            w[j] = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true));
+        } else {
+            const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(y[1]), __float_as_uint(y[0]), 0x0c0c0400u);
+            const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(y[3]), __float_as_uint(y[2]), 0x04000c0cu);
+            w[j] = lo | hi;
+        }
+    }
+    return w;
+}
+template <int CTRL>
+__device__ __forceinline__ float quad(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
+}
+
+// Four dwords of four bytes, turned: byte j of out[i] is byte i of in[j].
+__device__ __forceinline__ void turn4(const uint32_t (&in)[4], uint32_t (&out)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(in[1], in[0], 0x05010400u), b = __builtin_amdgcn_perm(in[3], in[2], 0x05010400u);
+    const uint32_t c = __builtin_amdgcn_perm(in[1], in[0], 0x07030602u), d = __builtin_amdgcn_perm(in[3], in[2], 0x07030602u);
+    out[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    out[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    out[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+    out[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+}
+// A page's value codes in LDS: [token][kPitch bytes].  The turn between tokens
+// and channels reads and writes it in dwords, a lane group g at tokens 4 g on:
+// 16 dwords over a multiple of 64 keeps the four groups on banks of their own.
+template <int LB>
+constexpr int kValuePitch = (8 << LB) + 16;
+
 // Write: one workgroup per (tile, head).  1 << LB lanes (eight channels each)
-// take a token: row maximum by shuffles, key codes straight to the token's
-// row, value codes to LDS as [token][Dp]; then the value tile leaves
-// transposed, 16 bytes a lane where a lane's 16 tokens are all new, else four
-// tokens or one at a time (bytes of other tokens are never touched).
+// take a token, up to four tokens of theirs in flight: row maximum across
+// lanes, key codes straight to the token's row, value codes to LDS; then the
+// value tile leaves turned, four channels of 16 tokens a lane, 16 bytes at a
+// time where those tokens are all new, else four tokens or one at a time
+// (bytes of other tokens are never touched).
 template <typename T, bool FP8, int LB, bool VEC>
 __global__ __launch_bounds__(kThreads) void kv_write_kernel(const T* __restrict__ k, const T* __restrict__ v,
                                                             int64_t k_stride, int64_t v_stride,
@@ -135,74 +218,106 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(const T* __restrict_
                                                             const int32_t* __restrict__ offsets,
                                                             const int32_t* __restrict__ start, KvCache c, int n_seqs,
                                                             int n_rows, int capacity) {
-    constexpr int kPitch = (8 << LB) + 4;
-    __shared__ uint32_t vt[kKvPage * kPitch / 4];
+    constexpr int kPitch = kValuePitch<LB>, kPer = kThreads >> LB, kPasses = kKvPage / kPer < 4 ? kKvPage / kPer : 4;
+    __shared__ __attribute__((aligned(16))) uint32_t vt[kKvPage * kPitch / 4];
     __shared__ int ok[kKvPage];
     const Tile tile = find_tile(offsets, start, n_seqs, capacity);
     if (tile.seq >= n_seqs) return;
     const int page = c.page(tile.seq, tile.p);
     if (page < 0) return;  // nowhere to write: dropped
-    const int h = blockIdx.y, Dp = c.Dp();
+    const int h = blockIdx.x, Dp = c.Dp();
     const int64_t cb = c.code_base(page, h), sb = c.scale_base(page, h);
     if (threadIdx.x < kKvPage) ok[threadIdx.x] = 0;
     __syncthreads();
     const int d = (threadIdx.x & ((1 << LB) - 1)) * 8;
-    for (int t = tile.t0 + (threadIdx.x >> LB); t < tile.t1; t += kThreads >> LB) {
-        int64_t row = tile.row0 + t;
-        if (rows) row = rows[row];
-        const bool in = row >= 0 && row < n_rows;  // (the same for all of a token's lanes)
-        if (!in) continue;
-        float x[8], y[8];
-        load8<VEC>(k + row * k_stride + h * c.D + d, c.D - d, x);
-        load8<VEC>(v + row * v_stride + h * c.D + d, c.D - d, y);
-        float mk = 0.0f, mv = 0.0f;
-        auto amax = [](float m, float a) { return a > m ? a : m; };
+    for (int t0 = tile.t0; t0 < tile.t1; t0 += kPasses * kPer) {
+        float x[kPasses][8], y[kPasses][8];
+        bool in[kPasses];  // (the same for all of a token's lanes)
+        int64_t row[kPasses];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) mk = amax(mk, fabsf(x[j])), mv = amax(mv, fabsf(y[j]));
-#pragma unroll
-        for (int o = 1; o < (1 << LB); o <<= 1) {
-            mk = amax(mk, __shfl_xor(mk, o, 64));
-            mv = amax(mv, __shfl_xor(mv, o, 64));
+        for (int i = 0; i < kPasses; ++i) {
+            const int t = t0 + i * kPer + (threadIdx.x >> LB);
+            row[i] = tile.row0 + min(t, tile.t1 - 1);
+            if (rows) row[i] = rows[row[i]];
+            in[i] = t < tile.t1 && row[i] >= 0 && row[i] < n_rows;
+            if (!in[i]) row[i] = 0;
         }
-        float sk, sv;
-        const u32x2_t wk = quant8<FP8>(x, mk, sk), wv = quant8<FP8>(y, mv, sv);
-        if (d < Dp) *reinterpret_cast<u32x2_t*>(c.k + cb + t * Dp + d) = wk;
-        vt[(t * kPitch + d) / 4] = wv[0];
-        vt[(t * kPitch + d) / 4 + 1] = wv[1];
-        if (d == 0) {
-            c.ks[sb + t] = sk;
-            c.vs[sb + t] = sv;
-            ok[t] = 1;
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            load8<VEC>(k + row[i] * k_stride + h * c.D, d, c.D, x[i]);
+            load8<VEC>(v + row[i] * v_stride + h * c.D, d, c.D, y[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            if (t0 + i * kPer >= tile.t1) break;
+            const int t = t0 + i * kPer + (threadIdx.x >> LB);
+            u32x2_t wk, wv;
+            float sk, sv;
+            auto umax = [](uint32_t m, uint32_t n) { return max(m, n); };
+            const uint32_t bk = row_max<LB>(magnitude(x[i]), umax), bv = row_max<LB>(magnitude(y[i]), umax);
+            // (from 2^-100 on, and of zeros, the scale's reciprocal is finite)
+            auto plain = [](uint32_t m) { return m - 0x0d800000u < 0x7f800000u - 0x0d800000u || m == 0; };
+            if (__ballot(!plain(bk) || !plain(bv)) == 0) {
+                // Even lanes divide for the keys, odd ones for the values.
+                const float m = __uint_as_float(threadIdx.x & 1 ? bv : bk);
+                const float scale = m > 0.0f ? m / (FP8 ? 448.0f : 127.0f) : 1.0f, inv = 1.0f / scale;
+                sk = quad<0xA0>(scale);  // quad_perm 0, 0, 2, 2
+                sv = quad<0xF5>(scale);  // quad_perm 1, 1, 3, 3
+                wk = quant8_plain<FP8>(x[i], quad<0xA0>(inv));
+                wv = quant8_plain<FP8>(y[i], quad<0xF5>(inv));
+            } else {
+                float mk = 0.0f, mv = 0.0f;
+                auto amax = [](float m, float a) { return a > m ? a : m; };  // NaN never wins
+#pragma unroll
+                for (int j = 0; j < 8; ++j) mk = amax(mk, fabsf(x[i][j])), mv = amax(mv, fabsf(y[i][j]));
+                wk = quant8<FP8>(x[i], row_max<LB>(mk, amax), sk);
+                wv = quant8<FP8>(y[i], row_max<LB>(mv, amax), sv);
+            }
+            if (!in[i]) continue;
+            if (d < Dp) *reinterpret_cast<u32x2_t*>(c.k + cb + t * Dp + d) = wk;
+            *reinterpret_cast<u32x2_t*>(vt + (t * kPitch + d) / 4) = wv;
+            if (d == 0) {
+                c.ks[sb + t] = sk;
+                c.vs[sb + t] = sv;
+                ok[t] = 1;
+            }
         }
     }
     __syncthreads();
     const uint64_t written = __ballot(ok[threadIdx.x & 63] != 0);
-    const uint8_t* vb = reinterpret_cast<const uint8_t*>(vt);
-    for (int i = threadIdx.x; i < Dp * 4; i += kThreads) {
-        const int g = i & 3, dd = i >> 2;
+    for (int i = threadIdx.x; i < Dp; i += kThreads) {
+        const int g = i & 3, dd = 4 * (i >> 2);
         uint8_t* out = c.v + cb + static_cast<int64_t>(dd) * kKvPage + 16 * g;
-        u32x4_t w;
+        u32x4_t w[4];
         uint32_t full = 0;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {  // q = 2s + h: tokens 16q + 4g + r
             const int t = 16 * q + 4 * g;
-            w[q] = 0;
+            uint32_t by_token[4], by_channel[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) w[q] |= static_cast<uint32_t>(vb[(t + r) * kPitch + dd]) << (8 * r);
+            for (int r = 0; r < 4; ++r) by_token[r] = vt[((t + r) * kPitch + dd) / 4];
+            turn4(by_token, by_channel);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j][q] = by_channel[j];
             full |= (((written >> t) & 15) == 15 ? 1u : 0u) << q;
         }
         if (full == 15) {
-            *reinterpret_cast<u32x4_t*>(out) = w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4_t*>(out + j * kKvPage) = w[j];
         } else {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int t = 16 * q + 4 * g;
-                if ((full >> q) & 1) {
-                    *reinterpret_cast<uint32_t*>(out + 4 * q) = w[q];
-                } else {
+                const uint32_t some = (written >> (16 * q + 4 * g)) & 15;
+                if (some == 15) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint32_t*>(out + j * kKvPage + 4 * q) = w[j][q];
+                } else if (some != 0) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        if ((written >> (t + r)) & 1) out[4 * q + r] = static_cast<uint8_t>(w[q] >> (8 * r));
+                        if ((some >> r) & 1)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                out[j * kKvPage + 4 * q + r] = static_cast<uint8_t>(w[j][q] >> (8 * r));
                 }
             }
         }
@@ -210,48 +325,66 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(const T* __restrict_
 }
 
 // Read: one workgroup per (tile, head): x = code * scale, rounded once to the
-// output type; the value tile is turned in LDS.  A position without a page
-// reads as zero.
+// output type; the value tile is turned in LDS while the keys are on their
+// way.  A position without a page reads as zero.
 template <typename T, bool FP8, int LB, bool VEC>
 __global__ __launch_bounds__(kThreads) void kv_read_kernel(KvCache c, const int32_t* __restrict__ offsets,
                                                            const int32_t* __restrict__ start, T* __restrict__ k_out,
                                                            T* __restrict__ v_out, int n_seqs, int capacity) {
-    constexpr int kPitch = (8 << LB) + 4;
-    __shared__ uint32_t vt[kKvPage * kPitch / 4];
+    constexpr int kPitch = kValuePitch<LB>, kPer = kThreads >> LB, kPasses = kKvPage / kPer < 4 ? kKvPage / kPer : 4;
+    __shared__ __attribute__((aligned(16))) uint32_t vt[kKvPage * kPitch / 4];
     const Tile tile = find_tile(offsets, start, n_seqs, capacity);
     if (tile.seq >= n_seqs) return;
     const int page = c.page(tile.seq, tile.p);
-    const int h = blockIdx.y, Dp = c.Dp();
+    const int h = blockIdx.x, Dp = c.Dp();
     const int64_t cb = c.code_base(max(page, 0), h), sb = c.scale_base(max(page, 0), h);
-    uint8_t* vb = reinterpret_cast<uint8_t*>(vt);
+    const int d = (threadIdx.x & ((1 << LB) - 1)) * 8;
+    u32x2_t wk[kPasses];
+    float sk[kPasses], sv[kPasses];
+    auto load_keys = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const int t = min(t0 + i * kPer + static_cast<int>(threadIdx.x >> LB), kKvPage - 1);
+            wk[i] = *reinterpret_cast<const u32x2_t*>(c.k + cb + t * Dp + (d < Dp ? d : 0));
+            sk[i] = c.ks[sb + t];
+            sv[i] = c.vs[sb + t];
+        }
+    };
     if (page >= 0) {
-        for (int i = threadIdx.x; i < Dp * 4; i += kThreads) {
-            const int g = i & 3, dd = i >> 2;
-            const u32x4_t w = *reinterpret_cast<const u32x4_t*>(c.v + cb + static_cast<int64_t>(dd) * kKvPage + 16 * g);
+        load_keys(tile.t0);
+        for (int i = threadIdx.x; i < Dp; i += kThreads) {
+            const int g = i & 3, dd = 4 * (i >> 2);
+            const uint8_t* from = c.v + cb + static_cast<int64_t>(dd) * kKvPage + 16 * g;
+            u32x4_t w[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+            for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const u32x4_t*>(from + j * kKvPage);
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    vb[(16 * q + 4 * g + r) * kPitch + dd] = static_cast<uint8_t>(w[q] >> (8 * r));
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t by_channel[4] = {w[0][q], w[1][q], w[2][q], w[3][q]};
+                uint32_t by_token[4];
+                turn4(by_channel, by_token);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) vt[((16 * q + 4 * g + r) * kPitch + dd) / 4] = by_token[r];
+            }
         }
     }
     __syncthreads();
-    const int d = (threadIdx.x & ((1 << LB) - 1)) * 8;
     if (d >= c.D) return;
-    for (int t = tile.t0 + (threadIdx.x >> LB); t < tile.t1; t += kThreads >> LB) {
-        const int64_t at = ((tile.row0 + t) * c.heads + h) * c.D + d;
-        float x[8] = {}, y[8] = {};
-        if (page >= 0) {
-            const u32x2_t wk = *reinterpret_cast<const u32x2_t*>(c.k + cb + t * Dp + d);
-            const float sk = c.ks[sb + t], sv = c.vs[sb + t];
+    for (int t0 = tile.t0; t0 < tile.t1; t0 += kPasses * kPer) {
+        if (page >= 0 && t0 > tile.t0) load_keys(t0);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[j] = code_value<FP8>(wk[j / 4], j & 3) * sk;
-                y[j] = code_value<FP8>(vt[(t * kPitch + d) / 4 + j / 4], j & 3) * sv;
+        for (int i = 0; i < kPasses; ++i) {
+            const int t = t0 + i * kPer + (threadIdx.x >> LB);
+            if (t >= tile.t1) break;
+            const int64_t at = ((tile.row0 + t) * c.heads + h) * c.D + d;
+            float x[8] = {}, y[8] = {};
+            if (page >= 0) {
+                values8<FP8>(wk[i], sk[i], x);
+                values8<FP8>(*reinterpret_cast<const u32x2_t*>(vt + (t * kPitch + d) / 4), sv[i], y);
             }
+            store8<VEC>(k_out + at, c.D - d, x);
+            store8<VEC>(v_out + at, c.D - d, y);
         }
-        store8<VEC>(k_out + at, c.D - d, x);
-        store8<VEC>(v_out + at, c.D - d, y);
     }
 }
 
@@ -261,6 +394,13 @@ unsigned tile_bound(int n_seqs, int capacity) {
     const int64_t seqs = std::min(n_seqs, capacity);
     const int64_t most = (static_cast<int64_t>(capacity) + 62 * seqs) / kKvPage + seqs;
     return static_cast<unsigned>(std::min<int64_t>(most, capacity));
+}
+
+// Heads, tiles: blockIdx.y + blockIdx.z * gridDim.y.  Workgroups that start
+// together have the heads of a token, whose rows lie side by side.
+dim3 tile_grid(int n_seqs, int capacity, int heads) {
+    const unsigned tiles = tile_bound(n_seqs, capacity), y = std::min(tiles, 32768u);
+    return dim3(heads, y, (tiles + y - 1) / y);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -292,7 +432,7 @@ int kv_write(const char* fn, const T* k, const T* v, int64_t k_stride, int64_t v
     LHQ_REQUIRE(k && v && offsets && start, "%s: null pointer", fn);
     constexpr int kPer16 = 16 / sizeof(T);
     const bool vec = c.D % 8 == 0 && aligned16(k) && aligned16(v) && k_stride % kPer16 == 0 && v_stride % kPer16 == 0;
-    const dim3 grid(tile_bound(n_seqs, capacity), c.heads);
+    const dim3 grid = tile_grid(n_seqs, capacity, c.heads);
     by_row(c.D, vec, [&](auto lb, auto ve) {
         auto launch = [&](auto fp8) {
             kv_write_kernel<T, fp8(), lb(), ve()><<<grid, kThreads, 0, as_stream(stream)>>>(
@@ -312,7 +452,7 @@ int kv_read(const char* fn, const KvCache& c, const int32_t* offsets, const int3
     if (int st = kv_check_pointers(fn, c)) return st;
     LHQ_REQUIRE(offsets && start && k_out && v_out, "%s: null pointer", fn);
     const bool vec = c.D % 8 == 0 && aligned16(k_out) && aligned16(v_out);
-    const dim3 grid(tile_bound(n_seqs, capacity), c.heads);
+    const dim3 grid = tile_grid(n_seqs, capacity, c.heads);
     by_row(c.D, vec, [&](auto lb, auto ve) {
         auto launch = [&](auto fp8) {
             kv_read_kernel<T, fp8(), lb(), ve()><<<grid, kThreads, 0, as_stream(stream)>>>(c, offsets, start, k_out,
