@@ -272,6 +272,11 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(const T* __restrict_
                 for (int j = 0; j < 8; ++j) mk = amax(mk, fabsf(x[i][j])), mv = amax(mv, fabsf(y[i][j]));
                 wk = quant8<FP8>(x[i], row_max<LB>(mk, amax), sk);
                 wv = quant8<FP8>(y[i], row_max<LB>(mv, amax), sv);
+                // An infinite reciprocal makes NaN of the zeros past D: their codes are zero all the same.
+                const int own = 8 * min(max(c.D - d, 0), 8);
+                const uint64_t keep = own == 64 ? ~uint64_t{0} : (uint64_t{1} << own) - 1;
+                wk &= __builtin_bit_cast(u32x2_t, keep);
+                wv &= __builtin_bit_cast(u32x2_t, keep);
             }
             if (!in[i]) continue;
             if (d < Dp) *reinterpret_cast<u32x2_t*>(c.k + cb + t * Dp + d) = wk;
