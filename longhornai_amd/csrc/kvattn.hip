@@ -171,6 +171,10 @@ __device__ __forceinline__ int key_swizzle(int r) {
     else if constexpr (KS == 8) return ((r & 1) << 2) | ((r & 2) << 2) | ((r >> 2) & 2);
     else return 0;
 }
+// The same for values, which lie as operands already (channel row c of 64 bytes,
+// lane group g's 16 at 16 g): group g's chunk of row c is in place g ^ this.
+__device__ __forceinline__ int value_swizzle(int c) { return (c >> 1) & 2; }
+
 // LDS DMA: 16 bytes a lane, from this lane's address + OFFSET to `to` + OFFSET +
 // 16 * lane.
 template <int OFFSET>
@@ -630,7 +634,8 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
             return 16 * (lane ^ key_swizzle<KS>((64 * n + lane) / (2 * KS)));
         });
         asm volatile("" ::: "memory");  // (the values last: the wait for the keys counts on it)
-        fetch<KS>(a.c.v + a.c.code_base(page, h), values, [lane](int) -> uint32_t { return 16 * lane; });
+        fetch<KS>(a.c.v + a.c.code_base(page, h), values,
+                  [lane](int) -> uint32_t { return 16 * (lane ^ value_swizzle(lane >> 2)); });
     };
     // pages p0 + wave, + NW, ...
     const int mine = u.p0 + wave < u.p1 ? (u.p1 - u.p0 - wave + NW - 1) / NW : 0;
@@ -663,7 +668,8 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
         factors[64 + lane] = z.factor(in ? vs : 0.0f);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
-        for (int i = 0; i < CT; ++i) v[i] = *reinterpret_cast<const u32x4_t*>(values + 1024 * i + 64 * c + 16 * g);
+        for (int i = 0; i < CT; ++i)
+            v[i] = *reinterpret_cast<const u32x4_t*>(values + 1024 * i + 64 * c + 16 * (g ^ value_swizzle(c)));
         const int next = it + 1 < mine ? page_id(it + 1) : -1;
         if (it + 1 < mine) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (this page has been read)
