@@ -5,6 +5,13 @@
 // kv head: scale = max|x| / 127 (448 for e4m3), 1 for a row of zeros, code =
 // x * (1 / scale) rounded to nearest even; NaN never wins the maximum.  The
 // same IEEE operations in the same order, no multiply-add fused.
+//
+// Both ways are bound by memory from a few thousand tokens on, below that by
+// the launch and one workgroup's chain of loads.  8 x 4096 tokens of 8 heads of
+// 128, bf16 and e4m3, 203 MB each way: write 42 us (4.8 TB/s, a copy's rate),
+// read 31 us (6.4, the results partly in the last-level cache); one token of 16
+// sequences: 4 and 3 us.  Turning the value tile in bytes rather than dwords,
+// one row after the other, took 55 and 42 us.
 #include <algorithm>
 #include <type_traits>
 

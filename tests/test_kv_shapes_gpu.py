@@ -87,6 +87,24 @@ def test_equal_scores_far_from_zero(oracle, ops):
         c.check()
 
 
+def test_missing_pages_ahead_of_far_scores(oracle, ops):
+    """Waves whose first pages are missing, then scores of -180 alone."""
+    c = Case(oracle, ops, "int8", 4, 1, 32, [2500], [2], seed=8)
+    c.c.k[...] = 0
+    c.c.k[..., 0] = 127
+    c.c.ks[...] = 1.0
+    c.q[...] = 0
+    c.q[..., 0] = D.to_bf16_bits(oracle, np.array([-8.0], np.float32))[0]
+    c.k[...] = 0
+    c.k[..., 0] = D.to_bf16_bits(oracle, np.array([127.0], np.float32))[0]
+    for gone in (range(0, 9), range(0, 39), range(0, 40)):
+        table = c.table.copy()
+        c.table[0, list(gone)] = -1
+        c.check()
+        c.check(new=False) if len(gone) < 40 else None
+        c.table = table
+
+
 @pytest.mark.parametrize("fmt", ["int8", "fp8"])
 def test_nan_stays_with_the_queries_that_see_it(oracle, ops, fmt):
     """A NaN key scale, a NaN value scale and (fp8) a NaN code of tokens that
