@@ -338,7 +338,7 @@ struct Sums {
     f32x4_t o[NQ][CT], x[NQ][4];
     float m[NQ], l[NQ];
     int e;       // o is relative to 2^(e - kTop)
-    bool fresh;  // no scores so far
+    bool fresh;  // a query of the wave has no scores so far
 
     __device__ __forceinline__ void clear() {
         fresh = true;
@@ -378,10 +378,10 @@ struct Sums {
     }
     // x (products q . k), times ks the scores -> weights; times w they are the
     // operands p of the second product.  The maximum follows when a score is
-    // over it by more than kLag; the wave's first scores set it.
+    // over it by more than kLag; a query's first scores set it.
     __device__ __forceinline__ void weigh(const f32x4_t (&ks)[4], const f32x4_t (&w)[4], u32x4_t (&p)[NQ][2]) {
         if (fresh) {
-            bool any = false;
+            bool all = true;
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
                 float top = -INFINITY;
@@ -389,11 +389,12 @@ struct Sums {
                 for (int t = 0; t < 4; ++t)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) top = fmaxf(top, x[n][t][j] * ks[t][j]);
-                m[n] = across(top);
-                any |= m[n] != -INFINITY;
-                if (m[n] == -INFINITY) m[n] = 0.0f;  // (nothing seen: every weight is zero)
+                top = across(top);
+                const bool first = across(l[n]) == 0.0f;  // (a maximum's own weight is at least 2^-kLag)
+                if (first && top != -INFINITY) m[n] = top;  // (a missing page, or a mask that leaves nothing, sets nothing)
+                all &= !first || top != -INFINITY;
             }
-            fresh = !__ballot(any);  // (a missing page sets nothing)
+            fresh = __ballot(!all) != 0;
         }
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
@@ -451,8 +452,8 @@ struct Sums {
         uint32_t seen[NQ];  // of those 32
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-            const int r = u.r0 + 16 * n + c, t = u.token(min(r, u.R - 1));
-            uint64_t word = r >= u.R ? 0 : late->tree ? late->tree[u.lo + t] : ~uint64_t{0} >> (63 - t);
+            const int t = u.token(min(u.r0 + 16 * n + c, u.R - 1));
+            uint64_t word = late->tree ? late->tree[u.lo + t] : ~uint64_t{0} >> (63 - t);
             word &= ~uint64_t{0} >> (64 - u.T);
             seen[n] = static_cast<uint32_t>(word >> t0);
         }
@@ -667,9 +668,14 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
     for (int n = 0; n < NQ; ++n) load_queries<KS>(a, u, u.r0 + 16 * n, q[n]);
     Sums<KS, NQ> z;
     z.clear();
+    // The new tokens first, 32 at a time, by the waves whose turn it is after the last page (at least four waves
+    // for at most 64 tokens): their rows are fetched while the first page is on its way.  After the pages they
+    // took 1 to 3% more of every measured call, and more registers.
+    const int turn = __builtin_amdgcn_readfirstlane((wave + NW - (u.p1 - u.p0) % NW) % NW);
+    if (late_args()->k_new && u.split == u.splits - 1 && 32 * turn < u.T) z.new_tokens(late_args(), u, 32 * turn, D, q);
     for (int it = 0; it < mine; ++it) {
         const int left = page < 0 ? 0 : min(u.L - (u.p0 + wave + it * NW) * kKvPage, kKvPage);
-        // The keys have landed: the CT loads of values were issued after them.
+        // The keys have landed: at least the CT loads of values were issued after them.
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CT) : "memory");
         u32x4_t k[(KS + 1) / 2][4], v[CT], w[NQ][2];
         read_keys<KS>(keys, k);
@@ -721,11 +727,7 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
         page = next;
     }
 
-    // the new tokens, 32 at a time, by the waves whose turn it is after the last page
     const LateArgs late = late_args();
-    const int turn = __builtin_amdgcn_readfirstlane((wave + NW - (u.p1 - u.p0) % NW) % NW);  // (at least four waves for at most 64 tokens)
-    if (late->k_new && u.split == u.splits - 1 && 32 * turn < u.T) z.new_tokens(late, u, 32 * turn, D, q);
-
     __syncthreads();  // (the pages' place is taken)
     float* sums = reinterpret_cast<float*>(attn_lds);
     z.put(sums + wave * sums_floats<KS, NQ>());

@@ -105,6 +105,28 @@ def test_missing_pages_ahead_of_far_scores(oracle, ops):
         c.table = table
 
 
+@pytest.mark.parametrize("T", [1, 3, 40, 64])
+@pytest.mark.parametrize("Hq,Dh", [(1, 32), (4, 128), (3, 256)])
+def test_far_scores_of_queries_that_see_none_of_a_waves_new_tokens(oracle, ops, Hq, Dh, T):
+    """Every score -180 or 180.  Queries that see new tokens share waves with
+    some that see none of them, or none of the 32 that the wave has."""
+    for q in (-8.0, 8.0):
+        c = Case(oracle, ops, "int8", Hq, 1, Dh, [130, 700, 0], [T, T, T], seed=T)
+        c.scale = float(np.float32(32 ** -0.5))
+        c.c.k[...] = 0
+        c.c.k[..., 0] = 127
+        c.c.ks[...] = 1.0
+        c.q[...] = 0
+        c.q[..., 0] = D.to_bf16_bits(oracle, np.array([q], np.float32))[0]
+        c.k[...] = 0
+        c.k[..., 0] = D.to_bf16_bits(oracle, np.array([127.0], np.float32))[0]
+        c.check()
+        c.tree[:] = [(1 << (i % T + 1)) - 1 for i in range(3 * T)]
+        c.check()
+        c.tree[::2] = 0
+        c.check()
+
+
 @pytest.mark.parametrize("fmt", ["int8", "fp8"])
 def test_nan_stays_with_the_queries_that_see_it(oracle, ops, fmt):
     """A NaN key scale, a NaN value scale and (fp8) a NaN code of tokens that
