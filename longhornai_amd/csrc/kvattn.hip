@@ -197,16 +197,14 @@ LHQ_DMA16(1024)
 LHQ_DMA16(2048)
 LHQ_DMA16(3072)
 #undef LHQ_DMA16
-// 2 KS KiB of a page: KiB n from `from` + 1024 n + place(n) to `to` + 1024 n + 16 * lane.
+// KiB 4 part .. 4 part + 3 of a page's 2 KS: KiB n from `from` + 1024 n + place(n) to `to` + 1024 n + 16 * lane.
 template <int KS, typename Place>
-__device__ __forceinline__ void fetch(const uint8_t* from, uint8_t* to, Place place) {
-#pragma unroll
-    for (int n = 0; n < 2 * KS; n += 4) {  // (four of them with one address on either side)
-        dma16<0>(from + 1024 * n + place(n), to + 1024 * n);
-        dma16<1024>(from + 1024 * n + place(n + 1), to + 1024 * n);
-        if (n + 2 < 2 * KS) dma16<2048>(from + 1024 * n + place(n + 2), to + 1024 * n);
-        if (n + 2 < 2 * KS) dma16<3072>(from + 1024 * n + place(n + 3), to + 1024 * n);
-    }
+__device__ __forceinline__ void fetch(int part, const uint8_t* from, uint8_t* to, Place place) {
+    const int n = 4 * part;  // (with one address on either side)
+    dma16<0>(from + 1024 * n + place(n), to + 1024 * n);
+    dma16<1024>(from + 1024 * n + place(n + 1), to + 1024 * n);
+    if (n + 2 < 2 * KS) dma16<2048>(from + 1024 * n + place(n + 2), to + 1024 * n);
+    if (n + 2 < 2 * KS) dma16<3072>(from + 1024 * n + place(n + 3), to + 1024 * n);
 }
 // A page's keys from LDS as operands: k steps 2 i and 2 i + 1 of tile t.
 template <int KS>
@@ -225,21 +223,19 @@ __device__ __forceinline__ void read_keys(const uint8_t* keys, u32x4_t (&k)[(KS 
             }
         }
 }
-// S^T of a page.
+// Step i of a page's S^T.
 template <int KS, int NQ, bool FP8>
-__device__ __forceinline__ void score(const u32x4_t (&k)[(KS + 1) / 2][4], const u32x4_t (&q)[NQ][KS],
+__device__ __forceinline__ void score(int i, const u32x4_t (&k)[(KS + 1) / 2][4], const u32x4_t (&q)[NQ][KS],
                                       f32x4_t (&x)[NQ][4]) {
-    // (a step of channels at a time over all tiles: no product waits for the one before it)
+    // (a step of channels over all tiles: no product waits for the one before it)
 #pragma unroll
-    for (int i = 0; i < KS; ++i)
+    for (int t = 0; t < 4; ++t) {
+        const u32x2_t lo = codes_bf16<FP8>(k[i / 2][t][2 * (i & 1)]), hi = codes_bf16<FP8>(k[i / 2][t][2 * (i & 1) + 1]);
+        const u32x4_t key = {lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const u32x2_t lo = codes_bf16<FP8>(k[i / 2][t][2 * (i & 1)]), hi = codes_bf16<FP8>(k[i / 2][t][2 * (i & 1) + 1]);
-            const u32x4_t key = {lo[0], lo[1], hi[0], hi[1]};
-#pragma unroll
-            for (int n = 0; n < NQ; ++n)
-                x[n][t] = mfma_bf16_16x16x32(key, q[n][i], i == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : x[n][t]);
-        }
+        for (int n = 0; n < NQ; ++n)
+            x[n][t] = mfma_bf16_16x16x32(key, q[n][i], i == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : x[n][t]);
+    }
 }
 
 // The waves of a workgroup at most; two a SIMD where 256 registers hold a
@@ -637,16 +633,30 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
     float* factors = reinterpret_cast<float*>(values + 2 * KS * 1024);  // of scores, of weights; by token
 
     float ks = 0.0f, vs = 0.0f;  // of token `lane`
-    auto load_page = [&](int page) {
+    // A page's fetch in parts: its scales and keys, then its values (the values last: the wait for the keys counts
+    // on it).
+    constexpr int kParts = (KS + 1) / 2;
+    const uint8_t *from_k = nullptr, *from_v = nullptr;
+    auto aim = [&](int page) {
         ks = a.c.ks[a.c.scale_base(page, h) + lane];
         vs = a.c.vs[a.c.scale_base(page, h) + lane];
-        const uint8_t* from = a.c.k + a.c.code_base(page, h);
-        fetch<KS>(from, keys, [lane](int n) -> uint32_t {
-            return 16 * (lane ^ key_swizzle<KS>((64 * n + lane) / (2 * KS)));
-        });
-        asm volatile("" ::: "memory");  // (the values last: the wait for the keys counts on it)
-        fetch<KS>(a.c.v + a.c.code_base(page, h), values,
-                  [lane](int) -> uint32_t { return 16 * (lane ^ value_swizzle(lane >> 2)); });
+        from_k = a.c.k + a.c.code_base(page, h);
+        from_v = a.c.v + a.c.code_base(page, h);
+    };
+    auto load_part = [&](int part) {
+        if (part < kParts)
+            fetch<KS>(part, from_k, keys, [lane](int n) -> uint32_t {
+                return 16 * (lane ^ key_swizzle<KS>((64 * n + lane) / (2 * KS)));
+            });
+        else
+            fetch<KS>(part - kParts, from_v, values,
+                      [lane](int) -> uint32_t { return 16 * (lane ^ value_swizzle(lane >> 2)); });
+        asm volatile("" ::: "memory");  // (in order)
+    };
+    auto load_page = [&](int page) {
+        aim(page);
+#pragma unroll
+        for (int part = 0; part < 2 * kParts; ++part) load_part(part);
     };
     // pages p0 + wave, + NW, ...
     const int mine = u.p0 + wave < u.p1 ? (u.p1 - u.p0 - wave + NW - 1) / NW : 0;
@@ -687,15 +697,24 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
         for (int i = 0; i < CT; ++i)
             v[i] = *reinterpret_cast<const u32x4_t*>(values + 1024 * i + 64 * c + 16 * (g ^ value_swizzle(c)));
         const int next = it + 1 < mine ? page_id(it + 1) : -1;
-        if (it + 1 < mine) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (this page has been read)
-            load_page(max(next, 0));
-        }
+        const bool more = it + 1 < mine;
         __builtin_amdgcn_sched_barrier(0);
         // The SIMD's other wave is kept off the matrix cores until this one's product is through: left
         // alone the two run every product and every softmax at the same time, one unit idle in turn.
         __builtin_amdgcn_s_setprio(2);
-        score<KS, NQ, FP8>(k, q, z.x);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            score<KS, NQ, FP8>(i, k, q, z.x);
+            if (more) {  // parts of the next page's fetch between the steps
+                if (i == 0) {
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (this page has been read)
+                    aim(max(next, 0));
+                }
+#pragma unroll
+                for (int part = i * 2 * kParts / KS; part < (i + 1) * 2 * kParts / KS; ++part) load_part(part);
+            }
+            
+        }
         __builtin_amdgcn_s_setprio(0);
         if (left < kKvPage) {
             z.cut(left);
