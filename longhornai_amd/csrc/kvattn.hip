@@ -22,11 +22,13 @@
 //
 // Measured (32 or 64 query heads over 8 kv heads of 128): decode of 4 x 131072
 // tokens 193 us, 5.7 TB/s, where a 2 GiB copy moves 4.9 -- bound by memory.
-// Trees of 64 over 4 x 8192 tokens 92 us, 750 TFLOP/s of the 1246 of a large
-// library product: the matrix cores are busy 37% of the cycles, the vector
-// units 69%, converting codes and weighing scores, and a SIMD's two waves
-// overlap the two little.  Small calls are bound by their ends: 4 us to find a
-// workgroup's share and fetch its queries and first page, 2 to 3 to join.
+// Trees of 64 over 4 x 8192 tokens 87 to 99 us, 700 to 790 TFLOP/s of the 1246
+// of a large library product: the matrix cores are busy 37% of the cycles.  A
+// page of 32 queries takes a wave 317 vector instructions besides its 64 MFMAs,
+// converting codes and weighing scores, and a wave issues one every 5 clocks
+// (exponentials 9), whatever the SIMD's other wave does.  Small calls are bound
+// by their ends: 4 us to find a workgroup's share and fetch its queries and
+// first page, 2 to 3 to join.
 // Tried and slower: 64 queries a wave with a SIMD to itself (trees of 64 152
 // us); pages shared by the query waves of a workgroup with a barrier a page,
 // its halves in turn at the products and the softmax (110).
@@ -680,7 +682,7 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
     z.clear();
     // The new tokens first, 32 at a time, by the waves whose turn it is after the last page (at least four waves
     // for at most 64 tokens): their rows are fetched while the first page is on its way.  After the pages they
-    // took 1 to 3% more of every measured call, and more registers.
+    // took up to 4% of a call more (decode of 64 ragged sequences 44.3 us, now 42.9), and more registers.
     const int turn = __builtin_amdgcn_readfirstlane((wave + NW - (u.p1 - u.p0) % NW) % NW);
     if (late_args()->k_new && u.split == u.splits - 1 && 32 * turn < u.T) z.new_tokens(late_args(), u, 32 * turn, D, q);
     for (int it = 0; it < mine; ++it) {
@@ -705,7 +707,7 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
             score<KS, NQ, FP8>(i, k, q, z.x);
-            if (more) {  // parts of the next page's fetch between the steps
+            if (more) {  // parts of the next page's fetch between the steps (all before them: 42.9 us for 42.2)
                 if (i == 0) {
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (this page has been read)
                     aim(max(next, 0));
