@@ -17,8 +17,13 @@
 // rescaling factor are one register.
 // Precision: key codes are exact in bf16 and meet the queries' own bf16; value
 // codes are exact in fp16, and a weight times its value scale is rounded once
-// to fp16 (2^-11 of itself).  To keep that product in fp16's normal range it
-// is held relative to 2^e, e the running exponent of the largest value scale.
+// to fp16.  That product is held relative to 2^e, e the running exponent of the
+// largest value scale that the wave has met: the rounding is 2^-11 of itself
+// down to 2^-25 of the largest scale, under that 2^-36 of the largest scale.
+// New tokens have their own exponents and each query one for those it sees, so
+// a query's result depends on nothing that it does not see, to the bit; 0.15 us
+// of a decode call, 0.5 of a tree's (one exponent for all of a wave's new
+// tokens erased what stood beside an unseen 2^40).
 //
 // Measured (32 or 64 query heads over 8 kv heads of 128): decode of 4 x 131072
 // tokens 193 us, 5.7 TB/s, where a 2 GiB copy moves 4.9 -- bound by memory.
@@ -51,6 +56,12 @@ typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
 // times value scales held at 2^kTop, stay within fp16's 65504.
 constexpr float kLag = 4.0f;
 constexpr int kTop = 11;
+// New tokens: the exponent that a query has while it sees none; the room that
+// fp32 sums have over an exponent e, so that 32 products of 2^29, at to <= e +
+// kRoom, stay under 2^(34 - 29 + kTop + kRoom) = 2^100; the highest e that new
+// tokens set.  A query's excess is at most 129 - kHighest - kRoom = 105: the sum
+// of its weights, 2^-105 or more, is a normal number.
+constexpr int kNothing = -400, kRoom = 84, kHighest = -60;
 
 constexpr int kJoinRows = 4;     // rows of a workgroup that joins splits, a wave each
 constexpr int kMostSplits = 64;  // of a sequence: a lane each when they are joined
@@ -374,45 +385,50 @@ struct Sums {
         }
         return ldexpf(vs, kTop - e);
     }
-    // x (products q . k), times ks the scores -> weights; times w they are the
-    // operands p of the second product.  The maximum follows when a score is
-    // over it by more than kLag; a query's first scores set it.
-    __device__ __forceinline__ void weigh(const f32x4_t (&ks)[4], const f32x4_t (&w)[4], u32x4_t (&p)[NQ][2]) {
-        if (fresh) {
-            bool all = true;
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) top = fmaxf(top, x[n][t][j] * ks[t][j]);
-                top = across(top);
-                const bool first = across(l[n]) == 0.0f;  // (a maximum's own weight is at least 2^-kLag)
-                if (first && top != -INFINITY) m[n] = top;  // (a missing page, or a mask that leaves nothing, sets nothing)
-                all &= !first || top != -INFINITY;
-            }
-            fresh = __ballot(!all) != 0;
-        }
+    // Of x (products q . k), times ks the scores: a query's first ones set its maximum.
+    __device__ __forceinline__ void start(const f32x4_t (&ks)[4]) {
+        bool all = true;
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             float top = -INFINITY;
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    x[n][t][j] = __builtin_fmaf(x[n][t][j], ks[t][j], -m[n]);
-                    top = fmaxf(top, x[n][t][j]);
-                }
-            if (__ballot(top > kLag)) {
-                const float to = m[n] + fmaxf(across(top), 0.0f), by = to - m[n], f = exp2_(-by);
-                m[n] = to;
-                l[n] *= f;
+                for (int j = 0; j < 4; ++j) top = fmaxf(top, x[n][t][j] * ks[t][j]);
+            top = across(top);
+            const bool first = across(l[n]) == 0.0f;  // (a maximum's own weight is at least 2^-kLag, and 2^-105 with an excess)
+            if (first && top != -INFINITY) m[n] = top;  // (a missing page, or a mask that leaves nothing, sets nothing)
+            all &= !first || top != -INFINITY;
+        }
+        fresh = __ballot(!all) != 0;
+    }
+    // Products of query tile n -> scores less the maximum, which follows when one is over it by more than kLag.
+    __device__ __forceinline__ void follow(int n, const f32x4_t (&ks)[4]) {
+        float top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < CT; ++i) o[n][i] *= f;
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int t = 0; t < 4; ++t) x[n][t] -= by;
+            for (int j = 0; j < 4; ++j) {
+                x[n][t][j] = __builtin_fmaf(x[n][t][j], ks[t][j], -m[n]);
+                top = fmaxf(top, x[n][t][j]);
             }
+        if (__ballot(top > kLag)) {
+            top = across(top);  // (of the other queries nothing moves: what they see decides nothing here)
+            const float to = m[n] + (top > kLag ? top : 0.0f), by = to - m[n], f = exp2_(-by);
+            m[n] = to;
+            l[n] *= f;
+#pragma unroll
+            for (int i = 0; i < CT; ++i) o[n][i] *= f;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) x[n][t] -= by;
+        }
+    }
+    // Products -> weights; times w they are the operands p of the second product.
+    __device__ __forceinline__ void weigh(const f32x4_t (&ks)[4], const f32x4_t (&w)[4], u32x4_t (&p)[NQ][2]) {
+        if (fresh) start(ks);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            follow(n, ks);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 f32x4_t y;
@@ -444,7 +460,9 @@ struct Sums {
         return in == 4 ? 0xffffffffu : (1u << (8 * in)) - 1;
     }
 
-    // The new tokens' own keys and values: tokens t0 .. t0 + 31 that there are (at least one).
+    // The new tokens' own keys and values: tokens t0 .. t0 + 31 that there are (at least one), before any page.
+    // Each has an exponent of its own, that of its largest value, and each query one of the largest weighted value
+    // that it sees: what a query does not see, however large, takes no bits from what it does.
     __device__ __forceinline__ void new_tokens(LateArgs late, const Unit& u, int t0, int D, const u32x4_t (&q)[NQ][KS]) {
         const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
         uint32_t seen[NQ];  // of those 32
@@ -474,11 +492,11 @@ struct Sums {
         };
         if constexpr (NQ == 1) load_raw();  // (early where registers are free)
         const uint16_t* new_keys = late->k_new + u.lo * late->k_stride + u.h * D;
-        f32x4_t ks[4], f[4];
+        f32x4_t ks[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) ks[t][j] = late->scale2, f[t][j] = ldexpf(1.0f, kTop);
+            for (int j = 0; j < 4; ++j) ks[t][j] = late->scale2;
 #pragma unroll
             for (int n = 0; n < NQ; ++n) x[n][t] = f32x4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             if (t >= 2) continue;
@@ -496,20 +514,24 @@ struct Sums {
                     if ((seen[n] >> (16 * t + 4 * g + j)) & 1) x[n][t][j] = y[j];
             }
         }
-        u32x4_t p[NQ][2];
-        weigh(ks, f, p);
+        start(ks);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) follow(n, ks);
         if constexpr (NQ > 1) load_raw();
-        u16x2_t size = {0, 0};
+        u16x2_t size[4];  // the largest of this lane's channels of two tokens, as in raw
         auto grow = [&] {
-            size = u16x2_t{0, 0};
 #pragma unroll
-            for (int i = 0; i < CT; ++i)
+            for (int j = 0; j < 4; ++j) {
+                size[j] = u16x2_t{0, 0};
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    size = __builtin_elementwise_max(size, __builtin_bit_cast(u16x2_t, raw[i][j] & 0x7fff7fffu));
+                for (int i = 0; i < CT; ++i)
+                    size[j] = __builtin_elementwise_max(size[j], __builtin_bit_cast(u16x2_t, raw[i][j] & 0x7fff7fffu));
+            }
         };
         grow();
-        const uint64_t not_finite = __ballot(max(size[0], size[1]) >= 0x7f80);
+        const u16x2_t all = __builtin_elementwise_max(__builtin_elementwise_max(size[0], size[1]),
+                                                      __builtin_elementwise_max(size[2], size[3]));
+        const uint64_t not_finite = __ballot(max(all[0], all[1]) >= 0x7f80);
         if (not_finite) {  // kept out of the product, in which they would reach queries that do not see them
             uint32_t inf = 0x7f80u;
             asm volatile("" : "+s"(inf));  // (else made 64 selects on every call)
@@ -522,20 +544,67 @@ struct Sums {
                 }
             grow();
         }
-        float big = bf16_to_f32(max(size[0], size[1]));
-        for (int d = 32; d; d >>= 1) big = fmaxf(big, __shfl_xor(big, d, 64));
-        // the values themselves as fp16, their largest under 2^15 (fp16's normal range holds 2^-29 of that)
-        const int want = __builtin_amdgcn_readfirstlane(exponent(big)) - 15;
-        if (big > 0.0f && want > e) raise(want);
+        // Each of this lane group's eight tokens, whose weights this lane has too: the exponent of its largest value
+        // (biased by 126, at least 14, of 2^-112: smaller ones keep fp16's precision by that), x[n][t][j]'s in te[t][j].
+        u16x2_t exps[4];
+        float te[2][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const u16x2_t top = row_max<4>(size[j], [](u16x2_t a, u16x2_t b) { return __builtin_elementwise_max(a, b); });
+            exps[j] = __builtin_elementwise_max(top >> 7, u16x2_t{14, 14});
+#pragma unroll
+            for (int half = 0; half < 2; ++half) te[j / 2][2 * (j % 2) + half] = static_cast<float>(exps[j][half]) - 126.0f;
+        }
+        // Values as fp16 under 2^15 and weights up to 2^14 of the query's largest (either keeps a normal number down
+        // to 2^-28 of that): the products are relative to 2^(to - 29).
+        int to[NQ], most = kNothing;
+        u32x4_t p[NQ];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            float top = static_cast<float>(kNothing);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    l[n] += exp2_(x[n][t][j]);
+                    x[n][t][j] += te[t][j];
+                    top = fmaxf(top, x[n][t][j]);
+                }
+            top = ceilf(across(top));
+            to[n] = static_cast<int>(top);
+            most = max(most, to[n]);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                f32x4_t y;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = exp2_(x[n][t][j] - (top - 14.0f));
+                p[n][2 * t] = pack_f16x2(y[0], y[1]);
+                p[n][2 * t + 1] = pack_f16x2(y[2], y[3]);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < CT; ++i) {
             u32x4_t val;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                val[j] = pack_f16x2(ldexpf(__uint_as_float(raw[i][j] << 16), -e),
-                                    ldexpf(__uint_as_float(raw[i][j] & 0xffff0000u), -e));
+                val[j] = pack_f16x2(ldexpf(__uint_as_float(raw[i][j] << 16), 141 - exps[j][0]),
+                                    ldexpf(__uint_as_float(raw[i][j] & 0xffff0000u), 141 - exps[j][1]));
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) o[n][i] = mfma_f16_16x16x32(val, p[n][0], o[n][i]);
+            for (int n = 0; n < NQ; ++n) o[n][i] = mfma_f16_16x16x32(val, p[n], o[n][i]);
+        }
+        // To one exponent, so low that a page's value scales keep their bits beside it (the sums are fp32 and lose
+        // none).  A query whose values are too large for that takes the excess into its maximum.
+        most = row_max<4>(most, [](int a, int b) { return max(a, b); });
+        e = min(max(__builtin_amdgcn_readfirstlane(most) - kRoom, -200), kHighest);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            const int excess = max(to[n] - e - kRoom, 0);
+            m[n] += static_cast<float>(excess);
+            l[n] = ldexpf(l[n], -excess);
+#pragma unroll
+            for (int i = 0; i < CT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[n][i][j] = ldexpf(o[n][i][j], to[n] - 29 + kTop - e - excess);
         }
         if (not_finite)  // a query that sees such a value takes it as it is, the others do not
 #pragma unroll 1

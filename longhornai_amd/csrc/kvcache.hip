@@ -145,20 +145,6 @@ __device__ __forceinline__ Tile find_tile(const int32_t* offsets, const int32_t*
     return {u.seq, static_cast<int>(max<int64_t>(a, 0)), static_cast<int>(min<int64_t>(b, kKvPage)), p, lo - a};
 }
 
-// Maximum over 1 << LB adjacent lanes (8, 16 or 32), the same in all of them.
-template <int LB, typename T, typename Max>
-__device__ __forceinline__ T row_max(T m, Max max_of) {
-#define LHQ_MAX_STEP(ctrl)                                                                               \
-    m = max_of(m, __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, m), ctrl, \
-                                                                    0xf, 0xf, false)))
-    LHQ_MAX_STEP(0xB1);   // quad_perm 1, 0, 3, 2
-    LHQ_MAX_STEP(0x4E);   // quad_perm 2, 3, 0, 1
-    LHQ_MAX_STEP(0x141);  // row_half_mirror: the other quad of 8 lanes
-    if constexpr (LB >= 4) LHQ_MAX_STEP(0x140);  // row_mirror: the other half of 16
-#undef LHQ_MAX_STEP
-    if constexpr (LB >= 5) m = max_of(m, __shfl_xor(m, 16, 64));
-    return m;
-}
 __device__ __forceinline__ uint32_t magnitude(const float (&x)[8]) {  // bits of max |x|; NaN is over infinity
     uint32_t m = 0;
 #pragma unroll
