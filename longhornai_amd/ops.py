@@ -253,6 +253,7 @@ def gemm_w8a8_i32(Aq, Bt, M, N, K, C=None):
 # ---------------------------------------------------------------------------
 
 KV_PAGE = 64
+KV_MAX_NEW = 64  # new tokens of one sequence that a call of kv_attn attends
 _KV_FORMATS = {"int8": 0, "fp8": 1}  # LHQ_KV_INT8, LHQ_KV_FP8
 
 
@@ -390,12 +391,17 @@ def kv_attn_workspace(cache: KvCache, n_seqs: int, n: int, max_new: int, max_pag
 
 def kv_attn(cache: KvCache, q: torch.Tensor, offsets: torch.Tensor, lengths: torch.Tensor,
             block_table: torch.Tensor, k_new: torch.Tensor | None, v_new: torch.Tensor | None,
-            tree: torch.Tensor | None = None, scale: float | None = None, max_new: int = 1,
+            tree: torch.Tensor | None = None, scale: float | None = None, max_new: int | None = None,
             workspace: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of new tokens (q [n, heads * head_dim], bf16 as int16 bits)
     over the first lengths[s] cached tokens of their sequence and over the new
     ones (k_new, v_new) that tree (int64, a bit for each) names -- None: those
-    up to the token itself.  Returns out [n, heads, head_dim], int16 bits."""
+    up to the token itself.  Returns out [n, heads, head_dim], int16 bits.
+    max_new bounds the new tokens of one sequence, 64 at most; the closer, the
+    better the kernel's shape (1 in plain decode).  Rows past it in a sequence,
+    and rows of q that offsets give to none, are not computed: they stay what
+    ``out`` held.  None: as many as q has rows, 64 at most, and what is not
+    computed is zero in a result that is made here."""
     H, D = cache.n_kv_heads, cache.head_dim
     B, width = _kv_tables("kv_attn", offsets, lengths, block_table)
     shape = q.shape
@@ -413,13 +419,17 @@ def kv_attn(cache: KvCache, q: torch.Tensor, offsets: torch.Tensor, lengths: tor
             raise ValueError(f"kv_attn: {n} queries with {n_keys} new keys and {n_values} values")
     if tree is not None and (tree.dtype != torch.int64 or tree.numel() != n or not tree.is_contiguous()):
         raise ValueError(f"kv_attn: tree must hold {n} contiguous int64 words")
+    bound = min(n, KV_MAX_NEW) if max_new is None else max_new
     if out is None:
-        out = q.new_empty((n, heads, D))
+        if max_new is not None and n > B * max_new:
+            raise ValueError(f"kv_attn: {n} rows of {B} sequences are over max_new = {max_new} each, and no out is "
+                             "given for those that are not computed")
+        out = q.new_empty((n, heads, D)) if max_new is not None else q.new_zeros((n, heads, D))
     elif out.dtype != torch.int16 or out.numel() != n * heads * D or not out.is_contiguous():
         raise ValueError(f"kv_attn: out must be contiguous [{n}, {heads}, {D}] int16")
     nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
     lib().call("lhq_kv_attn_bf16", q.data_ptr(), qs, P(k_new), ks, P(v_new), vs, P(tree), offsets.data_ptr(),
                lengths.data_ptr(), block_table.data_ptr(), *cache.pointers(), out.data_ptr(), _KV_FORMATS[cache.fmt],
-               B, n, max_new, width, cache.n_pages, heads, H, D, D ** -0.5 if scale is None else scale, P(workspace),
+               B, n, bound, width, cache.n_pages, heads, H, D, D ** -0.5 if scale is None else scale, P(workspace),
                nbytes, stream())
     return out

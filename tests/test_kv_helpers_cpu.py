@@ -1,0 +1,32 @@
+"""The cache's Python helpers: arguments that they must refuse before anything
+is enqueued.  No GPU: whatever passes the checks would fail on the launch."""
+import pytest
+import torch
+
+from longhornai_amd import ops
+from tests import _kv
+
+I32 = dict(dtype=torch.int32)
+
+
+def host_cache():
+    c = _kv.HostCache("int8", 4, 2, 40)
+    return ops.KvCache("int8", 4, 2, 40, *(torch.from_numpy(a) for a in (c.k, c.v, c.ks, c.vs)))
+
+
+def call(**kw):
+    """kv_attn on six rows of two sequences."""
+    a = dict(cache=host_cache(), q=torch.zeros((6, 160), dtype=torch.int16), offsets=torch.tensor([0, 3, 6], **I32),
+             lengths=torch.zeros(2, **I32), block_table=torch.zeros((2, 2), **I32),
+             k_new=torch.zeros((6, 80), dtype=torch.int16), v_new=torch.zeros((6, 80), dtype=torch.int16))
+    a.update(kw)
+    return ops.kv_attn(**a)
+
+
+def test_attn_refuses_a_result_with_rows_that_it_would_leave_unwritten():
+    """Six rows of two sequences of at most two tokens: two rows or more would
+    hold whatever the new memory held."""
+    with pytest.raises(ValueError, match="max_new"):
+        call(max_new=2)
+    with pytest.raises(ValueError, match="max_new"):
+        call(max_new=1, tree=torch.zeros(6, dtype=torch.int64))
