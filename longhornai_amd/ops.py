@@ -427,7 +427,11 @@ def kv_attn(cache: KvCache, q: torch.Tensor, offsets: torch.Tensor, lengths: tor
         out = q.new_empty((n, heads, D)) if max_new is not None else q.new_zeros((n, heads, D))
     elif out.dtype != torch.int16 or out.numel() != n * heads * D or not out.is_contiguous():
         raise ValueError(f"kv_attn: out must be contiguous [{n}, {heads}, {D}] int16")
-    nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    nbytes = 0
+    if workspace is not None:
+        if not workspace.is_contiguous():
+            raise ValueError(f"kv_attn: workspace must be contiguous (strides {tuple(workspace.stride())})")
+        nbytes = workspace.numel() * workspace.element_size()
     lib().call("lhq_kv_attn_bf16", q.data_ptr(), qs, P(k_new), ks, P(v_new), vs, P(tree), offsets.data_ptr(),
                lengths.data_ptr(), block_table.data_ptr(), *cache.pointers(), out.data_ptr(), _KV_FORMATS[cache.fmt],
                B, n, bound, width, cache.n_pages, heads, H, D, D ** -0.5 if scale is None else scale, P(workspace),

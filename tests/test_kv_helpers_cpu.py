@@ -30,3 +30,11 @@ def test_attn_refuses_a_result_with_rows_that_it_would_leave_unwritten():
         call(max_new=2)
     with pytest.raises(ValueError, match="max_new"):
         call(max_new=1, tree=torch.zeros(6, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("workspace", [torch.zeros(4096, dtype=torch.uint8)[::2],
+                                       torch.zeros((64, 64), dtype=torch.float32).t()[:, :32]])
+def test_attn_refuses_a_workspace_with_gaps(workspace):
+    """The kernels would write the elements between those of the slice."""
+    with pytest.raises(ValueError, match="workspace"):
+        call(max_new=3, workspace=workspace)
