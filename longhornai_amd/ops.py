@@ -326,13 +326,13 @@ def _kv_tables(fn: str, offsets: torch.Tensor, start: torch.Tensor, table: torch
     i32 = torch.int32
     if offsets.dtype is not i32 or start.dtype is not i32 or table.dtype is not i32:
         raise ValueError(f"{fn}: offsets, positions and block table must be int32")
-    B, shape = start.shape[0], table.shape
-    if offsets.shape[0] != B + 1 or len(shape) != 2 or shape[0] != B:
-        raise ValueError(f"{fn}: {B} positions with {offsets.shape[0]} offsets and a block table of "
-                         f"{tuple(shape)}")
+    positions, offs, shape = start.shape, offsets.shape, table.shape
+    if len(positions) != 1 or len(offs) != 1 or len(shape) != 2 or offs[0] != positions[0] + 1 or shape[0] != positions[0]:
+        raise ValueError(f"{fn}: positions {tuple(positions)}, offsets {tuple(offs)} and block table {tuple(shape)} are "
+                         "not [B], [B + 1] and [B, pages]")
     if not (offsets.is_contiguous() and start.is_contiguous() and table.is_contiguous()):
         raise ValueError(f"{fn}: offsets, positions and block table must be contiguous")
-    return B, shape[1]
+    return positions[0], shape[1]
 
 
 _KV_BITS, _KV_ROWS = (torch.int16,), (torch.int16, torch.float32)
@@ -405,7 +405,7 @@ def kv_attn(cache: KvCache, q: torch.Tensor, offsets: torch.Tensor, lengths: tor
     H, D = cache.n_kv_heads, cache.head_dim
     B, width = _kv_tables("kv_attn", offsets, lengths, block_table)
     shape = q.shape
-    heads = shape[1] // D if len(shape) == 2 else shape[1]
+    heads = shape[1] // D if len(shape) == 2 else shape[1] if len(shape) == 3 else 0
     n, qs = _kv_rows("kv_attn", "q", q, heads, D, _KV_BITS)
     if heads % H != 0:
         raise ValueError(f"kv_attn: {heads} query heads over {H} kv heads")

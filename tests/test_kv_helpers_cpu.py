@@ -38,3 +38,22 @@ def test_attn_refuses_a_workspace_with_gaps(workspace):
     """The kernels would write the elements between those of the slice."""
     with pytest.raises(ValueError, match="workspace"):
         call(max_new=3, workspace=workspace)
+
+
+@pytest.mark.parametrize("kw", [dict(offsets=torch.zeros((3, 2), **I32)), dict(lengths=torch.zeros((2, 2), **I32)),
+                                dict(lengths=torch.zeros((), **I32)), dict(offsets=torch.zeros((), **I32)),
+                                dict(q=torch.zeros(160, dtype=torch.int16)), dict(q=torch.zeros((), dtype=torch.int16)),
+                                dict(q=torch.zeros((6, 4, 40, 1), dtype=torch.int16))])
+def test_tensors_of_other_ranks(kw):
+    """Tables of more than a number a sequence would be read as if they had one."""
+    with pytest.raises(ValueError):
+        call(max_new=3, **kw)
+    if "q" in kw:
+        return
+    c, k = host_cache(), torch.zeros((6, 80), dtype=torch.int16)
+    tables = (kw.get("offsets", torch.tensor([0, 3, 6], **I32)), kw.get("lengths", torch.zeros(2, **I32)),
+              torch.zeros((2, 2), **I32))
+    with pytest.raises(ValueError):
+        ops.kv_write(c, k, k, *tables)
+    with pytest.raises(ValueError):
+        ops.kv_read(c, *tables, 6)
