@@ -284,6 +284,8 @@ class KvCache:
             if t.dtype != dt or not t.is_contiguous() or t.numel() * t.element_size() != nbytes:
                 raise ValueError(f"KvCache: {name} must be {nbytes} contiguous bytes of {dt}, "
                                  f"got {tuple(t.shape)} {t.dtype}")
+            if t.device != self.k.device:
+                raise ValueError(f"KvCache: {name} is on {t.device}, k on {self.k.device}")
 
     def pointers(self):
         return self.k.data_ptr(), self.k_scales.data_ptr(), self.v.data_ptr(), self.v_scales.data_ptr()
@@ -301,6 +303,17 @@ def kv_cache(fmt: str, n_pages: int, n_kv_heads: int, head_dim: int) -> KvCache:
 
 # These checks run before every call, ahead of kernels of a few microseconds:
 # each attribute of a tensor is read once, the usual case decided first.
+
+def _kv_on_gpu(fn: str, cache: KvCache, *tensors: torch.Tensor | None) -> None:
+    """The cache and what goes with it lie on one GPU: the kernels fault on other
+    addresses (0.1 us a tensor)."""
+    at = cache.k.get_device()
+    if at < 0:
+        raise ValueError(f"{fn}: the cache is not on a GPU")
+    for t in tensors:
+        if t is not None and t.get_device() != at:
+            raise ValueError(f"{fn}: a tensor of {t.device} with a cache on GPU {at}")
+
 
 def _kv_rows(fn: str, name: str, t: torch.Tensor, heads: int, D: int, dtypes) -> tuple[int, int]:
     """Checks new tokens' rows [n, heads * D] or [n, heads, D], heads packed;
@@ -354,6 +367,7 @@ def kv_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, offsets: torch.Te
         raise ValueError(f"kv_write: {n_rows} rows of keys and {n_values} of values")
     if rows is not None and (rows.dtype != torch.int32 or not rows.is_contiguous()):
         raise ValueError("kv_write: rows must be contiguous int32")
+    _kv_on_gpu("kv_write", cache, k, v, offsets, start, block_table, rows)
     n = n_rows if rows is None else rows.numel()
     lib().call("lhq_kv_write_f32" if dt == torch.float32 else "lhq_kv_write_bf16", k.data_ptr(), v.data_ptr(), ks, vs,
                P(rows), offsets.data_ptr(), start.data_ptr(), block_table.data_ptr(), *cache.pointers(),
@@ -364,7 +378,8 @@ def kv_read(cache: KvCache, offsets: torch.Tensor, start: torch.Tensor, block_ta
             bf16: bool = True, out: tuple[torch.Tensor, torch.Tensor] | None = None):
     """Cached tokens as values: row i of sequence s's rows offsets[s] ..
     offsets[s+1] is its position start[s] + i.  n rows in all; returns (k, v)
-    [n, heads, head_dim], bf16 as int16 bits or fp32."""
+    [n, heads, head_dim], bf16 as int16 bits or fp32.  Rows that offsets give to
+    no sequence are not written."""
     H, D = cache.n_kv_heads, cache.head_dim
     B, width = _kv_tables("kv_read", offsets, start, block_table)
     dt = torch.int16 if bf16 else torch.float32
@@ -375,6 +390,7 @@ def kv_read(cache: KvCache, offsets: torch.Tensor, start: torch.Tensor, block_ta
         for t in out:
             if t.dtype != dt or tuple(t.shape) != (n, H, D) or not t.is_contiguous():
                 raise ValueError(f"kv_read: outputs must be contiguous [{n}, {H}, {D}] {dt}")
+    _kv_on_gpu("kv_read", cache, offsets, start, block_table, *out)
     lib().call("lhq_kv_read_bf16" if bf16 else "lhq_kv_read_f32", *cache.pointers(), offsets.data_ptr(),
                start.data_ptr(), block_table.data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
                _KV_FORMATS[cache.fmt], B, n, width, cache.n_pages, H, D, stream())
@@ -432,6 +448,7 @@ def kv_attn(cache: KvCache, q: torch.Tensor, offsets: torch.Tensor, lengths: tor
         if not workspace.is_contiguous():
             raise ValueError(f"kv_attn: workspace must be contiguous (strides {tuple(workspace.stride())})")
         nbytes = workspace.numel() * workspace.element_size()
+    _kv_on_gpu("kv_attn", cache, q, offsets, lengths, block_table, k_new, v_new, tree, workspace, out)
     lib().call("lhq_kv_attn_bf16", q.data_ptr(), qs, P(k_new), ks, P(v_new), vs, P(tree), offsets.data_ptr(),
                lengths.data_ptr(), block_table.data_ptr(), *cache.pointers(), out.data_ptr(), _KV_FORMATS[cache.fmt],
                B, n, bound, width, cache.n_pages, heads, H, D, D ** -0.5 if scale is None else scale, P(workspace),

@@ -57,3 +57,15 @@ def test_tensors_of_other_ranks(kw):
         ops.kv_write(c, k, k, *tables)
     with pytest.raises(ValueError):
         ops.kv_read(c, *tables, 6)
+
+
+def test_host_memory_is_refused():
+    """Tensors of the host: the kernels would fault on their addresses."""
+    c, k = host_cache(), torch.zeros((6, 80), dtype=torch.int16)
+    tables = torch.tensor([0, 3, 6], **I32), torch.zeros(2, **I32), torch.zeros((2, 2), **I32)
+    with pytest.raises(ValueError, match="GPU"):
+        call(max_new=3)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.kv_write(c, k, k, *tables)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.kv_read(c, *tables, 6)
