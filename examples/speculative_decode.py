@@ -103,6 +103,8 @@ def plain_attention(layer: Layer, s: int, q, k, v, masks) -> np.ndarray:
 
 def main(fmt: str = "int8", steps: int = 4, prompts: tuple[int, ...] = (300, 64, 129, 1), T: int = 12) -> float:
     """Returns the last step's largest error, relative to its largest value."""
+    if steps < 1:
+        raise ValueError("speculative_decode: the last step is checked, so there must be one")
     g, tg = np.random.default_rng(1), torch.Generator(device="cuda").manual_seed(1)
     layer = Layer(fmt, len(prompts), max(prompts) + steps * T, seed=2)
     left = list(prompts)
@@ -128,9 +130,16 @@ def main(fmt: str = "int8", steps: int = 4, prompts: tuple[int, ...] = (300, 64,
     return worst
 
 
-if __name__ == "__main__":
+def run(argv: list[str] | None = None) -> int:
+    """The command: 0 where the last step holds to 64 bits, else 1."""
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--fmt", choices=("int8", "fp8"), default="int8")
     ap.add_argument("--steps", type=int, default=4)
-    a = ap.parse_args()
-    sys.exit(main(a.fmt, a.steps) > 2.0 ** -8)
+    a = ap.parse_args(argv)
+    if a.steps < 1:
+        ap.error("--steps must be 1 or more")
+    return 0 if main(a.fmt, a.steps) <= 2.0 ** -8 else 1  # (a NaN is no success)
+
+
+if __name__ == "__main__":
+    sys.exit(run())
