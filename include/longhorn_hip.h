@@ -443,7 +443,12 @@ int lhq_kv_read_bf16(const uint8_t* k_codes, const float* k_scales, const uint8_
  * sequence; of one that has more, those past max_new are not computed and
  * their rows of out [row_capacity, n_heads, head_dim] are left as they are.
  * lengths are clamped to [0, 64 * max_pages].  scale must be finite and
- * positive.
+ * positive.  What a row does not see, whatever it holds, changes nothing of its
+ * result.  Rounding: queries, keys and codes enter the products as they are; a
+ * softmax weight times the scale of its value is rounded to fp16 (2^-11 of
+ * itself, or 2^-35 of the largest value scale of the sequence where that is
+ * more, whatever the weight there), a new token's weight likewise; scores and
+ * sums are fp32, the result is rounded once more to bf16.
  * workspace: the sequences' tokens are split over workgroups, whose partial
  * sums meet there and are added in order of position (deterministic).  Up to
  * lhq_kv_attn_workspace_bytes bytes are used; with less, or NULL, there are

@@ -19,21 +19,24 @@
 // codes are exact in fp16, and a weight times its value scale is rounded once
 // to fp16.  That product is held relative to 2^e, e the running exponent of the
 // largest value scale that the wave has met: the rounding is 2^-11 of itself
-// down to 2^-25 of the largest scale, under that 2^-36 of the largest scale.
-// New tokens have their own exponents and each query one for those it sees, so
-// a query's result depends on nothing that it does not see, to the bit; 0.15 us
-// of a decode call, 0.5 of a tree's (one exponent for all of a wave's new
-// tokens erased what stood beside an unseen 2^40).
+// down to 2^-24 of that scale, under that 2^-35 of the scale.  New tokens have
+// their own exponents and each query one for those it sees, so a query's result
+// depends on nothing that it does not see, to the bit; 0.15 us of a decode call,
+// 0.5 of a tree's (one exponent for all of a wave's new tokens erased what stood
+// beside an unseen 2^40).
 //
-// Measured (32 or 64 query heads over 8 kv heads of 128): decode of 4 x 131072
-// tokens 193 us, 5.7 TB/s, where a 2 GiB copy moves 4.9 -- bound by memory.
-// Trees of 64 over 4 x 8192 tokens 87 to 99 us, 700 to 790 TFLOP/s of the 1246
-// of a large library product: the matrix cores are busy 37% of the cycles.  A
-// page of 32 queries takes a wave 317 vector instructions besides its 64 MFMAs,
-// converting codes and weighing scores, and a wave issues one every 5 clocks
-// (exponentials 9), whatever the SIMD's other wave does.  Small calls are bound
-// by their ends: 4 us to find a workgroup's share and fetch its queries and
-// first page, 2 to 3 to join.
+// Measured with inputs that change (32 or 64 query heads over 8 kv heads of
+// 128): decode of 4 x 131072 tokens 193 us, 5.7 TB/s, where a 4 GiB read streams
+// at 6.35 -- bound by memory.  Trees of 64 over 4 x 8192 tokens 88 to 97 us at
+// settled clocks, 710 to 780 TFLOP/s of the 1246 of a large library product (103
+// to 117 us in the first 200 calls after a pause).  There the matrix cores are
+// busy 35% of a SIMD's cycles and vector instructions issue in 67%, together all
+// of them: the two hardly overlap.  A page of 32 queries takes a wave 64 MFMAs
+// of 16 clocks and about 400 vector instructions, converting codes and weighing
+// scores; two waves of a SIMD share its vector unit, which takes 4.2 to 4.4
+// clocks for a conversion, a permute or a multiply-add, 8.2 for an exponential,
+// 2.2 for a sum.  Small calls are bound by their ends: 4 us to find a workgroup's
+// share and fetch its queries and first page, 2 to 3 to join.
 // Tried and slower: 64 queries a wave with a SIMD to itself (trees of 64 152
 // us); pages shared by the query waves of a workgroup with a barrier a page,
 // its halves in turn at the products and the softmax (110).
@@ -396,7 +399,8 @@ struct Sums {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) top = fmaxf(top, x[n][t][j] * ks[t][j]);
             top = across(top);
-            const bool first = across(l[n]) == 0.0f;  // (a maximum's own weight is at least 2^-kLag, and 2^-105 with an excess)
+            // (a maximum's own weight is at least 2^-kLag, 2^-105 where new tokens took an excess)
+            const bool first = across(l[n]) == 0.0f;
             if (first && top != -INFINITY) m[n] = top;  // (a missing page, or a mask that leaves nothing, sets nothing)
             all &= !first || top != -INFINITY;
         }
@@ -544,8 +548,8 @@ struct Sums {
                 }
             grow();
         }
-        // Each of this lane group's eight tokens, whose weights this lane has too: the exponent of its largest value
-        // (biased by 126, at least 14, of 2^-112: smaller ones keep fp16's precision by that), x[n][t][j]'s in te[t][j].
+        // Each of this lane group's eight tokens, whose weights this lane has too: the exponent of its largest value,
+        // biased by 126 and at least 14 (2^-112, by which smaller values are exact in fp16 too); x[n][t][j]'s is te[t][j].
         u16x2_t exps[4];
         float te[2][4];
 #pragma unroll
@@ -751,7 +755,8 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
     z.clear();
     // The new tokens first, 32 at a time, by the waves whose turn it is after the last page (at least four waves
     // for at most 64 tokens): their rows are fetched while the first page is on its way.  After the pages they
-    // took up to 4% of a call more (decode of 64 ragged sequences 44.3 us, now 42.9), and more registers.
+    // took up to 4% of a call more (decode of 64 ragged sequences, replays over one set of inputs, 44.3 us for 42.9),
+    // and more registers.
     const int turn = __builtin_amdgcn_readfirstlane((wave + NW - (u.p1 - u.p0) % NW) % NW);
     if (late_args()->k_new && u.split == u.splits - 1 && 32 * turn < u.T) z.new_tokens(late_args(), u, 32 * turn, D, q);
     for (int it = 0; it < mine; ++it) {
@@ -784,7 +789,6 @@ __global__ __launch_bounds__(64 * most_waves<KS>(), KS <= 4 ? 2 : 1) void kv_att
 #pragma unroll
                 for (int part = i * 2 * kParts / KS; part < (i + 1) * 2 * kParts / KS; ++part) load_part(part);
             }
-            
         }
         __builtin_amdgcn_s_setprio(0);
         if (left < kKvPage) {
@@ -906,6 +910,11 @@ int64_t unit_bound(int n_seqs, int capacity, int max_new, int G, int block) {
 // splits 14.6 us, in one 19.4; of 16 x 2048 in one 19.2, in two 21.7; trees of
 // 12 over 2500 ragged tokens in 3 or 5 splits 24, in one 31; trees of 64 over 4 x
 // 8192 in one 97, in two 116.
+// A split is a share of the table's width, of which a sequence far shorter than
+// that has few: one token over 8192 takes 12.4 us with a table of 128 or 256
+// pages, 14.6 with 512, 18.7 with 1024, 26.7 with 2048 (16 such sequences 48 us
+// with any).  And with kMostSplits one sequence and one kv head have 64
+// workgroups at most: 131072 tokens of 4 query heads 24 us, 1.4 TB/s.
 Plan make_plan(int n_seqs, int capacity, int max_new, int max_pages, int heads, int kv_heads, int D, int64_t ws_bytes) {
     const int G = heads / kv_heads, KS = kv_padded(D) / 32;
     Plan p{};

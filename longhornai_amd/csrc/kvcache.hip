@@ -8,10 +8,11 @@
 //
 // Both ways are bound by memory from a few thousand tokens on, below that by
 // the launch and one workgroup's chain of loads.  8 x 4096 tokens of 8 heads of
-// 128, bf16 and e4m3, 203 MB each way: write 42 us (4.8 TB/s, a copy's rate),
-// read 31 us (6.4, the results partly in the last-level cache); one token of 16
-// sequences: 4 and 3 us.  Turning the value tile in bytes rather than dwords,
-// one row after the other, took 55 and 42 us.
+// 128, bf16 and e4m3, 203 MB each way: write 57 us with inputs that change (3.6
+// TB/s; 42 to 49 where they lie partly in the last-level cache), read 31 us (6.5,
+// the results partly in that cache); one token of 16 sequences: 5.7 and 3.8 us.
+// Turning the value tile in bytes rather than dwords, one row after the other,
+// took 55 and 42 us where this takes 42 and 31.
 #include <algorithm>
 #include <type_traits>
 
