@@ -442,8 +442,8 @@ int lhq_kv_read_bf16(const uint8_t* k_codes, const float* k_scales, const uint8_
  * sees nothing gives zeros.  max_new <= 64 bounds the new tokens of a
  * sequence; of one that has more, those past max_new are not computed and
  * their rows of out [row_capacity, n_heads, head_dim] are left as they are.
- * lengths are clamped to [0, 64 * max_pages].  scale must be finite and
- * positive.  What a row does not see, whatever it holds, changes nothing of its
+ * lengths are clamped to [0, 64 * max_pages].  scale must be positive and
+ * finite, also times log2 e.  What a row does not see, whatever it holds, changes nothing of its
  * result.  Rounding: queries, keys and codes enter the products as they are; a
  * softmax weight times the scale of its value is rounded to fp16 (2^-11 of
  * itself, or 2^-35 of the largest value scale of the sequence where that is

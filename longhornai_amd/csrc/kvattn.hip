@@ -1007,7 +1007,9 @@ int lhq_kv_attn_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k_new,
     LHQ_SUPPORTED(n_heads <= 65535, "%s: %d query heads are over 65535", fn, n_heads);
     LHQ_REQUIRE(max_new >= 0, "%s: bad max_new %d", fn, max_new);
     LHQ_SUPPORTED(max_new <= kKvMaxNew, "%s: max_new %d is over %d", fn, max_new, kKvMaxNew);
-    LHQ_REQUIRE(std::isfinite(scale) && scale > 0.0f, "%s: scale %g is not finite and positive", fn, scale);
+    const float scale2 = scale * 1.4426950408889634f;  // weights are powers of two
+    LHQ_REQUIRE(std::isfinite(scale2) && scale > 0.0f, "%s: scale %g is not positive and finite, also times log2 e", fn,
+                scale);
     LHQ_REQUIRE((k_new == nullptr) == (v_new == nullptr), "%s: new keys without values, or values without keys", fn);
     LHQ_REQUIRE(q_stride >= static_cast<int64_t>(n_heads) * head_dim, "%s: q rows of stride %lld are under %d heads of %d",
                 fn, static_cast<long long>(q_stride), n_heads, head_dim);
@@ -1022,7 +1024,7 @@ int lhq_kv_attn_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k_new,
     LHQ_REQUIRE(q && offsets && lengths && out, "%s: null pointer", fn);
     auto odd = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; };
     AttnArgs a{q,        q_stride, k_new,  k_stride,     v_new,   v_stride, tree, offsets, lengths, c, out,
-               n_seqs, row_capacity, max_new, n_heads, n_heads / n_kv_heads, scale * 1.4426950408889634f};
+               n_seqs, row_capacity, max_new, n_heads, n_heads / n_kv_heads, scale2};
     if (num_pages == 0) a.c.max_pages = 0;  // (no page to stand in for a missing one)
     a.vec_out = head_dim % 4 == 0 && !odd(out, 8);
     const Plan p = make_plan(n_seqs, row_capacity, max_new, max_pages, n_heads, n_kv_heads, head_dim,

@@ -3,8 +3,9 @@ is enqueued.  No GPU: whatever passes the checks would fail on the launch."""
 import pytest
 import torch
 
-from longhornai_amd import ops
+from longhornai_amd import capi, ops
 from tests import _kv
+from tests.test_kv_cpu import attn_args
 
 I32 = dict(dtype=torch.int32)
 
@@ -69,3 +70,11 @@ def test_host_memory_is_refused():
         ops.kv_write(c, k, k, *tables)
     with pytest.raises(ValueError, match="GPU"):
         ops.kv_read(c, *tables, 6)
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38])
+def test_attn_refuses_a_scale_that_is_infinite_as_a_power_of_two(scale):
+    """The kernel's weights are powers of two: scale times log2 e must be finite too."""
+    args = attn_args(scale=scale)
+    assert capi.load().status("lhq_kv_attn_bf16", *args) == capi.LHQ_ERR_INVALID
+    assert "scale" in capi.load().last_error()
