@@ -465,6 +465,88 @@ int lhq_kv_attn_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k_new,
                      int n_kv_heads, int head_dim, float scale, void* workspace,
                      int64_t workspace_bytes, void* stream);
 
+/* ---- a prompt's way through an attention layer ---------------------------- */
+/* No reference counterpart on the quantized-GEMM path: tables, positions and
+ * attention of prompts, beside the cache above. */
+/* A step's tables from the requests' lengths.  Sequence s holds lengths[s]
+ * tokens (clamped to [0, 64 * max_pages]) and gets new_tokens[s] more; where
+ * that is negative the sequence is over, gets none, and the pages of its tokens
+ * go back (its row of the table stays as it is and means nothing).
+ *   offsets [n_seqs + 1]: the rows of the new tokens, as above, at most row_capacity
+ *   block_table [n_seqs][max_pages]: entries ceil(lengths / 64) .. up to the last
+ *     new token get a page each, or -1 where there is none left; other entries are
+ *     not touched
+ *   positions [row_capacity]: lengths[s] + i for row i of a sequence, with a tree
+ *     (its words as in lhq_kv_attn_bf16, or NULL) lengths[s] + the tokens above it
+ *     in the tree; -1 in rows of no sequence
+ *   slots [row_capacity] (or NULL): 64 * page + place of token lengths[s] + i in
+ *     the cache; -1 where it has no page, and in rows of no sequence
+ * free_pages [num_pages] is a stack of which the first left[0] entries count
+ * (clamped to [0, num_pages]): pages that go back are pushed in order of sequence
+ * and page (entries outside [0, num_pages) are no pages), then new ones are popped
+ * in that order.  left_out [2]: what is left on the stack, and how many pages were
+ * wanted and not there.  left_out may be left, for tables that live from step to
+ * step.  A page that two sequences share goes back once for each that is over:
+ * taking care of that is the caller's. */
+int lhq_kv_plan(const int32_t* lengths, const int32_t* new_tokens, const uint64_t* tree,
+                const int32_t* left, int32_t* left_out, int32_t* free_pages, int32_t* block_table,
+                int32_t* offsets, int32_t* positions, int64_t* slots, int n_seqs, int row_capacity,
+                int max_pages, int num_pages, void* stream);
+/* Queries and keys turned by their positions, their heads RMS-normed in the same
+ * pass where a weight [head_dim] is given (NULL: not): y = x / sqrt(mean(x^2) +
+ * eps) * weight of each head, then each pair (a, b) of its first rot_dim channels
+ * becomes gain * (a cos - b sin, b cos + a sin); the other channels are y.  Pairs
+ * are (i, i + rot_dim / 2), with interleaved = 1 (2i, 2i + 1).  The angle of pair
+ * i is positions[row] * turns[i], turns [rot_dim / 2] being the fraction of a full
+ * turn per position in units of 2^-64; whole turns fall away in the product, so
+ * it is exact for every position.  fp32 from the input to one rounding.  Rows of
+ * negative positions are passed on as they are.  Row r starts at element r *
+ * stride, heads one after the other.  A result may lie where its input does (one
+ * pointer, one stride), else not overlap an input or the other result.  Either
+ * side may have no heads.  head_dim <= 256, n_rows <= 2^23. */
+int lhq_rope_f32(const float* q, int64_t q_stride, const float* k, int64_t k_stride,
+                 const int32_t* positions, const uint64_t* turns, const float* q_weight,
+                 const float* k_weight, float eps, float gain, float* q_out, int64_t q_out_stride,
+                 float* k_out, int64_t k_out_stride, int interleaved, int n_rows, int n_heads,
+                 int n_kv_heads, int head_dim, int rot_dim, void* stream);
+int lhq_rope_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride,
+                  const int32_t* positions, const uint64_t* turns, const uint16_t* q_weight,
+                  const uint16_t* k_weight, float eps, float gain, uint16_t* q_out,
+                  int64_t q_out_stride, uint16_t* k_out, int64_t k_out_stride, int interleaved,
+                  int n_rows, int n_heads, int n_kv_heads, int head_dim, int rot_dim, void* stream);
+/* Causal attention of any number of new tokens a sequence:  out = softmax(scale *
+ * q K^T) V per query head, query head i reading kv head i / (n_heads /
+ * n_kv_heads); bf16 in and out, fp32 sums.  New token i of a sequence sees its new
+ * tokens 0 .. i and, in lhq_kv_prefill_bf16, before them the first lengths[s]
+ * tokens of the cache (clamped to [0, 64 * max_pages]; those of a missing page are
+ * not seen).  k_new, v_new both NULL there: only the cache is seen.  A row that
+ * sees nothing gives zeros, rows of no sequence are left as they are; what a row
+ * does not see, whatever it holds, changes nothing of its result.  Offsets,
+ * strides, scale, table and cache as for lhq_kv_attn_bf16, which is the faster for
+ * a few new tokens a sequence.  out [row_capacity, n_heads, head_dim].  Rounding:
+ * queries, keys and codes enter the products as they are; a softmax weight, of a
+ * cached token times the scale of its value, is rounded to bf16 (2^-8 of itself);
+ * scores and sums are fp32, the result is rounded once more to bf16.
+ * workspace: where there are few rows their keys are split over workgroups, whose
+ * partial sums meet there and are added in order of position (deterministic).  Up
+ * to lhq_prefill_workspace_bytes bytes are used; with less, or NULL, there are
+ * fewer splits or none.  Device memory, 16-byte aligned, any contents, not shared
+ * with a call running concurrently. */
+int64_t lhq_prefill_workspace_bytes(int n_seqs, int row_capacity, int n_heads, int n_kv_heads,
+                                    int head_dim);
+int lhq_attn_prompt_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride,
+                         const uint16_t* v, int64_t v_stride, const int32_t* offsets, uint16_t* out,
+                         int n_seqs, int row_capacity, int n_heads, int n_kv_heads, int head_dim,
+                         float scale, void* workspace, int64_t workspace_bytes, void* stream);
+int lhq_kv_prefill_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k_new,
+                        int64_t k_stride, const uint16_t* v_new, int64_t v_stride,
+                        const int32_t* offsets, const int32_t* lengths, const int32_t* block_table,
+                        const uint8_t* k_codes, const float* k_scales, const uint8_t* v_codes,
+                        const float* v_scales, uint16_t* out, int format, int n_seqs,
+                        int row_capacity, int max_pages, int num_pages, int n_heads, int n_kv_heads,
+                        int head_dim, float scale, void* workspace, int64_t workspace_bytes,
+                        void* stream);
+
 /* ---- fp32 GEMM: gemm.hpp:13-29 / gemm.cpp:5-75 -------------------------- */
 /* lh::gemm semantics (beta first; beta == 0 never reads C). */
 int lhq_gemm_f32(const float* A, const float* B, float* C, int M, int N, int K,

@@ -92,6 +92,12 @@ SIGNATURES = {
     "lhq_kv_read_bf16": [_p] * 9 + [_i] * 7 + [_p],
     "lhq_kv_attn_workspace_bytes": [_i] * 7,
     "lhq_kv_attn_bf16": [_p, _i64, _p, _i64, _p, _i64] + [_p] * 9 + [_i] * 9 + [_f, _p, _i64, _p],
+    "lhq_kv_plan": [_p] * 10 + [_i] * 4 + [_p],
+    "lhq_rope_f32": [_p, _i64, _p, _i64] + [_p] * 4 + [_f, _f] + [_p, _i64, _p, _i64] + [_i] * 6 + [_p],
+    "lhq_rope_bf16": [_p, _i64, _p, _i64] + [_p] * 4 + [_f, _f] + [_p, _i64, _p, _i64] + [_i] * 6 + [_p],
+    "lhq_prefill_workspace_bytes": [_i] * 5,
+    "lhq_attn_prompt_bf16": [_p, _i64] * 3 + [_p] * 2 + [_i] * 5 + [_f, _p, _i64, _p],
+    "lhq_kv_prefill_bf16": [_p, _i64] * 3 + [_p] * 8 + [_i] * 8 + [_f, _p, _i64, _p],
     "lhq_gemm_f32": [_p, _p, _p, _i, _i, _i, _f, _f, _p],
     "lhq_gemm_f32_ref": [_p, _p, _p, _i, _i, _i, _f, _f, _p],
     "lhq_gemm_f32_batched": [_p, _p, _p, _i, _i, _i, _i, _f, _f, _p],
@@ -118,6 +124,7 @@ _RESTYPES = {
     "lhq_kv_codes_bytes": _i64,
     "lhq_kv_scales_bytes": _i64,
     "lhq_kv_attn_workspace_bytes": _i64,
+    "lhq_prefill_workspace_bytes": _i64,
     "lhq_gemm_w4a16_workspace_bytes": _i64,
     "lhq_gemm_w4a16_bf16_workspace_bytes": _i64,
     "lhq_gemm_w4a16_bf16_grouped_workspace_bytes": _i64,

@@ -98,7 +98,6 @@ __device__ __forceinline__ int split_count(const AttnArgs& a, int length) {
     const int pages = (length + kKvPage - 1) / kKvPage;
     return max(1, (pages + a.pages_per_split - 1) / a.pages_per_split);
 }
-__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Four codes as two pairs of bf16 or of fp16 (exact either way).
 template <bool FP8>
@@ -133,33 +132,6 @@ __device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {  // rounds to
 __device__ __forceinline__ f32x4_t mfma_f16_16x16x32(u32x4_t a, u32x4_t b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
                                                   0, 0, 0);
-}
-
-// Eight bf16 of a row from channel ch on, those past D as zero: one 16-byte
-// load at any alignment, of the row's last 8 channels where fewer are left
-// (and shifted down).  SMALL: D may be under 8.
-template <bool SMALL>
-__device__ __forceinline__ u32x4_t load_channels(const uint16_t* row, int ch, int D) {
-    uint64_t w[2] = {0, 0};
-    if (SMALL && D < 8) {
-        if (ch == 0)
-#pragma unroll 1
-            for (int j = D - 1; j >= 0; --j) {
-                w[1] = (w[1] << 16) | (w[0] >> 48);
-                w[0] = (w[0] << 16) | row[j];
-            }
-    } else {
-        const int at = min(ch, D - 8), down = 16 * (ch - at), by = down & 63;
-        __builtin_memcpy(w, row + at, 16);
-        if (D % 8) {
-            const uint64_t lo = down >= 64 ? w[1] : w[0], hi = down >= 64 ? 0 : w[1];
-            w[0] = (lo >> by) | ((hi << 1) << (63 - by));
-            w[1] = hi >> by;
-        }
-        if (ch >= D) w[0] = w[1] = 0;
-    }
-    return {static_cast<uint32_t>(w[0]), static_cast<uint32_t>(w[0] >> 32), static_cast<uint32_t>(w[1]),
-            static_cast<uint32_t>(w[1] >> 32)};
 }
 
 // The arguments once more, from where the launch left them: a kernel that

@@ -111,6 +111,35 @@ __device__ __forceinline__ KvUnit kv_find_unit(uint32_t unit, int n_seqs, Count 
     return {n_seqs, 0, 0};
 }
 
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Eight bf16 of a row from channel ch on, those past D as zero: one 16-byte
+// load at any alignment, of the row's last 8 channels where fewer are left
+// (and shifted down).  SMALL: D may be under 8.
+template <bool SMALL>
+__device__ __forceinline__ u32x4_t load_channels(const uint16_t* row, int ch, int D) {
+    uint64_t w[2] = {0, 0};
+    if (SMALL && D < 8) {
+        if (ch == 0)
+#pragma unroll 1
+            for (int j = D - 1; j >= 0; --j) {
+                w[1] = (w[1] << 16) | (w[0] >> 48);
+                w[0] = (w[0] << 16) | row[j];
+            }
+    } else {
+        const int at = min(ch, D - 8), down = 16 * (ch - at), by = down & 63;
+        __builtin_memcpy(w, row + at, 16);
+        if (D % 8) {
+            const uint64_t lo = down >= 64 ? w[1] : w[0], hi = down >= 64 ? 0 : w[1];
+            w[0] = (lo >> by) | ((hi << 1) << (63 - by));
+            w[1] = hi >> by;
+        }
+        if (ch >= D) w[0] = w[1] = 0;
+    }
+    return {static_cast<uint32_t>(w[0]), static_cast<uint32_t>(w[0] >> 32), static_cast<uint32_t>(w[1]),
+            static_cast<uint32_t>(w[1] >> 32)};
+}
+
 // Checks that all entry points of the cache share; `fn` names the caller.
 inline int kv_check(const char* fn, const KvCache& c, int format, int n_seqs, int row_capacity) {
     LHQ_REQUIRE(format == LHQ_KV_INT8 || format == LHQ_KV_FP8, "%s: unknown cache format %d", fn, format);

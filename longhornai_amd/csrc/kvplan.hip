@@ -1,0 +1,229 @@
+// kvplan.hip -- a serving step's tables from the requests' lengths, for gfx950:
+// pages handed back and out, offsets, positions and cache slots of the new
+// rows (lhq_kv_plan).
+//
+// The free pages are a stack.  Pages of sequences that are over are pushed in
+// order of sequence and page, then those of new tokens are popped in that order
+// (all pushes come first, whatever the order of sequences), so every entry's
+// place follows from prefix sums and no atomic decides anything.  The sums run
+// over all sequences, so one workgroup does them; the rows, which only read
+// what it wrote, are done by it too where they are few and by a launch of their
+// own where they are many.
+#include <algorithm>
+
+#include "kvcommon.hpp"
+
+namespace lhq {
+namespace {
+
+constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+// Rows that the planning workgroup does itself: four a thread.
+constexpr int kPlanRows = 4 * kPlanThreads;
+constexpr int kRowThreads = 256;
+
+struct PlanArgs {
+    const int32_t* lengths;
+    const int32_t* new_tokens;
+    const uint64_t* tree;
+    const int32_t* left;
+    int32_t* left_out;
+    int32_t* free_pages;
+    int32_t* table;
+    int32_t* offsets;
+    int32_t* positions;
+    int64_t* slots;
+    int n_seqs, capacity, max_pages, num_pages;
+};
+
+// Tokens that a sequence holds, as its table row can name them.
+__device__ __forceinline__ int held(const PlanArgs& a, int s) {
+    return static_cast<int>(min<int64_t>(max(a.lengths[s], 0), static_cast<int64_t>(a.max_pages) * kKvPage));
+}
+__device__ __forceinline__ int pages_of(int64_t tokens) { return static_cast<int>((tokens + kKvPage - 1) / kKvPage); }
+
+// Sums over the threads before this one (below 2^32 in all, else held there);
+// `total` is that of all threads.
+__device__ __forceinline__ uint32_t scan_before(uint32_t x, uint32_t* lds, uint32_t& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t upto = kv_scan(x);
+    __syncthreads();  // (lds may still be read)
+    if (lane == 63) lds[wave] = upto;
+    __syncthreads();
+    uint32_t before = 0;
+    total = 0;
+    for (int w = 0; w < kPlanWaves; ++w) {
+        if (w == wave) before = total;
+        total = __builtin_elementwise_add_sat(total, lds[w]);
+    }
+    return __builtin_elementwise_add_sat(before, upto - x);
+}
+
+// Row r: the last sequence whose offset is not over r owns it, if its rows
+// reach that far.
+__device__ __forceinline__ void plan_row(const PlanArgs& a, const int32_t* offsets, int r) {
+    int lo = 0, hi = a.n_seqs;  // offsets[lo] <= r (offsets[0] = 0), offsets[hi] > r or hi = n_seqs
+    while (hi - lo > 1) {
+        const int mid = lo + (hi - lo) / 2;
+        if (offsets[mid] <= r) lo = mid;
+        else hi = mid;
+    }
+    int position = -1;
+    int64_t slot = -1;
+    if (a.n_seqs > 0 && r < offsets[lo + 1]) {
+        const int first = offsets[lo], length = held(a, lo), i = r - first;
+        const int64_t at = static_cast<int64_t>(length) + i, p = at / kKvPage;
+        int64_t depth = i;
+        if (a.tree) {  // ancestors of a drafted token, itself among them
+            const int T = min(offsets[lo + 1] - first, 64);
+            const uint64_t own = T == 64 ? ~uint64_t{0} : (uint64_t{1} << T) - 1;
+            depth = max(static_cast<int>(__popcll(a.tree[r] & own)) - 1, 0);
+        }
+        position = static_cast<int>(min<int64_t>(length + depth, INT32_MAX));
+        const int page = p < a.max_pages ? a.table[static_cast<int64_t>(lo) * a.max_pages + p] : -1;
+        if (page >= 0 && page < a.num_pages) slot = static_cast<int64_t>(page) * kKvPage + at % kKvPage;
+    }
+    a.positions[r] = position;
+    if (a.slots) a.slots[r] = slot;
+}
+
+// ROWS: the rows too (n_seqs <= kPlanThreads, capacity <= kPlanRows).
+template <bool ROWS>
+__global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
+    __shared__ uint32_t sums[kPlanWaves];
+    __shared__ int first[kPlanThreads], count[kPlanThreads], rank[kPlanThreads];
+    __shared__ int offs[kPlanThreads + 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t have = static_cast<uint32_t>(min(max(a.left[0], 0), a.num_pages));  // pages on the stack
+
+    // Pages of sequences that are over, 1024 sequences at a time.
+    for (int base = 0; base < a.n_seqs; base += kPlanThreads) {
+        const int s = base + static_cast<int>(threadIdx.x);
+        const int had = s < a.n_seqs && a.new_tokens[s] < 0 ? pages_of(held(a, s)) : 0;
+        if (!__syncthreads_or(had)) continue;
+        first[threadIdx.x] = had;
+        __syncthreads();
+        // valid entries of each, a wave a sequence
+        for (int i = wave; i < kPlanThreads; i += kPlanWaves) {
+            const int n = first[i];
+            int valid = 0;
+            for (int p = 0; p < n; p += 64) {
+                const int id = p + lane < n ? a.table[static_cast<int64_t>(base + i) * a.max_pages + p + lane] : -1;
+                valid += __popcll(__ballot(id >= 0 && id < a.num_pages));
+            }
+            if (lane == 0) count[i] = valid;
+        }
+        __syncthreads();
+        uint32_t total;
+        const uint32_t before = scan_before(static_cast<uint32_t>(count[threadIdx.x]), sums, total);
+        rank[threadIdx.x] = static_cast<int>(min(before, 0x7fffffffu));
+        __syncthreads();
+        for (int i = wave; i < kPlanThreads; i += kPlanWaves) {
+            const int n = first[i];
+            int64_t at = static_cast<int64_t>(have) + rank[i];
+            for (int p = 0; p < n; p += 64) {
+                const int id = p + lane < n ? a.table[static_cast<int64_t>(base + i) * a.max_pages + p + lane] : -1;
+                const bool valid = id >= 0 && id < a.num_pages;
+                const uint64_t all = __ballot(valid);
+                const int64_t to = at + __popcll(all & ((uint64_t{1} << lane) - 1));
+                // (more pages than there are: some were handed back twice; the stack keeps to its size)
+                if (valid && to < a.num_pages) a.free_pages[to] = id;
+                at += __popcll(all);
+            }
+        }
+        have = min(__builtin_elementwise_add_sat(have, total), static_cast<uint32_t>(a.num_pages));
+        __syncthreads();
+    }
+
+    // Offsets, and the new tokens' pages.
+    uint32_t rows = 0, asked = 0;
+    for (int base = 0; base < a.n_seqs; base += kPlanThreads) {
+        const int s = base + static_cast<int>(threadIdx.x);
+        const uint32_t want = s < a.n_seqs ? static_cast<uint32_t>(max(a.new_tokens[s], 0)) : 0u;
+        uint32_t total;
+        const uint32_t cap = static_cast<uint32_t>(a.capacity);
+        const uint32_t before = __builtin_elementwise_add_sat(rows, scan_before(want, sums, total));
+        const int lo = static_cast<int>(min(before, cap)), hi = static_cast<int>(min(__builtin_elementwise_add_sat(before, want), cap));
+        rows = __builtin_elementwise_add_sat(rows, total);
+        int from = 0, takes = 0;
+        if (s < a.n_seqs) {
+            a.offsets[s + 1] = hi;
+            if (s == 0) a.offsets[0] = 0;
+            if constexpr (ROWS) {
+                offs[s + 1] = hi;
+                if (s == 0) offs[0] = 0;
+            }
+            const int length = held(a, s);
+            from = pages_of(length);
+            if (hi > lo) takes = max(min(pages_of(static_cast<int64_t>(length) + hi - lo), a.max_pages) - from, 0);
+        }
+        const uint32_t mine = __builtin_elementwise_add_sat(asked, scan_before(static_cast<uint32_t>(takes), sums, total));
+        asked = __builtin_elementwise_add_sat(asked, total);
+        auto take = [&](int seq, int p, uint32_t nth) {
+            a.table[static_cast<int64_t>(seq) * a.max_pages + p] = nth < have ? a.free_pages[have - 1 - nth] : -1;
+        };
+        // one or two pages by the sequence's thread, more by a wave
+        if (takes <= 2) {
+            for (int i = 0; i < takes; ++i) take(s, from + i, __builtin_elementwise_add_sat(mine, static_cast<uint32_t>(i)));
+            takes = 0;
+        }
+        if (__syncthreads_or(takes)) {
+            first[threadIdx.x] = from;
+            count[threadIdx.x] = takes;
+            rank[threadIdx.x] = static_cast<int>(mine);
+            __syncthreads();
+            for (int i = wave; i < kPlanThreads; i += kPlanWaves)
+                for (int p = lane; p < count[i]; p += 64)
+                    take(base + i, first[i] + p,
+                         __builtin_elementwise_add_sat(static_cast<uint32_t>(rank[i]), static_cast<uint32_t>(p)));
+        }
+    }
+    __syncthreads();  // (left may be left_out: everyone has read it)
+    if (threadIdx.x == 0) {
+        a.left_out[0] = static_cast<int32_t>(have - min(have, asked));
+        a.left_out[1] = static_cast<int32_t>(min(asked - min(have, asked), 0x7fffffffu));
+        if (a.n_seqs == 0) a.offsets[0] = 0;
+    }
+    if constexpr (ROWS) {
+        for (int r = threadIdx.x; r < a.capacity; r += kPlanThreads) plan_row(a, offs, r);
+    }
+}
+
+__global__ __launch_bounds__(kRowThreads) void kv_plan_rows_kernel(PlanArgs a) {
+    const int r = static_cast<int>(blockIdx.x * kRowThreads + threadIdx.x);
+    if (r < a.capacity) plan_row(a, a.offsets, r);
+}
+
+}  // namespace
+}  // namespace lhq
+
+using namespace lhq;
+
+extern "C" int lhq_kv_plan(const int32_t* lengths, const int32_t* new_tokens, const uint64_t* tree,
+                           const int32_t* left, int32_t* left_out, int32_t* free_pages, int32_t* block_table,
+                           int32_t* offsets, int32_t* positions, int64_t* slots, int n_seqs, int row_capacity,
+                           int max_pages, int num_pages, void* stream) {
+    const char* fn = "kv_plan";
+    LHQ_REQUIRE(n_seqs >= 0 && row_capacity >= 0, "%s: bad counts (%d sequences, %d rows)", fn, n_seqs, row_capacity);
+    LHQ_REQUIRE(max_pages >= 0 && num_pages >= 0, "%s: bad page counts (%d of a sequence, %d in all)", fn, max_pages,
+                num_pages);
+    LHQ_SUPPORTED(static_cast<int64_t>(max_pages) * kKvPage < (int64_t{1} << 31), "%s: sequences of 2^31 tokens", fn);
+    LHQ_SUPPORTED(row_capacity <= INT32_MAX - kPlanRows && n_seqs <= INT32_MAX - kPlanThreads,
+                  "%s: %d rows of %d sequences are over 2^31 - 4097 or 2^31 - 1025", fn, row_capacity, n_seqs);
+    LHQ_REQUIRE(left && left_out && offsets, "%s: null pointer", fn);
+    LHQ_REQUIRE(n_seqs == 0 || (lengths && new_tokens), "%s: null lengths", fn);
+    LHQ_REQUIRE(num_pages == 0 || free_pages, "%s: null list of free pages", fn);
+    LHQ_REQUIRE(n_seqs == 0 || max_pages == 0 || block_table, "%s: null block table", fn);
+    LHQ_REQUIRE(row_capacity == 0 || positions, "%s: null positions", fn);
+    const PlanArgs a{lengths, new_tokens, tree,  left,   left_out,     free_pages, block_table,
+                     offsets, positions,  slots, n_seqs, row_capacity, max_pages,  num_pages};
+    const hipStream_t s = as_stream(stream);
+    if (n_seqs <= kPlanThreads && row_capacity <= kPlanRows) {
+        kv_plan_kernel<true><<<1, kPlanThreads, 0, s>>>(a);
+        return check_launch(fn);
+    }
+    kv_plan_kernel<false><<<1, kPlanThreads, 0, s>>>(a);
+    if (int st = check_launch(fn)) return st;
+    if (row_capacity == 0) return LHQ_OK;
+    kv_plan_rows_kernel<<<(row_capacity + kRowThreads - 1) / kRowThreads, kRowThreads, 0, s>>>(a);
+    return check_launch(fn);
+}

@@ -1,0 +1,697 @@
+// prefill.hip -- causal attention of prompts and of prompts' chunks, with the
+// paged 8-bit cache (layout in kvcommon.hpp) or without, for gfx950.
+//
+//   s_j = scale * q . k_j           over the sequence's cached tokens and its new
+//   o   = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m)     ones up to the token itself
+//
+// One pass with a running maximum and sum.  A workgroup has 256 (new token, query
+// head) rows of one kv head, eight waves of 32 rows each, and walks the keys 64 at
+// a time: pages of the cache, then tiles of the new tokens.  A tile comes to LDS
+// once for all waves, in bf16 (codes are exact there), while they work on the one
+// before it.  Both products are 32x32x16 MFMAs on transposed tiles: S^T = K Q^T
+// leaves a lane with 4 adjacent keys of one row, four times over, which is what it
+// needs as the B operand of O^T = V^T P^T when V^T's keys come in that order; a
+// row's maximum and sum are one register each.
+// Precision: scores, weights' sums and results are fp32; a weight (of a cached
+// token, times its value scale) is rounded once to bf16, which has the range of
+// both and needs no exponent of its own, at 2^-8 of itself; the result is rounded
+// to bf16.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "kvcommon.hpp"
+
+namespace lhq {
+namespace {
+
+#define LHQ_LDS_AS __attribute__((address_space(3)))
+typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+
+constexpr int kWaves = 8, kThreads = 64 * kWaves;
+constexpr int kRows = 32 * kWaves;  // of a workgroup
+// The running maximum follows the scores only when one is over it by more than
+// 2^kLag: weights go up to 2^kLag, which costs none of their bits.
+constexpr float kLag = 6.0f;
+constexpr int kMostSplits = 64;  // of a block's keys
+constexpr int kLeastTiles = 16;  // of a split: the launch that joins takes as long as some tiles
+constexpr int kJoinRows = 64;    // of a workgroup that joins splits
+
+struct PrefillArgs {
+    const uint16_t* q;
+    int64_t q_stride;
+    const uint16_t* k_new;
+    int64_t k_stride;
+    const uint16_t* v_new;
+    int64_t v_stride;
+    const int32_t* offsets;
+    const int32_t* lengths;
+    KvCache c;
+    uint16_t* out;
+    int n_seqs, capacity, heads, group;  // group: query heads of a kv head
+    float scale2;          // scale * log2 e: weights are powers of two
+    bool vec_new;          // rows of k_new, v_new: 16-byte loads
+    bool vec_out;          // rows of out: 16-byte stores
+    int slots;             // workgroups of a kv head that splitting aims at, 0: no splitting
+    int part_rows;         // rows of a part in the workspace
+    float* ws_o;           // [kv head][part][part_rows][Dp]
+    float* ws_ml;          // [kv head][part][part_rows] {maximum, sum}
+};
+
+// Bytes of LDS: two tiles of keys and values, two of factors, a flag.
+template <int KS>
+constexpr int lds_bytes() { return 2 * (2 * KS * 4096 + 512) + 16; }
+
+// A sequence: its first row, new tokens, cached tokens; the list of blocks.
+struct Seq {
+    int lo, T, L, blocks, tiles;
+};
+__device__ __forceinline__ Seq seq_of(const PrefillArgs& a, int s) {
+    if (s >= a.n_seqs) return {0, 0, 0, 0, 0};
+    const KvRows r = kv_rows(a.offsets, s, a.capacity);
+    Seq q;
+    q.lo = r.lo;
+    q.T = r.hi - r.lo;
+    q.L = a.c.max_pages == 0 ? 0 : static_cast<int>(min<int64_t>(max(a.lengths[s], 0), static_cast<int64_t>(a.c.max_pages) * kKvPage));
+    q.blocks = (q.T * a.group + kRows - 1) / kRows;
+    q.tiles = (q.L + kKvPage - 1) / kKvPage + (a.k_new ? (q.T + kKvPage - 1) / kKvPage : 0);
+    return q;
+}
+// Tiles that a split has at least: all blocks' tiles over the workgroups wanted.
+// Blocks that have more are split, into less than 2 * slots parts in all (a block
+// of t > target tiles has ceil(t / target) < 2 t / target of them).
+__device__ __forceinline__ int split_target(const PrefillArgs& a, const Seq& first) {
+    if (a.slots == 0) return INT32_MAX;
+    double work = 0.0;
+    for (int base = 0; base < a.n_seqs; base += 64) {
+        const Seq q = base == 0 ? first : seq_of(a, base + (threadIdx.x & 63));
+        work += static_cast<double>(q.blocks) * q.tiles;
+    }
+    for (int d = 32; d; d >>= 1) work += __shfl_xor(work, d, 64);
+    return max(kLeastTiles, static_cast<int>(min(work / a.slots, 2147483000.0)) + 1);
+}
+__device__ __forceinline__ int split_count(const Seq& q, int target) {
+    return q.tiles <= target ? 1 : min((q.tiles + target - 1) / target, kMostSplits);
+}
+// The unit with number `unit` in the list that has count(sequence, splits) units
+// of each sequence in turn: the sequence, the unit's number within it, and the
+// parts (split blocks times their splits) of the sequences before it.  seq =
+// n_seqs past the end of the list.
+struct Found { int seq, nth, splits, parts; Seq q; };
+template <typename Count>
+__device__ __forceinline__ Found find_unit(const PrefillArgs& a, uint32_t unit, Count count) {
+    const int lane = threadIdx.x & 63;
+    const Seq first = seq_of(a, lane);
+    const int target = split_target(a, first);
+    uint32_t parts = 0;
+    for (int base = 0; base < a.n_seqs; base += 64) {
+        const Seq q = base == 0 ? first : seq_of(a, base + lane);
+        const int splits = split_count(q, target);
+        const uint32_t sum = kv_scan(count(q, splits)), own = splits > 1 ? q.blocks * splits : 0, upto = kv_scan(own);
+        const uint64_t over = __ballot(sum > unit);
+        if (over) {
+            const int l = __builtin_ctzll(over);
+            auto of = [l](int x) { return __builtin_amdgcn_readlane(x, l); };
+            const uint32_t before = l > 0 ? __builtin_amdgcn_readlane(sum, l - 1) : 0u;
+            return {base + l, static_cast<int>(unit - before), of(splits), static_cast<int>(parts) + of(upto - own),
+                    {of(q.lo), of(q.T), of(q.L), of(q.blocks), of(q.tiles)}};
+        }
+        unit -= __builtin_amdgcn_readlane(sum, 63);
+        parts += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return {a.n_seqs, 0, 1, 0, {0, 0, 0, 0, 0}};
+}
+
+// ---- tiles in LDS -----------------------------------------------------------
+// Keys, and values of new tokens: [32 channels][64 tokens][64 bytes], the 16-byte
+// chunk j of token t at place j ^ ((t >> 2) & 3): the 16 lanes of an operand read
+// that LDS serves at a time have one chunk of 16 tokens, which lie in 16 different
+// places of 256 bytes.
+// Values of cached tokens: [channel][128 bytes], the chunk of keys 16 s + {4 h ..
+// 4 h + 3, 8 + 4 h .. + 3} at place (2 s + h) ^ ((channel >> 1) & 7), as above.
+__device__ __forceinline__ int token_place(int t, int chunk) { return t * 64 + 16 * (chunk ^ ((t >> 2) & 3)); }
+__device__ __forceinline__ int value_place(int ch, int chunk) { return ch * 128 + 16 * (chunk ^ ((ch >> 1) & 7)); }
+
+__device__ __attribute__((aligned(16))) const uint32_t kZeros[4] = {0, 0, 0, 0};
+
+// 16 bytes a lane from its address to `to` + 16 * lane.
+__device__ __forceinline__ void dma16(const void* from, void* to) {
+    __builtin_amdgcn_global_load_lds(from, (LHQ_LDS_AS void*)to, 16, 0, 0);
+}
+
+// New tokens j0 .. j0 + 63 of a sequence of T from row lo on, kv head h, to LDS.
+// Tokens past the last one are that one again (no row sees them); channels past D
+// are zero in keys and anything in values, whose results there are not kept.
+template <int KS>
+__device__ __forceinline__ void stage_new(const PrefillArgs& a, int lo, int T, int h, int j0, uint8_t* keys, uint8_t* values) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), D = a.c.D;
+    if (a.vec_new) {
+        const int t = 16 * (wave & 3) + (lane >> 2), j = (lane & 3) ^ ((lane >> 4) & 3);
+        const int64_t row = lo + min(j0 + t, T - 1);
+        const uint16_t* k = a.k_new + row * a.k_stride + h * D;
+        const uint16_t* v = a.v_new + row * a.v_stride + h * D;
+#pragma unroll
+        for (int m = 0; m < (KS + 1) / 2; ++m) {
+            const int kb = (wave >> 2) + 2 * m, ch = 32 * kb + 8 * j, at = 4096 * kb + 1024 * (wave & 3);
+            if (kb >= KS) break;
+            dma16(ch < D ? static_cast<const void*>(k + ch) : kZeros, keys + at);
+            dma16(v + min(ch, D - 8), values + at);
+        }
+    } else {
+        for (int n = threadIdx.x; n < 64 * 4 * KS; n += kThreads) {
+            const int t = n & 63, ch = 8 * (n >> 6);
+            const int64_t row = lo + min(j0 + t, T - 1);
+            const int at = (ch >> 5) * 4096 + token_place(t, (ch >> 3) & 3);
+            *reinterpret_cast<u32x4_t*>(keys + at) = load_channels<KS == 1>(a.k_new + row * a.k_stride + h * D, ch, D);
+            *reinterpret_cast<u32x4_t*>(values + at) = load_channels<KS == 1>(a.v_new + row * a.v_stride + h * D, ch, D);
+        }
+    }
+}
+
+// Four codes as two pairs of bf16 (exact).
+template <bool FP8>
+__device__ __forceinline__ u32x2_t codes_bf16(uint32_t w) {
+    if constexpr (FP8) {
+        return {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false)),
+                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))};
+    } else {
+        auto f = [w](int j) { return static_cast<float>(static_cast<int8_t>(w >> (8 * j))); };
+        return {pack_bf16x2(f(0), f(1)), pack_bf16x2(f(2), f(3))};
+    }
+}
+
+// A page on its way: 32 codes of keys (a token's 32 channels) or of values (a
+// channel's 32 keys of one half) a thread and task, and a scale.
+template <int KS>
+struct PageLoad {
+    static constexpr int kTasks = (KS + 3) / 4;
+    u32x4_t w[kTasks][2];
+    float factor;
+
+    __device__ __forceinline__ void load(const KvCache& c, int page, int h) {
+        const uint8_t *k = c.k + c.code_base(page, h), *v = c.v + c.code_base(page, h);
+        const int tid = threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < kTasks; ++i) {
+            const int n = tid + kThreads * i;  // (the same side for all of a wave)
+            if (n < 64 * KS) {
+                w[i][0] = *reinterpret_cast<const u32x4_t*>(k + 32 * n);
+                w[i][1] = *reinterpret_cast<const u32x4_t*>(k + 32 * n + 16);
+            } else if (n < 128 * KS) {
+                const int m = n - 64 * KS;  // channel m >> 1, keys' half m & 1
+                w[i][0] = *reinterpret_cast<const u32x4_t*>(v + 64 * (m >> 1) + 16 * (m & 1));
+                w[i][1] = *reinterpret_cast<const u32x4_t*>(v + 64 * (m >> 1) + 16 * (m & 1) + 32);
+            }
+        }
+        if (tid < 64) factor = c.ks[c.scale_base(page, h) + tid];
+        else if (tid < 128) factor = c.vs[c.scale_base(page, h) + tid - 64];
+    }
+    // `left` tokens of the page count; codes and value scales of the others become zero.
+    template <bool FP8>
+    __device__ __forceinline__ void store(int left, float scale2, uint8_t* keys, uint8_t* values, float* factors) {
+        const int tid = threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < kTasks; ++i) {
+            const int n = tid + kThreads * i;
+            if (n < 64 * KS) {
+                const int t = n / KS, kb = n % KS;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const u32x2_t lo = codes_bf16<FP8>(w[i][j >> 1][2 * (j & 1)]), hi = codes_bf16<FP8>(w[i][j >> 1][2 * (j & 1) + 1]);
+                    *reinterpret_cast<u32x4_t*>(keys + 4096 * kb + token_place(t, j)) = u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+                }
+            } else if (n < 128 * KS) {
+                const int m = n - 64 * KS, ch = m >> 1, half = m & 1;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    uint32_t x = w[i][0][s], y = w[i][1][s];  // keys 16 s + 4 half on, and 8 further
+                    if (left < kKvPage) {
+                        auto keep = [left](uint32_t codes, int t) {
+                            const int in = left - t;
+                            return in >= 4 ? codes : in <= 0 ? 0u : codes & ((1u << (8 * in)) - 1);
+                        };
+                        x = keep(x, 16 * s + 4 * half);
+                        y = keep(y, 16 * s + 4 * half + 8);
+                    }
+                    const u32x2_t lo = codes_bf16<FP8>(x), hi = codes_bf16<FP8>(y);
+                    *reinterpret_cast<u32x4_t*>(values + value_place(ch, 2 * s + half)) = u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+                }
+            }
+        }
+        if (tid < 64) factors[tid] = factor * scale2;
+        else if (tid < 128) factors[tid] = tid - 64 < left ? factor : 0.0f;
+    }
+};
+
+// The halves of a dword that are bf16 infinities or NaN, as a mask.
+__device__ __forceinline__ uint32_t odd_halves(uint32_t w) {
+    return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+}
+// A product with a zero weight would make NaN of such a value: in tiles that some
+// row does not see whole, they become zeros here (each wave those that it brought)
+// and are added at the end to the rows that see them.  Returns whether there were any.
+template <int KS>
+__device__ __forceinline__ bool clear_odd(const PrefillArgs& a, uint8_t* values) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    bool any = false;
+    auto clear = [&](uint8_t* at) {
+        u32x4_t w = *reinterpret_cast<const u32x4_t*>(at), bad;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bad[j] = odd_halves(w[j]);
+        if ((bad[0] | bad[1] | bad[2] | bad[3]) == 0) return;
+        any = true;
+        *reinterpret_cast<u32x4_t*>(at) = w & ~bad;
+    };
+    if (a.vec_new) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        for (int kb = wave >> 2; kb < KS; kb += 2) clear(values + 4096 * kb + 1024 * (wave & 3) + 16 * lane);
+    } else {
+        for (int n = threadIdx.x; n < 64 * 4 * KS; n += kThreads) clear(values + (n >> 8) * 4096 + token_place(n & 63, (n >> 6) & 3));
+    }
+    return __ballot(any) != 0;
+}
+
+// ---- a wave's rows ----------------------------------------------------------
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+
+// A wave's 32 rows: row lane & 31 is this lane's, with keys and channels 8 a + 4
+// (lane >> 5) + (0..3) of every 32.
+template <int KS>
+struct Rows {
+    static constexpr int NT = KS <= 4 ? 2 : 1;  // 32-key tiles whose scores are held at a time
+    u32x4_t q[2 * KS];
+    f32x16_t o[KS];
+    float m, above, l;  // maximum, the score that moves it, this lane's part of the weights' sum
+
+    __device__ __forceinline__ void clear() {
+        m = l = 0.0f;
+        above = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
+    }
+    // A score is over the maximum by more than 2^kLag in some row of the wave:
+    // those rows' maximum moves.  What other rows see decides nothing.
+    __device__ __forceinline__ void raise(float top) {
+        top = fmaxf(top, other_half(top));
+        if (top > above) {
+            const float f = above == -INFINITY ? 0.0f : exp2_(m - top);
+            m = top;
+            above = top + kLag;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) o[i] *= f;
+        }
+    }
+    // One tile.  masked (the same for the wave): a row sees the first `limit` keys of it.
+    template <bool CACHED>
+    __device__ __forceinline__ void step(const PrefillArgs& a, const uint8_t* keys, const uint8_t* values, const float* factors,
+                                         bool masked, int limit) {
+        const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
+        const uint8_t* k0 = keys + token_place(c, g);
+        const uint8_t* k1 = keys + token_place(c, 2 + g);
+#pragma unroll
+        for (int t0 = 0; t0 < 2; t0 += NT) {
+            f32x16_t x[NT];
+#pragma unroll
+            for (int i = 0; i < 2 * KS; ++i)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const u32x4_t k = *reinterpret_cast<const u32x4_t*>((i & 1 ? k1 : k0) + 4096 * (i >> 1) + 2048 * (t0 + t));
+                    if (i == 0)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) x[t][j] = 0.0f;
+                    x[t] = mfma_bf16_32x32x16(k, q[i], x[t]);
+                }
+            float top = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    f32x4_t f;
+                    if constexpr (CACHED) f = *reinterpret_cast<const f32x4_t*>(factors + 32 * (t0 + t) + 8 * b + 4 * g);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float y = x[t][4 * b + j];
+                        if constexpr (CACHED) y *= f[j];
+                        x[t][4 * b + j] = y;
+                    }
+                }
+            if (masked) {
+                int left = limit - 32 * t0 - 4 * g;
+                asm volatile("" : "+v"(left));  // (else made selects on every tile)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) x[t][j] = 32 * t + 8 * (j >> 2) + (j & 3) < left ? x[t][j] : -INFINITY;
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) top = fmaxf(top, x[t][j]);
+            if constexpr (!CACHED) top *= a.scale2;
+            if (__ballot(top > above)) raise(top);
+            u32x4_t p[2 * NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    f32x4_t f, y;
+                    if constexpr (CACHED) f = *reinterpret_cast<const f32x4_t*>(factors + 64 + 32 * (t0 + t) + 8 * b + 4 * g);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        y[j] = exp2_(CACHED ? x[t][4 * b + j] - m : __builtin_fmaf(x[t][4 * b + j], a.scale2, -m));
+                        l += y[j];
+                        if constexpr (CACHED) y[j] *= f[j];
+                    }
+                    p[2 * t + (b >> 1)][2 * (b & 1)] = pack_bf16x2(y[0], y[1]);
+                    p[2 * t + (b >> 1)][2 * (b & 1) + 1] = pack_bf16x2(y[2], y[3]);
+                }
+            if constexpr (CACHED) {
+#pragma unroll
+                for (int s = 0; s < 2 * NT; ++s)
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) {
+                        const u32x4_t v = *reinterpret_cast<const u32x4_t*>(values + 4096 * i + value_place(c, 2 * (2 * t0 + s) + g));
+                        o[i] = mfma_bf16_32x32x16(v, p[s], o[i]);
+                    }
+            } else {
+                // a lane's address in a transposing read: token 4 g + (lane & 15) / 4, channels 16 (lane >> 4 & 1) + 4 (lane & 3) on
+                const int tok = 4 * g + ((lane & 15) >> 2), chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+                const uint8_t* at[2] = {values + token_place(tok, chunk) + 8 * (lane & 1), values + token_place(tok + 8, chunk) + 8 * (lane & 1)};
+                auto operand = [&](int s, int i) {
+                    u32x2_t w[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        w[e] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                   (LHQ_LDS_AS s16x4_t*)(at[e] + 4096 * i + 1024 * (2 * t0 + s))));
+                    return u32x4_t{w[0][0], w[0][1], w[1][0], w[1][1]};
+                };
+#pragma unroll
+                for (int s = 0; s < 2 * NT; ++s)
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) o[i] = mfma_bf16_32x32x16(operand(s, i), p[s], o[i]);
+            }
+        }
+    }
+};
+
+// MODE 0: no cache, 1: int8, 2: e4m3.
+template <int KS, int MODE>
+__global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t prefill_lds[];
+    constexpr int kTile = KS * 4096;
+    const Found u = find_unit(a, blockIdx.y + blockIdx.z * gridDim.y,
+                              [](const Seq& q, int splits) { return static_cast<uint32_t>(q.blocks) * splits; });
+    if (u.seq >= a.n_seqs) return;
+    const int h = blockIdx.x, G = a.group, D = a.c.D, R = u.q.T * G, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // the blocks with the most keys first
+    const int block = u.q.blocks - 1 - u.nth / u.splits, split = u.nth % u.splits;
+    const int r0 = block * kRows, pages = (u.q.L + kKvPage - 1) / kKvPage;
+    const int tiles = pages + (a.k_new ? ((min(r0 + kRows, R) - 1) / G) / kKvPage + 1 : 0);
+    const int first = static_cast<int>(static_cast<int64_t>(tiles) * split / u.splits);
+    const int end = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / u.splits);
+    auto keys = [&](int buf) { return prefill_lds + buf * 2 * kTile; };
+    auto factors = [&](int buf) { return reinterpret_cast<float*>(prefill_lds + 4 * kTile) + 128 * buf; };
+    int* odd = reinterpret_cast<int*>(prefill_lds + 4 * kTile + 1024);  // infinite or NaN values were cleared
+    if (threadIdx.x == 0) *odd = 0;
+    __syncthreads();
+
+    // this wave's rows: (token, query head) pairs of the kv head; past the last one, that again, which is not kept
+    const bool some = r0 + 32 * wave < R;
+    const int r = min(r0 + 32 * wave + (lane & 31), R - 1), token = r / G;
+    const int low = __builtin_amdgcn_readlane(token, 0), high = __builtin_amdgcn_readlane(token, 31);
+    Rows<KS> z;
+    {
+        const uint16_t* from = a.q + (u.q.lo + token) * a.q_stride + static_cast<int64_t>(h * G + r - token * G) * D;
+#pragma unroll
+        for (int i = 0; i < 2 * KS; ++i) z.q[i] = load_channels<KS == 1>(from, 16 * i + 8 * (lane >> 5), D);
+    }
+    z.clear();
+
+    PageLoad<KS> page_load;
+    int ids = 0;
+    auto page_id = [&](int t) {  // 64 entries of the block table at a time, one a lane
+        if (((t - first) & 63) == 0) ids = t + lane < pages ? a.c.page(u.seq, t + lane) : -1;
+        return __builtin_amdgcn_readlane(ids, (t - first) & 63);
+    };
+    auto fetch = [&](int t, int buf) {  // returns whether the tile is there
+        if (MODE != 0 && t < pages) {
+            const int id = page_id(t);
+            if (id >= 0) page_load.load(a.c, id, h);
+            return id >= 0;
+        }
+        stage_new<KS>(a, u.q.lo, u.q.T, h, (t - pages) * kKvPage, keys(buf), keys(buf) + kTile);
+        return true;
+    };
+    // the first tile of new tokens that some row of the block does not see whole
+    const int partly = pages + (r0 / G + 1) / kKvPage;
+    auto arrive = [&](int t, int buf, bool there) {
+        if (t >= partly && clear_odd<KS>(a, keys(buf) + kTile) && lane == 0) *odd = 1;
+        if (MODE != 0 && t < pages && there)
+            page_load.template store<MODE == 2>(min(u.q.L - t * kKvPage, kKvPage), a.scale2, keys(buf), keys(buf) + kTile, factors(buf));
+    };
+    bool there = false, next_there = false;
+    if (first < end) {
+        there = fetch(first, 0);
+        arrive(first, 0, there);
+    }
+    __syncthreads();
+    for (int t = first; t < end; ++t) {
+        const int buf = (t - first) & 1;
+        if (t + 1 < end) next_there = fetch(t + 1, buf ^ 1);
+        if (some && there) {
+            const uint8_t *k = keys(buf), *v = k + kTile;
+            if (MODE != 0 && t < pages) {
+                const int left = min(u.q.L - t * kKvPage, kKvPage);
+                z.template step<true>(a, k, v, factors(buf), left < kKvPage, left);
+            } else {
+                const int j0 = (t - pages) * kKvPage;
+                if (j0 <= high) z.template step<false>(a, k, v, nullptr, j0 + kKvPage - 1 > low, token - j0 + 1);
+            }
+        }
+        if (t + 1 < end) arrive(t + 1, buf ^ 1, next_there);
+        there = next_there;
+        __syncthreads();
+    }
+
+    if (!some) return;
+    z.l += other_half(z.l);
+    const bool mine = r0 + 32 * wave + (lane & 31) < R;
+    const int g = lane >> 5;
+    if (!mine) return;
+    // Infinite or NaN values that the row sees: added to what was written (a sum
+    // with them is what they are, whatever the weight).
+    auto add_odd = [&](auto* to, auto put) {
+        if (*odd == 0) return;
+        const int last = min((end - pages) * kKvPage, token + 1);
+        for (int n = max(first, partly) * kKvPage - pages * kKvPage; n < last; ++n) {
+            const uint16_t* row = a.v_new + (u.q.lo + static_cast<int64_t>(n)) * a.v_stride + h * D;
+            for (int ch = 4 * g; ch < D; ch += ch % 4 == 3 ? 5 : 1) {
+                const float y = bf16_to_f32(row[ch]);
+                if (!(fabsf(y) < INFINITY)) put(to + ch, y);
+            }
+        }
+    };
+    if (u.splits > 1) {
+        const int64_t part = static_cast<int64_t>(h) * 2 * a.slots + u.parts + block * u.splits + split;
+        const int64_t at = part * a.part_rows + 32 * wave + (lane & 31);
+        if (g == 0) {
+            a.ws_ml[2 * at] = z.l == 0.0f ? -INFINITY : z.m;
+            a.ws_ml[2 * at + 1] = z.l;
+        }
+        float* to = a.ws_o + at * (32 * KS);
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                *reinterpret_cast<f32x4_t*>(to + 32 * i + 8 * b + 4 * g) =
+                    f32x4_t{z.o[i][4 * b], z.o[i][4 * b + 1], z.o[i][4 * b + 2], z.o[i][4 * b + 3]};
+        add_odd(to, [](float* p, float y) { *p += y; });
+        return;
+    }
+    const float by = z.l == 0.0f ? 0.0f : 1.0f / z.l;  // nothing seen: zeros
+    uint16_t* to = a.out + (static_cast<int64_t>(u.q.lo + token) * a.heads + h * G + r - token * G) * D;
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int ch = 32 * i + 8 * b + 4 * g;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (ch + j < D) to[ch + j] = f32_to_bf16(z.l == 0.0f ? 0.0f : z.o[i][4 * b + j] * by);
+        }
+    add_odd(to, [](uint16_t* p, float y) { *p = f32_to_bf16(bf16_to_f32(*p) + y); });
+}
+
+// Joins the parts of split blocks in order of position: kJoinRows rows of a
+// block a workgroup, four channels a thread at a time.
+__global__ __launch_bounds__(256) void prefill_join_kernel(PrefillArgs a) {
+    const Found u = find_unit(a, blockIdx.y + blockIdx.z * gridDim.y, [](const Seq& q, int splits) {
+        return splits > 1 ? static_cast<uint32_t>(q.blocks) * (kRows / kJoinRows) : 0u;
+    });
+    if (u.seq >= a.n_seqs) return;
+    const int h = blockIdx.x, G = a.group, D = a.c.D, Dp = a.c.Dp(), R = u.q.T * G;
+    const int block = u.nth / (kRows / kJoinRows), from = (u.nth % (kRows / kJoinRows)) * kJoinRows;
+    const int64_t part = static_cast<int64_t>(h) * 2 * a.slots + u.parts + block * u.splits;
+    for (int n = threadIdx.x; n < kJoinRows * (Dp / 4); n += 256) {
+        const int row = from + n / (Dp / 4), ch = 4 * (n % (Dp / 4)), r = block * kRows + row;
+        if (r >= R) return;
+        const int64_t at = part * a.part_rows + row;
+        float top = -INFINITY, weight = 0.0f;
+        for (int s = 0; s < u.splits; ++s) top = fmaxf(top, a.ws_ml[2 * (at + static_cast<int64_t>(s) * a.part_rows)]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < u.splits; ++s) {
+            const int64_t p = at + static_cast<int64_t>(s) * a.part_rows;
+            const float f = exp2_(a.ws_ml[2 * p] - ref);
+            weight += a.ws_ml[2 * p + 1] * f;
+            sum += *reinterpret_cast<const f32x4_t*>(a.ws_o + p * Dp + ch) * f;
+        }
+        uint16_t* out = a.out + (static_cast<int64_t>(u.q.lo + r / G) * a.heads + h * G + r % G) * D;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (ch + j < D) out[ch + j] = f32_to_bf16(weight == 0.0f ? 0.0f : sum[j] / weight);
+    }
+}
+
+// ---- host -------------------------------------------------------------------
+
+int compute_units() {
+    int dev = 0, n = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) {
+        (void)hipGetLastError();
+        return 256;
+    }
+    return n;
+}
+// Workgroups of a kv head that splitting aims at: one a CU.  None where the rows
+// fill the chip as they are, or where no block can have two splits' tiles.
+int want_slots(int capacity, int heads, int kv_heads, int64_t most_tiles) {
+    const int cus = compute_units();
+    const int64_t rows = static_cast<int64_t>(capacity) * (heads / kv_heads);
+    if (rows / kRows * kv_heads >= cus || most_tiles <= kLeastTiles) return 0;
+    return std::max(1, cus / kv_heads);
+}
+int64_t part_bytes(int rows, int D) { return static_cast<int64_t>(rows) * (kv_padded(D) + 2) * 4; }
+int part_rows(int capacity, int heads, int kv_heads) {
+    return static_cast<int>(std::min<int64_t>(kRows, static_cast<int64_t>(capacity) * (heads / kv_heads)));
+}
+
+dim3 unit_grid(int heads, int64_t units) {
+    const unsigned y = static_cast<unsigned>(std::min<int64_t>(units, 32768));
+    return dim3(heads, y, static_cast<unsigned>((units + y - 1) / y));
+}
+
+template <int KS, int MODE>
+int launch(const char* fn, const PrefillArgs& a, dim3 grid, hipStream_t s) {
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&prefill_kernel<KS, MODE>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    if (attr != hipSuccess) return set_error(LHQ_ERR_HIP, "%s: dynamic LDS attribute: %s", fn, hipGetErrorString(attr));
+    prefill_kernel<KS, MODE><<<grid, kThreads, lds_bytes<KS>(), s>>>(a);
+    return check_launch(fn);
+}
+
+bool odd(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; }
+
+int prefill(const char* fn, PrefillArgs a, int mode, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+    const int D = a.c.D, kv_heads = a.c.heads;
+    LHQ_REQUIRE(a.heads > 0 && a.heads % kv_heads == 0, "%s: %d query heads are no multiple of %d kv heads", fn, a.heads, kv_heads);
+    LHQ_SUPPORTED(a.heads <= 65535, "%s: %d query heads are over 65535", fn, a.heads);
+    a.group = a.heads / kv_heads;
+    LHQ_SUPPORTED(static_cast<int64_t>(a.capacity) * a.heads < INT32_MAX - kRows, "%s: %d rows of %d heads are over 2^31", fn, a.capacity, a.heads);
+    a.scale2 = scale * 1.4426950408889634f;  // weights are powers of two
+    LHQ_REQUIRE(std::isfinite(a.scale2) && scale > 0.0f, "%s: scale %g is not positive and finite, also times log2 e", fn, scale);
+    LHQ_REQUIRE((a.k_new == nullptr) == (a.v_new == nullptr), "%s: new keys without values, or values without keys", fn);
+    LHQ_REQUIRE(a.q_stride >= static_cast<int64_t>(a.heads) * D, "%s: q rows of stride %lld are under %d heads of %d", fn,
+                static_cast<long long>(a.q_stride), a.heads, D);
+    LHQ_REQUIRE(!a.k_new || (a.k_stride >= static_cast<int64_t>(kv_heads) * D && a.v_stride >= static_cast<int64_t>(kv_heads) * D),
+                "%s: new rows of strides %lld, %lld are under %d heads of %d", fn, static_cast<long long>(a.k_stride),
+                static_cast<long long>(a.v_stride), kv_heads, D);
+    LHQ_REQUIRE(workspace_bytes >= 0, "%s: negative workspace size", fn);
+    LHQ_REQUIRE(!odd(workspace, 16), "%s: workspace must be 16-byte aligned", fn);
+    if (a.n_seqs == 0 || a.capacity == 0) return LHQ_OK;
+    if (mode != 0)
+        if (int st = kv_check_pointers(fn, a.c)) return st;
+    LHQ_REQUIRE(a.q && a.offsets && a.out && (mode == 0 || a.lengths), "%s: null pointer", fn);
+    if (mode == 0) LHQ_REQUIRE(a.k_new, "%s: null pointer", fn);
+    if (a.c.num_pages == 0) a.c.max_pages = 0;
+    a.vec_new = D % 8 == 0 && !odd(a.k_new, 16) && !odd(a.v_new, 16) && a.k_stride % 8 == 0 && a.v_stride % 8 == 0;
+    a.vec_out = D % 8 == 0 && !odd(a.out, 16);
+    const int64_t tiles = a.c.max_pages + (a.k_new ? (static_cast<int64_t>(a.capacity) + kKvPage - 1) / kKvPage : 0);
+    a.part_rows = part_rows(a.capacity, a.heads, kv_heads);
+    // as many parts as there is room for, two a slot
+    const int64_t room = workspace ? workspace_bytes / part_bytes(a.part_rows, D) / (2 * kv_heads) : 0;
+    a.slots = static_cast<int>(std::min<int64_t>(want_slots(a.capacity, a.heads, kv_heads, tiles), room));
+    const int64_t parts = static_cast<int64_t>(kv_heads) * 2 * a.slots;
+    a.ws_o = static_cast<float*>(workspace);
+    a.ws_ml = a.ws_o + parts * a.part_rows * kv_padded(D);
+    const int64_t rows = static_cast<int64_t>(a.capacity) * a.group;
+    const int64_t units = rows / kRows + std::min(a.n_seqs, a.capacity) + 2 * a.slots;
+    LHQ_SUPPORTED(units * kv_heads < INT32_MAX / kThreads, "%s: %lld query blocks of %d heads are over the grid", fn,
+                  static_cast<long long>(units), kv_heads);
+    const dim3 grid = unit_grid(kv_heads, units);
+    const hipStream_t s = as_stream(stream);
+    int st = LHQ_OK;
+    auto go = [&](auto ks) {
+        st = mode == 0 ? launch<ks(), 0>(fn, a, grid, s) : mode == 1 ? launch<ks(), 1>(fn, a, grid, s) : launch<ks(), 2>(fn, a, grid, s);
+    };
+    switch (kv_padded(D) / 32) {
+        case 1: go(std::integral_constant<int, 1>{}); break;
+        case 2: go(std::integral_constant<int, 2>{}); break;
+        case 3: go(std::integral_constant<int, 3>{}); break;
+        case 4: go(std::integral_constant<int, 4>{}); break;
+        case 5: go(std::integral_constant<int, 5>{}); break;
+        case 6: go(std::integral_constant<int, 6>{}); break;
+        case 7: go(std::integral_constant<int, 7>{}); break;
+        default: go(std::integral_constant<int, 8>{}); break;
+    }
+    if (st != LHQ_OK || a.slots == 0) return st;
+    // (less than one split block a slot)
+    prefill_join_kernel<<<unit_grid(kv_heads, static_cast<int64_t>(a.slots) * (kRows / kJoinRows)), 256, 0, s>>>(a);
+    return check_launch(fn);
+}
+
+}  // namespace
+}  // namespace lhq
+
+using namespace lhq;
+
+extern "C" {
+
+int64_t lhq_prefill_workspace_bytes(int n_seqs, int row_capacity, int n_heads, int n_kv_heads, int head_dim) {
+    if (n_seqs <= 0 || row_capacity <= 0 || n_kv_heads <= 0 || n_kv_heads > 65535 || n_heads <= 0 || n_heads % n_kv_heads != 0 ||
+        head_dim <= 0 || head_dim > kKvMaxDim)
+        return 0;
+    return static_cast<int64_t>(n_kv_heads) * 2 * want_slots(row_capacity, n_heads, n_kv_heads, INT64_MAX) *
+           part_bytes(part_rows(row_capacity, n_heads, n_kv_heads), head_dim);
+}
+
+int lhq_attn_prompt_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride, const uint16_t* v,
+                         int64_t v_stride, const int32_t* offsets, uint16_t* out, int n_seqs, int row_capacity,
+                         int n_heads, int n_kv_heads, int head_dim, float scale, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
+    const char* fn = "attn_prompt_bf16";
+    const KvCache c{nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0, n_kv_heads, head_dim};
+    if (int st = kv_check(fn, c, LHQ_KV_INT8, n_seqs, row_capacity)) return st;
+    const PrefillArgs a{q, q_stride, k, k_stride, v, v_stride, offsets, nullptr, c, out, n_seqs, row_capacity, n_heads};
+    return prefill(fn, a, 0, scale, workspace, workspace_bytes, stream);
+}
+
+int lhq_kv_prefill_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k_new, int64_t k_stride,
+                        const uint16_t* v_new, int64_t v_stride, const int32_t* offsets, const int32_t* lengths,
+                        const int32_t* block_table, const uint8_t* k_codes, const float* k_scales,
+                        const uint8_t* v_codes, const float* v_scales, uint16_t* out, int format, int n_seqs,
+                        int row_capacity, int max_pages, int num_pages, int n_heads, int n_kv_heads, int head_dim,
+                        float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* fn = "kv_prefill_bf16";
+    const KvCache c{const_cast<uint8_t*>(k_codes), const_cast<float*>(k_scales), const_cast<uint8_t*>(v_codes),
+                    const_cast<float*>(v_scales), block_table, max_pages, num_pages, n_kv_heads, head_dim};
+    if (int st = kv_check(fn, c, format, n_seqs, row_capacity)) return st;
+    const PrefillArgs a{q, q_stride, k_new, k_stride, v_new, v_stride, offsets, lengths, c, out, n_seqs, row_capacity, n_heads};
+    return prefill(fn, a, format == LHQ_KV_FP8 ? 2 : 1, scale, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

@@ -454,3 +454,243 @@ def kv_attn(cache: KvCache, q: torch.Tensor, offsets: torch.Tensor, lengths: tor
                B, n, bound, width, cache.n_pages, heads, H, D, D ** -0.5 if scale is None else scale, P(workspace),
                nbytes, stream())
     return out
+
+
+# ---------------------------------------------------------------------------
+# A prompt's way through an attention layer
+# ---------------------------------------------------------------------------
+
+@dataclass(frozen=True)
+class KvPlan:
+    """A step's tables (lhq_kv_plan): offsets int32 [B + 1], positions int32 [n],
+    slots int64 [n], left int32 [2] (pages left, pages missing)."""
+    offsets: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+    left: torch.Tensor
+
+
+def _on_one_gpu(fn: str, *tensors: torch.Tensor | None) -> None:
+    """All of them on the current GPU, on whose stream the call is launched."""
+    at = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for t in tensors:
+        if t is not None and (t.get_device() != at or at < 0):
+            raise ValueError(f"{fn}: a tensor of {t.device}, the current GPU is {at}")
+
+
+def _packed(fn: str, name: str, t: torch.Tensor, dtype, shape) -> None:
+    if t.dtype is not dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{fn}: {name} must be contiguous {list(shape)} {dtype}, got {tuple(t.shape)} {t.dtype}")
+
+
+def kv_plan(lengths: torch.Tensor, new_tokens: torch.Tensor, free_pages: torch.Tensor, left: torch.Tensor,
+            block_table: torch.Tensor, n: int, tree: torch.Tensor | None = None,
+            out: KvPlan | None = None) -> KvPlan:
+    """A step's tables from the requests' lengths (int32 [B]): sequence s holds
+    lengths[s] tokens and gets new_tokens[s] more, or is over where that is
+    negative.  Pages go back to and come off the stack ``free_pages`` (int32, one
+    entry for each page there is), whose first left[0] entries count; block_table
+    [B, pages] gets the new ones.  n: rows there are room for.  tree (int64 [n]):
+    drafted tokens' ancestors, for their positions.  ``out`` may hold ``left``
+    itself, for tables that live from step to step."""
+    i32, shape = torch.int32, block_table.shape
+    if len(shape) != 2 or n < 0:
+        raise ValueError(f"kv_plan: block table {tuple(shape)} is not [B, pages], or {n} rows")
+    B, width = shape
+    _packed("kv_plan", "block_table", block_table, i32, (B, width))
+    _packed("kv_plan", "lengths", lengths, i32, (B,))
+    _packed("kv_plan", "new_tokens", new_tokens, i32, (B,))
+    _packed("kv_plan", "left", left, i32, (2,))
+    if free_pages.dtype is not i32 or len(free_pages.shape) != 1 or not free_pages.is_contiguous():
+        raise ValueError(f"kv_plan: free_pages must be contiguous [pages] int32, got {tuple(free_pages.shape)}")
+    if tree is not None:
+        _packed("kv_plan", "tree", tree, torch.int64, (n,))
+    if out is None:
+        out = KvPlan(lengths.new_empty(B + 1), lengths.new_empty(n), lengths.new_empty(n, dtype=torch.int64),
+                     lengths.new_empty(2))
+    else:
+        _packed("kv_plan", "out.offsets", out.offsets, i32, (B + 1,))
+        _packed("kv_plan", "out.positions", out.positions, i32, (n,))
+        _packed("kv_plan", "out.slots", out.slots, torch.int64, (n,))
+        _packed("kv_plan", "out.left", out.left, i32, (2,))
+    _on_one_gpu("kv_plan", lengths, new_tokens, free_pages, left, block_table, tree, out.offsets, out.positions,
+                out.slots, out.left)
+    lib().call("lhq_kv_plan", lengths.data_ptr(), new_tokens.data_ptr(), P(tree), left.data_ptr(), out.left.data_ptr(),
+               free_pages.data_ptr(), block_table.data_ptr(), out.offsets.data_ptr(), out.positions.data_ptr(),
+               out.slots.data_ptr(), B, n, width, free_pages.shape[0], stream())
+    return out
+
+
+@dataclass(frozen=True)
+class RopePlan:
+    """How heads are turned: for each pair of the first rot_dim channels the
+    fraction of a full turn per position, in units of 2^-64 (as int64 bits)."""
+    head_dim: int
+    rot_dim: int
+    turns: torch.Tensor
+    interleaved: bool
+    gain: float
+
+
+def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
+                     original: int = 4096, slow: float = 1.0, fast: float = 32.0) -> np.ndarray:
+    """Radians per position of each pair, theta^(-2i / rot_dim), for contexts
+    ``factor`` times the ``original`` length:
+      "linear"  all divided by factor (positions interpolated)
+      "ntk"     theta times factor^(rot_dim / (rot_dim - 2)): the slowest pair is
+                divided by factor, the fastest kept
+      "yarn"    pairs that make under ``slow`` turns in the original length divided
+                by factor, those over ``fast`` kept, between them in proportion"""
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"rope_frequencies: scaling {scaling!r} is not None, 'linear', 'ntk' or 'yarn'")
+    if rot_dim < 0 or rot_dim % 2 or not 1.0 <= theta < np.inf or not 1.0 <= factor < np.inf:
+        raise ValueError(f"rope_frequencies: rot_dim {rot_dim}, theta {theta}, factor {factor}: an even number, and "
+                         "finite ones of 1 or more, are wanted")
+    if scaling == "ntk":
+        if rot_dim == 2:
+            raise ValueError("rope_frequencies: one pair alone has no slowest and fastest")
+        theta = theta * factor ** (rot_dim / (rot_dim - 2)) if rot_dim else theta
+    f = float(theta) ** (-np.arange(0, rot_dim, 2, dtype=np.float64) / max(rot_dim, 1))
+    if scaling == "linear":
+        f = f / factor
+    if scaling == "yarn":
+        if not (original > 0 and fast > slow):
+            raise ValueError(f"rope_frequencies: original {original}, slow {slow}, fast {fast}")
+        keep = np.clip((original * f / (2 * np.pi) - slow) / (fast - slow), 0.0, 1.0)
+        f = f / factor * (1 - keep) + f * keep
+    return f
+
+
+def rope_plan(head_dim: int, rot_dim: int | None = None, theta: float = 10000.0, interleaved: bool = False,
+              scaling: str | None = None, factor: float = 1.0, original: int = 4096, slow: float = 1.0,
+              fast: float = 32.0, gain: float | None = None) -> RopePlan:
+    """The plan that ``rope`` takes, made once (rope_frequencies says what the
+    numbers are).  gain multiplies the turned channels; None: 0.1 ln(factor) + 1
+    with "yarn", else 1."""
+    rot = head_dim if rot_dim is None else rot_dim
+    if not 0 <= rot <= head_dim:
+        raise ValueError(f"rope_plan: rot_dim {rot} is no part of head_dim {head_dim}")
+    f = rope_frequencies(rot, theta, scaling, factor, original, slow, fast)
+    turns = np.array([int(x) for x in f / (2 * np.pi) * 2.0 ** 64], np.uint64)
+    if gain is None:
+        gain = 0.1 * float(np.log(factor)) + 1.0 if scaling == "yarn" else 1.0
+    return RopePlan(head_dim, rot, dev(turns.view(np.int64)), bool(interleaved), float(gain))
+
+
+def rope(plan: RopePlan, q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor,
+         q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+         out: tuple[torch.Tensor | None, torch.Tensor | None] | None = None):
+    """Queries and keys (fp32, or bf16 as int16 bits, [n, heads * head_dim] or [n,
+    heads, head_dim], rows may be strided; either may be None) turned by their
+    positions (int32 [n]; rows of negative ones are passed on as they are), each
+    head RMS-normed first where a weight [head_dim] is given.  Returns (q, k) [n,
+    heads, head_dim], in new tensors or in ``out``, which may be (q, k)."""
+    D = plan.head_dim
+    some = q if q is not None else k
+    if some is None:
+        raise ValueError("rope: neither queries nor keys")
+    dt, n = some.dtype, some.shape[0] if some.dim() else 0
+    if out is None:
+        out = tuple(None if t is None or t.dim() < 2 else t.new_empty((n, t[0].numel() // D if n else 0, D)) for t in (q, k))
+    args, heads = [], []
+    for name, t, w, o in (("q", q, q_weight, out[0]), ("k", k, k_weight, out[1])):
+        if t is None:
+            if o is not None or w is not None:
+                raise ValueError(f"rope: a weight or a result of {name} without {name}")
+            args.append((0, 0, 0, 0, 0))
+            heads.append(0)
+            continue
+        shape = t.shape
+        H = shape[1] // D if len(shape) == 2 else shape[1] if len(shape) == 3 else 0
+        rows, stride = _kv_rows("rope", name, t, H, D, (dt,) if dt in _KV_ROWS else _KV_ROWS)
+        if o is None:
+            raise ValueError(f"rope: no result for {name}")
+        o_rows, o_stride = _kv_rows("rope", f"the result of {name}", o, H, D, (dt,))
+        if rows != n or o_rows != n:
+            raise ValueError(f"rope: {n} rows, {rows} of {name}, {o_rows} of its result")
+        if w is not None:
+            _packed("rope", f"the weight of {name}", w, dt, (D,))
+        args.append((t.data_ptr(), stride, P(w), o.data_ptr(), o_stride))
+        heads.append(H)
+    _packed("rope", "positions", positions, torch.int32, (n,))
+    _on_one_gpu("rope", q, k, positions, plan.turns, q_weight, k_weight, *out)
+    (qp, qs, qw, qo, qos), (kp, ks, kw, ko, kos) = args
+    lib().call("lhq_rope_f32" if dt == torch.float32 else "lhq_rope_bf16", qp, qs, kp, ks, positions.data_ptr(),
+               plan.turns.data_ptr(), qw, kw, eps, plan.gain, qo, qos, ko, kos, int(plan.interleaved), n, heads[0],
+               heads[1], D, plan.rot_dim, stream())
+    return out
+
+
+def prefill_workspace(n_seqs: int, n: int, n_heads: int, n_kv_heads: int, head_dim: int) -> torch.Tensor | None:
+    """A device workspace of the size that attn_prompt and kv_prefill can use (None: they need none)."""
+    nbytes = lib().lhq_prefill_workspace_bytes(n_seqs, n, n_heads, n_kv_heads, head_dim)
+    return empty((nbytes,), np.uint8) if nbytes > 0 else None
+
+
+def _prefill_rows(fn: str, q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None, H: int | None, D: int,
+                  out: torch.Tensor | None, workspace: torch.Tensor | None):
+    """Checks rows, result and workspace; returns (n, heads, kv heads, strides, out, workspace bytes)."""
+    shape = q.shape
+    heads = shape[1] // D if len(shape) == 2 else shape[1] if len(shape) == 3 else 0
+    n, qs = _kv_rows(fn, "q", q, heads, D, _KV_BITS)
+    if (k is None) != (v is None):
+        raise ValueError(f"{fn}: new keys without values, or values without keys")
+    ks = vs = 0
+    if k is not None:
+        if H is None:
+            H = k.shape[1] // D if k.dim() == 2 else k.shape[1] if k.dim() == 3 else 0
+        n_keys, ks = _kv_rows(fn, "k", k, H, D, _KV_BITS)
+        n_values, vs = _kv_rows(fn, "v", v, H, D, _KV_BITS)
+        if n_keys != n or n_values != n:
+            raise ValueError(f"{fn}: {n} queries with {n_keys} new keys and {n_values} values")
+    if not H or heads == 0 or heads % H != 0:
+        raise ValueError(f"{fn}: {heads} query heads over {H} kv heads")
+    if out is None:
+        out = q.new_zeros((n, heads, D))  # (rows that offsets give to none stay zeros)
+    elif out.dtype != torch.int16 or out.numel() != n * heads * D or not out.is_contiguous():
+        raise ValueError(f"{fn}: out must be contiguous [{n}, {heads}, {D}] int16")
+    nbytes = 0
+    if workspace is not None:
+        if not workspace.is_contiguous():
+            raise ValueError(f"{fn}: workspace must be contiguous (strides {tuple(workspace.stride())})")
+        nbytes = workspace.numel() * workspace.element_size()
+    return n, heads, H, (qs, ks, vs), out, nbytes
+
+
+def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, head_dim: int,
+                scale: float | None = None, workspace: torch.Tensor | None = None,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of whole prompts, packed: q [n, heads * head_dim], k and v
+    [n, kv heads * head_dim] (bf16 as int16 bits, rows may be strided), sequence s
+    having rows offsets[s] .. offsets[s + 1] (int32 [B + 1]).  Returns out [n,
+    heads, head_dim], int16 bits; rows that offsets give to no sequence are not
+    computed: zeros in a result that is made here, else what ``out`` held."""
+    fn, D = "attn_prompt", head_dim
+    if offsets.dtype is not torch.int32 or offsets.dim() != 1 or offsets.shape[0] == 0 or not offsets.is_contiguous():
+        raise ValueError(f"{fn}: offsets must be contiguous [B + 1] int32, got {tuple(offsets.shape)} {offsets.dtype}")
+    n, heads, H, (qs, ks, vs), out, nbytes = _prefill_rows(fn, q, k, v, None, D, out, workspace)
+    _on_one_gpu(fn, q, k, v, offsets, workspace, out)
+    lib().call("lhq_attn_prompt_bf16", q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, offsets.data_ptr(),
+               out.data_ptr(), offsets.shape[0] - 1, n, heads, H, D, D ** -0.5 if scale is None else scale,
+               P(workspace), nbytes, stream())
+    return out
+
+
+def kv_prefill(cache: KvCache, q: torch.Tensor, offsets: torch.Tensor, lengths: torch.Tensor,
+               block_table: torch.Tensor, k_new: torch.Tensor | None, v_new: torch.Tensor | None,
+               scale: float | None = None, workspace: torch.Tensor | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of any number of new tokens a sequence over its first lengths[s]
+    cached tokens and, causal, over the new ones: kv_attn without its bound of 64
+    and without trees.  Rows as in attn_prompt.  Returns out [n, heads, head_dim],
+    int16 bits; rows that offsets give to no sequence are not computed: zeros in a
+    result that is made here, else what ``out`` held."""
+    fn, H, D = "kv_prefill", cache.n_kv_heads, cache.head_dim
+    B, width = _kv_tables(fn, offsets, lengths, block_table)
+    n, heads, H, (qs, ks, vs), out, nbytes = _prefill_rows(fn, q, k_new, v_new, H, D, out, workspace)
+    _on_one_gpu(fn, cache.k, q, offsets, lengths, block_table, k_new, v_new, workspace, out)
+    lib().call("lhq_kv_prefill_bf16", q.data_ptr(), qs, P(k_new), ks, P(v_new), vs, offsets.data_ptr(),
+               lengths.data_ptr(), block_table.data_ptr(), *cache.pointers(), out.data_ptr(), _KV_FORMATS[cache.fmt],
+               B, n, width, cache.n_pages, heads, H, D, D ** -0.5 if scale is None else scale, P(workspace), nbytes,
+               stream())
+    return out
