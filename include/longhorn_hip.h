@@ -520,8 +520,9 @@ int lhq_rope_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_
  * tokens 0 .. i and, in lhq_kv_prefill_bf16, before them the first lengths[s]
  * tokens of the cache (clamped to [0, 64 * max_pages]; those of a missing page are
  * not seen).  k_new, v_new both NULL there: only the cache is seen.  A row that
- * sees nothing gives zeros, rows of no sequence are left as they are; what a row
- * does not see, whatever it holds, changes nothing of its result.  Offsets,
+ * sees nothing gives zeros; rows before the first sequence's and behind the last
+ * one's are left as they are, with clear_rest = 1 they become zeros; what a row does
+ * not see, whatever it holds, changes nothing of its result.  Offsets,
  * strides, scale, table and cache as for lhq_kv_attn_bf16, which is the faster for
  * a few new tokens a sequence.  out [row_capacity, n_heads, head_dim].  Rounding:
  * queries, keys and codes enter the products as they are; a softmax weight, of a
@@ -537,15 +538,16 @@ int64_t lhq_prefill_workspace_bytes(int n_seqs, int row_capacity, int n_heads, i
 int lhq_attn_prompt_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride,
                          const uint16_t* v, int64_t v_stride, const int32_t* offsets, uint16_t* out,
                          int n_seqs, int row_capacity, int n_heads, int n_kv_heads, int head_dim,
-                         float scale, void* workspace, int64_t workspace_bytes, void* stream);
+                         float scale, int clear_rest, void* workspace, int64_t workspace_bytes,
+                         void* stream);
 int lhq_kv_prefill_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k_new,
                         int64_t k_stride, const uint16_t* v_new, int64_t v_stride,
                         const int32_t* offsets, const int32_t* lengths, const int32_t* block_table,
                         const uint8_t* k_codes, const float* k_scales, const uint8_t* v_codes,
                         const float* v_scales, uint16_t* out, int format, int n_seqs,
                         int row_capacity, int max_pages, int num_pages, int n_heads, int n_kv_heads,
-                        int head_dim, float scale, void* workspace, int64_t workspace_bytes,
-                        void* stream);
+                        int head_dim, float scale, int clear_rest, void* workspace,
+                        int64_t workspace_bytes, void* stream);
 
 /* ---- fp32 GEMM: gemm.hpp:13-29 / gemm.cpp:5-75 -------------------------- */
 /* lh::gemm semantics (beta first; beta == 0 never reads C). */

@@ -96,8 +96,8 @@ SIGNATURES = {
     "lhq_rope_f32": [_p, _i64, _p, _i64] + [_p] * 4 + [_f, _f] + [_p, _i64, _p, _i64] + [_i] * 6 + [_p],
     "lhq_rope_bf16": [_p, _i64, _p, _i64] + [_p] * 4 + [_f, _f] + [_p, _i64, _p, _i64] + [_i] * 6 + [_p],
     "lhq_prefill_workspace_bytes": [_i] * 5,
-    "lhq_attn_prompt_bf16": [_p, _i64] * 3 + [_p] * 2 + [_i] * 5 + [_f, _p, _i64, _p],
-    "lhq_kv_prefill_bf16": [_p, _i64] * 3 + [_p] * 8 + [_i] * 8 + [_f, _p, _i64, _p],
+    "lhq_attn_prompt_bf16": [_p, _i64] * 3 + [_p] * 2 + [_i] * 5 + [_f, _i, _p, _i64, _p],
+    "lhq_kv_prefill_bf16": [_p, _i64] * 3 + [_p] * 8 + [_i] * 8 + [_f, _i, _p, _i64, _p],
     "lhq_gemm_f32": [_p, _p, _p, _i, _i, _i, _f, _f, _p],
     "lhq_gemm_f32_ref": [_p, _p, _p, _i, _i, _i, _f, _f, _p],
     "lhq_gemm_f32_batched": [_p, _p, _p, _i, _i, _i, _i, _f, _f, _p],

@@ -28,8 +28,9 @@ namespace {
 #define LHQ_LDS_AS __attribute__((address_space(3)))
 typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 
-constexpr int kWaves = 8, kThreads = 64 * kWaves;
-constexpr int kRows = 32 * kWaves;  // of a workgroup
+// Waves of a workgroup, each with 32 rows.  MODE 0: no cache, 1: int8, 2: e4m3.
+template <int KS, int MODE>
+constexpr int waves_of() { return MODE == 0 && KS <= 4 ? 4 : 8; }
 // The running maximum follows the scores only when one is over it by more than
 // 2^kLag: weights go up to 2^kLag, which costs none of their bits.
 constexpr float kLag = 6.0f;
@@ -49,10 +50,13 @@ struct PrefillArgs {
     KvCache c;
     uint16_t* out;
     int n_seqs, capacity, heads, group;  // group: query heads of a kv head
-    float scale2;          // scale * log2 e: weights are powers of two
-    bool vec_new;          // rows of k_new, v_new: 16-byte loads
+    float scale2, unscale; // scale * log2 e (weights are powers of two), and 1 / that
+    bool vec_new;          // rows of k_new, v_new: 16-byte loads at 32-bit offsets from a tile's first
     bool vec_out;          // rows of out: 16-byte stores
+    bool clear_rest;       // rows of no sequence become zeros
     int slots;             // workgroups of a kv head that splitting aims at, 0: no splitting
+    int block_rows;        // rows of a workgroup
+    int resident;          // workgroups of a kv head that are on the chip at once
     int part_rows;         // rows of a part in the workspace
     float* ws_o;           // [kv head][part][part_rows][Dp]
     float* ws_ml;          // [kv head][part][part_rows] {maximum, sum}
@@ -73,7 +77,7 @@ __device__ __forceinline__ Seq seq_of(const PrefillArgs& a, int s) {
     q.lo = r.lo;
     q.T = r.hi - r.lo;
     q.L = a.c.max_pages == 0 ? 0 : static_cast<int>(min<int64_t>(max(a.lengths[s], 0), static_cast<int64_t>(a.c.max_pages) * kKvPage));
-    q.blocks = (q.T * a.group + kRows - 1) / kRows;
+    q.blocks = (q.T * a.group + a.block_rows - 1) / a.block_rows;
     q.tiles = (q.L + kKvPage - 1) / kKvPage + (a.k_new ? (q.T + kKvPage - 1) / kKvPage : 0);
     return q;
 }
@@ -95,8 +99,8 @@ __device__ __forceinline__ int split_count(const Seq& q, int target) {
 }
 // The unit with number `unit` in the list that has count(sequence, splits) units
 // of each sequence in turn: the sequence, the unit's number within it, and the
-// parts (split blocks times their splits) of the sequences before it.  seq =
-// n_seqs past the end of the list.
+// parts (split blocks times their splits) of the sequences before it.  Past the
+// end of the list seq is n_seqs and nth counts from there.
 struct Found { int seq, nth, splits, parts; Seq q; };
 template <typename Count>
 __device__ __forceinline__ Found find_unit(const PrefillArgs& a, uint32_t unit, Count count) {
@@ -119,7 +123,7 @@ __device__ __forceinline__ Found find_unit(const PrefillArgs& a, uint32_t unit, 
         unit -= __builtin_amdgcn_readlane(sum, 63);
         parts += __builtin_amdgcn_readlane(upto, 63);
     }
-    return {a.n_seqs, 0, 1, 0, {0, 0, 0, 0, 0}};
+    return {a.n_seqs, static_cast<int>(unit), 1, 0, {0, 0, 0, 0, 0}};
 }
 
 // ---- tiles in LDS -----------------------------------------------------------
@@ -139,34 +143,58 @@ __device__ __forceinline__ void dma16(const void* from, void* to) {
     __builtin_amdgcn_global_load_lds(from, (LHQ_LDS_AS void*)to, 16, 0, 0);
 }
 
-// New tokens j0 .. j0 + 63 of a sequence of T from row lo on, kv head h, to LDS.
-// Tokens past the last one are that one again (no row sees them); channels past D
-// are zero in keys and anything in values, whose results there are not kept.
-template <int KS>
-__device__ __forceinline__ void stage_new(const PrefillArgs& a, int lo, int T, int h, int j0, uint8_t* keys, uint8_t* values) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), D = a.c.D;
-    if (a.vec_new) {
-        const int t = 16 * (wave & 3) + (lane >> 2), j = (lane & 3) ^ ((lane >> 4) & 3);
-        const int64_t row = lo + min(j0 + t, T - 1);
-        const uint16_t* k = a.k_new + row * a.k_stride + h * D;
-        const uint16_t* v = a.v_new + row * a.v_stride + h * D;
+// New tokens of a sequence on their way to LDS, 64 from j0 on.  Tokens past the
+// last one are that one again (no row sees them); channels past D are zero in keys
+// and anything in values, whose results there are not kept.
+template <int KS, int W>
+struct NewLoad {
+    uint32_t k_at, v_at;  // this lane's row of a whole tile, bytes from the tile's first
+
+    // A wave brings 16 tokens (wave & 3) of every (W / 4)th 32 channels; four lanes a token.
+    static __device__ __forceinline__ int token() { return 16 * ((threadIdx.x >> 6) & 3) + ((threadIdx.x & 63) >> 2); }
+    static __device__ __forceinline__ int channel() {  // within 32
+        const int lane = threadIdx.x & 63;
+        return 8 * ((lane & 3) ^ ((lane >> 4) & 3));
+    }
+    __device__ __forceinline__ void aim(const PrefillArgs& a) {
+        k_at = token() * static_cast<uint32_t>(2 * a.k_stride) + 2 * channel();
+        v_at = token() * static_cast<uint32_t>(2 * a.v_stride) + 2 * channel();
+    }
+    __device__ __forceinline__ void load(const PrefillArgs& a, int lo, int T, int h, int j0, uint8_t* keys, uint8_t* values) const {
+        const int D = a.c.D;
+        const uint8_t* k = reinterpret_cast<const uint8_t*>(a.k_new + (lo + static_cast<int64_t>(j0)) * a.k_stride + h * D);
+        const uint8_t* v = reinterpret_cast<const uint8_t*>(a.v_new + (lo + static_cast<int64_t>(j0)) * a.v_stride + h * D);
+        if (a.vec_new) {
+            const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+            uint32_t ka = k_at, va = v_at;
+            if (j0 + kKvPage > T) {
+                const uint32_t t = min(token(), T - 1 - j0);
+                ka = t * static_cast<uint32_t>(2 * a.k_stride) + 2 * channel();
+                va = t * static_cast<uint32_t>(2 * a.v_stride) + 2 * channel();
+            }
 #pragma unroll
-        for (int m = 0; m < (KS + 1) / 2; ++m) {
-            const int kb = (wave >> 2) + 2 * m, ch = 32 * kb + 8 * j, at = 4096 * kb + 1024 * (wave & 3);
-            if (kb >= KS) break;
-            dma16(ch < D ? static_cast<const void*>(k + ch) : kZeros, keys + at);
-            dma16(v + min(ch, D - 8), values + at);
-        }
-    } else {
-        for (int n = threadIdx.x; n < 64 * 4 * KS; n += kThreads) {
-            const int t = n & 63, ch = 8 * (n >> 6);
-            const int64_t row = lo + min(j0 + t, T - 1);
-            const int at = (ch >> 5) * 4096 + token_place(t, (ch >> 3) & 3);
-            *reinterpret_cast<u32x4_t*>(keys + at) = load_channels<KS == 1>(a.k_new + row * a.k_stride + h * D, ch, D);
-            *reinterpret_cast<u32x4_t*>(values + at) = load_channels<KS == 1>(a.v_new + row * a.v_stride + h * D, ch, D);
+            for (int m = 0; m < (KS + W / 4 - 1) / (W / 4); ++m) {
+                const int kb = (wave >> 2) + W / 4 * m, at = 4096 * kb + 1024 * (wave & 3);
+                if (kb >= KS) break;
+                if (D == 32 * KS) {
+                    dma16(k + 64 * kb + ka, keys + at);
+                    dma16(v + 64 * kb + va, values + at);
+                } else {
+                    const int ch = 32 * kb + channel();
+                    dma16(ch < D ? k + 64 * kb + ka : reinterpret_cast<const uint8_t*>(kZeros), keys + at);
+                    dma16(ch < D ? v + 64 * kb + va : reinterpret_cast<const uint8_t*>(kZeros), values + at);
+                }
+            }
+        } else {
+            for (int n = threadIdx.x; n < 64 * 4 * KS; n += 64 * W) {
+                const int t = n & 63, ch = 8 * (n >> 6), at = (ch >> 5) * 4096 + token_place(t, (ch >> 3) & 3);
+                const int64_t row = min(t, T - 1 - j0);
+                *reinterpret_cast<u32x4_t*>(keys + at) = load_channels<KS == 1>(reinterpret_cast<const uint16_t*>(k) + row * a.k_stride, ch, D);
+                *reinterpret_cast<u32x4_t*>(values + at) = load_channels<KS == 1>(reinterpret_cast<const uint16_t*>(v) + row * a.v_stride, ch, D);
+            }
         }
     }
-}
+};
 
 // Four codes as two pairs of bf16 (exact).
 template <bool FP8>
@@ -182,9 +210,9 @@ __device__ __forceinline__ u32x2_t codes_bf16(uint32_t w) {
 
 // A page on its way: 32 codes of keys (a token's 32 channels) or of values (a
 // channel's 32 keys of one half) a thread and task, and a scale.
-template <int KS>
+template <int KS, int W>
 struct PageLoad {
-    static constexpr int kTasks = (KS + 3) / 4;
+    static constexpr int kTasks = (2 * KS + W - 1) / W;
     u32x4_t w[kTasks][2];
     float factor;
 
@@ -193,7 +221,7 @@ struct PageLoad {
         const int tid = threadIdx.x;
 #pragma unroll
         for (int i = 0; i < kTasks; ++i) {
-            const int n = tid + kThreads * i;  // (the same side for all of a wave)
+            const int n = tid + 64 * W * i;  // (the same side for all of a wave)
             if (n < 64 * KS) {
                 w[i][0] = *reinterpret_cast<const u32x4_t*>(k + 32 * n);
                 w[i][1] = *reinterpret_cast<const u32x4_t*>(k + 32 * n + 16);
@@ -212,7 +240,7 @@ struct PageLoad {
         const int tid = threadIdx.x;
 #pragma unroll
         for (int i = 0; i < kTasks; ++i) {
-            const int n = tid + kThreads * i;
+            const int n = tid + 64 * W * i;
             if (n < 64 * KS) {
                 const int t = n / KS, kb = n % KS;
 #pragma unroll
@@ -250,7 +278,7 @@ __device__ __forceinline__ uint32_t odd_halves(uint32_t w) {
 // A product with a zero weight would make NaN of such a value: in tiles that some
 // row does not see whole, they become zeros here (each wave those that it brought)
 // and are added at the end to the rows that see them.  Returns whether there were any.
-template <int KS>
+template <int KS, int W>
 __device__ __forceinline__ bool clear_odd(const PrefillArgs& a, uint8_t* values) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     bool any = false;
@@ -264,9 +292,9 @@ __device__ __forceinline__ bool clear_odd(const PrefillArgs& a, uint8_t* values)
     };
     if (a.vec_new) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        for (int kb = wave >> 2; kb < KS; kb += 2) clear(values + 4096 * kb + 1024 * (wave & 3) + 16 * lane);
+        for (int kb = wave >> 2; kb < KS; kb += W / 4) clear(values + 4096 * kb + 1024 * (wave & 3) + 16 * lane);
     } else {
-        for (int n = threadIdx.x; n < 64 * 4 * KS; n += kThreads) clear(values + (n >> 8) * 4096 + token_place(n & 63, (n >> 6) & 3));
+        for (int n = threadIdx.x; n < 64 * 4 * KS; n += 64 * W) clear(values + (n >> 8) * 4096 + token_place(n & 63, (n >> 6) & 3));
     }
     return __ballot(any) != 0;
 }
@@ -276,33 +304,37 @@ __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 
 
 // A wave's 32 rows: row lane & 31 is this lane's, with keys and channels 8 a + 4
 // (lane >> 5) + (0..3) of every 32.
-template <int KS>
+// HOLD: sixteen registers for what a product starts from (else made for each).
+template <int KS, bool HOLD>
 struct Rows {
     static constexpr int NT = KS <= 4 ? 2 : 1;  // 32-key tiles whose scores are held at a time
     u32x4_t q[2 * KS];
     f32x16_t o[KS];
-    float m, above, l;  // maximum, the score that moves it, this lane's part of the weights' sum
+    std::conditional_t<HOLD, f32x16_t, float> less;  // -m / scale2: what products of new tokens start from
+    float m, l;     // maximum, this lane's part of the weights' sum
+    float above;    // a score so far over the maximum moves it
 
     __device__ __forceinline__ void clear() {
         m = l = 0.0f;
         above = -INFINITY;
+        less = 0.0f;  // (every element)
 #pragma unroll
-        for (int i = 0; i < KS; ++i)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
+        for (int i = 0; i < KS; ++i) o[i] = 0.0f;
     }
-    // A score is over the maximum by more than 2^kLag in some row of the wave:
-    // those rows' maximum moves.  What other rows see decides nothing.
-    __device__ __forceinline__ void raise(float top) {
+    // A score is over the maximum by more than 2^kLag in some row of the wave, by
+    // `top` in this lane's keys: those rows' maximum moves (what other rows see
+    // decides nothing).  Returns by how much.
+    __device__ __forceinline__ float raise(float top, float unscale) {
         top = fmaxf(top, other_half(top));
-        if (top > above) {
-            const float f = above == -INFINITY ? 0.0f : exp2_(m - top);
-            m = top;
-            above = top + kLag;
-            l *= f;
+        if (!(top > above)) return 0.0f;
+        const float f = above == -INFINITY ? 0.0f : exp2_(-top);
+        above = kLag;
+        m += top;
+        l *= f;
+        less = fminf(fmaxf(-m * unscale, -3e38f), 3e38f);  // (NaN and infinite scores: the weights say so)
 #pragma unroll
-            for (int i = 0; i < KS; ++i) o[i] *= f;
-        }
+        for (int i = 0; i < KS; ++i) o[i] *= f;
+        return top;
     }
     // One tile.  masked (the same for the wave): a row sees the first `limit` keys of it.
     template <bool CACHED>
@@ -315,29 +347,28 @@ struct Rows {
         for (int t0 = 0; t0 < 2; t0 += NT) {
             f32x16_t x[NT];
 #pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                if constexpr (CACHED) x[t] = 0.0f;
+                else x[t] = less;
+            }
+#pragma unroll
             for (int i = 0; i < 2 * KS; ++i)
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     const u32x4_t k = *reinterpret_cast<const u32x4_t*>((i & 1 ? k1 : k0) + 4096 * (i >> 1) + 2048 * (t0 + t));
-                    if (i == 0)
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) x[t][j] = 0.0f;
                     x[t] = mfma_bf16_32x32x16(k, q[i], x[t]);
                 }
-            float top = -INFINITY;
+            // scores less the maximum (of new tokens: to be scaled)
+            if constexpr (CACHED) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    f32x4_t f;
-                    if constexpr (CACHED) f = *reinterpret_cast<const f32x4_t*>(factors + 32 * (t0 + t) + 8 * b + 4 * g);
+                    for (int b = 0; b < 4; ++b) {
+                        const f32x4_t f = *reinterpret_cast<const f32x4_t*>(factors + 32 * (t0 + t) + 8 * b + 4 * g);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float y = x[t][4 * b + j];
-                        if constexpr (CACHED) y *= f[j];
-                        x[t][4 * b + j] = y;
+                        for (int j = 0; j < 4; ++j) x[t][4 * b + j] = __builtin_fmaf(x[t][4 * b + j], f[j], -m);
                     }
-                }
+            }
             if (masked) {
                 int left = limit - 32 * t0 - 4 * g;
                 asm volatile("" : "+v"(left));  // (else made selects on every tile)
@@ -346,12 +377,18 @@ struct Rows {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) x[t][j] = 32 * t + 8 * (j >> 2) + (j & 3) < left ? x[t][j] : -INFINITY;
             }
+            float top = -INFINITY;
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) top = fmaxf(top, x[t][j]);
             if constexpr (!CACHED) top *= a.scale2;
-            if (__ballot(top > above)) raise(top);
+            if (__ballot(top > above)) {
+                float by = raise(top, a.unscale);
+                if constexpr (!CACHED) by *= a.unscale;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) x[t] -= by;
+            }
             u32x4_t p[2 * NT];
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -361,7 +398,7 @@ struct Rows {
                     if constexpr (CACHED) f = *reinterpret_cast<const f32x4_t*>(factors + 64 + 32 * (t0 + t) + 8 * b + 4 * g);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        y[j] = exp2_(CACHED ? x[t][4 * b + j] - m : __builtin_fmaf(x[t][4 * b + j], a.scale2, -m));
+                        y[j] = exp2_(CACHED ? x[t][4 * b + j] : x[t][4 * b + j] * a.scale2);
                         l += y[j];
                         if constexpr (CACHED) y[j] *= f[j];
                     }
@@ -397,18 +434,42 @@ struct Rows {
     }
 };
 
-// MODE 0: no cache, 1: int8, 2: e4m3.
+// Rows of no sequence: zeros, by the workgroups that have no block (one at least).
+__device__ void clear_rest(const PrefillArgs& a, int nth, int count) {
+    const int lo = a.n_seqs ? kv_rows(a.offsets, 0, a.capacity).lo : 0;
+    const int hi = a.n_seqs ? kv_rows(a.offsets, a.n_seqs - 1, a.capacity).hi : 0;
+    const int64_t width = static_cast<int64_t>(a.group) * a.c.D, at = blockIdx.x * width;  // a kv head's part of a row
+    for (int64_t row = nth; row < a.capacity; row += count) {
+        if (row >= lo && row < hi) {
+            row += (hi - 1 - row) / count * count;  // the last of this workgroup's that is inside
+            continue;
+        }
+        uint16_t* to = a.out + row * a.heads * a.c.D + at;
+        if (a.vec_out)
+            for (int64_t n = 8 * threadIdx.x; n < width; n += 8 * blockDim.x) *reinterpret_cast<u32x4_t*>(to + n) = u32x4_t{0, 0, 0, 0};
+        else
+            for (int64_t n = threadIdx.x; n < width; n += blockDim.x) to[n] = 0;
+    }
+}
+
 template <int KS, int MODE>
-__global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
+__global__ __launch_bounds__((64 * waves_of<KS, MODE>()), 2) void prefill_kernel(PrefillArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t prefill_lds[];
-    constexpr int kTile = KS * 4096;
-    const Found u = find_unit(a, blockIdx.y + blockIdx.z * gridDim.y,
-                              [](const Seq& q, int splits) { return static_cast<uint32_t>(q.blocks) * splits; });
-    if (u.seq >= a.n_seqs) return;
+    constexpr int kTile = KS * 4096, W = waves_of<KS, MODE>(), kRows = 32 * W;
+    const uint32_t unit = blockIdx.y + blockIdx.z * gridDim.y;
+    const Found u = find_unit(a, unit, [](const Seq& q, int splits) { return static_cast<uint32_t>(q.blocks) * splits; });
+    if (u.seq >= a.n_seqs) {
+        if (a.clear_rest) clear_rest(a, u.nth, static_cast<int>(gridDim.y * gridDim.z - unit) + u.nth);
+        return;
+    }
     const int h = blockIdx.x, G = a.group, D = a.c.D, R = u.q.T * G, lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // the blocks with the most keys first
-    const int block = u.q.blocks - 1 - u.nth / u.splits, split = u.nth % u.splits;
+    const int split = u.nth % u.splits;
+    // The blocks with the most keys first.  Where all are on the chip at once, the
+    // second half goes from the fewest keys up: it joins the first on the same CUs.
+    int block = u.nth / u.splits;
+    const int half = (u.q.blocks + 1) / 2;
+    block = u.splits == 1 && u.q.blocks <= a.resident && block >= half ? block - half : u.q.blocks - 1 - block;
     const int r0 = block * kRows, pages = (u.q.L + kKvPage - 1) / kKvPage;
     const int tiles = pages + (a.k_new ? ((min(r0 + kRows, R) - 1) / G) / kKvPage + 1 : 0);
     const int first = static_cast<int>(static_cast<int64_t>(tiles) * split / u.splits);
@@ -416,14 +477,41 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
     auto keys = [&](int buf) { return prefill_lds + buf * 2 * kTile; };
     auto factors = [&](int buf) { return reinterpret_cast<float*>(prefill_lds + 4 * kTile) + 128 * buf; };
     int* odd = reinterpret_cast<int*>(prefill_lds + 4 * kTile + 1024);  // infinite or NaN values were cleared
-    if (threadIdx.x == 0) *odd = 0;
-    __syncthreads();
 
     // this wave's rows: (token, query head) pairs of the kv head; past the last one, that again, which is not kept
     const bool some = r0 + 32 * wave < R;
     const int r = min(r0 + 32 * wave + (lane & 31), R - 1), token = r / G;
     const int low = __builtin_amdgcn_readlane(token, 0), high = __builtin_amdgcn_readlane(token, 31);
-    Rows<KS> z;
+    PageLoad<KS, W> page_load;
+    NewLoad<KS, W> new_load;
+    new_load.aim(a);
+    int ids = 0;
+    auto page_id = [&](int t) {  // 64 entries of the block table at a time, one a lane
+        if (((t - first) & 63) == 0) ids = t + lane < pages ? a.c.page(u.seq, t + lane) : -1;
+        return __builtin_amdgcn_readlane(ids, (t - first) & 63);
+    };
+    bool there = false, next_there = false;  // whether a page is
+    // the first tile of new tokens that some row of the block does not see whole
+    const int partly = pages + (r0 / G + 1) / kKvPage;
+    auto fetch_page = [&](int t) {
+        const int id = page_id(t);
+        next_there = id >= 0;
+        if (next_there) page_load.load(a.c, id, h);
+    };
+    auto page_arrives = [&](int t, int buf) {
+        there = next_there;
+        if (there) page_load.template store<MODE == 2>(min(u.q.L - t * kKvPage, kKvPage), a.scale2, keys(buf), keys(buf) + kTile, factors(buf));
+    };
+    auto fetch_new = [&](int t, int buf) {
+        new_load.load(a, u.q.lo, u.q.T, h, (t - pages) * kKvPage, keys(buf), keys(buf) + kTile);
+    };
+    auto new_arrives = [&](int t, int buf) {
+        if (t >= partly && clear_odd<KS, W>(a, keys(buf) + kTile) && lane == 0) *odd = 1;
+    };
+    const bool page_first = MODE != 0 && first < min(end, pages), new_first = !page_first && first < end;
+    if (page_first) fetch_page(first);
+    if (new_first) fetch_new(first, 0);
+    Rows<KS, MODE == 0> z;
     {
         const uint16_t* from = a.q + (u.q.lo + token) * a.q_stride + static_cast<int64_t>(h * G + r - token * G) * D;
 #pragma unroll
@@ -431,49 +519,32 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
     }
     z.clear();
 
-    PageLoad<KS> page_load;
-    int ids = 0;
-    auto page_id = [&](int t) {  // 64 entries of the block table at a time, one a lane
-        if (((t - first) & 63) == 0) ids = t + lane < pages ? a.c.page(u.seq, t + lane) : -1;
-        return __builtin_amdgcn_readlane(ids, (t - first) & 63);
-    };
-    auto fetch = [&](int t, int buf) {  // returns whether the tile is there
-        if (MODE != 0 && t < pages) {
-            const int id = page_id(t);
-            if (id >= 0) page_load.load(a.c, id, h);
-            return id >= 0;
-        }
-        stage_new<KS>(a, u.q.lo, u.q.T, h, (t - pages) * kKvPage, keys(buf), keys(buf) + kTile);
-        return true;
-    };
-    // the first tile of new tokens that some row of the block does not see whole
-    const int partly = pages + (r0 / G + 1) / kKvPage;
-    auto arrive = [&](int t, int buf, bool there) {
-        if (t >= partly && clear_odd<KS>(a, keys(buf) + kTile) && lane == 0) *odd = 1;
-        if (MODE != 0 && t < pages && there)
-            page_load.template store<MODE == 2>(min(u.q.L - t * kKvPage, kKvPage), a.scale2, keys(buf), keys(buf) + kTile, factors(buf));
-    };
-    bool there = false, next_there = false;
-    if (first < end) {
-        there = fetch(first, 0);
-        arrive(first, 0, there);
-    }
+    if (threadIdx.x == 0) *odd = 0;
     __syncthreads();
-    for (int t = first; t < end; ++t) {
-        const int buf = (t - first) & 1;
-        if (t + 1 < end) next_there = fetch(t + 1, buf ^ 1);
-        if (some && there) {
-            const uint8_t *k = keys(buf), *v = k + kTile;
-            if (MODE != 0 && t < pages) {
+    if (page_first) page_arrives(first, 0);
+    if (new_first) new_arrives(first, 0);
+    __syncthreads();
+    int t = first;
+    if constexpr (MODE != 0) {
+        for (; t < min(end, pages); ++t) {
+            const int buf = (t - first) & 1;
+            const bool page_next = t + 1 < min(end, pages), new_next = t + 1 == pages && t + 1 < end;
+            if (page_next) fetch_page(t + 1);
+            if (new_next) fetch_new(t + 1, buf ^ 1);
+            if (some && there) {
                 const int left = min(u.q.L - t * kKvPage, kKvPage);
-                z.template step<true>(a, k, v, factors(buf), left < kKvPage, left);
-            } else {
-                const int j0 = (t - pages) * kKvPage;
-                if (j0 <= high) z.template step<false>(a, k, v, nullptr, j0 + kKvPage - 1 > low, token - j0 + 1);
+                z.template step<true>(a, keys(buf), keys(buf) + kTile, factors(buf), left < kKvPage, left);
             }
+            if (page_next) page_arrives(t + 1, buf ^ 1);
+            if (new_next) new_arrives(t + 1, buf ^ 1);
+            __syncthreads();
         }
-        if (t + 1 < end) arrive(t + 1, buf ^ 1, next_there);
-        there = next_there;
+    }
+    for (; t < end; ++t) {
+        const int buf = (t - first) & 1, j0 = (t - pages) * kKvPage;
+        if (t + 1 < end) fetch_new(t + 1, buf ^ 1);
+        if (some && j0 <= high) z.template step<false>(a, keys(buf), keys(buf) + kTile, nullptr, j0 + kKvPage - 1 > low, token - j0 + 1);
+        if (t + 1 < end) new_arrives(t + 1, buf ^ 1);
         __syncthreads();
     }
 
@@ -529,15 +600,15 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
 // Joins the parts of split blocks in order of position: kJoinRows rows of a
 // block a workgroup, four channels a thread at a time.
 __global__ __launch_bounds__(256) void prefill_join_kernel(PrefillArgs a) {
-    const Found u = find_unit(a, blockIdx.y + blockIdx.z * gridDim.y, [](const Seq& q, int splits) {
-        return splits > 1 ? static_cast<uint32_t>(q.blocks) * (kRows / kJoinRows) : 0u;
+    const Found u = find_unit(a, blockIdx.y + blockIdx.z * gridDim.y, [&](const Seq& q, int splits) {
+        return splits > 1 ? static_cast<uint32_t>(q.blocks) * (a.block_rows / kJoinRows) : 0u;
     });
     if (u.seq >= a.n_seqs) return;
     const int h = blockIdx.x, G = a.group, D = a.c.D, Dp = a.c.Dp(), R = u.q.T * G;
-    const int block = u.nth / (kRows / kJoinRows), from = (u.nth % (kRows / kJoinRows)) * kJoinRows;
+    const int chunks = a.block_rows / kJoinRows, block = u.nth / chunks, from = u.nth % chunks * kJoinRows;
     const int64_t part = static_cast<int64_t>(h) * 2 * a.slots + u.parts + block * u.splits;
     for (int n = threadIdx.x; n < kJoinRows * (Dp / 4); n += 256) {
-        const int row = from + n / (Dp / 4), ch = 4 * (n % (Dp / 4)), r = block * kRows + row;
+        const int row = from + n / (Dp / 4), ch = 4 * (n % (Dp / 4)), r = block * a.block_rows + row;
         if (r >= R) return;
         const int64_t at = part * a.part_rows + row;
         float top = -INFINITY, weight = 0.0f;
@@ -569,15 +640,16 @@ int compute_units() {
 }
 // Workgroups of a kv head that splitting aims at: one a CU.  None where the rows
 // fill the chip as they are, or where no block can have two splits' tiles.
-int want_slots(int capacity, int heads, int kv_heads, int64_t most_tiles) {
+int block_rows(int mode, int D) { return 32 * (mode == 0 && D <= 128 ? waves_of<4, 0>() : waves_of<8, 1>()); }
+int want_slots(int block_rows, int capacity, int heads, int kv_heads, int64_t most_tiles) {
     const int cus = compute_units();
     const int64_t rows = static_cast<int64_t>(capacity) * (heads / kv_heads);
-    if (rows / kRows * kv_heads >= cus || most_tiles <= kLeastTiles) return 0;
+    if (rows / block_rows * kv_heads >= cus || most_tiles <= kLeastTiles) return 0;
     return std::max(1, cus / kv_heads);
 }
 int64_t part_bytes(int rows, int D) { return static_cast<int64_t>(rows) * (kv_padded(D) + 2) * 4; }
-int part_rows(int capacity, int heads, int kv_heads) {
-    return static_cast<int>(std::min<int64_t>(kRows, static_cast<int64_t>(capacity) * (heads / kv_heads)));
+int part_rows(int block_rows, int capacity, int heads, int kv_heads) {
+    return static_cast<int>(std::min<int64_t>(block_rows, static_cast<int64_t>(capacity) * (heads / kv_heads)));
 }
 
 dim3 unit_grid(int heads, int64_t units) {
@@ -590,20 +662,24 @@ int launch(const char* fn, const PrefillArgs& a, dim3 grid, hipStream_t s) {
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&prefill_kernel<KS, MODE>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (attr != hipSuccess) return set_error(LHQ_ERR_HIP, "%s: dynamic LDS attribute: %s", fn, hipGetErrorString(attr));
-    prefill_kernel<KS, MODE><<<grid, kThreads, lds_bytes<KS>(), s>>>(a);
+    prefill_kernel<KS, MODE><<<grid, 64 * waves_of<KS, MODE>(), lds_bytes<KS>(), s>>>(a);
     return check_launch(fn);
 }
 
 bool odd(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; }
 
-int prefill(const char* fn, PrefillArgs a, int mode, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+int prefill(const char* fn, PrefillArgs a, int mode, int clear_rest, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
     const int D = a.c.D, kv_heads = a.c.heads;
     LHQ_REQUIRE(a.heads > 0 && a.heads % kv_heads == 0, "%s: %d query heads are no multiple of %d kv heads", fn, a.heads, kv_heads);
     LHQ_SUPPORTED(a.heads <= 65535, "%s: %d query heads are over 65535", fn, a.heads);
     a.group = a.heads / kv_heads;
-    LHQ_SUPPORTED(static_cast<int64_t>(a.capacity) * a.heads < INT32_MAX - kRows, "%s: %d rows of %d heads are over 2^31", fn, a.capacity, a.heads);
+    a.block_rows = block_rows(mode, D);
+    a.resident = compute_units() * (a.block_rows == 128 ? 2 : 1) / kv_heads;
+    LHQ_SUPPORTED(static_cast<int64_t>(a.capacity) * a.heads < INT32_MAX - a.block_rows, "%s: %d rows of %d heads are over 2^31", fn, a.capacity, a.heads);
     a.scale2 = scale * 1.4426950408889634f;  // weights are powers of two
     LHQ_REQUIRE(std::isfinite(a.scale2) && scale > 0.0f, "%s: scale %g is not positive and finite, also times log2 e", fn, scale);
+    a.unscale = 1.0f / a.scale2;
+    LHQ_SUPPORTED(a.scale2 >= 0x1p-100f, "%s: scale %g is under 2^-100", fn, scale);
     LHQ_REQUIRE((a.k_new == nullptr) == (a.v_new == nullptr), "%s: new keys without values, or values without keys", fn);
     LHQ_REQUIRE(a.q_stride >= static_cast<int64_t>(a.heads) * D, "%s: q rows of stride %lld are under %d heads of %d", fn,
                 static_cast<long long>(a.q_stride), a.heads, D);
@@ -612,25 +688,27 @@ int prefill(const char* fn, PrefillArgs a, int mode, float scale, void* workspac
                 static_cast<long long>(a.v_stride), kv_heads, D);
     LHQ_REQUIRE(workspace_bytes >= 0, "%s: negative workspace size", fn);
     LHQ_REQUIRE(!odd(workspace, 16), "%s: workspace must be 16-byte aligned", fn);
-    if (a.n_seqs == 0 || a.capacity == 0) return LHQ_OK;
+    if (a.capacity == 0 || (a.n_seqs == 0 && !clear_rest)) return LHQ_OK;
     if (mode != 0)
         if (int st = kv_check_pointers(fn, a.c)) return st;
     LHQ_REQUIRE(a.q && a.offsets && a.out && (mode == 0 || a.lengths), "%s: null pointer", fn);
     if (mode == 0) LHQ_REQUIRE(a.k_new, "%s: null pointer", fn);
     if (a.c.num_pages == 0) a.c.max_pages = 0;
-    a.vec_new = D % 8 == 0 && !odd(a.k_new, 16) && !odd(a.v_new, 16) && a.k_stride % 8 == 0 && a.v_stride % 8 == 0;
+    a.vec_new = D % 8 == 0 && !odd(a.k_new, 16) && !odd(a.v_new, 16) && a.k_stride % 8 == 0 && a.v_stride % 8 == 0 &&
+                a.k_stride < (1 << 24) && a.v_stride < (1 << 24);
     a.vec_out = D % 8 == 0 && !odd(a.out, 16);
+    a.clear_rest = clear_rest != 0;
     const int64_t tiles = a.c.max_pages + (a.k_new ? (static_cast<int64_t>(a.capacity) + kKvPage - 1) / kKvPage : 0);
-    a.part_rows = part_rows(a.capacity, a.heads, kv_heads);
+    a.part_rows = part_rows(a.block_rows, a.capacity, a.heads, kv_heads);
     // as many parts as there is room for, two a slot
     const int64_t room = workspace ? workspace_bytes / part_bytes(a.part_rows, D) / (2 * kv_heads) : 0;
-    a.slots = static_cast<int>(std::min<int64_t>(want_slots(a.capacity, a.heads, kv_heads, tiles), room));
+    a.slots = static_cast<int>(std::min<int64_t>(want_slots(a.block_rows, a.capacity, a.heads, kv_heads, tiles), room));
     const int64_t parts = static_cast<int64_t>(kv_heads) * 2 * a.slots;
     a.ws_o = static_cast<float*>(workspace);
     a.ws_ml = a.ws_o + parts * a.part_rows * kv_padded(D);
     const int64_t rows = static_cast<int64_t>(a.capacity) * a.group;
-    const int64_t units = rows / kRows + std::min(a.n_seqs, a.capacity) + 2 * a.slots;
-    LHQ_SUPPORTED(units * kv_heads < INT32_MAX / kThreads, "%s: %lld query blocks of %d heads are over the grid", fn,
+    const int64_t units = rows / a.block_rows + std::min(a.n_seqs, a.capacity) + 2 * a.slots + (clear_rest ? 1 : 0);
+    LHQ_SUPPORTED(units * kv_heads < INT32_MAX / (2 * a.block_rows), "%s: %lld query blocks of %d heads are over the grid", fn,
                   static_cast<long long>(units), kv_heads);
     const dim3 grid = unit_grid(kv_heads, units);
     const hipStream_t s = as_stream(stream);
@@ -650,7 +728,7 @@ int prefill(const char* fn, PrefillArgs a, int mode, float scale, void* workspac
     }
     if (st != LHQ_OK || a.slots == 0) return st;
     // (less than one split block a slot)
-    prefill_join_kernel<<<unit_grid(kv_heads, static_cast<int64_t>(a.slots) * (kRows / kJoinRows)), 256, 0, s>>>(a);
+    prefill_join_kernel<<<unit_grid(kv_heads, static_cast<int64_t>(a.slots) * (a.block_rows / kJoinRows)), 256, 0, s>>>(a);
     return check_launch(fn);
 }
 
@@ -665,19 +743,22 @@ int64_t lhq_prefill_workspace_bytes(int n_seqs, int row_capacity, int n_heads, i
     if (n_seqs <= 0 || row_capacity <= 0 || n_kv_heads <= 0 || n_kv_heads > 65535 || n_heads <= 0 || n_heads % n_kv_heads != 0 ||
         head_dim <= 0 || head_dim > kKvMaxDim)
         return 0;
-    return static_cast<int64_t>(n_kv_heads) * 2 * want_slots(row_capacity, n_heads, n_kv_heads, INT64_MAX) *
-           part_bytes(part_rows(row_capacity, n_heads, n_kv_heads), head_dim);
+    int64_t most = 0;
+    for (int rows : {block_rows(0, head_dim), block_rows(1, head_dim)})
+        most = std::max(most, static_cast<int64_t>(n_kv_heads) * 2 * want_slots(rows, row_capacity, n_heads, n_kv_heads, INT64_MAX) *
+                                  part_bytes(part_rows(rows, row_capacity, n_heads, n_kv_heads), head_dim));
+    return most;
 }
 
 int lhq_attn_prompt_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride, const uint16_t* v,
                          int64_t v_stride, const int32_t* offsets, uint16_t* out, int n_seqs, int row_capacity,
-                         int n_heads, int n_kv_heads, int head_dim, float scale, void* workspace,
-                         int64_t workspace_bytes, void* stream) {
+                         int n_heads, int n_kv_heads, int head_dim, float scale, int clear_rest,
+                         void* workspace, int64_t workspace_bytes, void* stream) {
     const char* fn = "attn_prompt_bf16";
     const KvCache c{nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0, n_kv_heads, head_dim};
     if (int st = kv_check(fn, c, LHQ_KV_INT8, n_seqs, row_capacity)) return st;
     const PrefillArgs a{q, q_stride, k, k_stride, v, v_stride, offsets, nullptr, c, out, n_seqs, row_capacity, n_heads};
-    return prefill(fn, a, 0, scale, workspace, workspace_bytes, stream);
+    return prefill(fn, a, 0, clear_rest, scale, workspace, workspace_bytes, stream);
 }
 
 int lhq_kv_prefill_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k_new, int64_t k_stride,
@@ -685,13 +766,13 @@ int lhq_kv_prefill_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k_n
                         const int32_t* block_table, const uint8_t* k_codes, const float* k_scales,
                         const uint8_t* v_codes, const float* v_scales, uint16_t* out, int format, int n_seqs,
                         int row_capacity, int max_pages, int num_pages, int n_heads, int n_kv_heads, int head_dim,
-                        float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+                        float scale, int clear_rest, void* workspace, int64_t workspace_bytes, void* stream) {
     const char* fn = "kv_prefill_bf16";
     const KvCache c{const_cast<uint8_t*>(k_codes), const_cast<float*>(k_scales), const_cast<uint8_t*>(v_codes),
                     const_cast<float*>(v_scales), block_table, max_pages, num_pages, n_kv_heads, head_dim};
     if (int st = kv_check(fn, c, format, n_seqs, row_capacity)) return st;
     const PrefillArgs a{q, q_stride, k_new, k_stride, v_new, v_stride, offsets, lengths, c, out, n_seqs, row_capacity, n_heads};
-    return prefill(fn, a, format == LHQ_KV_FP8 ? 2 : 1, scale, workspace, workspace_bytes, stream);
+    return prefill(fn, a, format == LHQ_KV_FP8 ? 2 : 1, clear_rest, scale, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

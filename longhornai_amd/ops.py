@@ -629,7 +629,7 @@ def prefill_workspace(n_seqs: int, n: int, n_heads: int, n_kv_heads: int, head_d
 
 def _prefill_rows(fn: str, q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None, H: int | None, D: int,
                   out: torch.Tensor | None, workspace: torch.Tensor | None):
-    """Checks rows, result and workspace; returns (n, heads, kv heads, strides, out, workspace bytes)."""
+    """Checks rows, result and workspace; returns (n, heads, kv heads, strides, out, whether it was made here, workspace bytes)."""
     shape = q.shape
     heads = shape[1] // D if len(shape) == 2 else shape[1] if len(shape) == 3 else 0
     n, qs = _kv_rows(fn, "q", q, heads, D, _KV_BITS)
@@ -645,8 +645,9 @@ def _prefill_rows(fn: str, q: torch.Tensor, k: torch.Tensor | None, v: torch.Ten
             raise ValueError(f"{fn}: {n} queries with {n_keys} new keys and {n_values} values")
     if not H or heads == 0 or heads % H != 0:
         raise ValueError(f"{fn}: {heads} query heads over {H} kv heads")
-    if out is None:
-        out = q.new_zeros((n, heads, D))  # (rows that offsets give to none stay zeros)
+    made = out is None
+    if made:
+        out = q.new_empty((n, heads, D))
     elif out.dtype != torch.int16 or out.numel() != n * heads * D or not out.is_contiguous():
         raise ValueError(f"{fn}: out must be contiguous [{n}, {heads}, {D}] int16")
     nbytes = 0
@@ -654,7 +655,7 @@ def _prefill_rows(fn: str, q: torch.Tensor, k: torch.Tensor | None, v: torch.Ten
         if not workspace.is_contiguous():
             raise ValueError(f"{fn}: workspace must be contiguous (strides {tuple(workspace.stride())})")
         nbytes = workspace.numel() * workspace.element_size()
-    return n, heads, H, (qs, ks, vs), out, nbytes
+    return n, heads, H, (qs, ks, vs), out, int(made), nbytes
 
 
 def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, head_dim: int,
@@ -668,11 +669,11 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torc
     fn, D = "attn_prompt", head_dim
     if offsets.dtype is not torch.int32 or offsets.dim() != 1 or offsets.shape[0] == 0 or not offsets.is_contiguous():
         raise ValueError(f"{fn}: offsets must be contiguous [B + 1] int32, got {tuple(offsets.shape)} {offsets.dtype}")
-    n, heads, H, (qs, ks, vs), out, nbytes = _prefill_rows(fn, q, k, v, None, D, out, workspace)
+    n, heads, H, (qs, ks, vs), out, made, nbytes = _prefill_rows(fn, q, k, v, None, D, out, workspace)
     _on_one_gpu(fn, q, k, v, offsets, workspace, out)
     lib().call("lhq_attn_prompt_bf16", q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, offsets.data_ptr(),
                out.data_ptr(), offsets.shape[0] - 1, n, heads, H, D, D ** -0.5 if scale is None else scale,
-               P(workspace), nbytes, stream())
+               made, P(workspace), nbytes, stream())
     return out
 
 
@@ -687,10 +688,10 @@ def kv_prefill(cache: KvCache, q: torch.Tensor, offsets: torch.Tensor, lengths: 
     result that is made here, else what ``out`` held."""
     fn, H, D = "kv_prefill", cache.n_kv_heads, cache.head_dim
     B, width = _kv_tables(fn, offsets, lengths, block_table)
-    n, heads, H, (qs, ks, vs), out, nbytes = _prefill_rows(fn, q, k_new, v_new, H, D, out, workspace)
+    n, heads, H, (qs, ks, vs), out, made, nbytes = _prefill_rows(fn, q, k_new, v_new, H, D, out, workspace)
     _on_one_gpu(fn, cache.k, q, offsets, lengths, block_table, k_new, v_new, workspace, out)
     lib().call("lhq_kv_prefill_bf16", q.data_ptr(), qs, P(k_new), ks, P(v_new), vs, offsets.data_ptr(),
                lengths.data_ptr(), block_table.data_ptr(), *cache.pointers(), out.data_ptr(), _KV_FORMATS[cache.fmt],
-               B, n, width, cache.n_pages, heads, H, D, D ** -0.5 if scale is None else scale, P(workspace), nbytes,
+               B, n, width, cache.n_pages, heads, H, D, D ** -0.5 if scale is None else scale, made, P(workspace), nbytes,
                stream())
     return out

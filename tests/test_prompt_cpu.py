@@ -67,7 +67,7 @@ def test_rope_with_nothing_to_do_is_ok(L):
 
 def prompt_args(**kw):
     a = dict(q=FAKE, qs=4096, k=FAKE, ks=1024, v=FAKE, vs=1024, offsets=FAKE, out=FAKE, seqs=2, cap=5, heads=32, kv=8,
-             D=128, scale=C.c_float(0.1), ws=None, wsb=0, stream=None)
+             D=128, scale=C.c_float(0.1), rest=0, ws=None, wsb=0, stream=None)
     a.update(kw)
     return list(a.values())
 
@@ -75,7 +75,7 @@ def prompt_args(**kw):
 def prefill_args(**kw):
     a = dict(q=FAKE, qs=4096, k=FAKE, ks=1024, v=FAKE, vs=1024, offsets=FAKE, lengths=FAKE, table=FAKE, kc=FAKE, ksc=FAKE,
              vc=FAKE, vsc=FAKE, out=FAKE, fmt=0, seqs=2, cap=5, width=4, pages=9, heads=32, kv=8, D=128,
-             scale=C.c_float(0.1), ws=None, wsb=0, stream=None)
+             scale=C.c_float(0.1), rest=0, ws=None, wsb=0, stream=None)
     a.update(kw)
     return list(a.values())
 
