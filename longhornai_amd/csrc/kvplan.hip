@@ -42,25 +42,30 @@ __device__ __forceinline__ int held(const PlanArgs& a, int s) {
 __device__ __forceinline__ int pages_of(int64_t tokens) { return static_cast<int>((tokens + kKvPage - 1) / kKvPage); }
 
 // Sums over the threads before this one (below 2^32 in all, else held there);
-// `total` is that of all threads.
+// `total` is that of all threads.  lds: a place that no thread reads any more.
 __device__ __forceinline__ uint32_t scan_before(uint32_t x, uint32_t* lds, uint32_t& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t upto = kv_scan(x);
-    __syncthreads();  // (lds may still be read)
     if (lane == 63) lds[wave] = upto;
     __syncthreads();
-    uint32_t before = 0;
-    total = 0;
-    for (int w = 0; w < kPlanWaves; ++w) {
-        if (w == wave) before = total;
-        total = __builtin_elementwise_add_sat(total, lds[w]);
-    }
+    const uint32_t waves = kv_scan(lane < kPlanWaves ? lds[lane] : 0u);
+    total = __builtin_amdgcn_readlane(waves, kPlanWaves - 1);
+    const uint32_t before = wave > 0 ? __builtin_amdgcn_readlane(waves, wave - 1) : 0u;
     return __builtin_elementwise_add_sat(before, upto - x);
+}
+// f(lane, its x) for each lane of the wave that has x > 0, in order.
+template <typename F>
+__device__ __forceinline__ void each_lane(int x, F f) {
+    for (uint64_t some = __ballot(x > 0); some; some &= some - 1) {
+        const int l = __builtin_ctzll(some);
+        f(l, __builtin_amdgcn_readlane(x, l));
+    }
 }
 
 // Row r: the last sequence whose offset is not over r owns it, if its rows
 // reach that far.
-__device__ __forceinline__ void plan_row(const PlanArgs& a, const int32_t* offsets, int r) {
+template <typename Length>
+__device__ __forceinline__ void plan_row(const PlanArgs& a, const int32_t* offsets, Length length_of, int r) {
     int lo = 0, hi = a.n_seqs;  // offsets[lo] <= r (offsets[0] = 0), offsets[hi] > r or hi = n_seqs
     while (hi - lo > 1) {
         const int mid = lo + (hi - lo) / 2;
@@ -70,7 +75,7 @@ __device__ __forceinline__ void plan_row(const PlanArgs& a, const int32_t* offse
     int position = -1;
     int64_t slot = -1;
     if (a.n_seqs > 0 && r < offsets[lo + 1]) {
-        const int first = offsets[lo], length = held(a, lo), i = r - first;
+        const int first = offsets[lo], length = length_of(lo), i = r - first;
         const int64_t at = static_cast<int64_t>(length) + i, p = at / kKvPage;
         int64_t depth = i;
         if (a.tree) {  // ancestors of a drafted token, itself among them
@@ -89,93 +94,81 @@ __device__ __forceinline__ void plan_row(const PlanArgs& a, const int32_t* offse
 // ROWS: the rows too (n_seqs <= kPlanThreads, capacity <= kPlanRows).
 template <bool ROWS>
 __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
-    __shared__ uint32_t sums[kPlanWaves];
-    __shared__ int first[kPlanThreads], count[kPlanThreads], rank[kPlanThreads];
-    __shared__ int offs[kPlanThreads + 1];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ uint32_t sums[3][kPlanWaves];
+    __shared__ int offs[kPlanThreads + 1], lengths[kPlanThreads];
+    const int lane = threadIdx.x & 63, wave_first = static_cast<int>(threadIdx.x) - lane;
     uint32_t have = static_cast<uint32_t>(min(max(a.left[0], 0), a.num_pages));  // pages on the stack
+    // the first 1024 sequences' lengths and new tokens stay in registers
+    auto length_of = [&](int s) { return s < a.n_seqs ? held(a, s) : 0; };
+    auto new_of = [&](int s) { return s < a.n_seqs ? a.new_tokens[s] : 0; };
+    const int length0 = length_of(threadIdx.x), new0 = new_of(threadIdx.x);
 
-    // Pages of sequences that are over, 1024 sequences at a time.
+    // Pages of sequences that are over, 1024 sequences at a time, a wave its own 64.
     for (int base = 0; base < a.n_seqs; base += kPlanThreads) {
         const int s = base + static_cast<int>(threadIdx.x);
-        const int had = s < a.n_seqs && a.new_tokens[s] < 0 ? pages_of(held(a, s)) : 0;
+        const int n = base ? new_of(s) : new0, had = n < 0 ? pages_of(base ? length_of(s) : length0) : 0;
         if (!__syncthreads_or(had)) continue;
-        first[threadIdx.x] = had;
-        __syncthreads();
-        // valid entries of each, a wave a sequence
-        for (int i = wave; i < kPlanThreads; i += kPlanWaves) {
-            const int n = first[i];
-            int valid = 0;
-            for (int p = 0; p < n; p += 64) {
-                const int id = p + lane < n ? a.table[static_cast<int64_t>(base + i) * a.max_pages + p + lane] : -1;
-                valid += __popcll(__ballot(id >= 0 && id < a.num_pages));
-            }
-            if (lane == 0) count[i] = valid;
-        }
-        __syncthreads();
+        auto entry = [&](int l, int p, int pages) {
+            const int id = p < pages ? a.table[static_cast<int64_t>(base + wave_first + l) * a.max_pages + p] : -1;
+            return id < a.num_pages ? id : -1;
+        };
+        int valid = 0;  // entries of this lane's sequence that are pages
+        each_lane(had, [&](int l, int pages) {
+            int sum = 0;
+            for (int p = lane; p - lane < pages; p += 64) sum += __popcll(__ballot(entry(l, p, pages) >= 0));
+            if (lane == l) valid = sum;
+        });
         uint32_t total;
-        const uint32_t before = scan_before(static_cast<uint32_t>(count[threadIdx.x]), sums, total);
-        rank[threadIdx.x] = static_cast<int>(min(before, 0x7fffffffu));
-        __syncthreads();
-        for (int i = wave; i < kPlanThreads; i += kPlanWaves) {
-            const int n = first[i];
-            int64_t at = static_cast<int64_t>(have) + rank[i];
-            for (int p = 0; p < n; p += 64) {
-                const int id = p + lane < n ? a.table[static_cast<int64_t>(base + i) * a.max_pages + p + lane] : -1;
-                const bool valid = id >= 0 && id < a.num_pages;
-                const uint64_t all = __ballot(valid);
+        const uint32_t before = scan_before(static_cast<uint32_t>(valid), sums[0], total);
+        each_lane(had, [&](int l, int pages) {
+            int64_t at = static_cast<int64_t>(have) + static_cast<uint32_t>(__builtin_amdgcn_readlane(before, l));
+            for (int p = lane; p - lane < pages; p += 64) {
+                const int id = entry(l, p, pages);
+                const uint64_t all = __ballot(id >= 0);
                 const int64_t to = at + __popcll(all & ((uint64_t{1} << lane) - 1));
                 // (more pages than there are: some were handed back twice; the stack keeps to its size)
-                if (valid && to < a.num_pages) a.free_pages[to] = id;
+                if (id >= 0 && to < a.num_pages) a.free_pages[to] = id;
                 at += __popcll(all);
             }
-        }
+        });
         have = min(__builtin_elementwise_add_sat(have, total), static_cast<uint32_t>(a.num_pages));
-        __syncthreads();
     }
+    __syncthreads();  // (what is on the stack now is seen by all)
 
     // Offsets, and the new tokens' pages.
     uint32_t rows = 0, asked = 0;
     for (int base = 0; base < a.n_seqs; base += kPlanThreads) {
         const int s = base + static_cast<int>(threadIdx.x);
-        const uint32_t want = s < a.n_seqs ? static_cast<uint32_t>(max(a.new_tokens[s], 0)) : 0u;
+        const int length = base ? length_of(s) : length0;
+        const uint32_t want = static_cast<uint32_t>(max(base ? new_of(s) : new0, 0)), cap = static_cast<uint32_t>(a.capacity);
         uint32_t total;
-        const uint32_t cap = static_cast<uint32_t>(a.capacity);
-        const uint32_t before = __builtin_elementwise_add_sat(rows, scan_before(want, sums, total));
+        const uint32_t before = __builtin_elementwise_add_sat(rows, scan_before(want, sums[1], total));
         const int lo = static_cast<int>(min(before, cap)), hi = static_cast<int>(min(__builtin_elementwise_add_sat(before, want), cap));
         rows = __builtin_elementwise_add_sat(rows, total);
-        int from = 0, takes = 0;
+        const int from = pages_of(length);
+        int takes = 0;
         if (s < a.n_seqs) {
             a.offsets[s + 1] = hi;
             if (s == 0) a.offsets[0] = 0;
             if constexpr (ROWS) {
                 offs[s + 1] = hi;
                 if (s == 0) offs[0] = 0;
+                lengths[s] = length;
             }
-            const int length = held(a, s);
-            from = pages_of(length);
             if (hi > lo) takes = max(min(pages_of(static_cast<int64_t>(length) + hi - lo), a.max_pages) - from, 0);
         }
-        const uint32_t mine = __builtin_elementwise_add_sat(asked, scan_before(static_cast<uint32_t>(takes), sums, total));
+        const uint32_t mine = __builtin_elementwise_add_sat(asked, scan_before(static_cast<uint32_t>(takes), sums[2], total));
         asked = __builtin_elementwise_add_sat(asked, total);
         auto take = [&](int seq, int p, uint32_t nth) {
             a.table[static_cast<int64_t>(seq) * a.max_pages + p] = nth < have ? a.free_pages[have - 1 - nth] : -1;
         };
-        // one or two pages by the sequence's thread, more by a wave
-        if (takes <= 2) {
-            for (int i = 0; i < takes; ++i) take(s, from + i, __builtin_elementwise_add_sat(mine, static_cast<uint32_t>(i)));
-            takes = 0;
-        }
-        if (__syncthreads_or(takes)) {
-            first[threadIdx.x] = from;
-            count[threadIdx.x] = takes;
-            rank[threadIdx.x] = static_cast<int>(mine);
-            __syncthreads();
-            for (int i = wave; i < kPlanThreads; i += kPlanWaves)
-                for (int p = lane; p < count[i]; p += 64)
-                    take(base + i, first[i] + p,
-                         __builtin_elementwise_add_sat(static_cast<uint32_t>(rank[i]), static_cast<uint32_t>(p)));
-        }
+        // one page by the sequence's lane, more by its wave
+        if (takes == 1) take(s, from, mine);
+        each_lane(takes > 1 ? takes : 0, [&](int l, int pages) {
+            const int p0 = __builtin_amdgcn_readlane(from, l);
+            const uint32_t nth = __builtin_amdgcn_readlane(mine, l);
+            for (int p = lane; p < pages; p += 64) take(base + wave_first + l, p0 + p, __builtin_elementwise_add_sat(nth, static_cast<uint32_t>(p)));
+        });
     }
     __syncthreads();  // (left may be left_out: everyone has read it)
     if (threadIdx.x == 0) {
@@ -184,13 +177,13 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
         if (a.n_seqs == 0) a.offsets[0] = 0;
     }
     if constexpr (ROWS) {
-        for (int r = threadIdx.x; r < a.capacity; r += kPlanThreads) plan_row(a, offs, r);
+        for (int r = threadIdx.x; r < a.capacity; r += kPlanThreads) plan_row(a, offs, [&](int s) { return lengths[s]; }, r);
     }
 }
 
 __global__ __launch_bounds__(kRowThreads) void kv_plan_rows_kernel(PlanArgs a) {
     const int r = static_cast<int>(blockIdx.x * kRowThreads + threadIdx.x);
-    if (r < a.capacity) plan_row(a, a.offsets, r);
+    if (r < a.capacity) plan_row(a, a.offsets, [&](int s) { return held(a, s); }, r);
 }
 
 }  // namespace

@@ -19,6 +19,7 @@
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
+#include <utility>
 
 #include "kvcommon.hpp"
 
@@ -28,9 +29,6 @@ namespace {
 #define LHQ_LDS_AS __attribute__((address_space(3)))
 typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 
-// Waves of a workgroup, each with 32 rows.  MODE 0: no cache, 1: int8, 2: e4m3.
-template <int KS, int MODE>
-constexpr int waves_of() { return MODE == 0 && KS <= 4 ? 4 : 8; }
 // The running maximum follows the scores only when one is over it by more than
 // 2^kLag: weights go up to 2^kLag, which costs none of their bits.
 constexpr float kLag = 6.0f;
@@ -50,21 +48,20 @@ struct PrefillArgs {
     KvCache c;
     uint16_t* out;
     int n_seqs, capacity, heads, group;  // group: query heads of a kv head
-    float scale2, unscale; // scale * log2 e (weights are powers of two), and 1 / that
+    float scale2;          // scale * log2 e: weights are powers of two
     bool vec_new;          // rows of k_new, v_new: 16-byte loads at 32-bit offsets from a tile's first
     bool vec_out;          // rows of out: 16-byte stores
     bool clear_rest;       // rows of no sequence become zeros
     int slots;             // workgroups of a kv head that splitting aims at, 0: no splitting
     int block_rows;        // rows of a workgroup
-    int resident;          // workgroups of a kv head that are on the chip at once
     int part_rows;         // rows of a part in the workspace
     float* ws_o;           // [kv head][part][part_rows][Dp]
     float* ws_ml;          // [kv head][part][part_rows] {maximum, sum}
 };
 
-// Bytes of LDS: two tiles of keys and values, two of factors, a flag.
+// Bytes of LDS: two tiles of keys and values, two pages' factors, a flag.
 template <int KS>
-constexpr int lds_bytes() { return 2 * (2 * KS * 4096 + 512) + 16; }
+constexpr int lds_bytes() { return 4 * KS * 4096 + 1024 + 16; }
 
 // A sequence: its first row, new tokens, cached tokens; the list of blocks.
 struct Seq {
@@ -138,61 +135,84 @@ __device__ __forceinline__ int value_place(int ch, int chunk) { return ch * 128 
 
 __device__ __attribute__((aligned(16))) const uint32_t kZeros[4] = {0, 0, 0, 0};
 
-// 16 bytes a lane from its address to `to` + 16 * lane.
-__device__ __forceinline__ void dma16(const void* from, void* to) {
-    __builtin_amdgcn_global_load_lds(from, (LHQ_LDS_AS void*)to, 16, 0, 0);
+// 16 bytes a lane from `from` + lane_at + OFFSET to LDS address `to` + OFFSET + 16 *
+// lane, without a register on the way.  In assembly: the compiler makes every later
+// LDS read wait for the builtin's.  arrived() waits for them all.
+template <int OFFSET>
+__device__ __forceinline__ void dma16(const void* from, uint32_t lane_at, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3"
+                 :: "s"(to), "v"(lane_at), "s"(from), "n"(OFFSET) : "memory");
+}
+__device__ __forceinline__ void dma16_any(const void* from, uint32_t to) {  // an address a lane
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(to), "v"(from) : "memory");
+}
+__device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LHQ_LDS_AS const void*)p));
 }
 
-// New tokens of a sequence on their way to LDS, 64 from j0 on.  Tokens past the
-// last one are that one again (no row sees them); channels past D are zero in keys
-// and anything in values, whose results there are not kept.
+// Keys or values of a sequence's new tokens on their way to LDS, a tile of 64 after
+// the other.  Tokens past the last one are that one again (no row sees them); channels
+// past D are zero.
 template <int KS, int W>
-struct NewLoad {
-    uint32_t k_at, v_at;  // this lane's row of a whole tile, bytes from the tile's first
+struct NewTiles {
+    const uint16_t* from;  // the next tile's first row, this kv head
+    int64_t stride;        // of rows
+    uint32_t lane_at;      // this lane's bytes in a whole tile, from there
+    uint32_t wave_at;      // this wave's part of a tile in LDS
+    int j0, past;          // the next tile's first token, that past the last tile
 
     // A wave brings 16 tokens (wave & 3) of every (W / 4)th 32 channels; four lanes a token.
     static __device__ __forceinline__ int token() { return 16 * ((threadIdx.x >> 6) & 3) + ((threadIdx.x & 63) >> 2); }
-    static __device__ __forceinline__ int channel() {  // within 32
+    static __device__ __forceinline__ int channel() {  // of the first 32
         const int lane = threadIdx.x & 63;
-        return 8 * ((lane & 3) ^ ((lane >> 4) & 3));
+        return 32 * (threadIdx.x >> 8) + 8 * ((lane & 3) ^ ((lane >> 4) & 3));
     }
-    __device__ __forceinline__ void aim(const PrefillArgs& a) {
-        k_at = token() * static_cast<uint32_t>(2 * a.k_stride) + 2 * channel();
-        v_at = token() * static_cast<uint32_t>(2 * a.v_stride) + 2 * channel();
+    __device__ __forceinline__ void aim(const uint16_t* rows, int64_t stride_, int lo, int h, int D, int j0_, int past_) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        j0 = j0_;
+        past = past_;
+        stride = stride_;
+        from = rows + (lo + static_cast<int64_t>(j0)) * stride + h * D;
+        lane_at = token() * static_cast<uint32_t>(2 * stride) + 2 * channel();
+        wave_at = 4096 * (wave >> 2) + 1024 * (wave & 3);
     }
-    __device__ __forceinline__ void load(const PrefillArgs& a, int lo, int T, int h, int j0, uint8_t* keys, uint8_t* values) const {
+    template <int... M>
+    __device__ __forceinline__ void whole(uint32_t at, uint32_t to, std::integer_sequence<int, M...>) const {
+        constexpr int kStep = W / 4;
+        // (an odd number of 32 channels: the upper waves of eight have one fewer)
+        ((kStep * M + kStep <= KS || __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) + kStep * M < KS
+              ? dma16<64 * kStep * M>(from, at, to + (4096 - 64) * kStep * M) : void()), ...);
+    }
+    // The next tile to `to`, if there is one.
+    __device__ __forceinline__ void fetch(const PrefillArgs& a, int T, uint8_t* to) {
+        if (j0 >= past) return;
         const int D = a.c.D;
-        const uint8_t* k = reinterpret_cast<const uint8_t*>(a.k_new + (lo + static_cast<int64_t>(j0)) * a.k_stride + h * D);
-        const uint8_t* v = reinterpret_cast<const uint8_t*>(a.v_new + (lo + static_cast<int64_t>(j0)) * a.v_stride + h * D);
+        constexpr int kMost = (KS + W / 4 - 1) / (W / 4);
         if (a.vec_new) {
-            const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-            uint32_t ka = k_at, va = v_at;
-            if (j0 + kKvPage > T) {
-                const uint32_t t = min(token(), T - 1 - j0);
-                ka = t * static_cast<uint32_t>(2 * a.k_stride) + 2 * channel();
-                va = t * static_cast<uint32_t>(2 * a.v_stride) + 2 * channel();
-            }
+            uint32_t at = lane_at;
+            if (j0 + kKvPage > T) at = min(token(), T - 1 - j0) * static_cast<uint32_t>(2 * stride) + 2 * channel();
+            const uint32_t lds = lds_address(to) + wave_at;
+            if (D == 32 * KS) {
+                whole(at, lds, std::make_integer_sequence<int, kMost>{});
+            } else {
 #pragma unroll
-            for (int m = 0; m < (KS + W / 4 - 1) / (W / 4); ++m) {
-                const int kb = (wave >> 2) + W / 4 * m, at = 4096 * kb + 1024 * (wave & 3);
-                if (kb >= KS) break;
-                if (D == 32 * KS) {
-                    dma16(k + 64 * kb + ka, keys + at);
-                    dma16(v + 64 * kb + va, values + at);
-                } else {
-                    const int ch = 32 * kb + channel();
-                    dma16(ch < D ? k + 64 * kb + ka : reinterpret_cast<const uint8_t*>(kZeros), keys + at);
-                    dma16(ch < D ? v + 64 * kb + va : reinterpret_cast<const uint8_t*>(kZeros), values + at);
+                for (int m = 0; m < kMost; ++m) {
+                    const int more = 32 * (W / 4) * m;
+                    if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 8) + W / 4 * m >= KS) break;
+                    const uint8_t* lane = reinterpret_cast<const uint8_t*>(from) + at + 2 * more;
+                    dma16_any(channel() + more < D ? lane : reinterpret_cast<const uint8_t*>(kZeros), lds + 128 * more);
                 }
             }
         } else {
             for (int n = threadIdx.x; n < 64 * 4 * KS; n += 64 * W) {
-                const int t = n & 63, ch = 8 * (n >> 6), at = (ch >> 5) * 4096 + token_place(t, (ch >> 3) & 3);
-                const int64_t row = min(t, T - 1 - j0);
-                *reinterpret_cast<u32x4_t*>(keys + at) = load_channels<KS == 1>(reinterpret_cast<const uint16_t*>(k) + row * a.k_stride, ch, D);
-                *reinterpret_cast<u32x4_t*>(values + at) = load_channels<KS == 1>(reinterpret_cast<const uint16_t*>(v) + row * a.v_stride, ch, D);
+                const int t = n & 63, ch = 8 * (n >> 6);
+                const uint16_t* row = from + static_cast<int64_t>(min(t, T - 1 - j0)) * stride;
+                *reinterpret_cast<u32x4_t*>(to + (ch >> 5) * 4096 + token_place(t, (ch >> 3) & 3)) = load_channels<KS == 1>(row, ch, D);
             }
         }
+        from += kKvPage * stride;
+        j0 += kKvPage;
     }
 };
 
@@ -275,7 +295,7 @@ struct PageLoad {
 __device__ __forceinline__ uint32_t odd_halves(uint32_t w) {
     return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
 }
-// A product with a zero weight would make NaN of such a value: in tiles that some
+// (Once they have arrived.)  A product with a zero weight would make NaN of such a value: in tiles that some
 // row does not see whole, they become zeros here (each wave those that it brought)
 // and are added at the end to the rows that see them.  Returns whether there were any.
 template <int KS, int W>
@@ -291,7 +311,6 @@ __device__ __forceinline__ bool clear_odd(const PrefillArgs& a, uint8_t* values)
         *reinterpret_cast<u32x4_t*>(at) = w & ~bad;
     };
     if (a.vec_new) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         for (int kb = wave >> 2; kb < KS; kb += W / 4) clear(values + 4096 * kb + 1024 * (wave & 3) + 16 * lane);
     } else {
         for (int n = threadIdx.x; n < 64 * 4 * KS; n += 64 * W) clear(values + (n >> 8) * 4096 + token_place(n & 63, (n >> 6) & 3));
@@ -304,74 +323,142 @@ __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 
 
 // A wave's 32 rows: row lane & 31 is this lane's, with keys and channels 8 a + 4
 // (lane >> 5) + (0..3) of every 32.
-// HOLD: sixteen registers for what a product starts from (else made for each).
-template <int KS, bool HOLD>
+template <int KS>
 struct Rows {
     static constexpr int NT = KS <= 4 ? 2 : 1;  // 32-key tiles whose scores are held at a time
     u32x4_t q[2 * KS];
     f32x16_t o[KS];
-    std::conditional_t<HOLD, f32x16_t, float> less;  // -m / scale2: what products of new tokens start from
     float m, l;     // maximum, this lane's part of the weights' sum
     float above;    // a score so far over the maximum moves it
 
     __device__ __forceinline__ void clear() {
         m = l = 0.0f;
         above = -INFINITY;
-        less = 0.0f;  // (every element)
 #pragma unroll
         for (int i = 0; i < KS; ++i) o[i] = 0.0f;
     }
-    // A score is over the maximum by more than 2^kLag in some row of the wave, by
-    // `top` in this lane's keys: those rows' maximum moves (what other rows see
-    // decides nothing).  Returns by how much.
-    __device__ __forceinline__ float raise(float top, float unscale) {
+    // A score, `top` in this lane's keys, is over the maximum by more than 2^kLag in
+    // some row of the wave: those rows' maximum moves (what other rows see
+    // decides nothing).
+    __device__ __forceinline__ void raise(float top) {
         top = fmaxf(top, other_half(top));
-        if (!(top > above)) return 0.0f;
-        const float f = above == -INFINITY ? 0.0f : exp2_(-top);
-        above = kLag;
-        m += top;
+        if (!(top > above)) return;
+        const float f = above == -INFINITY ? 0.0f : exp2_(m - top);
+        m = top;
+        above = top + kLag;
         l *= f;
-        less = fminf(fmaxf(-m * unscale, -3e38f), 3e38f);  // (NaN and infinite scores: the weights say so)
 #pragma unroll
         for (int i = 0; i < KS; ++i) o[i] *= f;
-        return top;
     }
-    // One tile.  masked (the same for the wave): a row sees the first `limit` keys of it.
-    template <bool CACHED>
-    __device__ __forceinline__ void step(const PrefillArgs& a, const uint8_t* keys, const uint8_t* values, const float* factors,
-                                         bool masked, int limit) {
+    // Products of the rows with keys 32 t0 on of a tile, operands read kAhead ahead.
+    template <int N>
+    __device__ __forceinline__ void products(const uint8_t* keys, int t0, f32x16_t (&x)[N]) const {
+        constexpr int kAll = 2 * KS * N, kMost = KS <= 4 ? 8 : KS <= 6 ? 4 : 2, kAhead = kAll < kMost ? kAll : kMost;
         const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
         const uint8_t* k0 = keys + token_place(c, g);
         const uint8_t* k1 = keys + token_place(c, 2 + g);
+        auto key = [&](int n) {  // 32 keys n % N, channels 16 (n / N) on
+            return *reinterpret_cast<const u32x4_t*>((n / N & 1 ? k1 : k0) + 4096 * (n / N >> 1) + 2048 * (t0 + n % N));
+        };
+        u32x4_t k[kAhead];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) k[n] = key(n);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < kAll; ++n) {
+            if (n < N) x[n] = 0.0f;
+            x[n % N] = mfma_bf16_32x32x16(k[n % kAhead], q[n / N], x[n % N]);
+            if (n + kAhead < kAll) k[n % kAhead] = key(n + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // Only the first `limit` keys of the tile are seen; returns this lane's largest product with them.
+    template <int N>
+    __device__ __forceinline__ float mask(int t0, int limit, f32x16_t (&x)[N]) const {
+        int left = limit - 32 * t0 - 4 * static_cast<int>((threadIdx.x & 63) >> 5);
+        asm volatile("" : "+v"(left));  // (else made selects on every tile)
+        float top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                x[t][j] = 32 * t + 8 * (j >> 2) + (j & 3) < left ? x[t][j] : -INFINITY;
+                top = fmaxf(top, x[t][j]);
+            }
+        return top;
+    }
+    // Products after the mask and with the maximum moved where they are far over it.
+    template <int N>
+    __device__ __forceinline__ void settle(const PrefillArgs& a, int t0, bool masked, int limit, f32x16_t (&x)[N]) {
+        float top = -INFINITY;
+        if (masked) {
+            top = mask(t0, limit, x);
+        } else {
+#pragma unroll
+            for (int t = 0; t < N; ++t)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) top = fmaxf(top, x[t][j]);
+        }
+        top *= a.scale2;
+        if (__ballot(top > above)) raise(top);
+    }
+    // Products -> weights as operands.
+    template <int N>
+    __device__ __forceinline__ void weigh(const PrefillArgs& a, const f32x16_t (&x)[N], u32x4_t (&p)[2 * N]) {
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                f32x4_t y;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    y[j] = exp2_(__builtin_fmaf(x[t][4 * b + j], a.scale2, -m));
+                    l += y[j];
+                }
+                p[2 * t + (b >> 1)][2 * (b & 1)] = pack_bf16x2(y[0], y[1]);
+                p[2 * t + (b >> 1)][2 * (b & 1) + 1] = pack_bf16x2(y[2], y[3]);
+            }
+    }
+    // O^T += V^T P^T of new tokens 32 t0 on of a tile.
+    template <int N>
+    __device__ __forceinline__ void add(const uint8_t* values, int t0, const u32x4_t (&p)[2 * N]) {
+        const int lane = threadIdx.x & 63, g = lane >> 5;
+        // a lane's address in a transposing read: token 4 g + (lane & 15) / 4, channels 16 (lane >> 4 & 1) + 4 (lane & 3) on
+        const int tok = 4 * g + ((lane & 15) >> 2), chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+        const uint8_t* at[2] = {values + token_place(tok, chunk) + 8 * (lane & 1), values + token_place(tok + 8, chunk) + 8 * (lane & 1)};
+#pragma unroll
+        for (int s = 0; s < 2 * N; ++s)
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                u32x2_t w[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    w[e] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                               (LHQ_LDS_AS s16x4_t*)(at[e] + 4096 * i + 1024 * (2 * t0 + s))));
+                o[i] = mfma_bf16_32x32x16(u32x4_t{w[0][0], w[0][1], w[1][0], w[1][1]}, p[s], o[i]);
+            }
+    }
+    // One page.  masked (the same for the wave): a row sees the first `limit` tokens of it.
+    __device__ __forceinline__ void page(const uint8_t* keys, const uint8_t* values, const float* factors, bool masked,
+                                         int limit) {
+        const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
 #pragma unroll
         for (int t0 = 0; t0 < 2; t0 += NT) {
             f32x16_t x[NT];
+            products(keys, t0, x);
+            // scores
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                if constexpr (CACHED) x[t] = 0.0f;
-                else x[t] = less;
-            }
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int i = 0; i < 2 * KS; ++i)
+                for (int b = 0; b < 4; ++b) {
+                    const f32x4_t f = *reinterpret_cast<const f32x4_t*>(factors + 32 * (t0 + t) + 8 * b + 4 * g);
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const u32x4_t k = *reinterpret_cast<const u32x4_t*>((i & 1 ? k1 : k0) + 4096 * (i >> 1) + 2048 * (t0 + t));
-                    x[t] = mfma_bf16_32x32x16(k, q[i], x[t]);
+                    for (int j = 0; j < 4; ++j) x[t][4 * b + j] *= f[j];
                 }
-            // scores less the maximum (of new tokens: to be scaled)
-            if constexpr (CACHED) {
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const f32x4_t f = *reinterpret_cast<const f32x4_t*>(factors + 32 * (t0 + t) + 8 * b + 4 * g);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) x[t][4 * b + j] = __builtin_fmaf(x[t][4 * b + j], f[j], -m);
-                    }
-            }
             if (masked) {
                 int left = limit - 32 * t0 - 4 * g;
-                asm volatile("" : "+v"(left));  // (else made selects on every tile)
+                asm volatile("" : "+v"(left));  // (else made selects on every page)
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -382,54 +469,42 @@ struct Rows {
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) top = fmaxf(top, x[t][j]);
-            if constexpr (!CACHED) top *= a.scale2;
-            if (__ballot(top > above)) {
-                float by = raise(top, a.unscale);
-                if constexpr (!CACHED) by *= a.unscale;
-#pragma unroll
-                for (int t = 0; t < NT; ++t) x[t] -= by;
-            }
+            if (__ballot(top > above)) raise(top);
             u32x4_t p[2 * NT];
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    f32x4_t f, y;
-                    if constexpr (CACHED) f = *reinterpret_cast<const f32x4_t*>(factors + 64 + 32 * (t0 + t) + 8 * b + 4 * g);
+                    const f32x4_t f = *reinterpret_cast<const f32x4_t*>(factors + 64 + 32 * (t0 + t) + 8 * b + 4 * g);
+                    f32x4_t y;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        y[j] = exp2_(CACHED ? x[t][4 * b + j] : x[t][4 * b + j] * a.scale2);
+                        y[j] = exp2_(x[t][4 * b + j] - m);
                         l += y[j];
-                        if constexpr (CACHED) y[j] *= f[j];
+                        y[j] *= f[j];
                     }
                     p[2 * t + (b >> 1)][2 * (b & 1)] = pack_bf16x2(y[0], y[1]);
                     p[2 * t + (b >> 1)][2 * (b & 1) + 1] = pack_bf16x2(y[2], y[3]);
                 }
-            if constexpr (CACHED) {
 #pragma unroll
-                for (int s = 0; s < 2 * NT; ++s)
+            for (int s = 0; s < 2 * NT; ++s)
 #pragma unroll
-                    for (int i = 0; i < KS; ++i) {
-                        const u32x4_t v = *reinterpret_cast<const u32x4_t*>(values + 4096 * i + value_place(c, 2 * (2 * t0 + s) + g));
-                        o[i] = mfma_bf16_32x32x16(v, p[s], o[i]);
-                    }
-            } else {
-                // a lane's address in a transposing read: token 4 g + (lane & 15) / 4, channels 16 (lane >> 4 & 1) + 4 (lane & 3) on
-                const int tok = 4 * g + ((lane & 15) >> 2), chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-                const uint8_t* at[2] = {values + token_place(tok, chunk) + 8 * (lane & 1), values + token_place(tok + 8, chunk) + 8 * (lane & 1)};
-                auto operand = [&](int s, int i) {
-                    u32x2_t w[2];
+                for (int i = 0; i < KS; ++i) {
+                    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(values + 4096 * i + value_place(c, 2 * (2 * t0 + s) + g));
+                    o[i] = mfma_bf16_32x32x16(v, p[s], o[i]);
+                }
+        }
+    }
+    // One tile of new tokens, its products and then its weights.
+    __device__ __forceinline__ void tile(const PrefillArgs& a, const uint8_t* keys, const uint8_t* values, bool masked, int limit) {
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        w[e] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                   (LHQ_LDS_AS s16x4_t*)(at[e] + 4096 * i + 1024 * (2 * t0 + s))));
-                    return u32x4_t{w[0][0], w[0][1], w[1][0], w[1][1]};
-                };
-#pragma unroll
-                for (int s = 0; s < 2 * NT; ++s)
-#pragma unroll
-                    for (int i = 0; i < KS; ++i) o[i] = mfma_bf16_32x32x16(operand(s, i), p[s], o[i]);
-            }
+        for (int t0 = 0; t0 < 2; t0 += NT) {
+            f32x16_t x[NT];
+            u32x4_t p[2 * NT];
+            products(keys, t0, x);
+            settle(a, t0, masked, limit, x);
+            weigh(a, x, p);
+            add<NT>(values, t0, p);
         }
     }
 };
@@ -452,10 +527,11 @@ __device__ void clear_rest(const PrefillArgs& a, int nth, int count) {
     }
 }
 
-template <int KS, int MODE>
-__global__ __launch_bounds__((64 * waves_of<KS, MODE>()), 2) void prefill_kernel(PrefillArgs a) {
+// MODE 0: no cache, 1: int8, 2: e4m3.  W waves, each with 32 rows.
+template <int KS, int MODE, int W>
+__global__ __launch_bounds__(64 * W, 2) void prefill_kernel(PrefillArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t prefill_lds[];
-    constexpr int kTile = KS * 4096, W = waves_of<KS, MODE>(), kRows = 32 * W;
+    constexpr int kTile = KS * 4096, kRows = 32 * W;
     const uint32_t unit = blockIdx.y + blockIdx.z * gridDim.y;
     const Found u = find_unit(a, unit, [](const Seq& q, int splits) { return static_cast<uint32_t>(q.blocks) * splits; });
     if (u.seq >= a.n_seqs) {
@@ -465,17 +541,13 @@ __global__ __launch_bounds__((64 * waves_of<KS, MODE>()), 2) void prefill_kernel
     const int h = blockIdx.x, G = a.group, D = a.c.D, R = u.q.T * G, lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int split = u.nth % u.splits;
-    // The blocks with the most keys first.  Where all are on the chip at once, the
-    // second half goes from the fewest keys up: it joins the first on the same CUs.
-    int block = u.nth / u.splits;
-    const int half = (u.q.blocks + 1) / 2;
-    block = u.splits == 1 && u.q.blocks <= a.resident && block >= half ? block - half : u.q.blocks - 1 - block;
+    const int block = u.q.blocks - 1 - u.nth / u.splits;  // those with the most keys first
     const int r0 = block * kRows, pages = (u.q.L + kKvPage - 1) / kKvPage;
     const int tiles = pages + (a.k_new ? ((min(r0 + kRows, R) - 1) / G) / kKvPage + 1 : 0);
     const int first = static_cast<int>(static_cast<int64_t>(tiles) * split / u.splits);
     const int end = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / u.splits);
-    auto keys = [&](int buf) { return prefill_lds + buf * 2 * kTile; };
-    auto factors = [&](int buf) { return reinterpret_cast<float*>(prefill_lds + 4 * kTile) + 128 * buf; };
+    auto place = [&](int t) { return prefill_lds + ((t - first) & 1) * 2 * kTile; };  // of tile t
+    auto factors = [&](int t) { return reinterpret_cast<float*>(prefill_lds + 4 * kTile) + 128 * ((t - first) & 1); };
     int* odd = reinterpret_cast<int*>(prefill_lds + 4 * kTile + 1024);  // infinite or NaN values were cleared
 
     // this wave's rows: (token, query head) pairs of the kv head; past the last one, that again, which is not kept
@@ -483,8 +555,6 @@ __global__ __launch_bounds__((64 * waves_of<KS, MODE>()), 2) void prefill_kernel
     const int r = min(r0 + 32 * wave + (lane & 31), R - 1), token = r / G;
     const int low = __builtin_amdgcn_readlane(token, 0), high = __builtin_amdgcn_readlane(token, 31);
     PageLoad<KS, W> page_load;
-    NewLoad<KS, W> new_load;
-    new_load.aim(a);
     int ids = 0;
     auto page_id = [&](int t) {  // 64 entries of the block table at a time, one a lane
         if (((t - first) & 63) == 0) ids = t + lane < pages ? a.c.page(u.seq, t + lane) : -1;
@@ -498,20 +568,27 @@ __global__ __launch_bounds__((64 * waves_of<KS, MODE>()), 2) void prefill_kernel
         next_there = id >= 0;
         if (next_there) page_load.load(a.c, id, h);
     };
-    auto page_arrives = [&](int t, int buf) {
+    auto page_arrives = [&](int t) {
         there = next_there;
-        if (there) page_load.template store<MODE == 2>(min(u.q.L - t * kKvPage, kKvPage), a.scale2, keys(buf), keys(buf) + kTile, factors(buf));
+        if (there) page_load.template store<MODE == 2>(min(u.q.L - t * kKvPage, kKvPage), a.scale2, place(t), place(t) + kTile, factors(t));
     };
-    auto fetch_new = [&](int t, int buf) {
-        new_load.load(a, u.q.lo, u.q.T, h, (t - pages) * kKvPage, keys(buf), keys(buf) + kTile);
+    NewTiles<KS, W> keys, values;
+    const int page_end = MODE == 0 ? first : min(end, max(first, pages));
+    {
+        const int j0 = (page_end - pages) * kKvPage, past = (end - pages) * kKvPage;
+        keys.aim(a.k_new, a.k_stride, u.q.lo, h, D, j0, past);
+        values.aim(a.v_new, a.v_stride, u.q.lo, h, D, j0, past);
+    }
+    auto values_arrive = [&](int t, uint8_t* at) {
+        if (t < end && t >= partly && clear_odd<KS, W>(a, at) && lane == 0) *odd = 1;
     };
-    auto new_arrives = [&](int t, int buf) {
-        if (t >= partly && clear_odd<KS, W>(a, keys(buf) + kTile) && lane == 0) *odd = 1;
-    };
-    const bool page_first = MODE != 0 && first < min(end, pages), new_first = !page_first && first < end;
-    if (page_first) fetch_page(first);
-    if (new_first) fetch_new(first, 0);
-    Rows<KS, MODE == 0> z;
+    if (first < page_end) {
+        fetch_page(first);
+    } else {
+        keys.fetch(a, u.q.T, place(first));
+        values.fetch(a, u.q.T, place(first) + kTile);
+    }
+    Rows<KS> z;
     {
         const uint16_t* from = a.q + (u.q.lo + token) * a.q_stride + static_cast<int64_t>(h * G + r - token * G) * D;
 #pragma unroll
@@ -520,55 +597,71 @@ __global__ __launch_bounds__((64 * waves_of<KS, MODE>()), 2) void prefill_kernel
     z.clear();
 
     if (threadIdx.x == 0) *odd = 0;
+    arrived();
     __syncthreads();
-    if (page_first) page_arrives(first, 0);
-    if (new_first) new_arrives(first, 0);
+    if (first < page_end) page_arrives(first);
+    else values_arrive(first, place(first) + kTile);
     __syncthreads();
     int t = first;
     if constexpr (MODE != 0) {
-        for (; t < min(end, pages); ++t) {
-            const int buf = (t - first) & 1;
-            const bool page_next = t + 1 < min(end, pages), new_next = t + 1 == pages && t + 1 < end;
-            if (page_next) fetch_page(t + 1);
-            if (new_next) fetch_new(t + 1, buf ^ 1);
+        for (; t < page_end; ++t) {
+            uint8_t *now = place(t), *next = place(t + 1);
+            if (t + 1 < page_end) {
+                fetch_page(t + 1);
+            } else {
+                keys.fetch(a, u.q.T, next);
+                values.fetch(a, u.q.T, next + kTile);
+            }
             if (some && there) {
                 const int left = min(u.q.L - t * kKvPage, kKvPage);
-                z.template step<true>(a, keys(buf), keys(buf) + kTile, factors(buf), left < kKvPage, left);
+                z.page(now, now + kTile, factors(t), left < kKvPage, left);
             }
-            if (page_next) page_arrives(t + 1, buf ^ 1);
-            if (new_next) new_arrives(t + 1, buf ^ 1);
+            if (t + 1 < page_end) {
+                page_arrives(t + 1);
+            } else {
+                arrived();
+                values_arrive(t + 1, next + kTile);
+            }
             __syncthreads();
         }
     }
+    // New tokens.
+    auto masked = [&](int t) { return (t - pages) * kKvPage + kKvPage - 1 > low; };
+    auto limit = [&](int t) { return token - (t - pages) * kKvPage + 1; };
+    const int last = some ? min(end - 1, pages + high / kKvPage) : first - 1;  // the last tile that this wave sees
+    uint8_t *now = place(t), *next = place(t + 1);
     for (; t < end; ++t) {
-        const int buf = (t - first) & 1, j0 = (t - pages) * kKvPage;
-        if (t + 1 < end) fetch_new(t + 1, buf ^ 1);
-        if (some && j0 <= high) z.template step<false>(a, keys(buf), keys(buf) + kTile, nullptr, j0 + kKvPage - 1 > low, token - j0 + 1);
-        if (t + 1 < end) new_arrives(t + 1, buf ^ 1);
+        keys.fetch(a, u.q.T, next);
+        values.fetch(a, u.q.T, next + kTile);
+        if (t <= last) z.tile(a, now, now + kTile, masked(t), limit(t));
+        arrived();
+        values_arrive(t + 1, next + kTile);
         __syncthreads();
+        uint8_t* was = now;
+        now = next;
+        next = was;
     }
 
     if (!some) return;
     z.l += other_half(z.l);
-    const bool mine = r0 + 32 * wave + (lane & 31) < R;
-    const int g = lane >> 5;
-    if (!mine) return;
-    // Infinite or NaN values that the row sees: added to what was written (a sum
-    // with them is what they are, whatever the weight).
-    auto add_odd = [&](auto* to, auto put) {
+    const int g = lane >> 5, mine = 32 * wave + (lane & 31);
+    // Infinite or NaN values that this lane's row sees: add(channel, value) for each (a
+    // sum with them is what they are, whatever the weight).
+    auto each_odd = [&](auto add) {
         if (*odd == 0) return;
-        const int last = min((end - pages) * kKvPage, token + 1);
-        for (int n = max(first, partly) * kKvPage - pages * kKvPage; n < last; ++n) {
+        const int past = min((end - pages) * kKvPage, token + 1);
+        for (int n = (max(first, partly) - pages) * kKvPage; n < past; ++n) {
             const uint16_t* row = a.v_new + (u.q.lo + static_cast<int64_t>(n)) * a.v_stride + h * D;
             for (int ch = 4 * g; ch < D; ch += ch % 4 == 3 ? 5 : 1) {
                 const float y = bf16_to_f32(row[ch]);
-                if (!(fabsf(y) < INFINITY)) put(to + ch, y);
+                if (!(fabsf(y) < INFINITY)) add(ch, y);
             }
         }
     };
     if (u.splits > 1) {
+        if (r0 + mine >= R) return;
         const int64_t part = static_cast<int64_t>(h) * 2 * a.slots + u.parts + block * u.splits + split;
-        const int64_t at = part * a.part_rows + 32 * wave + (lane & 31);
+        const int64_t at = part * a.part_rows + mine;
         if (g == 0) {
             a.ws_ml[2 * at] = z.l == 0.0f ? -INFINITY : z.m;
             a.ws_ml[2 * at + 1] = z.l;
@@ -580,21 +673,44 @@ __global__ __launch_bounds__((64 * waves_of<KS, MODE>()), 2) void prefill_kernel
             for (int b = 0; b < 4; ++b)
                 *reinterpret_cast<f32x4_t*>(to + 32 * i + 8 * b + 4 * g) =
                     f32x4_t{z.o[i][4 * b], z.o[i][4 * b + 1], z.o[i][4 * b + 2], z.o[i][4 * b + 3]};
-        add_odd(to, [](float* p, float y) { *p += y; });
+        each_odd([&](int ch, float y) { to[ch] += y; });
         return;
     }
+    // Results to LDS (the tiles' place is free), from there in rows: the chunk j of row
+    // c at place j ^ (c & kTurn).
+    constexpr int kChunks = 4 * KS, kTurn = KS % 4 == 0 ? 15 : KS % 2 == 0 ? 7 : 3;
+    uint8_t* rows = prefill_lds + wave * 32 * 16 * kChunks;
+    auto chunk_at = [&](int row, int chunk) { return rows + 16 * (row * kChunks + (chunk ^ (row & kTurn))); };
     const float by = z.l == 0.0f ? 0.0f : 1.0f / z.l;  // nothing seen: zeros
-    uint16_t* to = a.out + (static_cast<int64_t>(u.q.lo + token) * a.heads + h * G + r - token * G) * D;
 #pragma unroll
     for (int i = 0; i < KS; ++i)
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            const int ch = 32 * i + 8 * b + 4 * g;
+            float y[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (ch + j < D) to[ch + j] = f32_to_bf16(z.l == 0.0f ? 0.0f : z.o[i][4 * b + j] * by);
+            for (int j = 0; j < 4; ++j) y[j] = z.l == 0.0f ? 0.0f : z.o[i][4 * b + j] * by;
+            *reinterpret_cast<u32x2_t*>(chunk_at(lane & 31, 4 * i + b) + 8 * g) = u32x2_t{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
         }
-    add_odd(to, [](uint16_t* p, float y) { *p = f32_to_bf16(bf16_to_f32(*p) + y); });
+    each_odd([&](int ch, float y) {
+        uint16_t* to = reinterpret_cast<uint16_t*>(chunk_at(lane & 31, ch >> 3)) + (ch & 7);
+        *to = f32_to_bf16(bf16_to_f32(*to) + y);
+    });
+    const int out_row = token * a.heads + r - token * G;  // of (sequence, kv head)
+    uint16_t* out = a.out + (static_cast<int64_t>(u.q.lo) * a.heads + h * G) * D;
+    for (int n = lane; n < 32 * kChunks; n += 64) {
+        const int row = n / kChunks, ch = 8 * (n % kChunks), left = D - ch;
+        uint16_t* to = out + static_cast<int64_t>(__shfl(out_row, row, 64)) * D + ch;
+        if (r0 + 32 * wave + row >= R) break;
+        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(chunk_at(row, n % kChunks));
+        if (left <= 0) continue;
+        if (a.vec_out) {
+            *reinterpret_cast<u32x4_t*>(to) = w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < left) to[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+        }
+    }
 }
 
 // Joins the parts of split blocks in order of position: kJoinRows rows of a
@@ -640,7 +756,19 @@ int compute_units() {
 }
 // Workgroups of a kv head that splitting aims at: one a CU.  None where the rows
 // fill the chip as they are, or where no block can have two splits' tiles.
-int block_rows(int mode, int D) { return 32 * (mode == 0 && D <= 128 ? waves_of<4, 0>() : waves_of<8, 1>()); }
+// Rows of a workgroup.  256, eight waves, bring a tile to LDS half as often; 128 make
+// two workgroups of a CU, which wait for different things, where LDS and registers
+// hold two (without a cache, up to 128 channels), and leave less over at the end.
+// Measured, 128 / 256 rows, 32 heads over 8: 2048 tokens 52 / 61 us, 16 prompts of up
+// to 2048 212 / 219, 4096 tokens 154 / 142, 16384 2054 / 2019; 64 channels, 8192
+// tokens 317 / 360; 96 channels 433 / 444; 16 heads over 4 of 192 483 / 384, of 256
+// 931 / 602.  With a cache a page is made bf16 by all waves: 256.
+int block_rows(int mode, int D, int n_seqs, int capacity, int heads) {
+    const int64_t blocks = static_cast<int64_t>(capacity) * heads / 256, cus = compute_units();
+    if (mode != 0) return 256;
+    if (D > 128) return blocks >= cus ? 256 : 128;
+    return D > 96 && blocks >= 2 * cus && capacity / std::max(n_seqs, 1) >= 4096 ? 256 : 128;
+}
 int want_slots(int block_rows, int capacity, int heads, int kv_heads, int64_t most_tiles) {
     const int cus = compute_units();
     const int64_t rows = static_cast<int64_t>(capacity) * (heads / kv_heads);
@@ -657,12 +785,12 @@ dim3 unit_grid(int heads, int64_t units) {
     return dim3(heads, y, static_cast<unsigned>((units + y - 1) / y));
 }
 
-template <int KS, int MODE>
+template <int KS, int MODE, int W>
 int launch(const char* fn, const PrefillArgs& a, dim3 grid, hipStream_t s) {
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&prefill_kernel<KS, MODE>),
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&prefill_kernel<KS, MODE, W>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (attr != hipSuccess) return set_error(LHQ_ERR_HIP, "%s: dynamic LDS attribute: %s", fn, hipGetErrorString(attr));
-    prefill_kernel<KS, MODE><<<grid, 64 * waves_of<KS, MODE>(), lds_bytes<KS>(), s>>>(a);
+    prefill_kernel<KS, MODE, W><<<grid, 64 * W, lds_bytes<KS>(), s>>>(a);
     return check_launch(fn);
 }
 
@@ -673,13 +801,10 @@ int prefill(const char* fn, PrefillArgs a, int mode, int clear_rest, float scale
     LHQ_REQUIRE(a.heads > 0 && a.heads % kv_heads == 0, "%s: %d query heads are no multiple of %d kv heads", fn, a.heads, kv_heads);
     LHQ_SUPPORTED(a.heads <= 65535, "%s: %d query heads are over 65535", fn, a.heads);
     a.group = a.heads / kv_heads;
-    a.block_rows = block_rows(mode, D);
-    a.resident = compute_units() * (a.block_rows == 128 ? 2 : 1) / kv_heads;
+    a.block_rows = block_rows(mode, D, a.n_seqs, a.capacity, a.heads);
     LHQ_SUPPORTED(static_cast<int64_t>(a.capacity) * a.heads < INT32_MAX - a.block_rows, "%s: %d rows of %d heads are over 2^31", fn, a.capacity, a.heads);
     a.scale2 = scale * 1.4426950408889634f;  // weights are powers of two
     LHQ_REQUIRE(std::isfinite(a.scale2) && scale > 0.0f, "%s: scale %g is not positive and finite, also times log2 e", fn, scale);
-    a.unscale = 1.0f / a.scale2;
-    LHQ_SUPPORTED(a.scale2 >= 0x1p-100f, "%s: scale %g is under 2^-100", fn, scale);
     LHQ_REQUIRE((a.k_new == nullptr) == (a.v_new == nullptr), "%s: new keys without values, or values without keys", fn);
     LHQ_REQUIRE(a.q_stride >= static_cast<int64_t>(a.heads) * D, "%s: q rows of stride %lld are under %d heads of %d", fn,
                 static_cast<long long>(a.q_stride), a.heads, D);
@@ -714,7 +839,8 @@ int prefill(const char* fn, PrefillArgs a, int mode, int clear_rest, float scale
     const hipStream_t s = as_stream(stream);
     int st = LHQ_OK;
     auto go = [&](auto ks) {
-        st = mode == 0 ? launch<ks(), 0>(fn, a, grid, s) : mode == 1 ? launch<ks(), 1>(fn, a, grid, s) : launch<ks(), 2>(fn, a, grid, s);
+        st = mode == 1 ? launch<ks(), 1, 8>(fn, a, grid, s) : mode == 2 ? launch<ks(), 2, 8>(fn, a, grid, s) :
+             a.block_rows == 128 ? launch<ks(), 0, 4>(fn, a, grid, s) : launch<ks(), 0, 8>(fn, a, grid, s);
     };
     switch (kv_padded(D) / 32) {
         case 1: go(std::integral_constant<int, 1>{}); break;
@@ -744,7 +870,7 @@ int64_t lhq_prefill_workspace_bytes(int n_seqs, int row_capacity, int n_heads, i
         head_dim <= 0 || head_dim > kKvMaxDim)
         return 0;
     int64_t most = 0;
-    for (int rows : {block_rows(0, head_dim), block_rows(1, head_dim)})
+    for (int rows : {128, 256})
         most = std::max(most, static_cast<int64_t>(n_kv_heads) * 2 * want_slots(rows, row_capacity, n_heads, n_kv_heads, INT64_MAX) *
                                   part_bytes(part_rows(rows, row_capacity, n_heads, n_kv_heads), head_dim));
     return most;

@@ -15,6 +15,7 @@
 // goes through the Taylor series of sine and cosine.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kvcommon.hpp"
 
@@ -126,6 +127,182 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs<T> a) {
     }
 }
 
+// Sum over 1 << LB adjacent lanes (4 to 32), the same in all of them.
+template <int LB, typename S>
+__device__ __forceinline__ S lanes_sum(S x) {
+#pragma unroll
+    for (int d = 1; d < 1 << LB; d <<= 1) x += __shfl_xor(x, d, 64);
+    return x;
+}
+// A vector is 16 bytes, at any alignment.
+template <typename T>
+constexpr int vector_of() { return 16 / sizeof(T); }
+template <typename T>
+__device__ __forceinline__ u32x4_t load_vector(const T* from) {
+    u32x4_t w;
+    __builtin_memcpy(&w, from, 16);
+    return w;
+}
+template <typename T>
+__device__ __forceinline__ void store_vector(T* to, u32x4_t w) { __builtin_memcpy(to, &w, 16); }
+__device__ __forceinline__ void unpack(u32x4_t w, float (&x)[8]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        x[2 * j] = __uint_as_float(w[j] << 16);
+        x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void unpack(u32x4_t w, float (&x)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(w[j]);
+}
+__device__ __forceinline__ u32x4_t pack(const float (&x)[8]) {
+    return u32x4_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+}
+__device__ __forceinline__ u32x4_t pack(const float (&x)[4]) {
+    return u32x4_t{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+}
+
+// Rows whose heads are whole vectors: a lane has two vectors of a head, of which each
+// pair has its channels in the lane, 1 << LB lanes a head, kHeads heads of a row beside
+// one another.  The workgroup makes its rows' cosines and sines once, one or two a
+// thread, through LDS, and a lane keeps its own for all the heads it goes through, of
+// which kBatch are on their way at a time.
+// Bound by memory: 32768 rows of 32 and 8 heads of 128 in bf16, 671 MB.
+constexpr int kHeads = 8, kBatch = 4;
+template <typename T, bool INTERLEAVED, int LB>
+__global__ __launch_bounds__(kRopeThreads) void rope_vec_kernel(RopeArgs<T> a) {
+    constexpr int V = vector_of<T>(), kRows = (kRopeThreads >> LB) / kHeads, kPairs = V << LB;
+    __shared__ __attribute__((aligned(16))) float cosines[kRows][kPairs], sines[kRows][kPairs];
+    const int pairs = a.rot / 2, first_row = blockIdx.x * kRows;
+    for (int n = threadIdx.x; n < kRows * kPairs; n += kRopeThreads) {
+        const int row = first_row + n / kPairs, i = n % kPairs;
+        if (row >= a.n_rows || i >= pairs) continue;
+        float c, s;
+        turn(static_cast<uint64_t>(max(a.positions[row], 0)) * a.turns[i], c, s);
+        cosines[n / kPairs][i] = c * a.gain;
+        sines[n / kPairs][i] = s * a.gain;
+    }
+    __syncthreads();
+    const int group = threadIdx.x >> LB, unit = threadIdx.x & ((1 << LB) - 1), r = group / kHeads;
+    const int64_t row = first_row + r;
+    const int units = a.D / (2 * V), heads = a.heads[0] + a.heads[1];
+    const bool turned = unit * V < pairs, in = unit < units;
+    if (row >= a.n_rows) return;
+    const bool somewhere = a.positions[row] >= 0;
+    // this lane's vectors of a head
+    const int at0 = turned && !INTERLEAVED ? unit * V : 2 * unit * V;
+    const int at1 = turned && !INTERLEAVED ? unit * V + pairs : 2 * unit * V + V;
+    float c[V], s[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        c[j] = cosines[r][unit * V + j];
+        s[j] = sines[r][unit * V + j];
+    }
+    float w0[V], w1[V];
+    int side = -1;
+    bool norm = false;
+    for (int h0 = blockIdx.y * kBatch * kHeads + group % kHeads; h0 < heads; h0 += gridDim.y * kBatch * kHeads) {
+        u32x4_t x0[kBatch], x1[kBatch];
+        T* to[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const int h = min(h0 + k * kHeads, heads - 1);  // (past the last one that again, not kept)
+            const int of = h >= a.heads[0], head = of ? h - a.heads[0] : h;
+            const T* from = (of ? a.x[1] + row * a.in_stride[1] : a.x[0] + row * a.in_stride[0]) + static_cast<int64_t>(head) * a.D;
+            to[k] = (of ? a.y[1] + row * a.out_stride[1] : a.y[0] + row * a.out_stride[0]) + static_cast<int64_t>(head) * a.D;
+            if (in) {
+                x0[k] = load_vector(from + at0);
+                x1[k] = load_vector(from + at1);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const int h = h0 + k * kHeads, of = h >= a.heads[0];
+            if (h >= heads) break;
+            if (of != side) {
+                side = of;
+                const T* w = a.weight[of];
+                norm = w != nullptr;
+                if (norm && in) {
+                    unpack(load_vector(w + at0), w0);
+                    unpack(load_vector(w + at1), w1);
+                }
+            }
+            if (somewhere) {
+                float y0[V], y1[V];
+                unpack(x0[k], y0);
+                unpack(x1[k], y1);
+                if (norm) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) sum += y0[j] * y0[j] + y1[j] * y1[j];
+                    sum = lanes_sum<LB>(in ? sum : 0.0f);
+                    const float mean = sum / static_cast<float>(a.D) + a.eps;
+                    float by = __builtin_amdgcn_rsqf(mean);
+                    if (!(mean >= 0x1p-60f && sum < 0x1p126f)) {  // squares out of fp32's range
+                        double all = 0.0;
+#pragma unroll
+                        for (int j = 0; j < V; ++j)
+                            all += static_cast<double>(y0[j]) * y0[j] + static_cast<double>(y1[j]) * y1[j];
+                        const double d = 1.0 / sqrt(lanes_sum<LB>(in ? all : 0.0) / a.D + a.eps);
+#pragma unroll
+                        for (int j = 0; j < V; ++j) {  // (the factor itself may be out of it)
+                            y0[j] = static_cast<float>(y0[j] * d);
+                            y1[j] = static_cast<float>(y1[j] * d);
+                        }
+                        by = 1.0f;
+                    }
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        y0[j] = y0[j] * by * w0[j];
+                        y1[j] = y1[j] * by * w1[j];
+                    }
+                }
+                if (turned) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        float& p = INTERLEAVED ? (2 * j < V ? y0[2 * j % V] : y1[2 * j % V]) : y0[j];
+                        float& q = INTERLEAVED ? (2 * j < V ? y0[2 * j % V + 1] : y1[2 * j % V + 1]) : y1[j];
+                        const float t = p * c[j] - q * s[j];
+                        q = q * c[j] + p * s[j];
+                        p = t;
+                    }
+                }
+                x0[k] = pack(y0);
+                x1[k] = pack(y1);
+            }
+            if (in) {
+                store_vector(to[k] + at0, x0[k]);
+                store_vector(to[k] + at1, x1[k]);
+            }
+        }
+    }
+}
+
+// Whether rope_vec_kernel takes a call: heads of whole vectors, pairs (or channels that
+// are not turned) in the same lane.
+template <typename T>
+bool whole_vectors(const RopeArgs<T>& a, bool interleaved) {
+    constexpr int V = vector_of<T>();
+    return a.D % (2 * V) == 0 && (interleaved ? a.rot % (2 * V) == 0 : a.rot / 2 % V == 0);
+}
+template <typename T, bool INTERLEAVED>
+void launch_vec(const RopeArgs<T>& a, hipStream_t s) {
+    const int units = a.D / (2 * vector_of<T>()), heads = a.heads[0] + a.heads[1];
+    auto go = [&](auto lb) {
+        constexpr int kRows = (kRopeThreads >> lb()) / kHeads;
+        const unsigned x = static_cast<unsigned>((a.n_rows + kRows - 1) / kRows);
+        // a workgroup for each batch of heads while there are too few for the chip
+        const unsigned y = std::min((heads + kBatch * kHeads - 1) / (kBatch * kHeads), static_cast<int>(1 + 2048 / x));
+        rope_vec_kernel<T, INTERLEAVED, lb()><<<dim3(x, y), kRopeThreads, 0, s>>>(a);
+    };
+    if (units <= 4) go(std::integral_constant<int, 2>{});
+    else if (units <= 8) go(std::integral_constant<int, 3>{});
+    else if (units <= 16) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 5>{});
+}
+
 template <typename T>
 int rope(const char* fn, const T* q, int64_t q_stride, const T* k, int64_t k_stride, const int32_t* positions,
          const uint64_t* turns, const T* q_weight, const T* k_weight, float eps, float gain, T* q_out,
@@ -165,9 +342,14 @@ int rope(const char* fn, const T* q, int64_t q_stride, const T* k, int64_t k_str
                 "%s: a result overlaps an input or the other result", fn);
     RopeArgs<T> a{{q, k},         {q_stride, k_stride}, {q_out, k_out}, {q_out_stride, k_out_stride},
                   {q_weight, k_weight}, {n_heads, n_kv_heads}, positions, turns, n_rows, D, rot, eps, gain};
+    const hipStream_t s = as_stream(stream);
+    if (whole_vectors(a, interleaved != 0)) {
+        if (interleaved) launch_vec<T, true>(a, s);
+        else launch_vec<T, false>(a, s);
+        return check_launch(fn);
+    }
     const int heads = n_heads + n_kv_heads;
     const dim3 grid(n_rows, std::min((heads + 3) / 4, 65535));
-    const hipStream_t s = as_stream(stream);
     if (interleaved) rope_kernel<T, true><<<grid, kRopeThreads, 0, s>>>(a);
     else rope_kernel<T, false><<<grid, kRopeThreads, 0, s>>>(a);
     return check_launch(fn);
