@@ -33,8 +33,8 @@ typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 // 2^kLag: weights go up to 2^kLag, which costs none of their bits.
 constexpr float kLag = 6.0f;
 constexpr int kMostSplits = 64;  // of a block's keys
-constexpr int kLeastTiles = 16;  // of a split: the launch that joins takes as long as some tiles
-constexpr int kJoinRows = 64;    // of a workgroup that joins splits
+constexpr int kLeastTiles = 8;   // of a split: the launch that joins takes as long as some tiles
+constexpr int kJoinRows = 8;     // of a workgroup that joins splits
 
 struct PrefillArgs {
     const uint16_t* q;
@@ -52,7 +52,7 @@ struct PrefillArgs {
     bool vec_new;          // rows of k_new, v_new: 16-byte loads at 32-bit offsets from a tile's first
     bool vec_out;          // rows of out: 16-byte stores
     bool clear_rest;       // rows of no sequence become zeros
-    int slots;             // workgroups of a kv head that splitting aims at, 0: no splitting
+    int slots;             // workgroups of a kv head that are on the chip at once, 0: no splitting
     int block_rows;        // rows of a workgroup
     int part_rows;         // rows of a part in the workspace
     float* ws_o;           // [kv head][part][part_rows][Dp]
@@ -78,21 +78,31 @@ __device__ __forceinline__ Seq seq_of(const PrefillArgs& a, int s) {
     q.tiles = (q.L + kKvPage - 1) / kKvPage + (a.k_new ? (q.T + kKvPage - 1) / kKvPage : 0);
     return q;
 }
-// Tiles that a split has at least: all blocks' tiles over the workgroups wanted.
-// Blocks that have more are split, into less than 2 * slots parts in all (a block
-// of t > target tiles has ceil(t / target) < 2 t / target of them).
-__device__ __forceinline__ int split_target(const PrefillArgs& a, const Seq& first) {
-    if (a.slots == 0) return INT32_MAX;
-    double work = 0.0;
-    for (int base = 0; base < a.n_seqs; base += 64) {
-        const Seq q = base == 0 ? first : seq_of(a, base + (threadIdx.x & 63));
-        work += static_cast<double>(q.blocks) * q.tiles;
-    }
-    for (int d = 32; d; d >>= 1) work += __shfl_xor(work, d, 64);
-    return max(kLeastTiles, static_cast<int>(min(work / a.slots, 2147483000.0)) + 1);
-}
 __device__ __forceinline__ int split_count(const Seq& q, int target) {
     return q.tiles <= target ? 1 : min((q.tiles + target - 1) / target, kMostSplits);
+}
+// Tiles that a split has at most: all blocks' tiles over the workgroups wanted, or
+// half of that where the parts would not all be on the chip at once (a finer grain
+// leaves less over at the end).  Blocks that have more are split, into less than 4 *
+// slots parts in all: a block of t > target tiles has ceil(t / target) < 2 t / target.
+__device__ __forceinline__ int split_target(const PrefillArgs& a, const Seq& first) {
+    if (a.slots == 0) return INT32_MAX;
+    auto over_all = [&](auto of) {  // (held at 2^32 - 1)
+        uint32_t sum = 0;
+        for (int base = 0; base < a.n_seqs; base += 64) {
+            const uint32_t x = of(base == 0 ? first : seq_of(a, base + (threadIdx.x & 63)));
+            sum = __builtin_elementwise_add_sat(sum, static_cast<uint32_t>(__builtin_amdgcn_readlane(kv_scan(x), 63)));
+        }
+        return sum;
+    };
+    const uint32_t work = over_all([](const Seq& q) {
+        return static_cast<uint32_t>(min(static_cast<uint64_t>(q.blocks) * q.tiles, uint64_t{0xffffffff}));
+    });
+    if (work == 0xffffffff) return INT32_MAX;  // (more than the chip has workgroups, by far)
+    auto target = [work](uint32_t slots) { return max(kLeastTiles, static_cast<int>(min(work / slots, 0x7ffffffeu)) + 1); };
+    const int once = target(a.slots);
+    const uint32_t units = over_all([once](const Seq& q) { return static_cast<uint32_t>(q.blocks) * split_count(q, once); });
+    return units <= static_cast<uint32_t>(a.slots) ? once : target(2 * a.slots);
 }
 // The unit with number `unit` in the list that has count(sequence, splits) units
 // of each sequence in turn: the sequence, the unit's number within it, and the
@@ -660,7 +670,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(PrefillArgs a) {
     };
     if (u.splits > 1) {
         if (r0 + mine >= R) return;
-        const int64_t part = static_cast<int64_t>(h) * 2 * a.slots + u.parts + block * u.splits + split;
+        const int64_t part = static_cast<int64_t>(h) * 4 * a.slots + u.parts + block * u.splits + split;
         const int64_t at = part * a.part_rows + mine;
         if (g == 0) {
             a.ws_ml[2 * at] = z.l == 0.0f ? -INFINITY : z.m;
@@ -715,32 +725,58 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(PrefillArgs a) {
 
 // Joins the parts of split blocks in order of position: kJoinRows rows of a
 // block a workgroup, four channels a thread at a time.
-__global__ __launch_bounds__(256) void prefill_join_kernel(PrefillArgs a) {
-    const Found u = find_unit(a, blockIdx.y + blockIdx.z * gridDim.y, [&](const Seq& q, int splits) {
-        return splits > 1 ? static_cast<uint32_t>(q.blocks) * (a.block_rows / kJoinRows) : 0u;
-    });
-    if (u.seq >= a.n_seqs) return;
+__device__ void join_rows(const PrefillArgs& a, const Found& u) {
     const int h = blockIdx.x, G = a.group, D = a.c.D, Dp = a.c.Dp(), R = u.q.T * G;
     const int chunks = a.block_rows / kJoinRows, block = u.nth / chunks, from = u.nth % chunks * kJoinRows;
-    const int64_t part = static_cast<int64_t>(h) * 2 * a.slots + u.parts + block * u.splits;
+    const int64_t part = static_cast<int64_t>(h) * 4 * a.slots + u.parts + block * u.splits;
     for (int n = threadIdx.x; n < kJoinRows * (Dp / 4); n += 256) {
         const int row = from + n / (Dp / 4), ch = 4 * (n % (Dp / 4)), r = block * a.block_rows + row;
         if (r >= R) return;
-        const int64_t at = part * a.part_rows + row;
+        const int64_t at = part * a.part_rows + row, step = a.part_rows;
+        // eight parts on their way at a time; past the last one, that again with no weight
+        constexpr int kBatch = 8;
         float top = -INFINITY, weight = 0.0f;
-        for (int s = 0; s < u.splits; ++s) top = fmaxf(top, a.ws_ml[2 * (at + static_cast<int64_t>(s) * a.part_rows)]);
-        const float ref = top == -INFINITY ? 0.0f : top;
         f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < u.splits; ++s) {
-            const int64_t p = at + static_cast<int64_t>(s) * a.part_rows;
-            const float f = exp2_(a.ws_ml[2 * p] - ref);
-            weight += a.ws_ml[2 * p + 1] * f;
-            sum += *reinterpret_cast<const f32x4_t*>(a.ws_o + p * Dp + ch) * f;
+        for (int s0 = 0; s0 < u.splits; s0 += kBatch) {
+            float m[kBatch], l[kBatch];
+            f32x4_t o[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int64_t p = at + min(s0 + k, u.splits - 1) * step;
+                m[k] = s0 + k < u.splits ? a.ws_ml[2 * p] : -INFINITY;
+                l[k] = a.ws_ml[2 * p + 1];
+                o[k] = *reinterpret_cast<const f32x4_t*>(a.ws_o + p * Dp + ch);
+            }
+            float most = top;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) most = fmaxf(most, m[k]);
+            if (most == -INFINITY) continue;
+            const float f = exp2_(top - most);
+            weight *= f;
+            sum *= f;
+            top = most;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const float y = exp2_(m[k] - most);
+                if (y != 0.0f) {  // (a part without weight may hold anything)
+                    weight += l[k] * y;
+                    sum += o[k] * y;
+                }
+            }
         }
         uint16_t* out = a.out + (static_cast<int64_t>(u.q.lo + r / G) * a.heads + h * G + r % G) * D;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (ch + j < D) out[ch + j] = f32_to_bf16(weight == 0.0f ? 0.0f : sum[j] / weight);
+    }
+}
+__global__ __launch_bounds__(256) void prefill_join_kernel(PrefillArgs a) {
+    const int chunks = a.block_rows / kJoinRows;
+    // (how many there are is known here alone; the grid is as many as run at once)
+    for (uint32_t unit = blockIdx.y;; unit += gridDim.y) {
+        const Found u = find_unit(a, unit, [&](const Seq& q, int splits) { return splits > 1 ? static_cast<uint32_t>(q.blocks) * chunks : 0u; });
+        if (u.seq >= a.n_seqs) return;
+        join_rows(a, u);
     }
 }
 
@@ -754,8 +790,8 @@ int compute_units() {
     }
     return n;
 }
-// Workgroups of a kv head that splitting aims at: one a CU.  None where the rows
-// fill the chip as they are, or where no block can have two splits' tiles.
+// Workgroups of a kv head that are on the chip at once: one a CU.  None where the
+// rows fill it four times over, or where splits would have too few tiles each.
 // Rows of a workgroup.  256, eight waves, bring a tile to LDS half as often; 128 make
 // two workgroups of a CU, which wait for different things, where LDS and registers
 // hold two (without a cache, up to 128 channels), and leave less over at the end.
@@ -772,7 +808,7 @@ int block_rows(int mode, int D, int n_seqs, int capacity, int heads) {
 int want_slots(int block_rows, int capacity, int heads, int kv_heads, int64_t most_tiles) {
     const int cus = compute_units();
     const int64_t rows = static_cast<int64_t>(capacity) * (heads / kv_heads);
-    if (rows / block_rows * kv_heads >= cus || most_tiles <= kLeastTiles) return 0;
+    if (rows / block_rows * kv_heads >= 4 * cus || most_tiles <= 2 * kLeastTiles) return 0;
     return std::max(1, cus / kv_heads);
 }
 int64_t part_bytes(int rows, int D) { return static_cast<int64_t>(rows) * (kv_padded(D) + 2) * 4; }
@@ -825,14 +861,14 @@ int prefill(const char* fn, PrefillArgs a, int mode, int clear_rest, float scale
     a.clear_rest = clear_rest != 0;
     const int64_t tiles = a.c.max_pages + (a.k_new ? (static_cast<int64_t>(a.capacity) + kKvPage - 1) / kKvPage : 0);
     a.part_rows = part_rows(a.block_rows, a.capacity, a.heads, kv_heads);
-    // as many parts as there is room for, two a slot
-    const int64_t room = workspace ? workspace_bytes / part_bytes(a.part_rows, D) / (2 * kv_heads) : 0;
+    // as many parts as there is room for, four a slot
+    const int64_t room = workspace ? workspace_bytes / part_bytes(a.part_rows, D) / (4 * kv_heads) : 0;
     a.slots = static_cast<int>(std::min<int64_t>(want_slots(a.block_rows, a.capacity, a.heads, kv_heads, tiles), room));
-    const int64_t parts = static_cast<int64_t>(kv_heads) * 2 * a.slots;
+    const int64_t parts = static_cast<int64_t>(kv_heads) * 4 * a.slots;
     a.ws_o = static_cast<float*>(workspace);
     a.ws_ml = a.ws_o + parts * a.part_rows * kv_padded(D);
     const int64_t rows = static_cast<int64_t>(a.capacity) * a.group;
-    const int64_t units = rows / a.block_rows + std::min(a.n_seqs, a.capacity) + 2 * a.slots + (clear_rest ? 1 : 0);
+    const int64_t units = rows / a.block_rows + std::min(a.n_seqs, a.capacity) + 4 * a.slots + (clear_rest ? 1 : 0);
     LHQ_SUPPORTED(units * kv_heads < INT32_MAX / (2 * a.block_rows), "%s: %lld query blocks of %d heads are over the grid", fn,
                   static_cast<long long>(units), kv_heads);
     const dim3 grid = unit_grid(kv_heads, units);
@@ -853,8 +889,9 @@ int prefill(const char* fn, PrefillArgs a, int mode, int clear_rest, float scale
         default: go(std::integral_constant<int, 8>{}); break;
     }
     if (st != LHQ_OK || a.slots == 0) return st;
-    // (less than one split block a slot)
-    prefill_join_kernel<<<unit_grid(kv_heads, static_cast<int64_t>(a.slots) * (a.block_rows / kJoinRows)), 256, 0, s>>>(a);
+    // (a split block has two parts or more: less than two a slot)
+    const int join_units = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(2 * a.slots) * (a.block_rows / kJoinRows), 2048 / kv_heads + 1));
+    prefill_join_kernel<<<dim3(kv_heads, join_units), 256, 0, s>>>(a);
     return check_launch(fn);
 }
 
@@ -871,7 +908,7 @@ int64_t lhq_prefill_workspace_bytes(int n_seqs, int row_capacity, int n_heads, i
         return 0;
     int64_t most = 0;
     for (int rows : {128, 256})
-        most = std::max(most, static_cast<int64_t>(n_kv_heads) * 2 * want_slots(rows, row_capacity, n_heads, n_kv_heads, INT64_MAX) *
+        most = std::max(most, static_cast<int64_t>(n_kv_heads) * 4 * want_slots(rows, row_capacity, n_heads, n_kv_heads, INT64_MAX) *
                                   part_bytes(part_rows(rows, row_capacity, n_heads, n_kv_heads), head_dim));
     return most;
 }

@@ -470,16 +470,20 @@ class KvPlan:
     left: torch.Tensor
 
 
-def _on_one_gpu(fn: str, *tensors: torch.Tensor | None) -> None:
+def _on_one_gpu(fn: str, first: torch.Tensor, *tensors: torch.Tensor | None) -> None:
     """All of them on the current GPU, on whose stream the call is launched."""
-    at = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    at = first.get_device()
+    if at < 0:
+        raise ValueError(f"{fn}: a tensor is on {first.device}, not on a GPU")
+    if at != torch.cuda.current_device():
+        raise ValueError(f"{fn}: a tensor of {first.device}, the current GPU is {torch.cuda.current_device()}")
     for t in tensors:
-        if t is not None and (t.get_device() != at or at < 0):
-            raise ValueError(f"{fn}: a tensor of {t.device}, the current GPU is {at}")
+        if t is not None and t.get_device() != at:
+            raise ValueError(f"{fn}: a tensor of {t.device} with one of {first.device}")
 
 
 def _packed(fn: str, name: str, t: torch.Tensor, dtype, shape) -> None:
-    if t.dtype is not dtype or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{fn}: {name} must be contiguous {list(shape)} {dtype}, got {tuple(t.shape)} {t.dtype}")
 
 
@@ -585,40 +589,53 @@ def rope(plan: RopePlan, q: torch.Tensor | None, k: torch.Tensor | None, positio
     positions (int32 [n]; rows of negative ones are passed on as they are), each
     head RMS-normed first where a weight [head_dim] is given.  Returns (q, k) [n,
     heads, head_dim], in new tensors or in ``out``, which may be (q, k)."""
-    D = plan.head_dim
+    D, turns = plan.head_dim, plan.turns
     some = q if q is not None else k
     if some is None:
         raise ValueError("rope: neither queries nor keys")
-    dt, n = some.dtype, some.shape[0] if some.dim() else 0
-    if out is None:
-        out = tuple(None if t is None or t.dim() < 2 else t.new_empty((n, t[0].numel() // D if n else 0, D)) for t in (q, k))
-    args, heads = [], []
-    for name, t, w, o in (("q", q, q_weight, out[0]), ("k", k, k_weight, out[1])):
-        if t is None:
-            if o is not None or w is not None:
-                raise ValueError(f"rope: a weight or a result of {name} without {name}")
-            args.append((0, 0, 0, 0, 0))
-            heads.append(0)
-            continue
-        shape = t.shape
-        H = shape[1] // D if len(shape) == 2 else shape[1] if len(shape) == 3 else 0
-        rows, stride = _kv_rows("rope", name, t, H, D, (dt,) if dt in _KV_ROWS else _KV_ROWS)
-        if o is None:
-            raise ValueError(f"rope: no result for {name}")
-        o_rows, o_stride = _kv_rows("rope", f"the result of {name}", o, H, D, (dt,))
-        if rows != n or o_rows != n:
-            raise ValueError(f"rope: {n} rows, {rows} of {name}, {o_rows} of its result")
-        if w is not None:
-            _packed("rope", f"the weight of {name}", w, dt, (D,))
-        args.append((t.data_ptr(), stride, P(w), o.data_ptr(), o_stride))
-        heads.append(H)
+    dt = some.dtype
+    if dt not in _KV_ROWS:
+        raise ValueError(f"rope: rows are {dt}, not one of {[str(d) for d in _KV_ROWS]}")
+    n, Hq, qs = _rope_rows("q", q, D, dt)
+    k_rows, Hk, ks = _rope_rows("k", k, D, dt)
+    if q is None:
+        n = k_rows
+    elif k is not None and k_rows != n:
+        raise ValueError(f"rope: {n} rows of q and {k_rows} of k")
     _packed("rope", "positions", positions, torch.int32, (n,))
-    _on_one_gpu("rope", q, k, positions, plan.turns, q_weight, k_weight, *out)
-    (qp, qs, qw, qo, qos), (kp, ks, kw, ko, kos) = args
-    lib().call("lhq_rope_f32" if dt == torch.float32 else "lhq_rope_bf16", qp, qs, kp, ks, positions.data_ptr(),
-               plan.turns.data_ptr(), qw, kw, eps, plan.gain, qo, qos, ko, kos, int(plan.interleaved), n, heads[0],
-               heads[1], D, plan.rot_dim, stream())
+    for name, t, w in (("q", q, q_weight), ("k", k, k_weight)):
+        if w is not None:
+            if t is None:
+                raise ValueError(f"rope: a weight of {name} without {name}")
+            _packed("rope", f"the weight of {name}", w, dt, (D,))
+    if out is None:
+        q_out = None if q is None else q.new_empty((n, Hq, D))
+        k_out = None if k is None else k.new_empty((n, Hk, D))
+        out, qos, kos = (q_out, k_out), Hq * D, Hk * D
+    else:
+        q_out, k_out = out
+        if (q_out is None) != (q is None) or (k_out is None) != (k is None):
+            raise ValueError("rope: results for the sides that are given, and for no others")
+        qo_rows, qo_heads, qos = _rope_rows("the result of q", q_out, D, dt)
+        ko_rows, ko_heads, kos = _rope_rows("the result of k", k_out, D, dt)
+        if (q is not None and (qo_rows, qo_heads) != (n, Hq)) or (k is not None and (ko_rows, ko_heads) != (n, Hk)):
+            raise ValueError(f"rope: results of {qo_rows} x {qo_heads} and {ko_rows} x {ko_heads} heads for "
+                             f"{n} x {Hq} and {n} x {Hk}")
+    _on_one_gpu("rope", positions, q, k, turns, q_weight, k_weight, q_out, k_out)
+    lib().call("lhq_rope_f32" if dt == torch.float32 else "lhq_rope_bf16", P(q), qs, P(k), ks, positions.data_ptr(),
+               turns.data_ptr(), P(q_weight), P(k_weight), eps, plan.gain, P(q_out), qos, P(k_out), kos,
+               int(plan.interleaved), n, Hq, Hk, D, plan.rot_dim, stream())
     return out
+
+
+def _rope_rows(name: str, t: torch.Tensor | None, D: int, dt) -> tuple[int, int, int]:
+    """(rows, heads, the stride between rows) of one side, zeros where there is none."""
+    if t is None:
+        return 0, 0, 0
+    shape = t.shape
+    heads = shape[1] // D if len(shape) == 2 else shape[1] if len(shape) == 3 else 0
+    n, stride = _kv_rows("rope", name, t, heads, D, (dt,))
+    return n, heads, stride
 
 
 def prefill_workspace(n_seqs: int, n: int, n_heads: int, n_kv_heads: int, head_dim: int) -> torch.Tensor | None:
