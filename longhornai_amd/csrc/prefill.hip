@@ -457,14 +457,14 @@ struct Rows {
         for (int t0 = 0; t0 < 2; t0 += NT) {
             f32x16_t x[NT];
             products(keys, t0, x);
-            // scores
+            // scores less the maximum
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     const f32x4_t f = *reinterpret_cast<const f32x4_t*>(factors + 32 * (t0 + t) + 8 * b + 4 * g);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x[t][4 * b + j] *= f[j];
+                    for (int j = 0; j < 4; ++j) x[t][4 * b + j] = __builtin_fmaf(x[t][4 * b + j], f[j], -m);
                 }
             if (masked) {
                 int left = limit - 32 * t0 - 4 * g;
@@ -479,7 +479,12 @@ struct Rows {
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) top = fmaxf(top, x[t][j]);
-            if (__ballot(top > above)) raise(top);
+            if (__ballot(top > above - m)) {
+                const float was = m;
+                raise(top + m);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) x[t] += was - m;
+            }
             u32x4_t p[2 * NT];
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -489,7 +494,7 @@ struct Rows {
                     f32x4_t y;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        y[j] = exp2_(x[t][4 * b + j] - m);
+                        y[j] = exp2_(x[t][4 * b + j]);
                         l += y[j];
                         y[j] *= f[j];
                     }
