@@ -728,6 +728,8 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(PrefillArgs a) {
     }
 }
 
+__device__ __forceinline__ float odd_or_zero(float x) { return fabsf(x) < INFINITY ? 0.0f : x; }
+
 // Joins the parts of split blocks in order of position: kJoinRows rows of a
 // block a workgroup, four channels a thread at a time.
 __device__ void join_rows(const PrefillArgs& a, const Found& u) {
@@ -738,7 +740,7 @@ __device__ void join_rows(const PrefillArgs& a, const Found& u) {
         const int row = from + n / (Dp / 4), ch = 4 * (n % (Dp / 4)), r = block * a.block_rows + row;
         if (r >= R) return;
         const int64_t at = part * a.part_rows + row, step = a.part_rows;
-        // eight parts on their way at a time; past the last one, that again with no weight
+        // eight parts on their way at a time; past the last one, that again, which does not count
         constexpr int kBatch = 8;
         float top = -INFINITY, weight = 0.0f;
         f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
@@ -755,24 +757,30 @@ __device__ void join_rows(const PrefillArgs& a, const Found& u) {
             float most = top;
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) most = fmaxf(most, m[k]);
-            if (most == -INFINITY) continue;
-            const float f = exp2_(top - most);
-            weight *= f;
-            sum *= f;
-            top = most;
+            if (most != -INFINITY) {
+                const float f = exp2_(top - most);
+                weight *= f;
+                sum *= f;
+                top = most;
+            }
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) {
-                const float y = exp2_(m[k] - most);
-                if (y != 0.0f) {  // (a part without weight may hold anything)
+                if (s0 + k >= u.splits) break;
+                const float y = m[k] == -INFINITY ? 0.0f : exp2_(m[k] - most);
+                if (y != 0.0f) {
                     weight += l[k] * y;
                     sum += o[k] * y;
+                } else {  // infinities and NaN have no weight that makes them nothing
+                    weight += odd_or_zero(l[k]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sum[j] += odd_or_zero(o[k][j]);
                 }
             }
         }
         uint16_t* out = a.out + (static_cast<int64_t>(u.q.lo + r / G) * a.heads + h * G + r % G) * D;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (ch + j < D) out[ch + j] = f32_to_bf16(weight == 0.0f ? 0.0f : sum[j] / weight);
+            if (ch + j < D) out[ch + j] = f32_to_bf16(weight == 0.0f ? odd_or_zero(sum[j]) : sum[j] / weight);
     }
 }
 __global__ __launch_bounds__(256) void prefill_join_kernel(PrefillArgs a) {

@@ -255,6 +255,84 @@ def test_many_sequences(oracle, ops):
     check(f32(ops, c.run(ops)), *c.want())
 
 
+# without a cache, where the rows are many: the larger row blocks, at every number of 32 channels
+# that has them (the call has the room; most rows are of no sequence)
+ROOMY = [
+    (32, 8, 128, [300], 4000), (32, 2, 100, [700, 3], 8000), (32, 32, 112, [130], 4000), (32, 4, 97, [65, 0, 70], 13000),
+    (16, 4, 256, [150, 600], 4000), (16, 16, 160, [70], 4096), (64, 1, 192, [40], 1100), (16, 2, 224, [129], 4096),
+    (32, 4, 255, [33, 90], 2100),
+]
+
+
+@pytest.mark.parametrize("Hq,H,dim,new,pad", ROOMY)
+def test_few_rows_in_a_large_call(oracle, ops, Hq, H, dim, new, pad):
+    c = Case(oracle, None, Hq, H, dim, [0] * len(new), new, seed=dim, pad=pad)
+    n = sum(new)
+    want, bound = c.want()
+    for workspace in (True, False):
+        got = f32(ops, c.run(ops, workspace=workspace))
+        check(got, want, bound, slice(0, n))
+        assert not got[n:].any()
+
+
+@pytest.mark.parametrize("dim,shift", [(128, 8), (128, 1), (104, 4), (99, 3)])
+def test_slices_of_one_projection_in_a_large_call(oracle, ops, dim, shift):
+    c = Case(oracle, None, 32, 8, dim, [0], [200], seed=dim, pad=3900)
+    assert np.array_equal(ops.host(c.run(ops, wide=True, shift=shift)), ops.host(c.run(ops)))
+
+
+@pytest.mark.parametrize("dim", [128, 99])
+@pytest.mark.parametrize("value", ODD)
+def test_odd_values_in_a_large_call(oracle, ops, dim, value):
+    c = Case(oracle, None, 32, 8, dim, [0], [200], seed=dim, pad=3900)
+    clean = ops.host(c.run(ops))
+    c.v[150, 1, 9] = value
+    c.k[200:], c.v[200:], c.q[200:] = 0x7fc0, 0x7fc0, 0x7fc0
+    got = ops.host(c.run(ops))
+    other = np.ones(got.shape, bool)
+    other[150:200, 4:8, 9] = False
+    assert np.array_equal(got[other], clean[other])
+    assert (got.view(np.uint16)[150:200, 4:8, 9] & 0x7fff >= 0x7f80).all()
+
+
+def test_a_prompt_of_four_thousand(oracle, ops):
+    """Two of the kv heads against 64 bits."""
+    from tests._prefill import attention
+    c = Case(oracle, None, 32, 8, 128, [0], [4133], seed=30)
+    got, f = f32(ops, c.run(ops)), D.bf16_bits_to_f32
+    for h in (0, 5):
+        q, k, v = f(c.q[:, 4 * h:4 * h + 2]), f(c.k[:, h:h + 1]), f(c.v[:, h:h + 1])
+        check(got[:, 4 * h:4 * h + 2], *attention(None, q, c.offs, c.lengths, None, k, v, c.scale))
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+def test_many_sequences_of_which_some_are_split(oracle, ops, fmt):
+    g = np.random.default_rng(31)
+    new = [int(x) for x in g.integers(0, 3, 140)]
+    lengths = [int(x) for x in g.integers(0, 150, 140)]
+    for s, n, t in ((3, 3000, 2), (70, 1, 40), (71, 2000, 1), (139, 2500, 9)):
+        lengths[s], new[s] = n, t
+    c = Case(oracle, fmt, 4, 2, 64, lengths, new, seed=31)
+    want, bound = c.want()
+    check(f32(ops, c.run(ops)), want, bound)
+    check(f32(ops, c.run(ops, workspace=False)), want, bound)
+
+
+@pytest.mark.parametrize("value", ODD)
+@pytest.mark.parametrize("gain", [1.0, 1e4])
+def test_odd_values_in_a_split_part_reach_who_sees_them(oracle, ops, gain, value):
+    """Whatever its part weighs beside the others (with large queries: nothing)."""
+    c = Case(oracle, "int8", 4, 2, 64, [3000], [20], seed=32, gain=gain)
+    clean = ops.host(c.run(ops))
+    c.v[7, 1, 9] = value
+    got = ops.host(c.run(ops))
+    other = np.ones(got.shape, bool)
+    other[7:, 2:, 9] = False
+    assert np.array_equal(got[other], clean[other])
+    hit = D.bf16_bits_to_f32(got.view(np.uint16))[7:, 2:, 9]
+    assert np.isnan(hit).all() if value == 0x7fc0 else (hit == (np.inf if value == 0x7f80 else -np.inf)).all()
+
+
 @pytest.mark.parametrize("fmt", [None, "fp8"])
 def test_captured_and_replayed(oracle, ops, fmt):
     """Graphs with workspaces of their own, on another stream, replayed with other
