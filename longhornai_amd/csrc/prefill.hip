@@ -34,7 +34,7 @@ typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 constexpr float kLag = 6.0f;
 constexpr int kMostSplits = 64;  // of a block's keys
 constexpr int kLeastTiles = 8;   // of a split: the launch that joins takes as long as some tiles
-constexpr int kJoinRows = 8;     // of a workgroup that joins splits
+constexpr int kJoinRows = 8;     // of a workgroup that joins splits: half a wave a row
 
 struct PrefillArgs {
     const uint16_t* q;
@@ -104,16 +104,15 @@ __device__ __forceinline__ int split_target(const PrefillArgs& a, const Seq& fir
     const uint32_t units = over_all([once](const Seq& q) { return static_cast<uint32_t>(q.blocks) * split_count(q, once); });
     return units <= static_cast<uint32_t>(a.slots) ? once : target(2 * a.slots);
 }
+// (`first` is the lane's of the first 64 sequences, `target` split_target's.)
 // The unit with number `unit` in the list that has count(sequence, splits) units
 // of each sequence in turn: the sequence, the unit's number within it, and the
 // parts (split blocks times their splits) of the sequences before it.  Past the
 // end of the list seq is n_seqs and nth counts from there.
 struct Found { int seq, nth, splits, parts; Seq q; };
 template <typename Count>
-__device__ __forceinline__ Found find_unit(const PrefillArgs& a, uint32_t unit, Count count) {
+__device__ __forceinline__ Found find_unit(const PrefillArgs& a, const Seq& first, int target, uint32_t unit, Count count) {
     const int lane = threadIdx.x & 63;
-    const Seq first = seq_of(a, lane);
-    const int target = split_target(a, first);
     uint32_t parts = 0;
     for (int base = 0; base < a.n_seqs; base += 64) {
         const Seq q = base == 0 ? first : seq_of(a, base + lane);
@@ -548,7 +547,8 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(PrefillArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t prefill_lds[];
     constexpr int kTile = KS * 4096, kRows = 32 * W;
     const uint32_t unit = blockIdx.y + blockIdx.z * gridDim.y;
-    const Found u = find_unit(a, unit, [](const Seq& q, int splits) { return static_cast<uint32_t>(q.blocks) * splits; });
+    const Seq first_seq = seq_of(a, threadIdx.x & 63);
+    const Found u = find_unit(a, first_seq, split_target(a, first_seq), unit, [](const Seq& q, int splits) { return static_cast<uint32_t>(q.blocks) * splits; });
     if (u.seq >= a.n_seqs) {
         if (a.clear_rest) clear_rest(a, u.nth, static_cast<int>(gridDim.y * gridDim.z - unit) + u.nth);
         return;
@@ -732,64 +732,87 @@ __device__ __forceinline__ float odd_or_zero(float x) { return fabsf(x) < INFINI
 
 // Joins the parts of split blocks in order of position: kJoinRows rows of a
 // block a workgroup, four channels a thread at a time.
+struct Joined {
+    float top = -INFINITY, weight = 0.0f;
+    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+
+    // The next N parts, on their way together: those of maxima and sums at ml, of products at o.
+    template <int N>
+    __device__ __forceinline__ void add(const float*& ml, int64_t ml_step, const float*& o, int64_t o_step) {
+        float m[N], l[N];
+        f32x4_t y[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            m[k] = ml[0];
+            l[k] = ml[1];
+            y[k] = *reinterpret_cast<const f32x4_t*>(o);
+            ml += ml_step;
+            o += o_step;
+        }
+        float most = top;
+#pragma unroll
+        for (int k = 0; k < N; ++k) most = fmaxf(most, m[k]);
+        if (most != -INFINITY) {
+            const float f = exp2_(top - most);
+            weight *= f;
+            sum *= f;
+            top = most;
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const float f = m[k] == -INFINITY ? 0.0f : exp2_(m[k] - most);
+            if (f != 0.0f) {
+                weight += l[k] * f;
+                sum += y[k] * f;
+            } else {  // infinities and NaN have no weight that makes them nothing
+                weight += odd_or_zero(l[k]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[j] += odd_or_zero(y[k][j]);
+            }
+        }
+    }
+};
 __device__ void join_rows(const PrefillArgs& a, const Found& u) {
     const int h = blockIdx.x, G = a.group, D = a.c.D, Dp = a.c.Dp(), R = u.q.T * G;
     const int chunks = a.block_rows / kJoinRows, block = u.nth / chunks, from = u.nth % chunks * kJoinRows;
     const int64_t part = static_cast<int64_t>(h) * 4 * a.slots + u.parts + block * u.splits;
-    for (int n = threadIdx.x; n < kJoinRows * (Dp / 4); n += 256) {
-        const int row = from + n / (Dp / 4), ch = 4 * (n % (Dp / 4)), r = block * a.block_rows + row;
-        if (r >= R) return;
-        const int64_t at = part * a.part_rows + row, step = a.part_rows;
-        // eight parts on their way at a time; past the last one, that again, which does not count
-        constexpr int kBatch = 8;
-        float top = -INFINITY, weight = 0.0f;
-        f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-        for (int s0 = 0; s0 < u.splits; s0 += kBatch) {
-            float m[kBatch], l[kBatch];
-            f32x4_t o[kBatch];
+    const int64_t ml_step = 2 * a.part_rows, o_step = static_cast<int64_t>(a.part_rows) * Dp;
+    // thread n: the channels 4 n on of the rows, Dp a row
+    const int row = from + static_cast<int>(threadIdx.x) / 32, r = block * a.block_rows + row;
+    if (r >= R) return;
+    const float* const ml0 = a.ws_ml + part * ml_step + 2 * row;
+    const float* const o0 = a.ws_o + part * o_step + static_cast<int64_t>(row) * Dp;
+    uint16_t* out = a.out + (static_cast<int64_t>(u.q.lo + r / G) * a.heads + h * G + r % G) * D;
+    for (int ch = 4 * (threadIdx.x % 32); ch < D; ch += 128) {
+        const float *ml = ml0, *o = o0 + ch;
+        Joined z;
+        int left = u.splits;
+        for (; left >= 8; left -= 8) z.add<8>(ml, ml_step, o, o_step);
+        if (left & 4) z.add<4>(ml, ml_step, o, o_step);
+        if (left & 2) z.add<2>(ml, ml_step, o, o_step);
+        if (left & 1) z.add<1>(ml, ml_step, o, o_step);
+        const float by = 1.0f / z.weight;
+        float y[4];
 #pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-                const int64_t p = at + min(s0 + k, u.splits - 1) * step;
-                m[k] = s0 + k < u.splits ? a.ws_ml[2 * p] : -INFINITY;
-                l[k] = a.ws_ml[2 * p + 1];
-                o[k] = *reinterpret_cast<const f32x4_t*>(a.ws_o + p * Dp + ch);
-            }
-            float most = top;
+        for (int j = 0; j < 4; ++j) y[j] = z.weight == 0.0f ? odd_or_zero(z.sum[j]) : z.sum[j] * by;
+        if (a.vec_out) {
+            *reinterpret_cast<u32x2_t*>(out + ch) = u32x2_t{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+        } else {
 #pragma unroll
-            for (int k = 0; k < kBatch; ++k) most = fmaxf(most, m[k]);
-            if (most != -INFINITY) {
-                const float f = exp2_(top - most);
-                weight *= f;
-                sum *= f;
-                top = most;
-            }
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-                if (s0 + k >= u.splits) break;
-                const float y = m[k] == -INFINITY ? 0.0f : exp2_(m[k] - most);
-                if (y != 0.0f) {
-                    weight += l[k] * y;
-                    sum += o[k] * y;
-                } else {  // infinities and NaN have no weight that makes them nothing
-                    weight += odd_or_zero(l[k]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) sum[j] += odd_or_zero(o[k][j]);
-                }
-            }
+            for (int j = 0; j < 4; ++j)
+                if (ch + j < D) out[ch + j] = f32_to_bf16(y[j]);
         }
-        uint16_t* out = a.out + (static_cast<int64_t>(u.q.lo + r / G) * a.heads + h * G + r % G) * D;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (ch + j < D) out[ch + j] = f32_to_bf16(weight == 0.0f ? odd_or_zero(sum[j]) : sum[j] / weight);
     }
 }
 __global__ __launch_bounds__(256) void prefill_join_kernel(PrefillArgs a) {
     const int chunks = a.block_rows / kJoinRows;
+    const Seq first = seq_of(a, threadIdx.x & 63);
+    const int target = split_target(a, first);
     // (how many there are is known here alone; the grid is as many as run at once)
-    for (uint32_t unit = blockIdx.y;; unit += gridDim.y) {
-        const Found u = find_unit(a, unit, [&](const Seq& q, int splits) { return splits > 1 ? static_cast<uint32_t>(q.blocks) * chunks : 0u; });
+    for (uint32_t unit = blockIdx.y;;) {
+        Found u = find_unit(a, first, target, unit, [&](const Seq& q, int splits) { return splits > 1 ? static_cast<uint32_t>(q.blocks) * chunks : 0u; });
         if (u.seq >= a.n_seqs) return;
-        join_rows(a, u);
+        for (; u.nth < u.q.blocks * chunks; u.nth += gridDim.y, unit += gridDim.y) join_rows(a, u);
     }
 }
 
