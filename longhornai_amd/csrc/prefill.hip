@@ -4,18 +4,29 @@
 //   s_j = scale * q . k_j           over the sequence's cached tokens and its new
 //   o   = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m)     ones up to the token itself
 //
-// One pass with a running maximum and sum.  A workgroup has 256 (new token, query
-// head) rows of one kv head, eight waves of 32 rows each, and walks the keys 64 at
-// a time: pages of the cache, then tiles of the new tokens.  A tile comes to LDS
-// once for all waves, in bf16 (codes are exact there), while they work on the one
-// before it.  Both products are 32x32x16 MFMAs on transposed tiles: S^T = K Q^T
-// leaves a lane with 4 adjacent keys of one row, four times over, which is what it
-// needs as the B operand of O^T = V^T P^T when V^T's keys come in that order; a
-// row's maximum and sum are one register each.
+// One pass with a running maximum and sum.  A workgroup has 128 or 256 (new token,
+// query head) rows of one kv head (block_rows says which), four or eight waves of 32
+// rows each, and walks the keys 64 at a time: pages of the cache, then tiles of the
+// new tokens.  A tile comes to LDS once for all waves, in bf16 (codes are exact
+// there), while they work on the one before it.  Both products are 32x32x16 MFMAs on
+// transposed tiles: S^T = K Q^T leaves a lane with 4 adjacent keys of one row, four
+// times over, which is what it needs as the B operand of O^T = V^T P^T when V^T's
+// keys come in that order; a row's maximum and sum are one register each.
 // Precision: scores, weights' sums and results are fp32; a weight (of a cached
 // token, times its value scale) is rounded once to bf16, which has the range of
 // both and needs no exponent of its own, at 2^-8 of itself; the result is rounded
 // to bf16.
+//
+// Bound: a tile for 256 rows of 128 channels is 2048 clocks of a SIMD's matrix work,
+// about 1900 of its vector work (exponentials half of it) and 256 KB of LDS reads,
+// 2048 clocks at the 128 bytes a clock that LDS gives at most; two waves a SIMD
+// overlap them to 3600.  Measured, 32 heads over 8 of 128: 16384 tokens 1.98 to 2.1
+// ms (1050 to 1110 TFLOPS, where a bf16 product of 8192^3 reaches 1190 to 1250), 16
+// prompts of up to 2048 208 us (760), 4 of up to 200 12.5 us.
+// Pages cost the conversion of their codes beside it: 512 tokens of 64 heads over
+// 32768 of e4m3 613 us (900 TFLOPS).  Of 64 rows a wave, which halves the LDS reads
+// but leaves one wave a SIMD: 2290 us where this takes 1985, also with the products
+// of the next tile interleaved with the weights of this one.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -731,7 +742,9 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(PrefillArgs a) {
 __device__ __forceinline__ float odd_or_zero(float x) { return fabsf(x) < INFINITY ? 0.0f : x; }
 
 // Joins the parts of split blocks in order of position: kJoinRows rows of a
-// block a workgroup, four channels a thread at a time.
+// block a workgroup, four channels a thread at a time.  Bound by latency (finding
+// the block, then the parts' loads), 5 us, and where there are many rows by memory: 14
+// us for 32768 rows of 128 channels in two parts, 34 MB written and read again.
 struct Joined {
     float top = -INFINITY, weight = 0.0f;
     f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
@@ -805,14 +818,14 @@ __device__ void join_rows(const PrefillArgs& a, const Found& u) {
     }
 }
 __global__ __launch_bounds__(256) void prefill_join_kernel(PrefillArgs a) {
-    const int chunks = a.block_rows / kJoinRows;
+    auto chunks = [&](const Seq& q) { return static_cast<uint32_t>(q.T * a.group + kJoinRows - 1) / kJoinRows; };
     const Seq first = seq_of(a, threadIdx.x & 63);
     const int target = split_target(a, first);
     // (how many there are is known here alone; the grid is as many as run at once)
     for (uint32_t unit = blockIdx.y;;) {
-        Found u = find_unit(a, first, target, unit, [&](const Seq& q, int splits) { return splits > 1 ? static_cast<uint32_t>(q.blocks) * chunks : 0u; });
+        Found u = find_unit(a, first, target, unit, [&](const Seq& q, int splits) { return splits > 1 ? chunks(q) : 0u; });
         if (u.seq >= a.n_seqs) return;
-        for (; u.nth < u.q.blocks * chunks; u.nth += gridDim.y, unit += gridDim.y) join_rows(a, u);
+        for (const int end = static_cast<int>(chunks(u.q)); u.nth < end; u.nth += gridDim.y, unit += gridDim.y) join_rows(a, u);
     }
 }
 
@@ -826,8 +839,6 @@ int compute_units() {
     }
     return n;
 }
-// Workgroups of a kv head that are on the chip at once: one a CU.  None where the
-// rows fill it four times over, or where splits would have too few tiles each.
 // Rows of a workgroup.  256, eight waves, bring a tile to LDS half as often; 128 make
 // two workgroups of a CU, which wait for different things, where LDS and registers
 // hold two (without a cache, up to 128 channels), and leave less over at the end.
@@ -841,6 +852,11 @@ int block_rows(int mode, int D, int n_seqs, int capacity, int heads) {
     if (D > 128) return blocks >= cus ? 256 : 128;
     return D > 96 && blocks >= 2 * cus && capacity / std::max(n_seqs, 1) >= 4096 ? 256 : 128;
 }
+// Workgroups of a kv head that are on the chip at once: one a CU.  None (no splits)
+// where the rows fill it four times over, or where splits would have too few tiles
+// each.  Measured with splits / without: 128 tokens over 16384, 32 heads over 8, 67 /
+// 579 us; 512 tokens of 64 heads over 32768 613 / 1141; 24 sequences, most of which
+// decode, over up to 4096 172 / 203.
 int want_slots(int block_rows, int capacity, int heads, int kv_heads, int64_t most_tiles) {
     const int cus = compute_units();
     const int64_t rows = static_cast<int64_t>(capacity) * (heads / kv_heads);
