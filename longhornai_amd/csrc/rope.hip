@@ -59,8 +59,8 @@ __device__ __forceinline__ void turn(uint64_t angle, float& c, float& s) {
 
 // A wave a (row, head): lane l has pairs l, l + 64 of the channels; those past
 // rot_dim go in twos that are not turned.  For the heads that rope_vec_kernel does not
-// take, of sizes that are no whole vectors: 32768 rows of 32 and 8 heads of 100, 326 us,
-// 1.6 TB/s, bound by its instructions, an element a lane at a time.
+// take: of an odd size (75 channels: 322 us for 32768 rows of 32 and 8 heads, 1.2
+// TB/s), or of more than 128 channels whose pairs are cut into no vectors.
 template <typename T, bool INTERLEAVED>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs<T> a) {
     const int lane = threadIdx.x & 63, pairs = a.rot / 2, units = (a.D + 1) / 2;
@@ -129,53 +129,59 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs<T> a) {
     }
 }
 
-// Sum over 1 << LB adjacent lanes (4 to 32), the same in all of them.
+// Sum over 1 << LB adjacent lanes (4 to 64), the same in all of them.
 template <int LB, typename S>
 __device__ __forceinline__ S lanes_sum(S x) {
 #pragma unroll
     for (int d = 1; d < 1 << LB; d <<= 1) x += __shfl_xor(x, d, 64);
     return x;
 }
-// A vector is 16 bytes, at any alignment.
-template <typename T>
-constexpr int vector_of() { return 16 / sizeof(T); }
-template <typename T>
-__device__ __forceinline__ u32x4_t load_vector(const T* from) {
-    u32x4_t w;
-    __builtin_memcpy(&w, from, 16);
-    return w;
-}
-template <typename T>
-__device__ __forceinline__ void store_vector(T* to, u32x4_t w) { __builtin_memcpy(to, &w, 16); }
-__device__ __forceinline__ void unpack(u32x4_t w, float (&x)[8]) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        x[2 * j] = __uint_as_float(w[j] << 16);
-        x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-    }
-}
-__device__ __forceinline__ void unpack(u32x4_t w, float (&x)[4]) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(w[j]);
-}
-__device__ __forceinline__ u32x4_t pack(const float (&x)[8]) {
-    return u32x4_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
-}
-__device__ __forceinline__ u32x4_t pack(const float (&x)[4]) {
-    return u32x4_t{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
-}
+// V channels, up to 16 bytes, at any alignment.
+template <typename T, int V>
+struct Vector {
+    static constexpr int kWords = (V * sizeof(T) + 3) / 4;
+    uint32_t w[kWords];
 
-// Rows whose heads are whole vectors: a lane has two vectors of a head, of which each
-// pair has its channels in the lane, 1 << LB lanes a head, kHeads heads of a row beside
-// one another.  The workgroup makes its rows' cosines and sines once, one or two a
-// thread, through LDS, and a lane keeps its own for all the heads it goes through, of
-// which kBatch are on their way at a time.
+    __device__ __forceinline__ void load(const T* from) {
+        w[0] = 0;  // (of one bf16 the upper half)
+        __builtin_memcpy(w, from, V * sizeof(T));
+    }
+    __device__ __forceinline__ void store(T* to) const { __builtin_memcpy(to, w, V * sizeof(T)); }
+    __device__ __forceinline__ void unpack(float (&x)[V]) const {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if constexpr (sizeof(T) == 4) x[j] = __uint_as_float(w[j]);
+            else x[j] = __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+        }
+    }
+    __device__ __forceinline__ void pack(const float (&x)[V]) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) w[j] = __float_as_uint(x[j]);
+        } else if constexpr (V == 1) {
+            w[0] = f32_to_bf16(x[0]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) w[j] = pack_bf16x2(x[2 * j], x[2 * j + 1]);
+        }
+    }
+};
+
+// Rows whose heads are whole vectors of V channels: a lane has two vectors of a head,
+// of which each pair has its channels in the lane, 1 << LB lanes a head, kHeads heads of
+// a row beside one another.  The workgroup makes its rows' cosines and sines once, one
+// or two a thread, through LDS, and a lane keeps its own for all the heads it goes
+// through, of which kBatch are on their way at a time.
 // Bound by memory: 32768 rows of 32 and 8 heads of 128 in bf16, 671 MB in and out, 123
-// us, 5.4 TB/s (a copy of 1 GiB: 5.1; rope_kernel 447).  A few rows: 4.2 us of launch and loads one after the other.
-constexpr int kHeads = 8, kBatch = 4;
-template <typename T, bool INTERLEAVED, int LB>
+// us, 5.4 TB/s (a copy of 1 GiB: 5.1; rope_kernel 447).  A few rows: 4.2 us of launch
+// and loads one after the other.
+template <int LB>
+constexpr int heads_of() { return std::min(8, kRopeThreads >> LB); }
+template <typename T, int V>
+constexpr int batch_of() { return V * sizeof(T) >= 8 ? 4 : 8; }
+template <typename T, int V, bool INTERLEAVED, int LB>
 __global__ __launch_bounds__(kRopeThreads) void rope_vec_kernel(RopeArgs<T> a) {
-    constexpr int V = vector_of<T>(), kRows = (kRopeThreads >> LB) / kHeads, kPairs = V << LB;
+    constexpr int kHeads = heads_of<LB>(), kBatch = batch_of<T, V>(), kRows = (kRopeThreads >> LB) / kHeads, kPairs = V << LB;
     __shared__ __attribute__((aligned(16))) float cosines[kRows][kPairs], sines[kRows][kPairs];
     const int pairs = a.rot / 2, first_row = blockIdx.x * kRows;
     for (int n = threadIdx.x; n < kRows * kPairs; n += kRopeThreads) {
@@ -206,7 +212,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_vec_kernel(RopeArgs<T> a) {
     int side = -1;
     bool norm = false;
     for (int h0 = blockIdx.y * kBatch * kHeads + group % kHeads; h0 < heads; h0 += gridDim.y * kBatch * kHeads) {
-        u32x4_t x0[kBatch], x1[kBatch];
+        Vector<T, V> x0[kBatch], x1[kBatch];
         T* to[kBatch];
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
@@ -215,8 +221,8 @@ __global__ __launch_bounds__(kRopeThreads) void rope_vec_kernel(RopeArgs<T> a) {
             const T* from = (of ? a.x[1] + row * a.in_stride[1] : a.x[0] + row * a.in_stride[0]) + static_cast<int64_t>(head) * a.D;
             to[k] = (of ? a.y[1] + row * a.out_stride[1] : a.y[0] + row * a.out_stride[0]) + static_cast<int64_t>(head) * a.D;
             if (in) {
-                x0[k] = load_vector(from + at0);
-                x1[k] = load_vector(from + at1);
+                x0[k].load(from + at0);
+                x1[k].load(from + at1);
             }
         }
 #pragma unroll
@@ -228,14 +234,17 @@ __global__ __launch_bounds__(kRopeThreads) void rope_vec_kernel(RopeArgs<T> a) {
                 const T* w = a.weight[of];
                 norm = w != nullptr;
                 if (norm && in) {
-                    unpack(load_vector(w + at0), w0);
-                    unpack(load_vector(w + at1), w1);
+                    Vector<T, V> v;
+                    v.load(w + at0);
+                    v.unpack(w0);
+                    v.load(w + at1);
+                    v.unpack(w1);
                 }
             }
             if (somewhere) {
                 float y0[V], y1[V];
-                unpack(x0[k], y0);
-                unpack(x1[k], y1);
+                x0[k].unpack(y0);
+                x1[k].unpack(y1);
                 if (norm) {
                     float sum = 0.0f;
 #pragma unroll
@@ -265,45 +274,63 @@ __global__ __launch_bounds__(kRopeThreads) void rope_vec_kernel(RopeArgs<T> a) {
                 if (turned) {
 #pragma unroll
                     for (int j = 0; j < V; ++j) {
-                        float& p = INTERLEAVED ? (2 * j < V ? y0[2 * j % V] : y1[2 * j % V]) : y0[j];
-                        float& q = INTERLEAVED ? (2 * j < V ? y0[2 * j % V + 1] : y1[2 * j % V + 1]) : y1[j];
+                        // (adjacent pairs: of the first vector, then of the second; of one channel each, both)
+                        constexpr bool kAdjacent = INTERLEAVED && V > 1;
+                        float& p = kAdjacent ? (2 * j < V ? y0[2 * j % V] : y1[2 * j % V]) : y0[j];
+                        float& q = kAdjacent ? (2 * j < V ? y0[(2 * j + 1) % V] : y1[(2 * j + 1) % V]) : y1[j];
                         const float t = p * c[j] - q * s[j];
                         q = q * c[j] + p * s[j];
                         p = t;
                     }
                 }
-                x0[k] = pack(y0);
-                x1[k] = pack(y1);
+                x0[k].pack(y0);
+                x1[k].pack(y1);
             }
             if (in) {
-                store_vector(to[k] + at0, x0[k]);
-                store_vector(to[k] + at1, x1[k]);
+                x0[k].store(to[k] + at0);
+                x1[k].store(to[k] + at1);
             }
         }
     }
 }
 
-// Whether rope_vec_kernel takes a call: heads of whole vectors, pairs (or channels that
-// are not turned) in the same lane.
-template <typename T>
+// Whether rope_vec_kernel takes a call with vectors of V channels: heads of whole ones on
+// 64 lanes, pairs (or channels that are not turned) in the same lane.
+template <typename T, int V>
 bool whole_vectors(const RopeArgs<T>& a, bool interleaved) {
-    constexpr int V = vector_of<T>();
-    return a.D % (2 * V) == 0 && (interleaved ? a.rot % (2 * V) == 0 : a.rot / 2 % V == 0);
+    return a.D % (2 * V) == 0 && a.D <= 128 * V && (interleaved ? a.rot % (2 * V) == 0 : a.rot / 2 % V == 0);
 }
-template <typename T, bool INTERLEAVED>
+template <typename T, int V, bool INTERLEAVED>
 void launch_vec(const RopeArgs<T>& a, hipStream_t s) {
-    const int units = a.D / (2 * vector_of<T>()), heads = a.heads[0] + a.heads[1];
+    const int units = a.D / (2 * V), heads = a.heads[0] + a.heads[1];
     auto go = [&](auto lb) {
-        constexpr int kRows = (kRopeThreads >> lb()) / kHeads;
+        constexpr int kHeads = heads_of<lb()>(), kBatch = batch_of<T, V>(), kRows = (kRopeThreads >> lb()) / kHeads;
         const unsigned x = static_cast<unsigned>((a.n_rows + kRows - 1) / kRows);
         // a workgroup for each batch of heads while there are too few for the chip
         const unsigned y = std::min((heads + kBatch * kHeads - 1) / (kBatch * kHeads), static_cast<int>(1 + 2048 / x));
-        rope_vec_kernel<T, INTERLEAVED, lb()><<<dim3(x, y), kRopeThreads, 0, s>>>(a);
+        rope_vec_kernel<T, V, INTERLEAVED, lb()><<<dim3(x, y), kRopeThreads, 0, s>>>(a);
     };
-    if (units <= 4) go(std::integral_constant<int, 2>{});
-    else if (units <= 8) go(std::integral_constant<int, 3>{});
-    else if (units <= 16) go(std::integral_constant<int, 4>{});
-    else go(std::integral_constant<int, 5>{});
+    // (as many lanes a head as kKvMaxDim channels can need)
+    if (units <= 4) return go(std::integral_constant<int, 2>{});
+    if (units <= 8) return go(std::integral_constant<int, 3>{});
+    if (units <= 16) return go(std::integral_constant<int, 4>{});
+    if constexpr (kKvMaxDim / (2 * V) > 16)
+        if (units <= 32) return go(std::integral_constant<int, 5>{});
+    if constexpr (kKvMaxDim / (2 * V) > 32) go(std::integral_constant<int, 6>{});
+}
+// The widest vectors that the call's channels can be cut into; whether there are any.
+// Measured, 32768 rows of 32 and 8 heads in bf16, widest vectors / rope_kernel: of 128
+// channels 115 / 447 us (vectors of 8), 124 of 128 turned 154 / 431 (2), 126 of 128 224 /
+// 432 (1), 40 40 / 315 (4), 100 105 / 325 (2); the same of 64 rows.
+template <typename T, int V>
+bool by_vectors(const RopeArgs<T>& a, bool interleaved, hipStream_t s) {
+    if (whole_vectors<T, V>(a, interleaved)) {
+        if (interleaved) launch_vec<T, V, true>(a, s);
+        else launch_vec<T, V, false>(a, s);
+        return true;
+    }
+    if constexpr (V > 1) return by_vectors<T, V / 2>(a, interleaved, s);
+    return false;
 }
 
 template <typename T>
@@ -346,11 +373,7 @@ int rope(const char* fn, const T* q, int64_t q_stride, const T* k, int64_t k_str
     RopeArgs<T> a{{q, k},         {q_stride, k_stride}, {q_out, k_out}, {q_out_stride, k_out_stride},
                   {q_weight, k_weight}, {n_heads, n_kv_heads}, positions, turns, n_rows, D, rot, eps, gain};
     const hipStream_t s = as_stream(stream);
-    if (whole_vectors(a, interleaved != 0)) {
-        if (interleaved) launch_vec<T, true>(a, s);
-        else launch_vec<T, false>(a, s);
-        return check_launch(fn);
-    }
+    if (by_vectors<T, 16 / sizeof(T)>(a, interleaved != 0, s)) return check_launch(fn);
     const int heads = n_heads + n_kv_heads;
     const dim3 grid(n_rows, std::min((heads + 3) / 4, 65535));
     if (interleaved) rope_kernel<T, true><<<grid, kRopeThreads, 0, s>>>(a);

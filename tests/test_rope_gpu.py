@@ -136,6 +136,38 @@ def test_rows_without_a_position_are_passed_on(oracle, ops):
         assert (np.abs(y - want) <= bound)[some].all()
 
 
+# channels that are cut into vectors of 8, 4, 2 and 1, and into none; more heads than a lane has at a time
+CUTS = [(2, 2), (6, 4), (40, 40), (40, 20), (64, 62), (100, 100), (100, 50), (128, 126), (126, 126), (130, 130),
+        (144, 136), (192, 188), (250, 250), (254, 126), (256, 252), (256, 254), (33, 32)]
+
+
+@pytest.mark.parametrize("dim,rot", CUTS)
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("norm", [False, True])
+def test_channels_of_any_number(oracle, ops, dtype, dim, rot, interleaved, norm):
+    c = Case(oracle, ops, dtype, 19, 41, 27, dim, norm, seed=dim, rot_dim=rot, interleaved=interleaved)
+    c.check(c.run(ops))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("dim,rot", [(40, 40), (128, 126), (100, 100)])
+def test_any_number_in_place_in_odd_slices(oracle, ops, dtype, dim, rot):
+    c = Case(oracle, ops, dtype, 50, 6, 2, dim, True, seed=6, rot_dim=rot)
+    want = c.run(ops)
+    width = 8 * dim + 3
+    buf = ops.dev(np.full(50 * width + 1, 9, c.q.dtype.type if c.bf16 else np.float32))
+    rows = buf[1:].view(50, width)
+    q, k, rest = rows.split([6 * dim, 2 * dim, 3], dim=1)
+    q.copy_(ops.dev(c.q).view(50, -1))
+    k.copy_(ops.dev(c.k).view(50, -1))
+    w = (None if x is None else ops.dev(x) for x in (c.qw, c.kw))
+    got = ops.rope(c.plan, q, k, ops.dev(c.pos), *w, out=(q, k))
+    for g, x in zip(got, want):
+        assert np.array_equal(c.host(ops, g.contiguous()).reshape(x.shape), x)
+    assert (ops.host(rest.contiguous()) == 9).all() and ops.host(buf)[0] == 9
+
+
 @pytest.mark.parametrize("side", ["q", "k"])
 def test_one_side_alone(oracle, ops, side):
     c = Case(oracle, ops, "bf16", 30, 4, 2, 64, False, seed=4)
