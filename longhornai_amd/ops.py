@@ -572,7 +572,7 @@ def rope_plan(head_dim: int, rot_dim: int | None = None, theta: float = 10000.0,
     numbers are).  gain multiplies the turned channels; None: 0.1 ln(factor) + 1
     with "yarn", else 1."""
     rot = head_dim if rot_dim is None else rot_dim
-    if not 0 <= rot <= head_dim:
+    if head_dim < 1 or not 0 <= rot <= head_dim:
         raise ValueError(f"rope_plan: rot_dim {rot} is no part of head_dim {head_dim}")
     f = rope_frequencies(rot, theta, scaling, factor, original, slow, fast)
     turns = np.array([int(x) for x in f / (2 * np.pi) * 2.0 ** 64], np.uint64)
@@ -684,6 +684,8 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torc
     heads, head_dim], int16 bits; rows that offsets give to no sequence are not
     computed: zeros in a result that is made here, else what ``out`` held."""
     fn, D = "attn_prompt", head_dim
+    if D < 1:
+        raise ValueError(f"{fn}: head_dim {D}")
     if offsets.dtype is not torch.int32 or offsets.dim() != 1 or offsets.shape[0] == 0 or not offsets.is_contiguous():
         raise ValueError(f"{fn}: offsets must be contiguous [B + 1] int32, got {tuple(offsets.shape)} {offsets.dtype}")
     n, heads, H, (qs, ks, vs), out, made, nbytes = _prefill_rows(fn, q, k, v, None, D, out, workspace)

@@ -206,3 +206,14 @@ def test_oracle_attention_of_known_weights():
     v[1, 0, 0] = np.inf
     out, _ = _prefill.attention(None, q, [0, 2], None, None, k, v, 1.0)
     assert np.array_equal(out[0], [[4.0, 0.0]]) and out[1, 0, 0] == np.inf and out[1, 0, 1] == 1.5
+
+
+def test_heads_of_no_channels_are_refused():
+    torch = pytest.importorskip("torch")
+    from longhornai_amd import ops
+    x, offs = torch.zeros((3, 8), dtype=torch.int16), torch.zeros(2, dtype=torch.int32)
+    for D in (0, -8):
+        with pytest.raises(ValueError, match="head_dim"):
+            ops.attn_prompt(x, x, x, offs, D)
+        with pytest.raises(ValueError, match="head_dim"):
+            ops.rope_plan(D, rot_dim=0)
