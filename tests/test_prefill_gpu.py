@@ -333,6 +333,22 @@ def test_odd_values_in_a_split_part_reach_who_sees_them(oracle, ops, gain, value
     assert np.isnan(hit).all() if value == 0x7fc0 else (hit == (np.inf if value == 0x7f80 else -np.inf)).all()
 
 
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+def test_sequences_that_share_pages(oracle, ops, fmt):
+    """A common prefix held once: the bits of a sequence that has it for itself."""
+    c = Case(oracle, fmt, 8, 2, 64, [192, 192, 192], [40, 1, 70], seed=33)
+    c.table[1, :2], c.table[2, :2] = c.table[0, :2], c.table[0, :2]
+    c.table[2, 2] = c.table[0, 0]  # and one page twice in a sequence
+    got = ops.host(c.run(ops))
+    check(D.bf16_bits_to_f32(got.view(np.uint16)), *c.want())
+    for name in ("k", "v", "ks", "vs"):  # page 1 of sequence 0 is copied for sequence 1
+        a = getattr(c.c, name)
+        spare = [p for p in range(c.c.pages) if p not in c.table]
+        a[spare[0]] = a[c.table[0, 1]]
+    c.table[1, 1] = spare[0]
+    assert np.array_equal(ops.host(c.run(ops)), got)
+
+
 @pytest.mark.parametrize("fmt", [None, "fp8"])
 def test_captured_and_replayed(oracle, ops, fmt):
     """Graphs with workspaces of their own, on another stream, replayed with other
