@@ -338,6 +338,8 @@ __device__ __forceinline__ bool clear_odd(const PrefillArgs& a, uint8_t* values)
     return __ballot(any) != 0;
 }
 
+__device__ __forceinline__ float odd_or_zero(float x) { return fabsf(x) < INFINITY ? 0.0f : x; }
+
 // ---- a wave's rows ----------------------------------------------------------
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
@@ -671,35 +673,54 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(PrefillArgs a) {
     if (!some) return;
     z.l += other_half(z.l);
     const int g = lane >> 5, mine = 32 * wave + (lane & 31);
-    // Infinite or NaN values that this lane's row sees: add(channel, value) for each (a
-    // sum with them is what they are, whatever the weight).
-    auto each_odd = [&](auto add) {
-        if (*odd == 0) return;
+    // Infinite or NaN values that a row sees: its sum is what they add to, whatever they
+    // weigh.  A tile that some row does not see whole holds none of them any more; in the
+    // others they left the products infinite or NaN (0 times infinity, where the weight or
+    // a move of the maximum is 0).  get(channel) and set(channel, value) are this lane's
+    // row's; all lanes of the wave call this.
+    const bool some_odd = *odd != 0;
+    float all = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) all = __builtin_fmaf(z.o[i][j], 0.0f, all);
+    auto settle_odd = [&](auto get, auto set) {
+        const bool sums = fabsf(z.l) < INFINITY && r0 + mine < R, blank = z.l == 0.0f && all != 0.0f;
+        if (!some_odd && __ballot(sums && all != 0.0f) == 0) return;
+        const int from = (max(first, pages) - pages) * kKvPage, whole = (min(end, max(first, partly)) - pages) * kKvPage;
         const int past = min((end - pages) * kKvPage, token + 1);
-        for (int n = (max(first, partly) - pages) * kKvPage; n < past; ++n) {
-            const uint16_t* row = a.v_new + (u.q.lo + static_cast<int64_t>(n)) * a.v_stride + h * D;
-            for (int ch = 4 * g; ch < D; ch += ch % 4 == 3 ? 5 : 1) {
-                const float y = bf16_to_f32(row[ch]);
-                if (!(fabsf(y) < INFINITY)) add(ch, y);
+        const uint16_t* rows = a.v_new + u.q.lo * a.v_stride + static_cast<int64_t>(h) * D;
+        auto value = [&](int n, int ch) { return odd_or_zero(bf16_to_f32(rows[n * a.v_stride + ch])); };
+        for (int ch = 0; ch < D; ++ch) {
+            const bool own = sums && (ch >> 2 & 1) == g;
+            float sum = 0.0f;
+            if (__ballot(own && (blank || !(fabsf(get(ch)) < INFINITY))) != 0) {  // the wave's rows see all of these alike
+                for (int n = from + lane; n < whole; n += 64) sum += value(n, ch);
+                for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
             }
+            if (some_odd)
+                for (int n = max(from, whole); n < past; ++n) sum += value(n, ch);
+            if (own && sum != 0.0f) set(ch, sum);
         }
     };
     if (u.splits > 1) {
-        if (r0 + mine >= R) return;
+        const bool kept = r0 + mine < R;
         const int64_t part = static_cast<int64_t>(h) * 4 * a.slots + u.parts + block * u.splits + split;
         const int64_t at = part * a.part_rows + mine;
-        if (g == 0) {
+        if (kept && g == 0) {
             a.ws_ml[2 * at] = z.l == 0.0f ? -INFINITY : z.m;
             a.ws_ml[2 * at + 1] = z.l;
         }
         float* to = a.ws_o + at * (32 * KS);
+        if (kept) {
 #pragma unroll
-        for (int i = 0; i < KS; ++i)
+            for (int i = 0; i < KS; ++i)
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
-                *reinterpret_cast<f32x4_t*>(to + 32 * i + 8 * b + 4 * g) =
-                    f32x4_t{z.o[i][4 * b], z.o[i][4 * b + 1], z.o[i][4 * b + 2], z.o[i][4 * b + 3]};
-        each_odd([&](int ch, float y) { to[ch] += y; });
+                for (int b = 0; b < 4; ++b)
+                    *reinterpret_cast<f32x4_t*>(to + 32 * i + 8 * b + 4 * g) =
+                        f32x4_t{z.o[i][4 * b], z.o[i][4 * b + 1], z.o[i][4 * b + 2], z.o[i][4 * b + 3]};
+        }
+        settle_odd([&](int ch) { return to[ch]; }, [&](int ch, float y) { to[ch] = y; });
         return;
     }
     // Results to LDS (the tiles' place is free), from there in rows: the chunk j of row
@@ -717,10 +738,8 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(PrefillArgs a) {
             for (int j = 0; j < 4; ++j) y[j] = z.l == 0.0f ? 0.0f : z.o[i][4 * b + j] * by;
             *reinterpret_cast<u32x2_t*>(chunk_at(lane & 31, 4 * i + b) + 8 * g) = u32x2_t{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
         }
-    each_odd([&](int ch, float y) {
-        uint16_t* to = reinterpret_cast<uint16_t*>(chunk_at(lane & 31, ch >> 3)) + (ch & 7);
-        *to = f32_to_bf16(bf16_to_f32(*to) + y);
-    });
+    auto result = [&](int ch) { return reinterpret_cast<uint16_t*>(chunk_at(lane & 31, ch >> 3)) + (ch & 7); };
+    settle_odd([&](int ch) { return bf16_to_f32(*result(ch)); }, [&](int ch, float y) { *result(ch) = f32_to_bf16(y); });
     const int out_row = token * a.heads + r - token * G;  // of (sequence, kv head)
     uint16_t* out = a.out + (static_cast<int64_t>(u.q.lo) * a.heads + h * G) * D;
     for (int n = lane; n < 32 * kChunks; n += 64) {
@@ -738,8 +757,6 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(PrefillArgs a) {
         }
     }
 }
-
-__device__ __forceinline__ float odd_or_zero(float x) { return fabsf(x) < INFINITY ? 0.0f : x; }
 
 // Joins the parts of split blocks in order of position: kJoinRows rows of a
 // block a workgroup, four channels a thread at a time.  Bound by latency (finding
@@ -767,8 +784,14 @@ struct Joined {
         for (int k = 0; k < N; ++k) most = fmaxf(most, m[k]);
         if (most != -INFINITY) {
             const float f = exp2_(top - most);
-            weight *= f;
-            sum *= f;
+            if (f != 0.0f) {
+                weight *= f;
+                sum *= f;
+            } else {  // infinities and NaN have no weight that makes them nothing
+                weight = odd_or_zero(weight);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[j] = odd_or_zero(sum[j]);
+            }
             top = most;
         }
 #pragma unroll
@@ -777,7 +800,7 @@ struct Joined {
             if (f != 0.0f) {
                 weight += l[k] * f;
                 sum += y[k] * f;
-            } else {  // infinities and NaN have no weight that makes them nothing
+            } else {
                 weight += odd_or_zero(l[k]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) sum[j] += odd_or_zero(y[k][j]);

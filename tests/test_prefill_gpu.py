@@ -423,3 +423,40 @@ def test_empty_calls(ops):
     assert not ops.attn_prompt(q, k, k, offs, 64).any()  # rows of no sequence
     offs = torch.zeros(3, dtype=torch.int32, device="cuda")
     assert not ops.attn_prompt(q, k, k, offs, 64).any()
+
+
+@pytest.mark.parametrize("fmt", [None, "int8"])
+@pytest.mark.parametrize("gain", [1.0, 1e4])
+@pytest.mark.parametrize("value", ODD)
+@pytest.mark.parametrize("token", [5, 700])
+def test_odd_values_far_back_reach_who_sees_them(oracle, ops, fmt, gain, value, token):
+    """In a tile that whole blocks see, in an early part of split ones: whatever the
+    value weighs (with large queries: nothing), split or not."""
+    c = Case(oracle, fmt, 2, 2, 64, [1500 if fmt else 0], [2600], seed=34, gain=gain)
+    for workspace in (True, False):
+        clean = ops.host(c.run(ops, workspace=workspace))
+        was = c.v[token, 1, 9]
+        c.v[token, 1, 9] = value
+        got = ops.host(c.run(ops, workspace=workspace))
+        c.v[token, 1, 9] = was
+        other = np.ones(got.shape, bool)
+        other[token:, 1, 9] = False
+        assert np.array_equal(got[other], clean[other])
+        hit = D.bf16_bits_to_f32(got.view(np.uint16))[token:, 1, 9]
+        assert np.isnan(hit).all() if value == 0x7fc0 else (hit == (np.inf if value == 0x7f80 else -np.inf)).all()
+
+
+@pytest.mark.parametrize("dim,wide", [(64, False), (61, True), (128, True), (256, False)])
+def test_odd_values_of_both_signs(oracle, ops, dim, wide):
+    """Infinity from one token on, NaN from the one on that has the other sign; a value of
+    another channel, another head and another sequence changes its own alone."""
+    c = Case(oracle, None, 2, 1, dim, [0, 0], [40, 900], seed=35, gain=1e3)
+    clean = ops.host(c.run(ops))
+    c.v[40 + 3, 0, 20], c.v[40 + 500, 0, 20], c.v[40 + 260, 0, dim - 1], c.v[7, 0, 2] = 0x7f80, 0xff80, 0x7fc0, 0xff80
+    got = ops.host(c.run(ops, wide=wide, shift=1 if dim % 8 else 8))
+    hit = D.bf16_bits_to_f32(got.view(np.uint16))
+    assert (hit[43:540, :, 20] == np.inf).all() and np.isnan(hit[540:, :, 20]).all()
+    assert np.isnan(hit[300:, :, dim - 1]).all() and (hit[7:40, :, 2] == -np.inf).all()
+    other = np.ones(got.shape, bool)
+    other[43:, :, 20], other[300:, :, dim - 1], other[7:40, :, 2] = False, False, False
+    assert np.array_equal(got[other], clean[other])
