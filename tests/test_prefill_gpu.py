@@ -460,3 +460,27 @@ def test_odd_values_of_both_signs(oracle, ops, dim, wide):
     other = np.ones(got.shape, bool)
     other[43:, :, 20], other[300:, :, dim - 1], other[7:40, :, 2] = False, False, False
     assert np.array_equal(got[other], clean[other])
+
+
+@pytest.mark.parametrize("fmt,Hq,H,lengths,new,least", [("fp8", 4, 2, [4000, 64], [20, 300], 1), (None, 2, 1, [0], [2600], 22)])
+@pytest.mark.parametrize("slots", [0, 1, 2, 3, 7, 20, 30])
+@pytest.mark.parametrize("parts", [-1, 0, 1])
+def test_a_workspace_of_some_parts_is_kept_to(oracle, ops, fmt, Hq, H, lengths, new, least, slots, parts):
+    """Room for some slots, a part more or less: fewer splits, nothing behind the room.
+    least: the slots from which something is split (41 blocks of up to 41 tiles, two parts a slot:
+    41 * 41 / 2 slots tiles a part, rounded up past the next whole number, are under 41 from 22 on)."""
+    import torch
+    c = Case(oracle, fmt, Hq, H, 64, lengths, new, seed=36)
+    part = (256 if fmt else 128) * (64 + 2) * 4  # bytes: a workgroup's rows, of padded channels, a maximum and a sum
+    room = max((slots * 4 * H + parts) * part, 0)
+    usable = room // part // (4 * H)             # whole slots
+    buf = torch.full((room + (1 << 20),), 0xa5, dtype=torch.uint8, device="cuda")
+    q, k, v = c.args(ops)
+    if fmt:
+        got = ops.kv_prefill(c.c.device(ops), q, ops.dev(c.offs), ops.dev(c.lengths), ops.dev(c.table), k, v,
+                             scale=c.scale, workspace=buf[:room])
+    else:
+        got = ops.attn_prompt(q, k, v, ops.dev(c.offs), 64, scale=c.scale, workspace=buf[:room])
+    check(f32(ops, got), *c.want())
+    assert bool((buf[usable * 4 * H * part:] == 0xa5).all())
+    assert bool((buf != 0xa5).any()) == (usable >= least)
