@@ -40,12 +40,13 @@ class Server:
         self.table = torch.full((places, PAGES_A_ROW), -1, dtype=torch.int32, device="cuda")
         self.free = ops.dev(g.permutation(pages).astype(np.int32))
         self.left = ops.dev(np.array([pages, 0], np.int32))
+        self.owned = torch.zeros(places, dtype=torch.int32, device="cuda")
         self.lengths = np.zeros(places, np.int32)  # the host's copy: it decides who gives what
 
     def tables(self, lengths: torch.Tensor, new: list[int]) -> ops.KvPlan:
         """The tables of a step with new[s] tokens of each place's request (-1: it is over)."""
         plan = ops.kv_plan(lengths, ops.dev(np.array(new, np.int32)), self.free, self.left, self.table,
-                           sum(t for t in new if t > 0))
+                           sum(t for t in new if t > 0), owned=self.owned)
         self.left = plan.left
         return plan
 

@@ -487,11 +487,31 @@ int lhq_kv_attn_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k_new,
  * in that order.  left_out [2]: what is left on the stack, and how many pages were
  * wanted and not there.  left_out may be left, for tables that live from step to
  * step.  A page that two sequences share goes back once for each that is over:
- * taking care of that is the caller's. */
+ * taking care of that is the caller's.
+ * What a sequence has here are the pages of its lengths, no others: after the call
+ * its lengths have to grow by all its new tokens (those of a full table or of rows
+ * past row_capacity excepted), else the next call takes other pages for the same
+ * entries and the first are lost; one that is over must have no length, or no
+ * negative new_tokens, in the next call, or its pages go back twice.  Where tokens may be rejected, pages run out,
+ * or a request ends before it has taken its tokens, lhq_kv_plan_owned. */
 int lhq_kv_plan(const int32_t* lengths, const int32_t* new_tokens, const uint64_t* tree,
                 const int32_t* left, int32_t* left_out, int32_t* free_pages, int32_t* block_table,
                 int32_t* offsets, int32_t* positions, int64_t* slots, int n_seqs, int row_capacity,
                 int max_pages, int num_pages, void* stream);
+/* The same, with what a sequence has counted: owned [n_seqs], in and out, is how many
+ * entries of its row, from the first one, hold pages that are its own (clamped to
+ * [0, max_pages]; 0 in a new row).  New tokens fill these first, and only entries past
+ * them get a page off the stack; those that find none become -1 and are not counted.
+ * Of a sequence that is over all of them go back, and owned becomes 0, so that one that
+ * stays over gives nothing back again.  So lengths may grow by fewer tokens than there
+ * were, as with rejected drafts, or not at all: a sequence that found too few pages
+ * comes again with the lengths it had, and keeps what it got.  (Tokens of slot -1
+ * are not in the cache; lengths that count them count what is not there.) */
+int lhq_kv_plan_owned(const int32_t* lengths, const int32_t* new_tokens, const uint64_t* tree,
+                      const int32_t* left, int32_t* left_out, int32_t* free_pages,
+                      int32_t* block_table, int32_t* owned, int32_t* offsets, int32_t* positions,
+                      int64_t* slots, int n_seqs, int row_capacity, int max_pages, int num_pages,
+                      void* stream);
 /* Queries and keys turned by their positions, their heads RMS-normed in the same
  * pass where a weight [head_dim] is given (NULL: not): y = x / sqrt(mean(x^2) +
  * eps) * weight of each head, then each pair (a, b) of its first rot_dim channels

@@ -93,6 +93,7 @@ SIGNATURES = {
     "lhq_kv_attn_workspace_bytes": [_i] * 7,
     "lhq_kv_attn_bf16": [_p, _i64, _p, _i64, _p, _i64] + [_p] * 9 + [_i] * 9 + [_f, _p, _i64, _p],
     "lhq_kv_plan": [_p] * 10 + [_i] * 4 + [_p],
+    "lhq_kv_plan_owned": [_p] * 11 + [_i] * 4 + [_p],
     "lhq_rope_f32": [_p, _i64, _p, _i64] + [_p] * 4 + [_f, _f] + [_p, _i64, _p, _i64] + [_i] * 6 + [_p],
     "lhq_rope_bf16": [_p, _i64, _p, _i64] + [_p] * 4 + [_f, _f] + [_p, _i64, _p, _i64] + [_i] * 6 + [_p],
     "lhq_prefill_workspace_bytes": [_i] * 5,

@@ -1,11 +1,14 @@
 // kvplan.hip -- a serving step's tables from the requests' lengths, for gfx950:
 // pages handed back and out, offsets, positions and cache slots of the new
-// rows (lhq_kv_plan).
+// rows (lhq_kv_plan, lhq_kv_plan_owned).
 //
 // The free pages are a stack.  Pages of sequences that are over are pushed in
 // order of sequence and page, then those of new tokens are popped in that order
 // (all pushes come first, whatever the order of sequences), so every entry's
-// place follows from prefix sums and no atomic decides anything.  The sums run
+// place follows from prefix sums and no atomic decides anything.  Which entries of
+// its row a sequence has pages in follows from its length, or is counted in `owned`:
+// those of rejected tokens, and those granted before the stack ran out, are the
+// sequence's then though its length does not reach them.  The sums run
 // over all sequences, so one workgroup does them; the rows, which only read
 // what it wrote, are done by it too where they are few and by a launch of their
 // own where they are many.  Bound by latency, a chain of loads and scans: 256 decoding
@@ -33,6 +36,7 @@ struct PlanArgs {
     int32_t* offsets;
     int32_t* positions;
     int64_t* slots;
+    int32_t* owned;  // entries of its row that a sequence has, or null: those of its tokens
     int n_seqs, capacity, max_pages, num_pages;
 };
 
@@ -40,6 +44,7 @@ struct PlanArgs {
 __device__ __forceinline__ int held(const PlanArgs& a, int s) {
     return static_cast<int>(min<int64_t>(max(a.lengths[s], 0), static_cast<int64_t>(a.max_pages) * kKvPage));
 }
+__device__ __forceinline__ int owned(const PlanArgs& a, int s) { return min(max(a.owned[s], 0), a.max_pages); }
 __device__ __forceinline__ int pages_of(int64_t tokens) { return static_cast<int>((tokens + kKvPage - 1) / kKvPage); }
 
 // Sums over the threads before this one (below 2^32 in all, else held there);
@@ -107,7 +112,8 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
     // Pages of sequences that are over, 1024 sequences at a time, a wave its own 64.
     for (int base = 0; base < a.n_seqs; base += kPlanThreads) {
         const int s = base + static_cast<int>(threadIdx.x);
-        const int n = base ? new_of(s) : new0, had = n < 0 ? pages_of(base ? length_of(s) : length0) : 0;
+        const int n = base ? new_of(s) : new0;
+        const int had = n >= 0 ? 0 : a.owned ? owned(a, s) : pages_of(base ? length_of(s) : length0);
         if (!__syncthreads_or(had)) continue;
         auto entry = [&](int l, int p, int pages) {
             const int id = p < pages ? a.table[static_cast<int64_t>(base + wave_first + l) * a.max_pages + p] : -1;
@@ -146,8 +152,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
         const uint32_t before = __builtin_elementwise_add_sat(rows, scan_before(want, sums[1], total));
         const int lo = static_cast<int>(min(before, cap)), hi = static_cast<int>(min(__builtin_elementwise_add_sat(before, want), cap));
         rows = __builtin_elementwise_add_sat(rows, total);
-        const int from = pages_of(length);
-        int takes = 0;
+        int from = pages_of(length), takes = 0;
         if (s < a.n_seqs) {
             a.offsets[s + 1] = hi;
             if (s == 0) a.offsets[0] = 0;
@@ -156,10 +161,15 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
                 if (s == 0) offs[0] = 0;
                 lengths[s] = length;
             }
+            if (a.owned) from = max(from, owned(a, s));
             if (hi > lo) takes = max(min(pages_of(static_cast<int64_t>(length) + hi - lo), a.max_pages) - from, 0);
         }
         const uint32_t mine = __builtin_elementwise_add_sat(asked, scan_before(static_cast<uint32_t>(takes), sums[2], total));
         asked = __builtin_elementwise_add_sat(asked, total);
+        if (a.owned && s < a.n_seqs) {
+            if ((base ? new_of(s) : new0) < 0) a.owned[s] = 0;
+            else if (takes > 0 && mine < have) a.owned[s] = from + static_cast<int>(min(static_cast<uint32_t>(takes), have - mine));
+        }
         auto take = [&](int seq, int p, uint32_t nth) {
             a.table[static_cast<int64_t>(seq) * a.max_pages + p] = nth < have ? a.free_pages[have - 1 - nth] : -1;
         };
@@ -192,32 +202,51 @@ __global__ __launch_bounds__(kRowThreads) void kv_plan_rows_kernel(PlanArgs a) {
 
 using namespace lhq;
 
-extern "C" int lhq_kv_plan(const int32_t* lengths, const int32_t* new_tokens, const uint64_t* tree,
-                           const int32_t* left, int32_t* left_out, int32_t* free_pages, int32_t* block_table,
-                           int32_t* offsets, int32_t* positions, int64_t* slots, int n_seqs, int row_capacity,
-                           int max_pages, int num_pages, void* stream) {
-    const char* fn = "kv_plan";
-    LHQ_REQUIRE(n_seqs >= 0 && row_capacity >= 0, "%s: bad counts (%d sequences, %d rows)", fn, n_seqs, row_capacity);
-    LHQ_REQUIRE(max_pages >= 0 && num_pages >= 0, "%s: bad page counts (%d of a sequence, %d in all)", fn, max_pages,
-                num_pages);
-    LHQ_SUPPORTED(static_cast<int64_t>(max_pages) * kKvPage < (int64_t{1} << 31), "%s: sequences of 2^31 tokens", fn);
-    LHQ_SUPPORTED(row_capacity <= INT32_MAX - kPlanRows && n_seqs <= INT32_MAX - kPlanThreads,
-                  "%s: %d rows of %d sequences are over 2^31 - 4097 or 2^31 - 1025", fn, row_capacity, n_seqs);
-    LHQ_REQUIRE(left && left_out && offsets, "%s: null pointer", fn);
-    LHQ_REQUIRE(n_seqs == 0 || (lengths && new_tokens), "%s: null lengths", fn);
-    LHQ_REQUIRE(num_pages == 0 || free_pages, "%s: null list of free pages", fn);
-    LHQ_REQUIRE(n_seqs == 0 || max_pages == 0 || block_table, "%s: null block table", fn);
-    LHQ_REQUIRE(row_capacity == 0 || positions, "%s: null positions", fn);
-    const PlanArgs a{lengths, new_tokens, tree,  left,   left_out,     free_pages, block_table,
-                     offsets, positions,  slots, n_seqs, row_capacity, max_pages,  num_pages};
+namespace {
+
+int plan(const char* fn, const PlanArgs& a, void* stream) {
+    LHQ_REQUIRE(a.n_seqs >= 0 && a.capacity >= 0, "%s: bad counts (%d sequences, %d rows)", fn, a.n_seqs, a.capacity);
+    LHQ_REQUIRE(a.max_pages >= 0 && a.num_pages >= 0, "%s: bad page counts (%d of a sequence, %d in all)", fn, a.max_pages,
+                a.num_pages);
+    LHQ_SUPPORTED(static_cast<int64_t>(a.max_pages) * kKvPage < (int64_t{1} << 31), "%s: sequences of 2^31 tokens", fn);
+    LHQ_SUPPORTED(a.capacity <= INT32_MAX - kPlanRows && a.n_seqs <= INT32_MAX - kPlanThreads,
+                  "%s: %d rows of %d sequences are over 2^31 - 4097 or 2^31 - 1025", fn, a.capacity, a.n_seqs);
+    LHQ_REQUIRE(a.left && a.left_out && a.offsets, "%s: null pointer", fn);
+    LHQ_REQUIRE(a.n_seqs == 0 || (a.lengths && a.new_tokens), "%s: null lengths", fn);
+    LHQ_REQUIRE(a.num_pages == 0 || a.free_pages, "%s: null list of free pages", fn);
+    LHQ_REQUIRE(a.n_seqs == 0 || a.max_pages == 0 || a.table, "%s: null block table", fn);
+    LHQ_REQUIRE(a.capacity == 0 || a.positions, "%s: null positions", fn);
     const hipStream_t s = as_stream(stream);
-    if (n_seqs <= kPlanThreads && row_capacity <= kPlanRows) {
+    if (a.n_seqs <= kPlanThreads && a.capacity <= kPlanRows) {
         kv_plan_kernel<true><<<1, kPlanThreads, 0, s>>>(a);
         return check_launch(fn);
     }
     kv_plan_kernel<false><<<1, kPlanThreads, 0, s>>>(a);
     if (int st = check_launch(fn)) return st;
-    if (row_capacity == 0) return LHQ_OK;
-    kv_plan_rows_kernel<<<(row_capacity + kRowThreads - 1) / kRowThreads, kRowThreads, 0, s>>>(a);
+    if (a.capacity == 0) return LHQ_OK;
+    kv_plan_rows_kernel<<<(a.capacity + kRowThreads - 1) / kRowThreads, kRowThreads, 0, s>>>(a);
     return check_launch(fn);
 }
+
+}  // namespace
+
+extern "C" {
+
+int lhq_kv_plan(const int32_t* lengths, const int32_t* new_tokens, const uint64_t* tree, const int32_t* left,
+                int32_t* left_out, int32_t* free_pages, int32_t* block_table, int32_t* offsets, int32_t* positions,
+                int64_t* slots, int n_seqs, int row_capacity, int max_pages, int num_pages, void* stream) {
+    return plan("kv_plan", {lengths, new_tokens, tree, left, left_out, free_pages, block_table, offsets, positions, slots,
+                            nullptr, n_seqs, row_capacity, max_pages, num_pages}, stream);
+}
+
+int lhq_kv_plan_owned(const int32_t* lengths, const int32_t* new_tokens, const uint64_t* tree, const int32_t* left,
+                      int32_t* left_out, int32_t* free_pages, int32_t* block_table, int32_t* owned, int32_t* offsets,
+                      int32_t* positions, int64_t* slots, int n_seqs, int row_capacity, int max_pages, int num_pages,
+                      void* stream) {
+    const char* fn = "kv_plan_owned";
+    LHQ_REQUIRE(n_seqs <= 0 || owned, "%s: null counts of owned pages", fn);
+    return plan(fn, {lengths, new_tokens, tree, left, left_out, free_pages, block_table, offsets, positions, slots, owned,
+                     n_seqs, row_capacity, max_pages, num_pages}, stream);
+}
+
+}  // extern "C"

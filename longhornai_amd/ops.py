@@ -489,14 +489,19 @@ def _packed(fn: str, name: str, t: torch.Tensor, dtype, shape) -> None:
 
 def kv_plan(lengths: torch.Tensor, new_tokens: torch.Tensor, free_pages: torch.Tensor, left: torch.Tensor,
             block_table: torch.Tensor, n: int, tree: torch.Tensor | None = None,
-            out: KvPlan | None = None) -> KvPlan:
+            out: KvPlan | None = None, owned: torch.Tensor | None = None) -> KvPlan:
     """A step's tables from the requests' lengths (int32 [B]): sequence s holds
     lengths[s] tokens and gets new_tokens[s] more, or is over where that is
     negative.  Pages go back to and come off the stack ``free_pages`` (int32, one
     entry for each page there is), whose first left[0] entries count; block_table
     [B, pages] gets the new ones.  n: rows there are room for.  tree (int64 [n]):
     drafted tokens' ancestors, for their positions.  ``out`` may hold ``left``
-    itself, for tables that live from step to step."""
+    itself, for tables that live from step to step.  owned (int32 [B], zeros at first,
+    kept from step to step): how many entries of its row a sequence has pages in, so that
+    new tokens may be rejected, come again after pages ran out, or never be taken, and a
+    request may stay over.  Without it a sequence has the pages of its lengths alone, which must
+    then grow by all its new tokens, and become 0 once it is over, or pages are lost or
+    go back twice."""
     i32, shape = torch.int32, block_table.shape
     if len(shape) != 2 or n < 0:
         raise ValueError(f"kv_plan: block table {tuple(shape)} is not [B, pages], or {n} rows")
@@ -509,6 +514,8 @@ def kv_plan(lengths: torch.Tensor, new_tokens: torch.Tensor, free_pages: torch.T
         raise ValueError(f"kv_plan: free_pages must be contiguous [pages] int32, got {tuple(free_pages.shape)}")
     if tree is not None:
         _packed("kv_plan", "tree", tree, torch.int64, (n,))
+    if owned is not None:
+        _packed("kv_plan", "owned", owned, i32, (B,))
     if out is None:
         out = KvPlan(lengths.new_empty(B + 1), lengths.new_empty(n), lengths.new_empty(n, dtype=torch.int64),
                      lengths.new_empty(2))
@@ -517,10 +524,11 @@ def kv_plan(lengths: torch.Tensor, new_tokens: torch.Tensor, free_pages: torch.T
         _packed("kv_plan", "out.positions", out.positions, i32, (n,))
         _packed("kv_plan", "out.slots", out.slots, torch.int64, (n,))
         _packed("kv_plan", "out.left", out.left, i32, (2,))
-    _on_one_gpu("kv_plan", lengths, new_tokens, free_pages, left, block_table, tree, out.offsets, out.positions,
-                out.slots, out.left)
-    lib().call("lhq_kv_plan", lengths.data_ptr(), new_tokens.data_ptr(), P(tree), left.data_ptr(), out.left.data_ptr(),
-               free_pages.data_ptr(), block_table.data_ptr(), out.offsets.data_ptr(), out.positions.data_ptr(),
+    _on_one_gpu("kv_plan", lengths, new_tokens, free_pages, left, block_table, tree, owned, out.offsets,
+                out.positions, out.slots, out.left)
+    lib().call("lhq_kv_plan" if owned is None else "lhq_kv_plan_owned", lengths.data_ptr(), new_tokens.data_ptr(), P(tree),
+               left.data_ptr(), out.left.data_ptr(), free_pages.data_ptr(), block_table.data_ptr(),
+               *(() if owned is None else (owned.data_ptr(),)), out.offsets.data_ptr(), out.positions.data_ptr(),
                out.slots.data_ptr(), B, n, width, free_pages.shape[0], stream())
     return out
 

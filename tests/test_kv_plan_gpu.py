@@ -185,3 +185,178 @@ def test_a_captured_loop_keeps_its_tables(ops):
         for a, b in zip((out.offsets, out.positions, out.slots, left, d[3], d[2]), (o, pos, slots, l, table, free)):
             assert np.array_equal(ops.host(a), b)
         torch.zeros(1000, device="cuda").add_(1)
+
+
+class Steps:
+    """Steps on tables that live on, what a sequence has counted in `owned`: each checked against
+    the rule in lists, and that every page is on the stack or in one row, once."""
+
+    def __init__(self, ops, B, width, pages, seed):
+        g = np.random.default_rng(seed)
+        self.ops, self.B, self.W, self.P = ops, B, width, pages
+        self.stack = [int(p) for p in g.permutation(pages)]
+        self.rows = [[] for _ in range(B)]  # the pages that a sequence has
+        self.length = np.zeros(B, np.int64)
+        self.table = ops.dev(np.full((B, width), -1, np.int32))
+        self.free = ops.dev(np.array(self.stack, np.int32))
+        self.left = ops.dev(np.array([pages, 0], np.int32))
+        self.owned = ops.dev(np.zeros(B, np.int32))
+
+    def step(self, new, n=None, tree=None):
+        """Returns the slots."""
+        ops, new = self.ops, np.asarray(new)
+        n = int(new.clip(0).sum()) if n is None else n
+        p = ops.kv_plan(ops.dev(self.length.astype(np.int32)), ops.dev(new.astype(np.int32)), self.free, self.left,
+                        self.table, n, tree=tree, owned=self.owned)
+        self.left = p.left
+        for s in np.nonzero(new < 0)[0]:
+            self.stack += self.rows[s]
+            self.rows[s] = []
+        missing, slots, lo = 0, np.full(n, -1, np.int64), 0
+        for s in range(self.B):
+            hi = min(n, lo + max(int(new[s]), 0))
+            L, row = int(self.length[s]), self.rows[s]
+            for _ in range(len(row), min(self.W, -(-(L + hi - lo) // 64)) if hi > lo else 0):
+                missing += not self.stack
+                if self.stack:
+                    row.append(self.stack.pop())
+            for i in range(lo, hi):
+                at = L + i - lo
+                if at // 64 < len(row):
+                    slots[i] = 64 * row[at // 64] + at % 64
+            lo = hi
+        got, owned, table = ops.host(p.slots), ops.host(self.owned), ops.host(self.table)
+        assert np.array_equal(got, slots)
+        assert ops.host(p.left).tolist() == [len(self.stack), missing]
+        assert owned.tolist() == [len(r) for r in self.rows]
+        assert all(table[s, :len(r)].tolist() == r for s, r in enumerate(self.rows))
+        assert ops.host(self.free)[:len(self.stack)].tolist() == self.stack
+        assert sorted(self.stack + [p for r in self.rows for p in r]) == list(range(self.P))
+        return got
+
+
+def test_rejected_drafts_lose_no_pages(ops):
+    """A prompt of 60, then drafts of 8 across the end of its page of which one is kept."""
+    t = Steps(ops, 1, 8, 10, seed=10)
+    assert (t.step([60]) >= 0).all()
+    t.length[0] = 60
+    for _ in range(4):
+        assert (t.step([8]) >= 0).all()
+        t.length[0] += 1
+    t.step([-1])
+    assert ops.host(t.left).tolist() == [10, 0]
+
+
+def test_a_shortage_can_be_tried_again(ops):
+    t = Steps(ops, 2, 8, 4, seed=11)
+    t.step([100, 0])
+    t.length[0] = 100
+    assert (t.step([1, 300])[1:] >= 0).sum() == 128  # two pages of the five
+    t.step([0, 300])                                 # none yet: it keeps the two
+    t.step([-1, 300])                                # two more
+    t.length[0] = 0
+    assert (t.step([0, 256]) >= 0).all()
+    t.step([0, -1])
+    assert ops.host(t.left).tolist() == [4, 0]
+
+
+def test_a_request_that_ends_before_its_tokens_were_taken(ops):
+    t = Steps(ops, 3, 4, 8, seed=12)
+    t.step([130, 64, 1])
+    t.step([-1, -1, -1])
+    assert ops.host(t.left).tolist() == [8, 0]
+
+
+def test_a_request_that_stays_over_gives_its_pages_back_once(ops):
+    t = Steps(ops, 2, 4, 8, seed=13)
+    t.step([130, 64])
+    t.length[:] = 130, 64
+    for _ in range(3):
+        t.step([-1, 0])
+    t.step([-1, 200])
+    t.length[0] = 0
+    t.step([256, 0])
+    assert ops.host(t.left).tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("B,width,pages,steps", [(1, 3, 3, 40), (5, 6, 20, 60), (40, 8, 150, 40), (70, 5, 400, 30),
+                                                 (1024, 4, 2000, 8), (1100, 6, 4000, 8), (2500, 4, 3000, 6)])
+def test_many_steps_of_drafts_shortages_and_ends(ops, B, width, pages, steps):
+    g = np.random.default_rng(B)
+    t = Steps(ops, B, width, pages, seed=B)
+    for _ in range(steps):
+        new = np.where(g.random(B) < 0.3, g.integers(0, 150, B), g.integers(0, 9, B))
+        new[g.random(B) < 0.15] = -1
+        total = int(new.clip(0).sum())
+        slots = t.step(new, n=total if g.random() < 0.7 else int(total * g.random()))
+        at = 0
+        for s in range(B):
+            k = max(int(new[s]), 0)
+            stored = slots[at:at + k]
+            there = int((stored >= 0).sum())  # the first ones
+            assert (stored[:there] >= 0).all()
+            at += k
+            if new[s] < 0:
+                t.length[s] = t.length[s] if g.random() < 0.5 else 0  # (the next step may still say that it is over)
+                if t.length[s]:
+                    new_over = np.zeros(B, np.int64)
+                    new_over[s] = -1
+                    if g.random() < 0.2:
+                        t.step(new_over)
+                    t.length[s] = 0
+            else:
+                t.length[s] += g.integers(0, there + 1)
+    t.step(np.full(B, -1))
+    assert ops.host(t.left).tolist() == [pages, 0]
+
+
+def test_counts_outside_the_row_are_clamped(ops):
+    t = Steps(ops, 2, 3, 9, seed=14)
+    t.owned.copy_(ops.dev(np.array([-5, -2 ** 31], np.int32)))
+    t.step([70, 1])
+    t.step([-1, -1])
+    import torch
+    table = ops.dev(np.array([[4, -1, 7]], np.int32))
+    free, left, owned = ops.dev(np.zeros(9, np.int32)), ops.dev(np.array([0, 0], np.int32)), ops.dev(np.array([2 ** 31 - 1], np.int32))
+    p = ops.kv_plan(ops.dev(np.zeros(1, np.int32)), ops.dev(np.array([-1], np.int32)), free, left, table, 0, owned=owned)
+    assert ops.host(p.left).tolist() == [2, 0] and ops.host(free)[:2].tolist() == [4, 7] and ops.host(owned).tolist() == [0]
+    assert torch.equal(table.cpu(), torch.tensor([[4, -1, 7]], dtype=torch.int32))
+
+
+def test_drafted_trees_with_owned_pages(ops):
+    """The tree changes positions, not pages."""
+    t = Steps(ops, 1, 4, 6, seed=15)
+    t.step([62], tree=ops.dev((1 << np.arange(1, 63, dtype=np.int64)) - 1))
+    t.length[0] = 62
+    for _ in range(3):
+        slots = t.step([4], tree=ops.dev(np.array([1, 3, 5, 9], np.int64)))
+        assert (slots >= 0).all()
+        t.length[0] += 1
+    t.step([-1])
+    assert ops.host(t.left).tolist() == [6, 0]
+
+
+def test_a_captured_loop_with_a_request_that_is_over(ops):
+    """The host has not looked yet: replays with the same counts give nothing back twice."""
+    import torch
+    lengths, new = ops.dev(np.array([100, 60], np.int32)), ops.dev(np.array([-1, 1], np.int32))
+    table = ops.dev(np.array([[3, 1, -1, -1], [0, -1, -1, -1]], np.int32))
+    free, left = ops.dev(np.array([2, 4, 5, -1, -1, -1], np.int32)), ops.dev(np.array([3, 0], np.int32))
+    owned = ops.dev(np.array([2, 1], np.int32))
+    i32 = dict(dtype=torch.int32, device="cuda")
+    out = ops.KvPlan(torch.empty(3, **i32), torch.empty(1, **i32), torch.empty(1, dtype=torch.int64, device="cuda"), left)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.kv_plan(lengths, new, free, left, table, 1, out=out, owned=owned)
+        lengths[1:].add_(1)
+    for step in range(7):
+        g.replay()
+        torch.cuda.synchronize()
+        L = 60 + step
+        row = [0] if L < 64 else [0, 1]
+        assert ops.host(left).tolist() == [5 if L < 64 else 4, 0]
+        assert ops.host(free)[:5 if L < 64 else 4].tolist() == [2, 4, 5, 3, 1][:5 if L < 64 else 4]
+        assert ops.host(owned).tolist() == [0, len(row)] and ops.host(table)[1, :len(row)].tolist() == row
+        assert ops.host(out.slots).tolist() == [64 * row[L // 64] + L % 64]
+        torch.zeros(1000, device="cuda").add_(1)

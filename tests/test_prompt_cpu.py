@@ -217,3 +217,23 @@ def test_heads_of_no_channels_are_refused():
             ops.attn_prompt(x, x, x, offs, D)
         with pytest.raises(ValueError, match="head_dim"):
             ops.rope_plan(D, rot_dim=0)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(seqs=-1), INV), (dict(cap=-1), INV), (dict(width=-1), INV), (dict(pages=-1), INV), (dict(width=1 << 25), UNS),
+    (dict(cap=2 ** 31 - 1), UNS), (dict(seqs=2 ** 31 - 1), UNS), (dict(lengths=None), INV), (dict(left=None), INV),
+    (dict(table=None), INV), (dict(owned=None), INV)])
+def test_plan_with_owned_pages_refusals(L, kw, code):
+    a = dict(zip(("lengths", "new", "tree", "left", "left_out", "free", "table"), plan_args()[:7])) | dict(owned=FAKE) | \
+        dict(zip(("offsets", "positions", "slots", "seqs", "cap", "width", "pages", "stream"), plan_args()[7:]))
+    a.update(kw)
+    assert L.status("lhq_kv_plan_owned", *a.values()) == code, L.last_error()
+    assert "kv_plan_owned" in L.last_error()
+
+
+def test_plan_helper_refuses_counts_of_another_kind():
+    i32 = dict(dtype=torch.int32)
+    for owned in (torch.zeros(3, **i32), torch.zeros(2, dtype=torch.int64), torch.zeros(4, **i32)[::2], torch.zeros((2, 1), **i32)):
+        with pytest.raises(ValueError, match="owned"):
+            ops.kv_plan(torch.zeros(2, **i32), torch.ones(2, **i32), torch.zeros(5, **i32), torch.zeros(2, **i32),
+                        torch.zeros((2, 3), **i32), 2, owned=owned)
