@@ -543,7 +543,8 @@ int lhq_rope_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_
  * sees nothing gives zeros; rows before the first sequence's and behind the last
  * one's are left as they are, with clear_rest = 1 they become zeros; what a row does
  * not see, whatever it holds, changes nothing of its result, and an infinite or NaN
- * value of a new token that it does see is in it whatever that token weighs.  Offsets,
+ * value of a new token that it does see is in it whatever that token weighs.  out may lie
+ * where q does, rows one after the other, else not overlap q, k_new or v_new.  Offsets,
  * strides, scale, table and cache as for lhq_kv_attn_bf16, which is the faster for
  * a few new tokens a sequence.  out [row_capacity, n_heads, head_dim].  Rounding:
  * queries, keys and codes enter the products as they are; a softmax weight, of a

@@ -929,6 +929,19 @@ int prefill(const char* fn, PrefillArgs a, int mode, int clear_rest, float scale
         if (int st = kv_check_pointers(fn, a.c)) return st;
     LHQ_REQUIRE(a.q && a.offsets && a.out && (mode == 0 || a.lengths), "%s: null pointer", fn);
     if (mode == 0) LHQ_REQUIRE(a.k_new, "%s: null pointer", fn);
+    // Workgroups read keys and values in no order with the writing of results; of the
+    // queries each reads its own before it writes them.
+    const int64_t q_width = static_cast<int64_t>(a.heads) * D, kv_width = static_cast<int64_t>(kv_heads) * D;
+    auto meets = [&a, q_width](const uint16_t* rows, int64_t stride, int64_t width) {
+        const int64_t out = reinterpret_cast<intptr_t>(a.out), x = reinterpret_cast<intptr_t>(rows);
+        const int64_t ahead = out - x - 2 * width;  // the first row that ends behind out's start
+        const int64_t row = ahead < 0 ? 0 : ahead / (2 * stride) + 1;
+        return row < a.capacity && x + 2 * stride * row < out + 2 * q_width * a.capacity;
+    };
+    const bool in_place = a.q == a.out && (a.q_stride == q_width || a.capacity == 1);
+    LHQ_REQUIRE((in_place || !meets(a.q, a.q_stride, q_width)) &&
+                    (!a.k_new || (!meets(a.k_new, a.k_stride, kv_width) && !meets(a.v_new, a.v_stride, kv_width))),
+                "%s: the result overlaps queries, new keys or new values", fn);
     if (a.c.num_pages == 0) a.c.max_pages = 0;
     a.vec_new = D % 8 == 0 && !odd(a.k_new, 16) && !odd(a.v_new, 16) && a.k_stride % 8 == 0 && a.v_stride % 8 == 0 &&
                 a.k_stride < (1 << 24) && a.v_stride < (1 << 24);

@@ -690,7 +690,9 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torc
     [n, kv heads * head_dim] (bf16 as int16 bits, rows may be strided), sequence s
     having rows offsets[s] .. offsets[s + 1] (int32 [B + 1]).  Returns out [n,
     heads, head_dim], int16 bits; rows that offsets give to no sequence are not
-    computed: zeros in a result that is made here, else what ``out`` held."""
+    computed: zeros in a result that is made here, else what ``out`` held.  ``out``
+    may be q itself where its rows lie one after the other, and else overlaps none of
+    q, k and v."""
     fn, D = "attn_prompt", head_dim
     if D < 1:
         raise ValueError(f"{fn}: head_dim {D}")

@@ -484,3 +484,32 @@ def test_a_workspace_of_some_parts_is_kept_to(oracle, ops, fmt, Hq, H, lengths, 
     check(f32(ops, got), *c.want())
     assert bool((buf[usable * 4 * H * part:] == 0xa5).all())
     assert bool((buf != 0xa5).any()) == (usable >= least)
+
+
+@pytest.mark.parametrize("fmt,lengths,new", [(None, [0, 0], [300, 70]), ("int8", [3000, 10], [40, 130])])
+def test_results_in_the_queries_place(oracle, ops, fmt, lengths, new):
+    c = Case(oracle, fmt, 4, 2, 64, lengths, new, seed=37)
+    want = ops.host(c.run(ops))
+    q, k, v = c.args(ops)
+    ws = ops.prefill_workspace(2, len(c.q), 4, 2, 64)
+    if fmt:
+        ops.kv_prefill(c.c.device(ops), q, ops.dev(c.offs), ops.dev(c.lengths), ops.dev(c.table), k, v, scale=c.scale,
+                       workspace=ws, out=q)
+    else:
+        ops.attn_prompt(q, k, v, ops.dev(c.offs), 64, scale=c.scale, workspace=ws, out=q)
+    assert np.array_equal(ops.host(q).reshape(want.shape), want)
+
+
+def test_results_beside_their_rows_of_one_buffer(oracle, ops):
+    """Out in front of and behind the projection's rows, with nothing between."""
+    import torch
+    c = Case(oracle, None, 4, 2, 64, [0], [90], seed=38)
+    want = ops.host(c.run(ops))
+    n, size = len(c.q), len(c.q) * 256
+    buf = torch.zeros(2 * size + n * 512, dtype=torch.int16, device="cuda")
+    rows = buf[size:-size].view(n, 512)
+    rows.copy_(ops.dev(np.concatenate([x.reshape(n, -1) for x in (c.q, c.k, c.v)], axis=1)))
+    q, k, v = rows.split([256, 128, 128], dim=1)
+    for out in (buf[:size], buf[-size:]):
+        ops.attn_prompt(q, k, v, ops.dev(c.offs), 64, scale=c.scale, out=out)
+        assert np.array_equal(ops.host(out).reshape(want.shape), want)

@@ -237,3 +237,21 @@ def test_plan_helper_refuses_counts_of_another_kind():
         with pytest.raises(ValueError, match="owned"):
             ops.kv_plan(torch.zeros(2, **i32), torch.ones(2, **i32), torch.zeros(5, **i32), torch.zeros(2, **i32),
                         torch.zeros((2, 3), **i32), 2, owned=owned)
+
+
+# 5 rows of 32 heads of 128 from `out` on, in bytes
+OUT, OUT_BYTES = 8 << 20, 5 * 4096 * 2
+
+
+@pytest.mark.parametrize("fn,args", [("lhq_attn_prompt_bf16", prompt_args), ("lhq_kv_prefill_bf16", prefill_args)])
+@pytest.mark.parametrize("kw", [
+    dict(k=OUT), dict(v=OUT), dict(k=OUT + OUT_BYTES - 2), dict(v=OUT - 5 * 1024 * 2 + 2), dict(q=OUT - 2), dict(q=OUT + 4096 * 2),
+    dict(q=OUT, qs=4104), dict(q=OUT + OUT_BYTES - 2), dict(q=OUT - OUT_BYTES + 2),
+    dict(k=OUT - 4 * 30000 * 2 - 2046, ks=30000),          # the last row's last element
+    dict(v=OUT - 3 * 30000 * 2 + OUT_BYTES - 2, vs=30000),  # a row in the middle
+])
+def test_results_over_what_others_read_are_refused(L, fn, args, kw):
+    """Workgroups read keys and values in no order with the writing of results."""
+    at = dict(q=16 << 20, k=24 << 20, v=32 << 20, out=OUT) | kw
+    assert L.status(fn, *args(**{n: C.c_void_p(x) if n in ("q", "k", "v", "out") else x for n, x in at.items()})) == INV
+    assert "overlap" in L.last_error()
