@@ -925,9 +925,10 @@ int prefill(const char* fn, PrefillArgs a, int mode, int clear_rest, float scale
     LHQ_REQUIRE(workspace_bytes >= 0, "%s: negative workspace size", fn);
     LHQ_REQUIRE(!odd(workspace, 16), "%s: workspace must be 16-byte aligned", fn);
     if (a.capacity == 0 || (a.n_seqs == 0 && !clear_rest)) return LHQ_OK;
+    if (a.n_seqs == 0) a.c.max_pages = 0;  // (no table and no lengths then)
     if (mode != 0)
         if (int st = kv_check_pointers(fn, a.c)) return st;
-    LHQ_REQUIRE(a.q && a.offsets && a.out && (mode == 0 || a.lengths), "%s: null pointer", fn);
+    LHQ_REQUIRE(a.q && a.offsets && a.out && (mode == 0 || a.n_seqs == 0 || a.lengths), "%s: null pointer", fn);
     if (mode == 0) LHQ_REQUIRE(a.k_new, "%s: null pointer", fn);
     // Workgroups read keys and values in no order with the writing of results; of the
     // queries each reads its own before it writes them.

@@ -513,3 +513,25 @@ def test_results_beside_their_rows_of_one_buffer(oracle, ops):
     for out in (buf[:size], buf[-size:]):
         ops.attn_prompt(q, k, v, ops.dev(c.offs), 64, scale=c.scale, out=out)
         assert np.array_equal(ops.host(out).reshape(want.shape), want)
+
+
+@pytest.mark.parametrize("width", [0, 3])
+def test_a_chunk_of_no_sequences(ops, width):
+    """Rows there are, sequences none: zeros, or what out held."""
+    import torch
+    i16, i32 = dict(dtype=torch.int16, device="cuda"), dict(dtype=torch.int32, device="cuda")
+    cache = ops.kv_cache("int8", 4, 2, 64)
+    q, k = torch.ones((3, 4 * 64), **i16), torch.ones((3, 2 * 64), **i16)
+    args = torch.zeros(1, **i32), torch.zeros(0, **i32), torch.zeros((0, width), **i32)
+    assert not ops.kv_prefill(cache, q, *args, k, k).any()
+    assert not ops.kv_prefill(cache, q, *args, None, None).any()
+    out = torch.full((3, 4, 64), 77, **i16)
+    ops.kv_prefill(cache, q, *args, k, k, out=out)
+    assert (out == 77).all()
+
+
+def test_chunks_over_a_table_of_no_pages(oracle, ops):
+    """Only the new tokens are seen."""
+    c = Case(oracle, "int8", 4, 2, 64, [0, 0], [70, 3], seed=39, width=0)
+    assert c.table.shape == (2, 0)
+    check(f32(ops, c.run(ops)), *c.want())
