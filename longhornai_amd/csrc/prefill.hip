@@ -157,15 +157,20 @@ __device__ __attribute__((aligned(16))) const uint32_t kZeros[4] = {0, 0, 0, 0};
 
 // 16 bytes a lane from `from` + lane_at + OFFSET to LDS address `to` + OFFSET + 16 *
 // lane, without a register on the way.  In assembly: the compiler makes every later
-// LDS read wait for the builtin's.  arrived() waits for them all.
+// LDS read wait for the builtin's.  arrived() waits for them all.  m0 is named as written:
+// the compiler keeps no variable there (and warns of that), but sets it ahead of
+// instructions of its own, and may take an earlier setting for still there.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 template <int OFFSET>
 __device__ __forceinline__ void dma16(const void* from, uint32_t lane_at, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3"
-                 :: "s"(to), "v"(lane_at), "s"(from), "n"(OFFSET) : "memory");
+                 :: "s"(to), "v"(lane_at), "s"(from), "n"(OFFSET) : "m0", "memory");
 }
 __device__ __forceinline__ void dma16_any(const void* from, uint32_t to) {  // an address a lane
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(to), "v"(from) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(to), "v"(from) : "m0", "memory");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
     return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LHQ_LDS_AS const void*)p));

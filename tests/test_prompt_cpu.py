@@ -255,3 +255,18 @@ def test_results_over_what_others_read_are_refused(L, fn, args, kw):
     at = dict(q=16 << 20, k=24 << 20, v=32 << 20, out=OUT) | kw
     assert L.status(fn, *args(**{n: C.c_void_p(x) if n in ("q", "k", "v", "out") else x for n, x in at.items()})) == INV
     assert "overlap" in L.last_error()
+
+
+def test_assembly_names_the_registers_it_writes():
+    """A statement that sets m0 says so, else the compiler may keep something there."""
+    import glob
+    import os
+    import re
+    sources = glob.glob(os.path.join(os.path.dirname(os.path.abspath(capi.__file__)), "csrc", "*.h*"))
+    found = 0
+    for path in sources:
+        for text in re.findall(r"asm\s+volatile\s*\((.*?)\)\s*;", open(path).read(), flags=re.S):
+            if re.search(r"\b[sv]_\w+\s+m0\s*,", text):
+                found += 1
+                assert '"m0"' in text.rsplit(":", 1)[1], (path, text)
+    assert found >= 2
