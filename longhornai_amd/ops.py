@@ -552,7 +552,11 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling: str | None =
       "ntk"     theta times factor^(rot_dim / (rot_dim - 2)): the slowest pair is
                 divided by factor, the fastest kept
       "yarn"    pairs that make under ``slow`` turns in the original length divided
-                by factor, those over ``fast`` kept, between them in proportion"""
+                by factor, those over ``fast`` kept, between them in proportion to
+                the turns they make, as the method's paper has it.  Checkpoints made
+                by its released code have a ramp in the pair's index, between
+                rounded ends, which differs in the middle (by a factor of up to 2 or
+                3): give rope_plan their own ``frequencies``"""
     if scaling not in (None, "linear", "ntk", "yarn"):
         raise ValueError(f"rope_frequencies: scaling {scaling!r} is not None, 'linear', 'ntk' or 'yarn'")
     if rot_dim < 0 or rot_dim % 2 or not 1.0 <= theta < np.inf or not 1.0 <= factor < np.inf:
@@ -575,15 +579,23 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling: str | None =
 
 def rope_plan(head_dim: int, rot_dim: int | None = None, theta: float = 10000.0, interleaved: bool = False,
               scaling: str | None = None, factor: float = 1.0, original: int = 4096, slow: float = 1.0,
-              fast: float = 32.0, gain: float | None = None) -> RopePlan:
+              fast: float = 32.0, gain: float | None = None, frequencies: np.ndarray | None = None) -> RopePlan:
     """The plan that ``rope`` takes, made once (rope_frequencies says what the
     numbers are).  gain multiplies the turned channels; None: 0.1 ln(factor) + 1
-    with "yarn", else 1."""
+    with "yarn", else 1.  frequencies: radians per position of each pair [rot_dim /
+    2], any finite ones, in place of theta's and the scaling's."""
     rot = head_dim if rot_dim is None else rot_dim
     if head_dim < 1 or not 0 <= rot <= head_dim:
         raise ValueError(f"rope_plan: rot_dim {rot} is no part of head_dim {head_dim}")
-    f = rope_frequencies(rot, theta, scaling, factor, original, slow, fast)
-    turns = np.array([int(x) for x in f / (2 * np.pi) * 2.0 ** 64], np.uint64)
+    if frequencies is None:
+        f = rope_frequencies(rot, theta, scaling, factor, original, slow, fast)
+    else:
+        f = np.asarray(frequencies, np.float64)
+        if scaling is not None or f.shape != (rot // 2,) or rot % 2 or not np.isfinite(f).all():
+            raise ValueError(f"rope_plan: frequencies {f.shape} are not finite ones of {rot} / 2 pairs, or there is "
+                             f"scaling {scaling!r} beside them")
+    # (whole turns per position change nothing; a fraction that rounds to one is none)
+    turns = np.array([int(x * 2.0 ** 64) % 2 ** 64 for x in f / (2 * np.pi) % 1.0], np.uint64)
     if gain is None:
         gain = 0.1 * float(np.log(factor)) + 1.0 if scaling == "yarn" else 1.0
     return RopePlan(head_dim, rot, dev(turns.view(np.int64)), bool(interleaved), float(gain))

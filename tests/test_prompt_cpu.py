@@ -270,3 +270,35 @@ def test_assembly_names_the_registers_it_writes():
                 found += 1
                 assert '"m0"' in text.rsplit(":", 1)[1], (path, text)
     assert found >= 2
+
+
+def test_the_middle_of_the_yarn_ramp_is_by_turns():
+    """Worked out by hand.  theta 10000 and 4 channels: 1 and 0.01 radians a position; in 4096
+    positions the second makes 4096 * 0.01 / (2 pi) = 6.518986469 turns, (6.518986469 - 1) / 31 =
+    0.178031822 of the way from 1 turn to 32: 0.0025 * 0.821968178 + 0.01 * 0.178031822."""
+    f = ops.rope_frequencies(4, theta=10000.0, scaling="yarn", factor=4.0, original=4096)
+    assert f[0] == 1.0 and math.isclose(f[1], 0.003835238663, rel_tol=1e-9)
+    # theta 16, original 64: 1, 1/2, 1/4 and 1/8 make 64 / (2 pi) = 10.18591635788 turns, 5.09295817894,
+    # 2.54647908947 and 1.273...; from 2 to 6 that is 1, 3.09295817894 / 4 = 0.773239544735,
+    # 0.54647908947 / 4 = 0.136619772368 and 0 of the way k, and (1 + k) / 2 of each frequency
+    f = ops.rope_frequencies(8, theta=16.0, scaling="yarn", factor=2.0, original=64, slow=2.0, fast=6.0)
+    assert np.allclose(f, [1.0, 0.25 * 1.773239544735, 0.125 * 1.136619772368, 0.0625], rtol=1e-9, atol=0)
+
+
+def test_plans_of_given_frequencies(monkeypatch):
+    monkeypatch.setattr(ops, "dev", torch.from_numpy)
+    f = ops.rope_frequencies(64, theta=500000.0, scaling="yarn", factor=4.0)
+    a = ops.rope_plan(128, 64, theta=500000.0, scaling="yarn", factor=4.0)
+    b = ops.rope_plan(128, 64, frequencies=f, gain=a.gain)
+    assert torch.equal(a.turns, b.turns) and (a.rot_dim, a.gain) == (b.rot_dim, b.gain)
+    assert ops.rope_plan(128, 64, frequencies=f).gain == 1.0
+    # a quarter turn, the same backwards, one and a quarter, none, nearly none backwards
+    quarter = np.pi / 2
+    turns = ops.rope_plan(10, frequencies=np.array([quarter, -quarter, 5 * quarter, 0.0, -1e-300])).turns
+    assert turns.numpy().view(np.uint64).tolist() == [1 << 62, 3 << 62, 1 << 62, 0, 0]
+    for kw in (dict(frequencies=f[:31]), dict(frequencies=f[None]), dict(frequencies=np.where(f < 1, f, np.nan)),
+               dict(frequencies=np.where(f < 1, f, np.inf)), dict(frequencies=f, scaling="linear"), dict(frequencies=[])):
+        with pytest.raises(ValueError, match="frequencies"):
+            ops.rope_plan(128, 64, **kw)
+    with pytest.raises(ValueError):
+        ops.rope_plan(128, 63, frequencies=f[:31])

@@ -230,3 +230,13 @@ def test_no_rows(ops):
     q, k = (torch.zeros((0, h * 64), dtype=torch.int16, device="cuda") for h in (4, 2))
     got = ops.rope(plan, q, k, torch.zeros(0, dtype=torch.int32, device="cuda"), out=(q, k))
     assert got[0].shape == (0, 256)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_frequencies_of_the_callers(oracle, ops, interleaved):
+    """Any of them: faster than a turn a position, backwards, none."""
+    c = Case(oracle, ops, "f32", 50, 3, 1, 64, False, seed=40, reach=3000, interleaved=interleaved)
+    f = np.random.default_rng(41).normal(0.0, 4.0, 32)
+    f[5] = 0.0
+    c.freq, c.plan = f, ops.rope_plan(64, interleaved=interleaved, frequencies=f)
+    c.check(c.run(ops))
