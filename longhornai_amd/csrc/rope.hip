@@ -363,7 +363,8 @@ int rope(const char* fn, const T* q, int64_t q_stride, const T* k, int64_t k_str
         const int64_t by = ((y - x) % xs + xs) % xs;  // columns of one wider matrix
         return xs == ys && by >= xw && by + yw <= xs;
     };
-    const bool q_in_place = q == q_out && q_stride == q_out_stride, k_in_place = k == k_out && k_stride == k_out_stride;
+    auto in_place = [n_rows](const T* x, int64_t xs, const T* y, int64_t ys) { return x == y && (xs == ys || n_rows == 1); };
+    const bool q_in_place = in_place(q, q_stride, q_out, q_out_stride), k_in_place = in_place(k, k_stride, k_out, k_out_stride);
     LHQ_REQUIRE((q_in_place || apart(q, q_stride, q_width, q_out, q_out_stride, q_width)) &&
                     (k_in_place || apart(k, k_stride, k_width, k_out, k_out_stride, k_width)) &&
                     apart(q, q_stride, q_width, k_out, k_out_stride, k_width) &&

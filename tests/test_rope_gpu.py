@@ -240,3 +240,19 @@ def test_frequencies_of_the_callers(oracle, ops, interleaved):
     f[5] = 0.0
     c.freq, c.plan = f, ops.rope_plan(64, interleaved=interleaved, frequencies=f)
     c.check(c.run(ops))
+
+
+@pytest.mark.parametrize("n", [1, 2])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_in_place_by_views_of_heads(oracle, ops, dtype, n):
+    """Slices of one projection as [n, heads, dim]: of one row such a view has a stride of its own."""
+    import torch
+    c = Case(oracle, ops, dtype, n, 4, 2, 64, True, seed=42)
+    want = c.run(ops)
+    wide = torch.cat([ops.dev(x).reshape(n, -1) for x in (c.q, c.k)], dim=1)
+    q, k = wide.split([256, 128], dim=1)
+    out = q.view(n, 4, 64), k.view(n, 2, 64)
+    w = [ops.dev(x) for x in (c.qw, c.kw)]
+    ops.rope(c.plan, q, k, ops.dev(c.pos), q_weight=w[0], k_weight=w[1], out=out)
+    for got, x in zip(out, want):
+        assert np.array_equal(c.host(ops, got.contiguous()), x)
