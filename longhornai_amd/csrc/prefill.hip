@@ -13,9 +13,9 @@
 // times over, which is what it needs as the B operand of O^T = V^T P^T when V^T's
 // keys come in that order; a row's maximum and sum are one register each.
 // Precision: scores, weights' sums and results are fp32; a weight (of a cached
-// token, times its value scale) is rounded once to bf16, which has the range of
-// both and needs no exponent of its own, at 2^-8 of itself; the result is rounded
-// to bf16.
+// token, times its value scale) is rounded once to bf16, at 2^-8 of itself, which has
+// the range of both and needs no exponent of its own (down to scales of 2^-115 or so:
+// below them weights leave its normal numbers); the result is rounded to bf16.
 //
 // Bound: a tile for 256 rows of 128 channels is 2048 clocks of a SIMD's matrix work,
 // about 1900 of its vector work (exponentials half of it) and 256 KB of LDS reads,

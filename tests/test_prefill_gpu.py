@@ -535,3 +535,20 @@ def test_chunks_over_a_table_of_no_pages(oracle, ops):
     c = Case(oracle, "int8", 4, 2, 64, [0, 0], [70, 3], seed=39, width=0)
     assert c.table.shape == (2, 0)
     check(f32(ops, c.run(ops)), *c.want())
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("by", [-100, -110, 110])
+def test_value_scales_far_down_and_up(oracle, ops, fmt, by):
+    """Weights times scales still are normal bf16 numbers, sums fp32 ones."""
+    c = Case(oracle, fmt, 4, 2, 64, [300], [20], seed=43)
+    c.c.vs *= np.float32(2.0) ** by
+    c.v[:] = 0
+    check(f32(ops, c.run(ops)), *c.want())
+
+
+def test_scores_of_minus_infinity_alone_give_zeros(oracle, ops):
+    c = Case(oracle, None, 2, 1, 64, [0], [140], seed=44)
+    c.q[..., 0], c.k[:5, 0, 0] = 0x3f80, 0xff80  # the first rows see no other keys
+    got = f32(ops, c.run(ops))
+    assert not got[:5].any() and np.isfinite(got).all()
