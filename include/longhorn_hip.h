@@ -492,8 +492,9 @@ int lhq_kv_attn_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k_new,
  * its lengths have to grow by all its new tokens (those of a full table or of rows
  * past row_capacity excepted), else the next call takes other pages for the same
  * entries and the first are lost; one that is over must have no length, or no
- * negative new_tokens, in the next call, or its pages go back twice.  Where tokens may be rejected, pages run out,
- * or a request ends before it has taken its tokens, lhq_kv_plan_owned. */
+ * negative new_tokens, in the next call, or its pages go back twice.  Where tokens
+ * may be rejected, pages run out, or a request ends before it has taken its tokens,
+ * lhq_kv_plan_owned. */
 int lhq_kv_plan(const int32_t* lengths, const int32_t* new_tokens, const uint64_t* tree,
                 const int32_t* left, int32_t* left_out, int32_t* free_pages, int32_t* block_table,
                 int32_t* offsets, int32_t* positions, int64_t* slots, int n_seqs, int row_capacity,
@@ -540,17 +541,18 @@ int lhq_rope_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_
  * tokens 0 .. i and, in lhq_kv_prefill_bf16, before them the first lengths[s]
  * tokens of the cache (clamped to [0, 64 * max_pages]; those of a missing page are
  * not seen).  k_new, v_new both NULL there: only the cache is seen.  A row that
- * sees nothing, or only scores of -infinity, gives zeros; rows before the first sequence's and behind the last
- * one's are left as they are, with clear_rest = 1 they become zeros; what a row does
- * not see, whatever it holds, changes nothing of its result, and an infinite or NaN
- * value of a new token that it does see is in it whatever that token weighs.  out may lie
- * where q does, rows one after the other, else not overlap q, k_new or v_new.  Offsets,
- * strides, scale, table and cache as for lhq_kv_attn_bf16, which is the faster for
- * a few new tokens a sequence.  out [row_capacity, n_heads, head_dim].  Rounding:
- * queries, keys and codes enter the products as they are; a softmax weight, of a
- * cached token times the scale of its value, is rounded to bf16 (2^-8 of itself, or
- * 2^-126 where that is more: cached values that are all under 1e-34 lose bits);
- * scores and sums are fp32, the result is rounded once more to bf16.
+ * sees nothing, or only scores of -infinity, gives zeros; rows before the first
+ * sequence's and behind the last one's are left as they are, with clear_rest = 1 they
+ * become zeros; what a row does not see, whatever it holds, changes nothing of its
+ * result, and an infinite or NaN value of a new token that it does see is in it
+ * whatever that token weighs.  out may lie where q does, rows one after the other,
+ * else not overlap q, k_new or v_new.  Offsets, strides, scale, table and cache as for
+ * lhq_kv_attn_bf16, which is the faster for a few new tokens a sequence.  out
+ * [row_capacity, n_heads, head_dim].  Rounding: queries, keys and codes enter the
+ * products as they are; a softmax weight, of a cached token times the scale of its
+ * value, is rounded to bf16 (2^-8 of itself, or 2^-126 where that is more: cached
+ * values that are all under 1e-34 lose bits); scores and sums are fp32, the result is
+ * rounded once more to bf16.
  * workspace: where there are few rows their keys are split over workgroups, whose
  * partial sums meet there and are added in order of position (deterministic).  Up
  * to lhq_prefill_workspace_bytes bytes are used; with less, or NULL, there are

@@ -12,7 +12,9 @@
 // over all sequences, so one workgroup does them; the rows, which only read
 // what it wrote, are done by it too where they are few and by a launch of their
 // own where they are many.  Bound by latency, a chain of loads and scans: 256 decoding
-// sequences 5.9 us (a pass 12.6, the host's), 48 prompts, 40243 rows, 12.3 and 4.1.
+// sequences 5.9 us (a pass 12.7, the host's); 48 prompts, 40243 rows, 12.1 to 12.6 and
+// 4.0, most of it the pages of those sequences, which are all one wave's: a wave serves
+// the 64 sequences beside one another of its lanes, one after the other.
 #include <algorithm>
 
 #include "kvcommon.hpp"

@@ -20,11 +20,12 @@
 // Bound: a tile for 256 rows of 128 channels is 2048 clocks of a SIMD's matrix work,
 // about 1900 of its vector work (exponentials half of it) and 256 KB of LDS reads,
 // 2048 clocks at the 128 bytes a clock that LDS gives at most; two waves a SIMD
-// overlap them to 3600.  Measured, 32 heads over 8 of 128: 16384 tokens 1.98 to 2.1
-// ms (1050 to 1110 TFLOPS, where a bf16 product of 8192^3 reaches 1190 to 1250), 16
-// prompts of up to 2048 208 us (760), 4 of up to 200 12.5 us.
+// overlap them to 3600.  Measured on several cards, 32 heads over 8 of 128: 16384
+// tokens 1.98 to 2.1 ms (1050 to 1110 TFLOPS, where a bf16 product of 8192^3 reaches
+// 1190 to 1250), 16 prompts of up to 2048 205 to 217 us (730 to 770), 4 of up to 200
+// 12.3 to 12.5 us.
 // Pages cost the conversion of their codes beside it: 512 tokens of 64 heads over
-// 32768 of e4m3 613 us (900 TFLOPS).  Of 64 rows a wave, which halves the LDS reads
+// 32768 of e4m3 601 to 640 us (870 to 920 TFLOPS).  Of 64 rows a wave, which halves the LDS reads
 // but leaves one wave a SIMD: 2290 us where this takes 1985, also with the products
 // of the next tile interleaved with the weights of this one.
 #include <algorithm>

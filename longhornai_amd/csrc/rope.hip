@@ -59,8 +59,8 @@ __device__ __forceinline__ void turn(uint64_t angle, float& c, float& s) {
 
 // A wave a (row, head): lane l has pairs l, l + 64 of the channels; those past
 // rot_dim go in twos that are not turned.  For the heads that rope_vec_kernel does not
-// take: of an odd size (75 channels: 322 us for 32768 rows of 32 and 8 heads, 1.2
-// TB/s), or of more than 128 channels whose pairs are cut into no vectors.
+// take: of an odd size (75 channels: 402 us for 32768 rows of 32 and 8 heads in bf16,
+// 1 TB/s), or of more than 128 channels whose pairs are cut into no vectors.
 template <typename T, bool INTERLEAVED>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs<T> a) {
     const int lane = threadIdx.x & 63, pairs = a.rot / 2, units = (a.D + 1) / 2;
@@ -172,8 +172,9 @@ struct Vector {
 // a row beside one another.  The workgroup makes its rows' cosines and sines once, one
 // or two a thread, through LDS, and a lane keeps its own for all the heads it goes
 // through, of which kBatch are on their way at a time.
-// Bound by memory: 32768 rows of 32 and 8 heads of 128 in bf16, 671 MB in and out, 123
-// us, 5.4 TB/s (a copy of 1 GiB: 5.1; rope_kernel 447).  A few rows: 4.2 us of launch
+// Bound by memory: 32768 rows of 32 and 8 heads of 128 in bf16, 671 MB in and out, 121
+// to 125 us, 5.4 to 5.5 TB/s (a copy of 1 GiB: 5.1; rope_kernel 435); 16384 in fp32, as
+// many bytes, 127 (273).  A few rows: 4.2 us of launch
 // and loads one after the other.
 template <int LB>
 constexpr int heads_of() { return std::min(8, kRopeThreads >> LB); }
@@ -319,9 +320,10 @@ void launch_vec(const RopeArgs<T>& a, hipStream_t s) {
     if constexpr (kKvMaxDim / (2 * V) > 32) go(std::integral_constant<int, 6>{});
 }
 // The widest vectors that the call's channels can be cut into; whether there are any.
-// Measured, 32768 rows of 32 and 8 heads in bf16, widest vectors / rope_kernel: of 128
-// channels 115 / 447 us (vectors of 8), 124 of 128 turned 154 / 431 (2), 126 of 128 224 /
-// 432 (1), 40 40 / 315 (4), 100 105 / 325 (2); the same of 64 rows.
+// Measured, 32768 rows of 32 and 8 heads in bf16, in place, two sets of inputs in turn,
+// widest vectors / rope_kernel: of 128 channels 121 / 435 us (vectors of 8), 124 of 128
+// turned 153 / 440 (2), 126 of 128 225 / 441 (1), 40 40 / 316 (4), 100 133 / 421 (2); of
+// 64 rows 10.6 / 10.6, the host's.
 template <typename T, int V>
 bool by_vectors(const RopeArgs<T>& a, bool interleaved, hipStream_t s) {
     if (whole_vectors<T, V>(a, interleaved)) {
