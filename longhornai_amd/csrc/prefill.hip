@@ -697,17 +697,25 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(PrefillArgs a) {
         const int past = min((end - pages) * kKvPage, token + 1);
         const uint16_t* rows = a.v_new + u.q.lo * a.v_stride + static_cast<int64_t>(h) * D;
         auto value = [&](int n, int ch) { return odd_or_zero(bf16_to_f32(rows[n * a.v_stride + ch])); };
-        for (int ch = 0; ch < D; ++ch) {
-            const bool own = sums && (ch >> 2 & 1) == g;
-            float sum = 0.0f;
-            if (__ballot(own && (blank || !(fabsf(get(ch)) < INFINITY))) != 0) {  // the wave's rows see all of these alike
-                for (int n = from + lane; n < whole; n += 64) sum += value(n, ch);
-                for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
-            }
-            if (some_odd)
-                for (int n = max(from, whole); n < past; ++n) sum += value(n, ch);
-            if (own && sum != 0.0f) set(ch, sum);
+        // those that all of the wave's rows see: a lane has channels lane, lane + 64, ..
+        float seen[(KS + 1) / 2] = {};
+        if (__ballot(sums && all != 0.0f) != 0) {
+#pragma unroll 8
+            for (int n = from; n < whole; ++n)
+#pragma unroll
+                for (int m = 0; m < (KS + 1) / 2; ++m) seen[m] += value(n, min(64 * m + lane, D - 1));
         }
+#pragma unroll
+        for (int m = 0; m < (KS + 1) / 2; ++m)
+            for (int c = 0; c < min(64, D - 64 * m); ++c) {
+                const int ch = 64 * m + c;
+                const bool own = sums && (ch >> 2 & 1) == g;
+                const float before = __shfl(seen[m], c, 64);
+                float sum = own && (blank || !(fabsf(get(ch)) < INFINITY)) ? before : 0.0f;
+                if (some_odd)
+                    for (int n = max(from, whole); n < past; ++n) sum += value(n, ch);
+                if (own && sum != 0.0f) set(ch, sum);
+            }
     };
     if (u.splits > 1) {
         const bool kept = r0 + mine < R;
