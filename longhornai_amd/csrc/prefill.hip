@@ -25,9 +25,9 @@
 // 1190 to 1250), 16 prompts of up to 2048 205 to 217 us (730 to 770), 4 of up to 200
 // 12.3 to 12.5 us.
 // Pages cost the conversion of their codes beside it: 512 tokens of 64 heads over
-// 32768 of e4m3 601 to 640 us (870 to 920 TFLOPS).  Of 64 rows a wave, which halves the LDS reads
-// but leaves one wave a SIMD: 2290 us where this takes 1985, also with the products
-// of the next tile interleaved with the weights of this one.
+// 32768 of e4m3 601 to 640 us (870 to 920 TFLOPS).  Of 64 rows a wave, which halves
+// the LDS reads but leaves one wave a SIMD: 2290 us where this takes 1985, also with
+// the products of the next tile interleaved with the weights of this one.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -683,7 +683,8 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(PrefillArgs a) {
     // weigh.  A tile that some row does not see whole holds none of them any more; in the
     // others they left the products infinite or NaN (0 times infinity, where the weight or
     // a move of the maximum is 0).  get(channel) and set(channel, value) are this lane's
-    // row's; all lanes of the wave call this.
+    // row's; all lanes of the wave call this.  Read in rows: a prompt of 16384 that holds
+    // such values takes up to 9.6 ms, 5.9 with one token of them, 2.3 without.
     const bool some_odd = *odd != 0;
     float all = 0.0f;
 #pragma unroll
